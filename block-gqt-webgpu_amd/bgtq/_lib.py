@@ -12,7 +12,7 @@ from pathlib import Path
 LIB_PATH = Path(os.environ.get("BGTQ_LIB", Path(__file__).resolve().parent.parent / "lib" / "libbgtq.so"))
 
 OK, ERR_RANGE, ERR_STATE, ERR_DEVICE, ERR_UNSUPPORTED, ERR_NOMEM = range(6)
-DTYPE_F32, DTYPE_F16 = 0, 1
+DTYPE_F32, DTYPE_F16, DTYPE_BF16, DTYPE_Q8 = 0, 1, 2, 3
 KEYS_FP16, KEYS_PACKED, KEYS_COMPRESSED = 0, 1, 2
 ROLES = {0: "persistent-k", 1: "persistent-v", 2: "shared", 3: "scratch"}
 
@@ -90,6 +90,43 @@ class PrefillDesc(ctypes.Structure):
                 ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
                 ("q_rotated", ctypes.c_int32)]
 
+
+class Pages(ctypes.Structure):
+    _fields_ = [("kv_heads", ctypes.c_int32), ("dim", ctypes.c_int32), ("key_format", ctypes.c_int32),
+                ("v_format", ctypes.c_int32), ("page_tokens", ctypes.c_int32), ("pages", ctypes.c_int64),
+                ("tables", ctypes.c_void_p * 16), ("packed", ctypes.c_void_p), ("packed_page_stride", ctypes.c_int64),
+                ("packed_head_stride", ctypes.c_int64), ("norms", ctypes.c_void_p),
+                ("norms_page_stride", ctypes.c_int64), ("norms_head_stride", ctypes.c_int64),
+                ("k_f16", ctypes.c_void_p), ("k_page_stride", ctypes.c_int64), ("k_head_stride", ctypes.c_int64),
+                ("v", ctypes.c_void_p), ("v_page_stride", ctypes.c_int64), ("v_head_stride", ctypes.c_int64),
+                ("v_scales", ctypes.c_void_p), ("v_scales_page_stride", ctypes.c_int64),
+                ("v_scales_head_stride", ctypes.c_int64)]
+
+
+class PagedRows(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_int64), ("slots", ctypes.c_void_p), ("k", ctypes.c_void_p),
+                ("k_dtype", ctypes.c_int32), ("k_row_stride", ctypes.c_int64), ("k_head_stride", ctypes.c_int64),
+                ("v", ctypes.c_void_p), ("v_dtype", ctypes.c_int32), ("v_row_stride", ctypes.c_int64),
+                ("v_head_stride", ctypes.c_int64)]
+
+
+class PagedDecodeDesc(ctypes.Structure):
+    _fields_ = [("batch", ctypes.c_int32), ("q_heads", ctypes.c_int32), ("q", ctypes.c_void_p),
+                ("out", ctypes.c_void_p), ("lengths", ctypes.c_void_p), ("page_table", ctypes.c_void_p),
+                ("page_table_stride", ctypes.c_int64), ("max_length", ctypes.c_uint32), ("splits", ctypes.c_int32),
+                ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t), ("q_rotated", ctypes.c_int32)]
+
+
+class PromptDesc(ctypes.Structure):
+    _fields_ = [("q_heads", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("dim", ctypes.c_int32),
+                ("dtype", ctypes.c_int32), ("sequences", ctypes.c_int32), ("tokens", ctypes.c_int64),
+                ("offsets", ctypes.c_void_p), ("q", ctypes.c_void_p), ("q_row_stride", ctypes.c_int64),
+                ("q_head_stride", ctypes.c_int64), ("k", ctypes.c_void_p), ("k_row_stride", ctypes.c_int64),
+                ("k_head_stride", ctypes.c_int64), ("v", ctypes.c_void_p), ("v_row_stride", ctypes.c_int64),
+                ("v_head_stride", ctypes.c_int64), ("out", ctypes.c_void_p), ("out_row_stride", ctypes.c_int64),
+                ("out_head_stride", ctypes.c_int64), ("scale", ctypes.c_float)]
+
+
 class Binding(ctypes.Structure):
     _fields_ = [("ptr", ctypes.c_void_p), ("bytes", ctypes.c_size_t), ("tables", ctypes.c_void_p)]
 
@@ -159,6 +196,12 @@ SIGNATURES = {
     "bgtq_prefill_workspace_size": (_I32, [ctypes.POINTER(PrefillDesc), ctypes.POINTER(ctypes.c_size_t)]),
     "bgtq_prefill": (_I32, [_VP, ctypes.POINTER(PrefillDesc)]),
     "bgtq_prefill_append": (_I32, [_VP, ctypes.POINTER(PrefillDesc), ctypes.POINTER(PrefillAppendDesc)]),
+    "bgtq_paged_write": (_I32, [_VP, ctypes.POINTER(Pages), ctypes.POINTER(PagedRows)]),
+    "bgtq_paged_read": (_I32, [_VP, ctypes.POINTER(Pages), ctypes.POINTER(PagedRows)]),
+    "bgtq_paged_decode_workspace_size": (_I32, [ctypes.POINTER(Pages), ctypes.POINTER(PagedDecodeDesc),
+                                                ctypes.POINTER(ctypes.c_size_t)]),
+    "bgtq_paged_decode": (_I32, [_VP, ctypes.POINTER(Pages), ctypes.POINTER(PagedDecodeDesc)]),
+    "bgtq_prompt_attention": (_I32, [_VP, ctypes.POINTER(PromptDesc)]),
     "bgtq_model_submit": (_I32, [_VP, ctypes.POINTER(ModelDispatch), _SZ]),
     "bgtq_allocate_bits": (_I32, [_VP, _SZ, ctypes.c_int64, _I32, _I32, _VP]),
     "bgtq_layout_groups": (_I32, [_VP, _SZ, _VP, _VP, _VP]),

@@ -30,7 +30,9 @@ DEVICE_SOURCES = ["encode.hip", "encode_bulk.hip", "encode_tile.hip", "encode_wa
                   "decode_fast_any64.hip", "decode_fast_any64_append.hip", "decode_fast_any64_prefill.hip",
                   "decode_fast_any128.hip",
                   "decode_fast_d64.hip", "decode_fast_d64_append.hip", "decode_fast_d64_prefill.hip",
-                  "decode_fast_d128.hip", "prefill.hip", "reconstruct.hip", "model_ops.hip", "decode_scratch.hip"]
+                  "decode_fast_d128.hip", "decode_paged_any64.hip", "decode_paged_any128.hip", "decode_paged_d64.hip",
+                  "decode_paged_d128.hip", "prefill.hip", "reconstruct.hip", "model_ops.hip", "decode_scratch.hip",
+                  "paged_rows.hip", "prompt.hip"]
 HOST_SOURCES = ["bgtq_api.cpp", "calibrate.cpp"]
 
 COMMON = ["-O3", "-std=c++17", "-fPIC", "-Wall", f"-I{INCLUDE}", f"-I{CSRC}"]
@@ -61,6 +63,8 @@ _MAX_ILP = ["-mllvm", "-amdgpu-sched-strategy=max-ilp"]
 SOURCE_FLAGS = {"prefill.hip": ["-fno-honor-nans"],
                 "decode_fast_d64.hip": _MAX_ILP,
                 "decode_fast_any64.hip": _MAX_ILP,
+                "decode_paged_d64.hip": _MAX_ILP,
+                "decode_paged_any64.hip": _MAX_ILP,
                 "decode_fast_d64_append.hip": _MAX_ILP + ["-mllvm", "-amdgpu-set-wave-priority"],
                 "decode_fast_any64_append.hip": ["-mllvm", "-amdgpu-sched-strategy=max-memory-clause"]}
 

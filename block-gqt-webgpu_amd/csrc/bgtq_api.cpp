@@ -1221,7 +1221,7 @@ static int fused_decode_splits(int64_t units, uint32_t max_length, int extra) {
 // four waves still holds the partials. Forced split counts keep four waves.
 static void choose_waves(DecodeParams &p, int nn) {
   p.waves = 4;
-  if (p.dim != 64 || p.splits_forced || nn < 0 || p.v_dtype != BGTQ_DTYPE_F16) return;
+  if (p.dim != 64 || p.splits_forced || nn < 0 || p.v_dtype == BGTQ_DTYPE_F32) return;
   if ((int64_t)p.batch * p.kv_heads * p.splits > device_cus()) return;
   p.waves = 8;
   p.splits = (int)std::min<int64_t>(p.splits, std::max<int64_t>(1, ((int64_t)p.max_length + 255) / 256));
@@ -1293,9 +1293,9 @@ bgtq_status bgtq_decode_workspace_size(const bgtq_decode_desc *d, size_t *bytes)
 // Whether the fused kernel reads p's V: FP16 rows, or FP32 rows in a decode
 // without an appended token; 16-byte aligned base and strides.
 static bool fused_v(const DecodeParams &p) {
-  const bool f32 = p.v_dtype == BGTQ_DTYPE_F32;
-  if (f32 ? p.k_new || p.starts : p.v_dtype != BGTQ_DTYPE_F16) return false;
-  const int64_t vb = f32 ? 4 : 2;
+  const bool f32 = p.v_dtype == BGTQ_DTYPE_F32, q8 = p.v_dtype == BGTQ_DTYPE_Q8;  // (Q8: pages only)
+  if (f32 ? p.k_new || p.starts || p.page_shift : p.v_dtype != BGTQ_DTYPE_F16 && !q8) return false;
+  const int64_t vb = f32 ? 4 : q8 ? 1 : 2;
   return (reinterpret_cast<uintptr_t>(p.v) & 15) == 0 && (p.v_seq_stride * vb) % 16 == 0 &&
          (p.v_head_stride * vb) % 16 == 0;
 }
@@ -1565,6 +1565,337 @@ static bgtq_status decode_impl(bgtq_context *ctx, const bgtq_decode_desc *d, con
     return BGTQ_OK;
   }
   return launch_decode_common(ctx, p, d->q, d->tables);
+}
+
+// ---------------------------------------------------------------- paged cache
+
+}  // extern "C"
+
+namespace {
+
+// The calling thread's device, set again on the way out: the paged calls run
+// on their context's device whatever device is current.
+struct DeviceScope {
+  int before = -1;
+  DeviceScope() {
+    if (hipGetDevice(&before) != hipSuccess) before = -1;
+  }
+  ~DeviceScope() {
+    if (before >= 0) (void)hipSetDevice(before);
+  }
+};
+
+// One array of a pool: its base and strides in bytes, and the bytes of a page's rows of one head.
+bgtq_status check_pool_array(const char *what, const void *base, int64_t page_stride, int64_t head_stride, int64_t rows,
+                             int64_t align, int64_t pages, int32_t heads) {
+  if (!base) return fail(BGTQ_ERR_RANGE, "pages: null %s", what);
+  if (page_stride < 0 || head_stride < 0) return fail(BGTQ_ERR_RANGE, "pages: negative %s stride", what);
+  if (reinterpret_cast<uintptr_t>(base) % (uintptr_t)align || page_stride % align || head_stride % align)
+    return fail(BGTQ_ERR_RANGE, "pages: %s base and strides must be multiples of %d bytes", what, (int)align);
+  if ((pages > 1 && page_stride < rows) || (heads > 1 && head_stride < rows))
+    return fail(BGTQ_ERR_RANGE, "pages: %s stride below the rows of a page", what);
+  return BGTQ_OK;
+}
+
+// A pool's fields as decode parameters (sequence strides: its pages').
+DecodeParams pool_params(const bgtq_pages *g) {
+  DecodeParams p{};
+  p.kv_heads = g->kv_heads;
+  p.dim = g->dim;
+  p.G = 1;
+  p.key_format = g->key_format == BGTQ_KEYS_PACKED ? 1 : 0;
+  p.packed = g->packed;
+  p.packed_seq_stride = g->packed_page_stride;
+  p.packed_head_stride = g->packed_head_stride;
+  p.norms = g->norms;
+  p.norms_seq_stride = g->norms_page_stride;
+  p.norms_head_stride = g->norms_head_stride;
+  p.k = g->k_f16;
+  p.k_seq_stride = g->k_page_stride;
+  p.k_head_stride = g->k_head_stride;
+  p.v = g->v;
+  p.v_dtype = g->v_format;
+  p.v_seq_stride = g->v_page_stride;
+  p.v_head_stride = g->v_head_stride;
+  p.v_scales = g->v_format == BGTQ_DTYPE_Q8 ? g->v_scales : nullptr;
+  p.v_scales_page_stride = g->v_scales_page_stride;
+  p.v_scales_head_stride = g->v_scales_head_stride;
+  p.page_shift = __builtin_ctz((unsigned)g->page_tokens);
+  p.pages = (int32_t)g->pages;
+  return p;
+}
+
+// The fused decode's instance for a pool's layout: nn and sg of a structured
+// one, nn -1 of any other it takes; false where it takes neither.
+bool pool_layout(const DecodeParams &p, const bgtq_pages *g, FastLayout *fl, int *nn, int *sg) {
+  if (fast_layout(p, g->tables, fl, nn, sg)) return true;
+  *nn = -1;
+  return general_layout(p, g->tables, fl);
+}
+
+bgtq_status check_pages(const bgtq_pages *g) {
+  if (!g) return fail(BGTQ_ERR_RANGE, "null pages");
+  if (g->kv_heads < 1 || g->kv_heads > kMaxKvHeads) return fail(BGTQ_ERR_RANGE, "pages: kv_heads must be in 1..%d", kMaxKvHeads);
+  if (g->dim != 64 && g->dim != 128) return fail(BGTQ_ERR_UNSUPPORTED, "pages hold heads of dim 64 or 128 (got %d)", g->dim);
+  if (g->page_tokens < 32 || g->page_tokens > 4096 || (g->page_tokens & (g->page_tokens - 1)))
+    return fail(BGTQ_ERR_RANGE, "page_tokens must be a power of two in 32..4096");
+  if (g->pages < 1 || g->pages > INT32_MAX) return fail(BGTQ_ERR_RANGE, "pages must be in 1..2^31 - 1");
+  if (g->v_format != BGTQ_DTYPE_F16 && g->v_format != BGTQ_DTYPE_Q8) return fail(BGTQ_ERR_RANGE, "pages: invalid V format");
+  const int64_t P = g->page_tokens;
+  if (g->key_format == BGTQ_KEYS_PACKED) {
+    int64_t row = 0, norm = 0;
+    for (int h = 0; h < g->kv_heads; ++h) {
+      if (!g->tables[h]) return fail(BGTQ_ERR_RANGE, "pages: null tables for KV head %d", h);
+      if (g->tables[h]->info.dim != g->dim) return fail(BGTQ_ERR_RANGE, "tables dim mismatch");
+      row = std::max<int64_t>(row, g->tables[h]->info.row_bytes);
+      norm = std::max<int64_t>(norm, g->tables[h]->info.norm_stride);
+    }
+    if (bgtq_status s = check_pool_array("packed K", g->packed, g->packed_page_stride, g->packed_head_stride, P * row, 16,
+                                         g->pages, g->kv_heads))
+      return s;
+    if (bgtq_status s = check_pool_array("scales", g->norms, 2 * g->norms_page_stride, 2 * g->norms_head_stride, 2 * P * norm,
+                                         16, g->pages, g->kv_heads))
+      return s;
+  } else if (g->key_format == BGTQ_KEYS_FP16) {
+    if (bgtq_status s = check_pool_array("FP16 K", g->k_f16, 2 * g->k_page_stride, 2 * g->k_head_stride, 2 * P * g->dim, 16,
+                                         g->pages, g->kv_heads))
+      return s;
+  } else {
+    return fail(BGTQ_ERR_RANGE, "pages: invalid key format");
+  }
+  const int64_t e = g->v_format == BGTQ_DTYPE_F16 ? 2 : 1;
+  if (bgtq_status s = check_pool_array("V", g->v, e * g->v_page_stride, e * g->v_head_stride, e * P * g->dim, 16, g->pages,
+                                       g->kv_heads))
+    return s;
+  if (g->v_format == BGTQ_DTYPE_Q8)
+    if (bgtq_status s = check_pool_array("V scales", g->v_scales, 2 * g->v_scales_page_stride, 2 * g->v_scales_head_stride,
+                                         2 * P, 4, g->pages, g->kv_heads))
+      return s;
+  FastLayout fl{};
+  int nn = 0, sg = 0;
+  if (!pool_layout(pool_params(g), g, &fl, &nn, &sg))
+    return fail(BGTQ_ERR_UNSUPPORTED, "pages hold the packed layouts of the fused decode");
+  return BGTQ_OK;
+}
+
+bgtq_status check_rows(const bgtq_paged_rows *r, bool both) {
+  if (!r) return fail(BGTQ_ERR_RANGE, "null rows");
+  if (r->rows < 0 || r->rows > INT32_MAX) return fail(BGTQ_ERR_RANGE, "rows must be in 0..2^31 - 1");
+  if (both ? !r->k || !r->v : !r->k && !r->v) return fail(BGTQ_ERR_RANGE, "null K or V rows");
+  struct {
+    const void *p;
+    int32_t dtype;
+    int64_t row, head;
+  } x[2] = {{r->k, r->k_dtype, r->k_row_stride, r->k_head_stride}, {r->v, r->v_dtype, r->v_row_stride, r->v_head_stride}};
+  for (auto &a : x) {
+    if (!a.p) continue;
+    if (a.dtype != BGTQ_DTYPE_F32 && a.dtype != BGTQ_DTYPE_F16 && a.dtype != BGTQ_DTYPE_BF16)
+      return fail(BGTQ_ERR_RANGE, "invalid rows dtype");
+    if (a.row < 0 || a.head < 0) return fail(BGTQ_ERR_RANGE, "negative rows stride");
+    if (reinterpret_cast<uintptr_t>(a.p) % (a.dtype == BGTQ_DTYPE_F32 ? 4 : 2))
+      return fail(BGTQ_ERR_RANGE, "rows must be aligned to their type");
+  }
+  if (r->rows && !r->slots) return fail(BGTQ_ERR_RANGE, "null slots");
+  if (reinterpret_cast<uintptr_t>(r->slots) % 8) return fail(BGTQ_ERR_RANGE, "slots must be 8-byte aligned");
+  return BGTQ_OK;
+}
+
+PagedWriteParams rows_params(const bgtq_pages *g, const bgtq_paged_rows *r) {
+  PagedWriteParams p{};
+  p.slots = {r->slots, r->rows, g->pages * g->page_tokens, __builtin_ctz((unsigned)g->page_tokens)};
+  p.kv_heads = g->kv_heads;
+  p.dim = g->dim;
+  if (g->key_format == BGTQ_KEYS_PACKED) {
+    for (int h = 0; h < g->kv_heads; ++h) {
+      p.tables[h] = g->tables[h]->dev();
+      p.enc_bytes[h] = (int32_t)g->tables[h]->h()->off_rot;
+      p.off_rot_t[h] = (int32_t)g->tables[h]->h()->off_rot_t;
+    }
+    p.packed = g->packed;
+    p.packed_page_stride = g->packed_page_stride;
+    p.packed_head_stride = g->packed_head_stride;
+    p.norms = g->norms;
+    p.norms_page_stride = g->norms_page_stride;
+    p.norms_head_stride = g->norms_head_stride;
+  } else {
+    p.k_f16 = g->k_f16;
+    p.kp_page_stride = g->k_page_stride;
+    p.kp_head_stride = g->k_head_stride;
+  }
+  p.v_pool = g->v;
+  p.vp_page_stride = g->v_page_stride;
+  p.vp_head_stride = g->v_head_stride;
+  if (g->v_format == BGTQ_DTYPE_Q8) {
+    p.v_scales = g->v_scales;
+    p.vs_page_stride = g->v_scales_page_stride;
+    p.vs_head_stride = g->v_scales_head_stride;
+  }
+  p.k = r->k;
+  p.v = r->v;
+  p.k_dtype = r->k_dtype;
+  p.v_dtype = r->v_dtype;
+  p.k_row_stride = r->k_row_stride;
+  p.k_head_stride = r->k_head_stride;
+  p.v_row_stride = r->v_row_stride;
+  p.v_head_stride = r->v_head_stride;
+  return p;
+}
+
+}  // namespace
+
+extern "C" {
+
+bgtq_status bgtq_paged_write(bgtq_context *ctx, const bgtq_pages *g, const bgtq_paged_rows *r) {
+  if (bgtq_status s = check_pages(g)) return s;
+  if (bgtq_status s = check_rows(r, true)) return s;
+  if (!ctx) return fail(BGTQ_ERR_RANGE, "null context");
+  if (!r->rows) return BGTQ_OK;
+  DeviceScope scope;
+  if (bgtq_status s = ctx->use()) return s;
+  const PagedWriteParams p = rows_params(g, r);
+  if (g->key_format == BGTQ_KEYS_PACKED) {
+    // Few rows: a wave per row, V in the same launch; many: the tile encoder,
+    // as for dense rows (bgtq_encode_batched).
+    EncodeTileSizes z{};
+    bool tile = r->k_row_stride <= kTileMaxStride;
+    int enc = 0;
+    for (int h = 0; h < g->kv_heads; ++h) {
+      const bgtq_tables_info &t = g->tables[h]->info;
+      tile &= g->tables[h]->tile_encode;
+      z.codebooks = std::max(z.codebooks, t.n_codebooks);
+      z.groups = std::max(z.groups, t.groups);
+      z.row_bytes = std::max(z.row_bytes, t.row_bytes);
+      enc = std::max(enc, p.enc_bytes[h]);
+    }
+    tile = tile && encode_tile_lds_bytes(g->dim, z.codebooks, z.groups, z.row_bytes) <= 160 * 1024;
+    const int lds = paged_write_lds_bytes(g->dim, enc);
+    const bool wave = lds <= 160 * 1024;
+    if (!tile && !wave) return fail(BGTQ_ERR_UNSUPPORTED, "paged write needs %d bytes of LDS (limit 163840)", lds);
+    if (!tile || (wave && r->rows * g->kv_heads < encode_wave_max_rows(g->dim, true))) {
+      HIP_TRY(launch_paged_write(p, true, lds, device_cus(), ctx->stream), "paged write launch");
+      return BGTQ_OK;
+    }
+    HIP_TRY(launch_encode_tile_paged(p, g->dim, device_cus(), z, ctx->stream), "paged encode launch");
+  }
+  HIP_TRY(launch_paged_write(p, false, 0, device_cus(), ctx->stream), "paged write launch");
+  return BGTQ_OK;
+}
+
+bgtq_status bgtq_paged_read(bgtq_context *ctx, const bgtq_pages *g, const bgtq_paged_rows *r) {
+  if (bgtq_status s = check_pages(g)) return s;
+  if (bgtq_status s = check_rows(r, false)) return s;
+  if (!ctx) return fail(BGTQ_ERR_RANGE, "null context");
+  if (!r->rows) return BGTQ_OK;
+  DeviceScope scope;
+  if (bgtq_status s = ctx->use()) return s;
+  HIP_TRY(launch_paged_read(rows_params(g, r), device_cus(), ctx->stream), "paged read launch");
+  return BGTQ_OK;
+}
+
+// Splits of a paged decode: the fused kernel's own choice, or the caller's.
+static bgtq_status plan_paged_decode(const bgtq_pages *g, const bgtq_paged_decode_desc *d, int *splits) {
+  if (bgtq_status s = check_pages(g)) return s;
+  if (!d) return fail(BGTQ_ERR_RANGE, "null descriptor");
+  if (d->batch < 1 || d->q_heads < g->kv_heads || d->q_heads % g->kv_heads || d->q_heads / g->kv_heads > 16)
+    return fail(BGTQ_ERR_RANGE, "invalid head geometry");
+  if (d->batch > 65535) return fail(BGTQ_ERR_UNSUPPORTED, "decode handles up to 65535 sequences per call");
+  if (d->max_length < 1 || d->max_length > (1u << 24)) return fail(BGTQ_ERR_RANGE, "max_length must be in 1..2^24");
+  if (!d->q || !d->out || !d->lengths || !d->page_table) return fail(BGTQ_ERR_RANGE, "null q/out/lengths/page table");
+  if (reinterpret_cast<uintptr_t>(d->q) % 16 || reinterpret_cast<uintptr_t>(d->out) % 16)
+    return fail(BGTQ_ERR_RANGE, "q and out must be 16-byte aligned");
+  if (reinterpret_cast<uintptr_t>(d->lengths) % 4 || reinterpret_cast<uintptr_t>(d->page_table) % 4)
+    return fail(BGTQ_ERR_RANGE, "lengths and page table must be 4-byte aligned");
+  const int64_t need = ((int64_t)d->max_length + g->page_tokens - 1) / g->page_tokens;
+  if (d->page_table_stride < need)
+    return fail(BGTQ_ERR_RANGE, "page table rows hold fewer than the %lld pages of max_length", (long long)need);
+  if (d->q_rotated != 0 && d->q_rotated != 1) return fail(BGTQ_ERR_RANGE, "q_rotated must be 0 or 1");
+  if (d->q_rotated && g->key_format != BGTQ_KEYS_PACKED) return fail(BGTQ_ERR_RANGE, "q_rotated needs packed K");
+  const int64_t units = (int64_t)d->batch * g->kv_heads;
+  *splits = d->splits > 0 ? choose_splits(units, d->max_length, d->splits) : fused_decode_splits(units, d->max_length, 0);
+  return BGTQ_OK;
+}
+
+bgtq_status bgtq_paged_decode_workspace_size(const bgtq_pages *g, const bgtq_paged_decode_desc *d, size_t *bytes) {
+  int splits = 1;
+  if (bgtq_status s = plan_paged_decode(g, d, &splits)) return s;
+  if (!bytes) return fail(BGTQ_ERR_RANGE, "null output");
+  *bytes = decode_ws((int64_t)d->batch * g->kv_heads, (int64_t)d->batch * d->q_heads, g->dim, splits).total;
+  return BGTQ_OK;
+}
+
+bgtq_status bgtq_paged_decode(bgtq_context *ctx, const bgtq_pages *g, const bgtq_paged_decode_desc *d) {
+  int splits = 1;
+  if (bgtq_status s = plan_paged_decode(g, d, &splits)) return s;
+  const DecodeWorkspace w = decode_ws((int64_t)d->batch * g->kv_heads, (int64_t)d->batch * d->q_heads, g->dim, splits);
+  if (!d->workspace || d->workspace_bytes < w.total) return fail(BGTQ_ERR_RANGE, "workspace of %zu bytes required", w.total);
+  if (reinterpret_cast<uintptr_t>(d->workspace) % 16) return fail(BGTQ_ERR_RANGE, "workspace must be 16-byte aligned");
+  if (!ctx) return fail(BGTQ_ERR_RANGE, "null context");
+  DeviceScope scope;
+  if (bgtq_status s = ctx->use()) return s;
+  DecodeParams p = pool_params(g);
+  for (int h = 0; h < g->kv_heads; ++h) p.tables[h] = p.key_format == 1 ? g->tables[h]->dev() : nullptr;
+  p.batch = d->batch;
+  p.q_heads = d->q_heads;
+  p.G = d->q_heads / g->kv_heads;
+  p.page_table = d->page_table;
+  p.page_table_stride = d->page_table_stride;
+  p.table_pages = (int32_t)(((int64_t)d->max_length + g->page_tokens - 1) / g->page_tokens);
+  uint8_t *ws = static_cast<uint8_t *>(d->workspace);
+  p.counters = reinterpret_cast<uint32_t *>(ws + w.counters);
+  p.counter_stride = kCounterStride;
+  p.part = reinterpret_cast<float *>(ws + w.part);
+  p.q = d->q;
+  p.lengths = d->lengths;
+  p.q_rotated = d->q_rotated;
+  p.max_length = (int32_t)d->max_length;
+  p.splits = splits;
+  p.splits_forced = d->splits > 0;
+  p.inv_sqrt_d = (float)(1.0 / std::sqrt((double)g->dim));
+  p.out = d->out;
+  FastLayout fl{};
+  int nn = 0, sg = 0;
+  if (!pool_layout(p, g, &fl, &nn, &sg)) return fail(BGTQ_ERR_UNSUPPORTED, "pages hold the packed layouts of the fused decode");
+  choose_waves(p, nn);
+  HIP_TRY(launch_decode_fast(p, fl, nn, sg, ctx->stream), "paged decode launch");
+  return BGTQ_OK;
+}
+
+// ---------------------------------------------------------------- attention over packed prompts
+bgtq_status bgtq_prompt_attention(bgtq_context *ctx, const bgtq_prompt_desc *d) {
+  if (!d) return fail(BGTQ_ERR_RANGE, "null descriptor");
+  if (d->kv_heads < 1 || d->q_heads < d->kv_heads || d->q_heads % d->kv_heads || d->q_heads > 65535)
+    return fail(BGTQ_ERR_RANGE, "invalid head geometry");
+  if (d->dim != 64 && d->dim != 128)
+    return fail(BGTQ_ERR_UNSUPPORTED, "prompt attention is built for dim 64 and 128 (got %d)", d->dim);
+  if (d->dtype != BGTQ_DTYPE_F16 && d->dtype != BGTQ_DTYPE_BF16) return fail(BGTQ_ERR_RANGE, "invalid dtype");
+  if (d->sequences < 0 || d->sequences > 65535) return fail(BGTQ_ERR_RANGE, "sequences must be in 0..65535");
+  if (d->tokens < 0 || d->tokens > INT32_MAX) return fail(BGTQ_ERR_RANGE, "tokens must be in 0..2^31 - 1");
+  if (!(d->scale >= 0.0f && d->scale <= 3.0e38f)) return fail(BGTQ_ERR_RANGE, "scale must be finite and not negative");
+  const bool none = !d->sequences || !d->tokens;
+  if (!none && (!d->offsets || !d->q || !d->k || !d->v || !d->out)) return fail(BGTQ_ERR_RANGE, "null offsets/q/k/v/out");
+  if (reinterpret_cast<uintptr_t>(d->offsets) % 4) return fail(BGTQ_ERR_RANGE, "offsets must be 4-byte aligned");
+  struct {
+    const void *p;
+    int64_t row, head;
+    int32_t heads;
+  } x[4] = {{d->q, d->q_row_stride, d->q_head_stride, d->q_heads},
+            {d->k, d->k_row_stride, d->k_head_stride, d->kv_heads},
+            {d->v, d->v_row_stride, d->v_head_stride, d->kv_heads},
+            {d->out, d->out_row_stride, d->out_head_stride, d->q_heads}};
+  for (auto &a : x) {
+    if (a.row < 0 || a.head < 0 || a.row % 8 || a.head % 8 || reinterpret_cast<uintptr_t>(a.p) % 16)
+      return fail(BGTQ_ERR_RANGE, "q/k/v/out: 16-byte aligned bases, strides multiples of 8 elements and not negative");
+    if (a.row > kPromptMaxStride) return fail(BGTQ_ERR_RANGE, "q/k/v/out: row strides up to %lld elements", (long long)kPromptMaxStride);
+  }
+  if ((d->tokens > 1 && d->out_row_stride < d->dim) || (d->q_heads > 1 && d->out_head_stride < d->dim))
+    return fail(BGTQ_ERR_RANGE, "out: strides below dim");
+  if (prompt_workgroups(*d) > INT32_MAX) return fail(BGTQ_ERR_UNSUPPORTED, "prompt attention: too many (row, head) pairs for one call");
+  if (!ctx) return fail(BGTQ_ERR_RANGE, "null context");
+  if (none) return BGTQ_OK;
+  DeviceScope scope;
+  if (bgtq_status s = ctx->use()) return s;
+  HIP_TRY(launch_prompt_attention(*d, ctx->stream), "prompt attention launch");
+  return BGTQ_OK;
 }
 
 // ---------------------------------------------------------------- chunked prefill

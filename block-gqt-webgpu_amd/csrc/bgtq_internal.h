@@ -162,6 +162,41 @@ __device__ inline const BGTQ_GLOBAL float *tables_rot_t(const BGTQ_GLOBAL DevTab
 }
 #endif
 
+// Rows of a paged call and their places in the pool.
+struct PagedSlots {
+  const int64_t *slots;
+  int64_t rows, pool_slots;  // rows of the call; slots of the pool (pages << page_shift)
+  int32_t page_shift;
+  // Row i's page and its row there; false where its slot is none of the pool's.
+  __device__ __forceinline__ bool find(int64_t i, int64_t &page, int &at) const {
+    const int64_t s = slots[i];
+    page = s >> page_shift;
+    at = (int)(s & ((1 << page_shift) - 1));
+    return s >= 0 && s < pool_slots;
+  }
+};
+// A paged write or read: the pool of bgtq_pages and the rows of bgtq_paged_rows.
+struct PagedWriteParams {
+  PagedSlots slots;
+  int32_t kv_heads, dim;
+  const DevTables *tables[kMaxKvHeads];  // packed K, else null
+  int32_t enc_bytes[kMaxKvHeads];        // bytes of each table set's header, code LUT and books
+  int32_t off_rot_t[kMaxKvHeads];
+  uint8_t *packed;
+  int64_t packed_page_stride, packed_head_stride;  // bytes
+  uint16_t *norms;
+  int64_t norms_page_stride, norms_head_stride;  // elements
+  uint16_t *k_f16;                               // FP16 K, else null
+  int64_t kp_page_stride, kp_head_stride;
+  void *v_pool;
+  int64_t vp_page_stride, vp_head_stride;
+  uint16_t *v_scales;  // 8-bit V, else null
+  int64_t vs_page_stride, vs_head_stride;
+  void *k, *v;  // the rows outside the pool
+  int32_t k_dtype, v_dtype;
+  int64_t k_row_stride, k_head_stride, v_row_stride, v_head_stride;  // elements
+};
+
 // Decode attention of one layer. Units are (sequence, KV head); each unit
 // serves G query heads (GQA). Work per unit is split over token ranges.
 struct DecodeParams {
@@ -223,6 +258,16 @@ struct DecodeParams {
   int32_t k_new_f32, v_new_f32;
   int64_t k_new_seq_stride, k_new_head_stride, v_new_seq_stride, v_new_head_stride;  // elements
   int64_t k_new_row_stride, v_new_row_stride;                                        // elements
+  // Decode over pages (null otherwise): the page of tokens i << page_shift ..
+  // of sequence b is page_table[b page_table_stride + i], an index 0 .. pages - 1
+  // (any other: no page, its tokens are left out), i < table_pages; the
+  // sequence strides above are then the pages'. v_scales: the FP16 scale of
+  // each 8-bit V row (null: FP16 V).
+  const int32_t *page_table;
+  int64_t page_table_stride;
+  int32_t page_shift, table_pages, pages;
+  const uint16_t *v_scales;
+  int64_t v_scales_page_stride, v_scales_head_stride;  // elements
   // Workgroups per (sequence, KV head) or row-wise unit that take the
   // appended rows (packed K: decode 1; row-wise prefill one row per wave),
   // after the splits in the split dimension; each leaves one partial.
@@ -429,6 +474,17 @@ hipError_t launch_encode_tile(const EncodeJobDev *jobs, int n_jobs, int dim, int
                               const EncodeTileSizes &z, hipStream_t stream);
 hipError_t launch_encode_tile_args(const EncodeTileLaunch &launch, int dim, int src_f32, int64_t max_rows, int cus,
                                    const EncodeTileSizes &z, hipStream_t stream);
+hipError_t launch_encode_tile_paged(const PagedWriteParams &p, int dim, int cus, const EncodeTileSizes &z,
+                                    hipStream_t stream);
+// Paged rows (paged_rows.hip). Write: packed K with a wave per row and, in
+// the same launch, V; or FP16 K and V alone (packed null). Read: both back.
+int paged_write_lds_bytes(int dim, int enc_bytes);
+hipError_t launch_paged_write(const PagedWriteParams &p, bool with_k, int lds_bytes, int cus, hipStream_t stream);
+hipError_t launch_paged_read(const PagedWriteParams &p, int cus, hipStream_t stream);
+// Causal attention over packed prompts (prompt.hip), and its workgroups.
+int64_t prompt_workgroups(const bgtq_prompt_desc &d);
+constexpr int64_t kPromptMaxStride = 1 << 22;  // elements: a block's byte offsets stay below 2^31
+hipError_t launch_prompt_attention(const bgtq_prompt_desc &d, hipStream_t stream);
 hipError_t launch_rotate_q(const DecodeParams &p, const float *q, float *qr, hipStream_t stream);
 // Device address of this device's bgtq_decode_noalloc scratch (decode_scratch.hip).
 hipError_t decode_scratch_setup(int device, hipStream_t stream, uint8_t **out);

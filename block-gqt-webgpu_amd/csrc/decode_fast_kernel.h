@@ -65,9 +65,10 @@ constexpr int kKindDecode = 1;   // decode, no appended rows (FP32 V included)
 constexpr int kKindAppend = 2;   // decode with an appended token (bgtq_decode_append)
 constexpr int kKindPrefill = 4;  // row-wise prefill (p.starts), with or without appended rows
 constexpr int kKindAll = 7;
+constexpr int kKindPaged = 8;  // decode over pages (p.page_table), instances of their own units
 
 inline int decode_fast_launch_kind(const DecodeParams &p) {
-  return p.starts ? kKindPrefill : p.k_new ? kKindAppend : kKindDecode;
+  return p.page_table ? kKindPaged : p.starts ? kKindPrefill : p.k_new ? kKindAppend : kKindDecode;
 }
 
 template <int D>
@@ -92,6 +93,10 @@ struct Geo {
 // 4 g + 0..3 (mod 16) XOR their piece index with 4 g, so the PV reads of the
 // four lane groups (rows 4 apart, the same 16 values) hit different banks.
 __host__ __device__ constexpr int swz32(int row) { return ((row >> 2) & 3) << 2; }
+// The same for a row of D 8-bit codes (D / 16 pieces): the 16 rows of a PV
+// read's 32 lanes, the same piece of each, lie in different banks.
+template <int D>
+__host__ __device__ constexpr int swz8(int row) { return D == 64 ? (row >> 2) & 3 : (row >> 1) & 7; }
 
 // Row-wise prefill stages its rotated queries (16 heads, rows padded to D + 4
 // floats) in dynamic LDS after the ring: no ring slot waits for the staging
@@ -99,7 +104,8 @@ __host__ __device__ constexpr int swz32(int row) { return ((row >> 2) & 3) << 2;
 __host__ __device__ constexpr int prefill_stage_bytes(int D) { return 16 * (D + 4) * 4; }
 
 // VF: the V rows' format, 0 = FP16 (2 bytes per value), 1, 2 = FP32 (4 bytes;
-// a ring of one slot per wave where two do not fit). NW: waves per workgroup.
+// a ring of one slot per wave where two do not fit), 3 = 8-bit codes with an
+// FP16 scale per row (pages). NW: waves per workgroup.
 template <int D, int KF, int NN, int VF = 0, int NW = kWaves>
 struct Slot {
   static constexpr int KS = D / 32;
@@ -109,17 +115,20 @@ struct Slot {
   static constexpr int NSC = KF == 1 ? 1 : KF == 2 ? NN : 0;  // scale DMAs per chunk
   static constexpr bool SMALL2 = KF == 2 && NN == 2 && D == 64;
   static constexpr int NBYTES = SMALL2 ? 384 : NSC * 64 * 4;
-  static constexpr int VBYTES = kChunk * D * (VF ? 4 : 2);
+  static constexpr int VBYTES = kChunk * D * (VF == 3 ? 1 : VF ? 4 : 2);
   static constexpr int VI = VBYTES / 1024;    // 16-byte DMA instructions per V chunk
   static constexpr int NOFF = VBYTES;         // scales
-  static constexpr int KOFF = NOFF + NBYTES;  // K
-  static constexpr int BYTES = KOFF + KI * 1024;
-  static constexpr int L = VI + KI + NSC;  // DMA instructions per chunk
+  static constexpr int NVS = VF == 3 ? 1 : 0;     // V scale DMAs per chunk
+  static constexpr int VSOFF = NOFF + NBYTES;     // V scales
+  static constexpr int KOFF = VSOFF + NVS * 256;  // K
+  // (8-bit V: at least the query staging's bytes)
+  static constexpr int BYTES = VF == 3 && KOFF + KI * 1024 < 16 * (D + 4) * 4 ? 16 * (D + 4) * 4 : KOFF + KI * 1024;
+  static constexpr int L = VI + KI + NSC + NVS;  // DMA instructions per chunk
   // Lookup tables (static LDS): KF 1, the K-steps' books; KF 2, the books'
   // code tables (CTABLES bytes), then kPairSlots pair tables of 2 KB.
   static constexpr int CTABLES = KF == 2 && D == 64 ? 3584 : KF >= 1 ? KS * 2048 : 0;
   static constexpr int TABLES = CTABLES + (KF == 2 ? kPairSlots * 2048 : 0);
-  static constexpr int RING = VF && kRing * NW * BYTES + TABLES > kLdsLimit ? 1 : kRing;
+  static constexpr int RING = (VF == 1 || VF == 2) && kRing * NW * BYTES + TABLES > kLdsLimit ? 1 : kRing;
   static constexpr int AHEAD = RING - 1;
   static constexpr int DYN = RING * NW * BYTES;  // dynamic LDS: the ring (the tables are static)
   // Decode-step append: the new token's wave encodes it with its last ring
@@ -163,7 +172,8 @@ __device__ __forceinline__ float exp_of(float d) {
   return __builtin_amdgcn_exp2f(NAT ? d * kLog2e : d);
 }
 
-template <int D, int SMAX, int NW, bool NAT>
+// PG: a head none of whose splits met a token gets zeros.
+template <int D, int SMAX, int NW, bool NAT, bool PG>
 __device__ __forceinline__ void merge_one_round(float *part, float *out, float *stats, int64_t head0, int G, int S,
                                              int wave, int lane) {
   constexpr int kWaves = NW;
@@ -222,7 +232,8 @@ __device__ __forceinline__ void merge_one_round(float *part, float *out, float *
         }
       }
 #pragma unroll
-      for (int dl = 0; dl < DL; ++dl) out[head * D + DL * lane + dl] = acc[dl] / Lsum;
+      for (int dl = 0; dl < DL; ++dl)
+        out[head * D + DL * lane + dl] = PG && M == -INFINITY ? 0.0f : acc[dl] / Lsum;
       if (lane == 0 && stats) {
         stats[head * 2] = NAT ? M : M * kLn2;
         stats[head * 2 + 1] = Lsum;
@@ -372,8 +383,9 @@ __device__ __forceinline__ void merge_rows(float *part, float *out, const MergeR
   "s"((int)fl.gnb[kv]), "s"((int)fl.gbstride[kv]), "s"((int)fl.gbnib[kv]), "s"(fl.gpair[kv]),                  \
   "s"((int)fl.grb[kv]), "s"((int)fl.gns[kv]));
 
-// AP: the launch's extra outputs, compiled in only where used: 0 none, 1 the
-// appended rows (decode or prefill append), 2 materialised logits (inspect()).
+// AP: what a launch does beside attention, compiled in only where used: 0
+// nothing, 1 the appended rows (decode or prefill append), 2 materialised
+// logits (inspect()), 3 K and V in pages (decode; a sequence may be empty).
 // RL: the workgroup's role in a launch with appended rows and packed K, known
 // from its split index before anything else: 1 a history split, 2 an append
 // workgroup; 0 either (decided at run time). The kernel below picks it.
@@ -381,19 +393,22 @@ template <int D, int KF, int NN, int SG, int PK = 0, int PF = 0, int VF = 0, int
 __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const FastLayout &fl, uint8_t *tabs) {
   using Gm = Geo<D>;
   using Sl = Slot<D, KF, NN, VF, NW>;
-  static_assert(VF == 0 || PF == 0, "FP32 V: decode only");
+  static_assert(VF == 0 || PF == 0, "FP32 and 8-bit V: decode only");
+  static_assert((AP == 3) >= (VF == 3) && (AP != 3 || (PF == 0 && VF != 1 && VF != 2 && Sl::AHEAD == 1)), "pages");
   static_assert(NW == 4 || NW == 8, "waves per workgroup");
   constexpr int kWaves = NW, kThreads = 64 * NW;
   static_assert(PF == 0 || PF == 8 || PF == 16, "row-wise unit width");
   constexpr int UC = PF ? PF : 16;  // columns of a row-wise unit
   static_assert(KF == 0 || row_enc::scratch_bytes(D) <= Sl::BYTES, "append scratch fits a ring slot");
   constexpr int KS = Gm::KS, DT = Gm::DT, PR = Gm::PR, VI = Sl::VI, KRI = Gm::KRI;
-  constexpr int VB = VF ? 4 : 2;  // bytes per V value
-  constexpr bool NAT = VF != 0;                // logits in natural units, else log2 domain
+  constexpr bool VF32 = VF == 1 || VF == 2, Q8 = VF == 3;
+  constexpr int VB = VF32 ? 4 : Q8 ? 1 : 2;  // bytes per V value
+  constexpr bool PG = AP == 3;               // K and V lie in pages
+  constexpr bool NAT = VF32;                 // logits in natural units, else log2 domain
   constexpr bool F32 = VF == 1 && KF >= 1;     // rotation and QK in FP32
   constexpr float kLogit = NAT ? 1.0f : kLn2;  // a logit's natural value
   // P is carried times 2^15 where it is split into FP16 parts; unscaled for FP32 V.
-  constexpr float kPShift = VF ? 0.0f : 15.0f, kPFactor = VF ? 1.0f : kPScale;
+  constexpr float kPShift = VF32 ? 0.0f : 15.0f, kPFactor = VF32 ? 1.0f : kPScale;
   constexpr int RB = Sl::RB, KI = Sl::KI, L = Sl::L, AHEAD = Sl::AHEAD;
   static_assert(NN >= 0 && NN <= KS && SG >= 1 && SG <= KS, "layout");
   static_assert(Sl::BYTES >= 16 * (D + 4) * 4, "q staging fits one ring slot");
@@ -415,6 +430,9 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
   // Every kernel argument the set-up reads, in one round trip (with the
   // role chosen by the kernel, already loaded there).
   BGTQ_LOAD_ARGS
+  if constexpr (PG)
+    asm volatile("" ::"s"(p.page_table), "s"(p.page_table_stride), "s"(p.page_shift), "s"(p.table_pages), "s"(p.pages),
+                 "s"(p.v_scales));
   __builtin_amdgcn_sched_barrier(0);
   const int unit = qrow * p.kv_heads + kv;
   uint32_t *const counter = p.counters + (int64_t)unit * (p.counter_stride > 0 ? p.counter_stride : 1);
@@ -461,14 +479,17 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
   // Each chunk's loads use buffer descriptors based at the chunk's first token
   // and sized to the chunk's tokens inside the sequence: the hardware range
   // check (which covers the per-lane offset) returns zeros past the length.
-  // V strides count values.
+  // V strides count values. Pages: the bases are page 0's, the sequence
+  // strides the pages' (a chunk adds its page's).
+  const int bs = PG ? 0 : b;
   const uint8_t *v_rows =
-      static_cast<const uint8_t *>(p.v) + ((int64_t)b * p.v_seq_stride + (int64_t)kv * p.v_head_stride) * VB;
+      static_cast<const uint8_t *>(p.v) + ((int64_t)bs * p.v_seq_stride + (int64_t)kv * p.v_head_stride) * VB;
   const _Float16 *v_base = reinterpret_cast<const _Float16 *>(v_rows);  // FP16 V: the appended row's store
-  const uint8_t *k_base = KF >= 1 ? p.packed + b * p.packed_seq_stride + kv * p.packed_head_stride
+  const uint8_t *k_base = KF >= 1 ? p.packed + bs * p.packed_seq_stride + kv * p.packed_head_stride
                                   : reinterpret_cast<const uint8_t *>(static_cast<const _Float16 *>(p.k) +
-                                                                      b * p.k_seq_stride + kv * p.k_head_stride);
-  const uint16_t *n_base = KF >= 1 ? p.norms + b * p.norms_seq_stride + kv * p.norms_head_stride : nullptr;
+                                                                      bs * p.k_seq_stride + kv * p.k_head_stride);
+  const uint16_t *n_base = KF >= 1 ? p.norms + bs * p.norms_seq_stride + kv * p.norms_head_stride : nullptr;
+  const uint16_t *vs_base = Q8 ? p.v_scales + kv * p.v_scales_head_stride : nullptr;
   // Packed row bytes and scales per row (runtime for KF 2).
   const int rb = KF == 2 ? fl.grb[kv] : RB;
   const int ns = KF == 2 ? fl.gns[kv] : 2;
@@ -478,8 +499,11 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
   uint32_t voff_rows[VI], koff_rows[KF == 0 ? KRI : 1];
 #pragma unroll
   for (int k = 0; k < VI; ++k) {
-    const int P = 64 * k + lane, r = P / (VF ? D / 4 : PR), c = P % (VF ? D / 4 : PR);
-    voff_rows[k] = VF ? r * (4 * D) + ((c ^ swz32(r)) * 16) : r * (2 * D) + ((c ^ swz<D>(r)) * 16);
+    constexpr int PV = VF32 ? D / 4 : Q8 ? D / 16 : PR;
+    const int P = 64 * k + lane, r = P / PV, c = P % PV;
+    voff_rows[k] = VF32 ? r * (4 * D) + ((c ^ swz32(r)) * 16)
+                   : Q8 ? r * D + ((c ^ swz8<D>(r)) * 16)
+                        : r * (2 * D) + ((c ^ swz<D>(r)) * 16);
   }
 #pragma unroll
   for (int k = 0; k < (KF == 0 ? KRI : 0); ++k) {
@@ -495,6 +519,24 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
   // these loads and stay in flight through the prologue.
   // FP32 V: the books' FP32 centroids (fl.mfma: the first book, rows of
   // max_centroids), in the places of the code tables.
+  // Pages: chunk i's page from the sequence's table, looked up two chunks
+  // ahead (chunks past the table's end read its last entry and stream
+  // nothing). A vector load: the wait before an iteration's PV covers it.
+  const int first_pg = (split * kWaves + wave) * kChunk, stride_pg = p.splits * kWaves * kChunk;
+  auto load_page = [&](int i) -> int {
+    const int at = min((first_pg + i * stride_pg) >> p.page_shift, p.table_pages - 1);
+    return p.page_table[(int64_t)b * p.page_table_stride + at];
+  };
+  // The page as an index into the pool: -1 where the table names none.
+  auto page_of = [&](int raw) -> int {
+    const int pg = __builtin_amdgcn_readfirstlane(raw);
+    return (uint32_t)pg < (uint32_t)p.pages ? pg : -1;
+  };
+  int raw0 = 0, raw1 = 0;
+  if constexpr (PG) {
+    raw0 = load_page(0);
+    raw1 = load_page(1);
+  }
   const int mc4 = F32 ? 4 * fl.gmc[kv] : 0;
   if (F32 && KF == 1 && wave == 0) {
 #pragma unroll
@@ -670,22 +712,33 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
   // a row-wise prefill chunk's history is read by every unit of its KV head,
   // so those loads keep the default policy and the units share it in L2.
   constexpr int kPol = PF ? kCached : kStream;
-  auto issue = [&](int i) {
+  auto issue = [&](int i, int pg = 0) {
     const int c0 = first + i * stride;
     // Tokens of the chunk inside the sequence; none for a chunk past the end
     // (a zero-sized descriptor: the DMA only writes zeros to LDS). A history
     // split's range ends before the appended token, so its row arrives as
     // zeros; the append workgroup streams nothing.
-    const int in_seq = app_wg ? 0 : min(T_att - c0, kChunk);
+    // Pages hold whole chunks; one of a page that is not in the pool streams nothing.
+    const int in_seq = app_wg || pg < 0 ? 0 : min(T_att - c0, kChunk);
     const uint32_t rest = __builtin_amdgcn_readfirstlane(in_seq > 0 ? in_seq : 0);  // wave-uniform: SGPR descriptor
     uint8_t *sb = slot_base(i % Sl::RING);
-    const __amdgpu_buffer_rsrc_t rV = rsrc(v_rows + (int64_t)c0 * D * VB, rest * (VB * D));
+    const int64_t pn = PG && pg > 0 ? pg : 0;
+    const int r0 = PG ? c0 & ((1 << p.page_shift) - 1) : c0;  // the chunk's first row at the bases
+    const uint8_t *v_rows_c = PG ? v_rows + pn * p.v_seq_stride * VB : v_rows;
+    const uint8_t *k_base_c = PG ? k_base + pn * (KF >= 1 ? p.packed_seq_stride : 2 * p.k_seq_stride) : k_base;
+    const uint16_t *n_base_c = PG && KF >= 1 ? n_base + pn * p.norms_seq_stride : n_base;
+    const __amdgpu_buffer_rsrc_t rV = rsrc(v_rows_c + (int64_t)r0 * D * VB, rest * (VB * D));
 #pragma unroll
     for (int k = 0; k < VI; ++k) dma16<kPol>(rV, sb + k * 1024, voff_rows[k], 0);
+    if constexpr (Q8) {
+      // (an odd chunk's last scale comes with the next row's: chunk_pv clears that)
+      const uint16_t *vs = vs_base + pn * p.v_scales_page_stride + r0;
+      dma4<kPol>(rsrc(vs, (rest * 2 + 3u) & ~3u), sb + Sl::VSOFF, lane * 4, 0);
+    }
     uint8_t *kb = sb + Sl::KOFF;
     if (KF == 1) {
-      const __amdgpu_buffer_rsrc_t rK = rsrc(k_base + (int64_t)c0 * RB, rest * RB);
-      const __amdgpu_buffer_rsrc_t rN = rsrc(n_base + (int64_t)c0 * 2, rest * 4);
+      const __amdgpu_buffer_rsrc_t rK = rsrc(k_base_c + (int64_t)r0 * RB, rest * RB);
+      const __amdgpu_buffer_rsrc_t rN = rsrc(n_base_c + (int64_t)r0 * 2, rest * 4);
 #pragma unroll
       for (int k = 0; k < KI; ++k) dma16<kPol>(rK, kb + k * 1024, k * 1024 + lane * 16, 0);
       dma4<kPol>(rN, sb + Sl::NOFF, lane * 4, 0);
@@ -696,15 +749,15 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
       // end on the access size (16 and 4 bytes): the last row's bytes arrive,
       // and the few bytes past it lie in the same aligned 16 bytes as the row's
       // end (both bases are 16-byte aligned, c0 a multiple of 32).
-      const __amdgpu_buffer_rsrc_t rK = rsrc(k_base + (int64_t)c0 * rb, (rest * rb + 15u) & ~15u);
-      const __amdgpu_buffer_rsrc_t rN = rsrc(n_base + (int64_t)c0 * ns, (rest * ns * 2 + 3u) & ~3u);
+      const __amdgpu_buffer_rsrc_t rK = rsrc(k_base_c + (int64_t)r0 * rb, (rest * rb + 15u) & ~15u);
+      const __amdgpu_buffer_rsrc_t rN = rsrc(n_base_c + (int64_t)r0 * ns, (rest * ns * 2 + 3u) & ~3u);
 #pragma unroll
       for (int k = 0; k < KI; ++k) dma16<kPol>(rK, kb + k * 1024, k * 1024 + lane * 16, 0);
 #pragma unroll
       for (int k = 0; k < Sl::NSC; ++k)
         if (k * 256 + lane * 4 < Sl::NBYTES) dma4<kPol>(rN, sb + Sl::NOFF + k * 256, k * 256 + lane * 4, 0);
     } else {
-      const __amdgpu_buffer_rsrc_t rK = rsrc(k_base + (int64_t)c0 * (2 * D), rest * (2 * D));
+      const __amdgpu_buffer_rsrc_t rK = rsrc(k_base_c + (int64_t)r0 * (2 * D), rest * (2 * D));
 #pragma unroll
       for (int k = 0; k < KI; ++k) dma16<kPol>(rK, kb + k * 1024, koff_rows[k], 0);
     }
@@ -829,6 +882,7 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
     if (KF == 0) load_piece(p.k_new, p.k_new_f32, k_off, k_raw);
   }
 
+  const int page0 = PG ? page_of(raw0) : 0;
   // Unconditional, so every wave has exactly AHEAD * L chunk loads in flight
   // behind its prologue loads (chunks past the end are zero-sized). The
   // scheduling barriers keep the prologue's loads ahead of them, so waiting
@@ -836,7 +890,7 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
   __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
   for (int i = 0; i < AHEAD; ++i)
-    if (!app_wg) issue(i);
+    if (!app_wg) issue(i, page0);
   __builtin_amdgcn_sched_barrier(0);
   float qv[KS][8];
 #pragma unroll
@@ -1248,7 +1302,8 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
   // This lane's logits of the chunk in ring slot sb (first token c0): head
   // col, tokens c0 + 16 u + 4 gq + r in x[4 u + r], log2 domain, masked past
   // the causal ends.
-  auto chunk_logits = [&](const uint8_t *sb, int c0, float (&x)[8]) {
+  // in_pool (pages): the chunk's page is one of the pool's; else it is masked whole.
+  auto chunk_logits = [&](const uint8_t *sb, int c0, float (&x)[8], bool in_pool = true) {
     const uint8_t *kbuf = sb + Sl::KOFF;
     // KF 2: transpose the scale rows (every read of the wave's slot precedes
     // its writes: one wave's LDS operations complete in order).
@@ -1497,19 +1552,52 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
         x[4 * u + r] = v * kq;
       }
     }
-    if (c0 + kChunk > lim_min) {
+    if (c0 + kChunk > lim_min || !in_pool) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int tok = c0 + 16 * (j >> 2) + 4 * gq + (j & 3);
-        x[j] = tok < lim ? x[j] : -INFINITY;
+        x[j] = tok < lim && in_pool ? x[j] : -INFINITY;
       }
     }
   };
   // PV of the chunk in ring slot sb: O += P V. FP16 V: P split into fp16 hi
   // (pha) and lo (pla) parts in A-operand order. FP32 V: the probabilities
   // pr themselves, on the FP32 matrix cores.
-  auto chunk_pv = [&](const uint8_t *sb, const half8 pha, const half8 pla, const float *pr) {
-    if constexpr (VF) {
+  // 8-bit V: v = RN16(s c), the FP16 value that a row's code and scale stand
+  // for, from the codes read transposed (as 1024 + (c + 128) in FP16, exact).
+  // rest: the chunk's tokens inside the sequence.
+  auto chunk_pv = [&](const uint8_t *sb, const half8 pha, const half8 pla, const float *pr, int rest = kChunk) {
+    if constexpr (Q8) {
+      typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+      const uint8_t *sc = sb + Sl::VSOFF + 8 * gq;
+      const u32x2 s0 = *reinterpret_cast<const u32x2 *>(sc), s1 = *reinterpret_cast<const u32x2 *>(sc + 32);
+      uint32_t s4[4] = {s0[0], s0[1], s1[0], s1[1]};  // tokens 4 gq + 0..3, 16 + 4 gq + 0..3
+      if (rest < kChunk) {  // (wave-uniform) no scale of a row past the sequence: it may hold anything
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int tok = 16 * (j >> 1) + 4 * gq + 2 * (j & 1);
+          s4[j] = tok + 1 < rest ? s4[j] : tok < rest ? s4[j] & 0xffffu : 0u;
+        }
+      }
+      const int r8 = col >> 1, vrow = 16 * (r8 >> 2) + 4 * gq + (r8 & 3);
+      u32x2 vc[DT];
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+        ds_read_tr8(sb + vrow * D + ((dt ^ swz8<D>(vrow)) * 16) + 8 * (col & 1), vc[dt]);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        wait_tr8<DT>(dt, vc[dt]);
+        u32x4 vb;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t h = __builtin_amdgcn_perm(0x64646464u, vc[dt][j >> 1] ^ 0x80808080u, j & 1 ? 0x04030402u : 0x04010400u);
+          const half2_t c = __builtin_bit_cast(half2_t, h) - half2_t{(_Float16)1152.0f, (_Float16)1152.0f};
+          vb[j] = __builtin_bit_cast(uint32_t, c * __builtin_bit_cast(half2_t, s4[j]));
+        }
+        O[dt] = mfma(pha, __builtin_bit_cast(half8, vb), O[dt]);
+        O[dt] = mfma(pla, __builtin_bit_cast(half8, vb), O[dt]);
+      }
+    } else if constexpr (VF32) {
       // Lane (gq, col) reads V[16 (j >> 2) + 4 gq + (j & 3)][16 dt + col], the
       // B operand of its probability j = 0..7 (row reads; the four lane
       // groups hit different banks through swz32). The 16x16x4 FP32 product
@@ -1608,6 +1696,8 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
       if (!app_wg) chunk_pv(slot_base(1), __builtin_bit_cast(half8, ph[1]), __builtin_bit_cast(half8, pl[1]), nullptr);
     }
   } else {
+    int raw_next = raw1;           // pages: the table entry of chunk i + 1
+    bool in_pool = page0 >= 0, in_pool_next = true;
     for (int i = 0; i < n_chunks; ++i) {
       const int c0 = first + i * stride;
       // Refill the buffer computed on last iteration with chunk i + AHEAD, then
@@ -1615,10 +1705,17 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
       // after it. With materialised logits the loop also stores, so wait for all.
       if (i + AHEAD < n_chunks) {
         wait_lds();
-        issue(i + AHEAD);
+        if constexpr (PG) {
+          const int pg = page_of(raw_next);
+          in_pool_next = pg >= 0;
+          issue(i + 1, pg);
+          raw_next = load_page(i + 2);
+        } else {
+          issue(i + AHEAD);
+        }
       }
       const int newer = lg ? 0 : min(n_chunks - 1 - i, AHEAD);
-      if (newer == AHEAD) wait_vm<AHEAD * L>();
+      if (newer == AHEAD) wait_vm<AHEAD * L + (PG ? 1 : 0)>();  // (pages: and the table entry's load)
       else if (AHEAD > 2 && newer == 2) wait_vm<2 * L>();
       else if (newer >= 1) wait_vm<L>();
       else wait_vm<0>();
@@ -1634,7 +1731,7 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
       }
 
       float x[8];
-      chunk_logits(sb, c0, x);
+      chunk_logits(sb, c0, x, in_pool);
       if (lg) {  // materialised logits for inspect() (natural units)
   #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -1657,7 +1754,7 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
       m_run = m_new;
       u32x4 ph{}, pl{};
   #pragma unroll
-      for (int k = 0; k < (VF ? 0 : 4); ++k) {
+      for (int k = 0; k < (VF32 ? 0 : 4); ++k) {
         uint32_t h, l;
         split2(pr[2 * k], pr[2 * k + 1], h, l);
         ph[k] = h;
@@ -1684,7 +1781,8 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
       // computed is waited for (at the top of the iteration).
       if (!PF) wait_vm<0>();
       const half8 pha = __builtin_bit_cast(half8, ph), pla = __builtin_bit_cast(half8, pl);
-      chunk_pv(sb, pha, pla, pr);
+      chunk_pv(sb, pha, pla, pr, PG ? min(T_att - c0, kChunk) : kChunk);
+      if constexpr (PG) in_pool = in_pool_next;
     }
   }
 
@@ -1739,7 +1837,7 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
       if (g >= G) continue;
       const int64_t head = (int64_t)qrow * Hq + hq0 + g;
       if (S == 1) {
-        p.out[head * D + dm] = Ov / Lsum;
+        p.out[head * D + dm] = PG && M == -INFINITY ? 0.0f : Ov / Lsum;  // (no token in a page: 0)
         if (dm == 0 && p.stats) {
           p.stats[head * 2] = M * kLogit;
           p.stats[head * 2 + 1] = Lsum;
@@ -1843,10 +1941,10 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
     return;
   }
   if (S <= kMergeOneRound) {
-    if (S <= 8) merge_one_round<D, 8, NW, NAT>(p.part, p.out, p.stats, (int64_t)qrow * Hq + hq0, G, S, wave, lane);
-    else if (S <= 16) merge_one_round<D, 16, NW, NAT>(p.part, p.out, p.stats, (int64_t)qrow * Hq + hq0, G, S, wave, lane);
-    else if (S <= 24) merge_one_round<D, 24, NW, NAT>(p.part, p.out, p.stats, (int64_t)qrow * Hq + hq0, G, S, wave, lane);
-    else merge_one_round<D, kMergeOneRound, NW, NAT>(p.part, p.out, p.stats, (int64_t)qrow * Hq + hq0, G, S, wave, lane);
+    if (S <= 8) merge_one_round<D, 8, NW, NAT, PG>(p.part, p.out, p.stats, (int64_t)qrow * Hq + hq0, G, S, wave, lane);
+    else if (S <= 16) merge_one_round<D, 16, NW, NAT, PG>(p.part, p.out, p.stats, (int64_t)qrow * Hq + hq0, G, S, wave, lane);
+    else if (S <= 24) merge_one_round<D, 24, NW, NAT, PG>(p.part, p.out, p.stats, (int64_t)qrow * Hq + hq0, G, S, wave, lane);
+    else merge_one_round<D, kMergeOneRound, NW, NAT, PG>(p.part, p.out, p.stats, (int64_t)qrow * Hq + hq0, G, S, wave, lane);
     if (tid == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     return;
   }
@@ -1872,7 +1970,7 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
       Lsum = __builtin_fmaf(wgt[tid * S + s], w, Lsum);
       mrow[tid * S + s] = w;
     }
-    for (int s = 0; s < S; ++s) wgt[tid * S + s] = mrow[tid * S + s] / Lsum;
+    for (int s = 0; s < S; ++s) wgt[tid * S + s] = PG && M == -INFINITY ? 0.0f : mrow[tid * S + s] / Lsum;
     if (p.stats) {
       const int64_t head = out_row(tid);
       p.stats[head * 2] = M * kLogit;
@@ -1953,6 +2051,15 @@ template <int KINDS, int D, int KF, int NN, int SG, int PK = 0>
 hipError_t launch_one(const DecodeParams &p, const FastLayout &fl, hipStream_t stream) {
   const int kind = decode_fast_launch_kind(p);
   if (!(kind & KINDS)) return hipErrorInvalidValue;
+  if constexpr ((KINDS & kKindPaged) != 0) {
+    static_assert(KINDS == kKindPaged, "pages have units of their own");
+    if constexpr (D == 64 && KF != 2)  // (the per-position path keeps four waves)
+      if (p.waves == 8)
+        return p.v_scales ? launch_mode<D, KF, NN, SG, PK, 0, 3, 8, 3>(p, fl, stream)
+                          : launch_mode<D, KF, NN, SG, PK, 0, 0, 8, 3>(p, fl, stream);
+    return p.v_scales ? launch_mode<D, KF, NN, SG, PK, 0, 3, kWaves, 3>(p, fl, stream)
+                      : launch_mode<D, KF, NN, SG, PK, 0, 0, kWaves, 3>(p, fl, stream);
+  }
   if (p.v_dtype == BGTQ_DTYPE_F32) {
     if constexpr ((KINDS & kKindDecode) != 0)
       if (kind == kKindDecode && (KF == 0 || p.qk_f32))  // (FP32 centroids: no pairs)

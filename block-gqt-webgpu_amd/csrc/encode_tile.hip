@@ -98,6 +98,18 @@ __host__ __device__ inline TileLds tile_lds(int n_codebooks, int groups, int row
   return L;
 }
 
+// Where a job's rows go: one after another from its first (DenseDst), or to
+// the slots of a pool of pages (PagedDst), whose blocks of 16 rows mostly are
+// consecutive rows of one page too and are then stored as whole words.
+struct DenseDst {
+  static constexpr bool kPaged = false;
+};
+struct PagedDst {
+  static constexpr bool kPaged = true;
+  PagedSlots slots;
+  int64_t packed_page_stride, norms_page_stride;  // bytes, elements
+};
+
 // Waves per SIMD that the register budget leaves room for.
 constexpr int tile_waves_per_simd(int D, bool src_f32) { return D != 64 ? 2 : src_f32 ? 3 : 4; }
 
@@ -110,10 +122,11 @@ constexpr int tile_waves_per_simd(int D, bool src_f32) { return D != 64 ? 2 : sr
 // chain meets a non-finite input. The chain runs over the 8-wide blocks that
 // touch the group (encode.hip; whole groups in encode_bulk.hip), or with
 // WHOLE_ROWS over the row (the wave encoder, for smaller calls).
-template <int D, bool SRC_F32, bool WHOLE_ROWS>
+template <int D, int SRC, bool WHOLE_ROWS, typename Dst = DenseDst>
 __device__ __forceinline__ void encode_tile_body(const EncodeTileJob &job, const int64_t rows, int max_codebooks,
-                                                 int max_groups, int max_row_bytes) {
+                                                 int max_groups, int max_row_bytes, const Dst &place = Dst{}) {
   using S = Tile<D>;
+  constexpr bool SRC_F32 = SRC == BGTQ_DTYPE_F32, SRC_BF16 = SRC == BGTQ_DTYPE_BF16;
   constexpr int KS = S::KS, NT = S::NT, NV = S::NV, W = tile_waves(D), TH = 64 * W;
   constexpr int kSelRow = NT + (NT == 4 ? 0 : 4);
   extern __shared__ __align__(16) uint8_t smem[];
@@ -129,8 +142,9 @@ __device__ __forceinline__ void encode_tile_body(const EncodeTileJob &job, const
   float *const cnt = reinterpret_cast<float *>(smem + L.cnt);
   uint8_t *const wv = smem + L.wave + wave * L.stride;
   // The image of a block's packed rows starts at the destination's byte in
-  // its word (the same for every block: 16 rows are whole words).
-  const uint32_t mis = (uint32_t)reinterpret_cast<uintptr_t>(job.packed) & 3u;
+  // its word (the same for every block: 16 rows are whole words; a block of
+  // consecutive rows of a page at its first row's, scattered rows at 0).
+  uint32_t mis = (uint32_t)reinterpret_cast<uintptr_t>(job.packed) & 3u;
 
   // A quarter of row col of block b per lane, in 16-byte pieces where the
   // source allows, through a buffer range that ends with the job's last row
@@ -176,6 +190,9 @@ __device__ __forceinline__ void encode_tile_body(const EncodeTileJob &job, const
                  (uint32_t)f32_to_f16_bits(__uint_as_float(raw[c / 4][c % 4 + 1])) << 16;
         else
           v[h] = raw[k / 2][2 * (k % 2) + h];
+        if (SRC_BF16)
+          v[h] = (uint32_t)f32_to_f16_bits(__uint_as_float(v[h] << 16)) |
+                 (uint32_t)f32_to_f16_bits(__uint_as_float(v[h] & 0xffff0000u)) << 16;
         typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
         const half2_t x = __builtin_bit_cast(half2_t, v[h]);
         squares = __builtin_amdgcn_fdot2(x, x, squares, false);
@@ -288,6 +305,26 @@ __device__ __forceinline__ void encode_tile_body(const EncodeTileJob &job, const
     // nibble pair shares a byte (its second store goes nowhere), byte codes
     // take one each.
     auto pair_pos = [&](int s) { return 4 * (s + (gq & 1)) + 2 * (gq >> 1); };
+    // Pages: this lane's row's destination (null: no slot of the pool), and
+    // whether the block's rows are consecutive rows of one page.
+    uint8_t *prow_pg = nullptr;
+    uint16_t *nrow_pg = nullptr;
+    bool run = true;
+    if constexpr (Dst::kPaged) {
+      const int nb = (int)min((int64_t)kTileRows, rows - b * kTileRows);
+      int64_t page;
+      int at;
+      if (col < nb && place.slots.find(b * kTileRows + col, page, at)) {
+        prow_pg = job.packed + page * place.packed_page_stride + (int64_t)at * RB;
+        nrow_pg = job.norms + page * place.norms_page_stride + (int64_t)at * NS;
+      }
+      const int lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)reinterpret_cast<uintptr_t>(prow_pg)),
+                hi = __builtin_amdgcn_readfirstlane((int)(reinterpret_cast<uintptr_t>(prow_pg) >> 32));
+      const uintptr_t first = (uintptr_t)(uint32_t)lo | (uintptr_t)(uint32_t)hi << 32;
+      const bool next = reinterpret_cast<uintptr_t>(prow_pg) == first + (uintptr_t)(col * RB);
+      run = first != 0 && __builtin_amdgcn_ballot_w64(col < nb && !next) == 0;
+      mis = run ? (uint32_t)first & 3u : 0u;
+    }
     uint8_t *const img0 = wv + mis;
     const int row_at = col * RB;
     // ATen's 8-lane sum of this row's leaves (leaf(s): position 4 s + gq) over
@@ -418,19 +455,33 @@ __device__ __forceinline__ void encode_tile_body(const EncodeTileJob &job, const
     // production_math.py:20-23: corrected_g = raw_g / max(sqrt(sum c^2), 1e-10).
     const int64_t row0 = b * kTileRows;
     const int nr = (int)min((int64_t)kTileRows, rows - row0);
-    BGTQ_GLOBAL uint16_t *nrow = to_global(job.norms) + (row0 + col) * NS;
+    BGTQ_GLOBAL uint16_t *nrow = Dst::kPaged ? to_global(nrow_pg) : to_global(job.norms) + (row0 + col) * NS;
+    const bool kept = Dst::kPaged ? nrow_pg != nullptr : col < nr;
     for (int h = 0; h < ngb; ++h) {
       const int g = gq + 4 * h;
       const float c = fmaxf(__builtin_sqrtf(tree_sum(h, [&](int s) { return c2[s]; })), 1e-10f);
       const uint16_t sc = f32_to_f16_bits((h == 0 ? raw_g[0] : raw_g[1]) / c);
-      if (g < ng && col < nr) nrow[g] = sc;
+      if (g < ng && kept) nrow[g] = sc;
     }
     for (int g = ng + gq; g < NS; g += 4)
-      if (col < nr) nrow[g] = 0;
+      if (kept) nrow[g] = 0;
     wave_sync();
+    if constexpr (Dst::kPaged) {
+      if (!run) {  // (uniform) lane group gq takes every fourth byte of its row
+        for (int o = gq; o < RB; o += 4)
+          if (prow_pg) to_global(prow_pg)[o] = img0[row_at + o];
+        wave_sync();
+        continue;
+      }
+    }
     // The image to the destination: whole words, then the bytes of the first
     // and last word when they are not whole.
     uint8_t *dst = job.packed + row0 * RB - mis;
+    if constexpr (Dst::kPaged) {  // (the first row's address, in scalar registers)
+      const uintptr_t a = reinterpret_cast<uintptr_t>(prow_pg);
+      dst = reinterpret_cast<uint8_t *>((uintptr_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)a) |
+                                        (uintptr_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(a >> 32)) << 32) - mis;
+    }
     const int e1 = (int)mis + nr * RB, w0 = mis ? 1 : 0, w1 = e1 / 4;
     for (int w = w0 + lane; w < w1; w += 64)
       *reinterpret_cast<BGTQ_GLOBAL uint32_t *>(to_global(dst) + 4 * w) = reinterpret_cast<const uint32_t *>(wv)[w];
@@ -486,10 +537,19 @@ __device__ __forceinline__ void encode_tile_body(const EncodeTileJob &job, const
       return total;
     };
     const int64_t row = b * kTileRows + col;
-    const bool stored = odd != 0 && row < rows;
+    bool stored = odd != 0 && row < rows;
+    uint8_t *prow_at = job.packed + row * RB;
+    uint16_t *nrow_at = job.norms + row * NS;
+    if constexpr (Dst::kPaged) {
+      int64_t page = 0;
+      int at = 0;
+      stored = stored && place.slots.find(row, page, at);
+      prow_at = job.packed + page * place.packed_page_stride + (int64_t)at * RB;
+      nrow_at = job.norms + page * place.norms_page_stride + (int64_t)at * NS;
+    }
     const float *R = reinterpret_cast<const float *>(Tg + T->off_rot);
-    BGTQ_GLOBAL uint8_t *prow = to_global(job.packed) + row * RB;
-    BGTQ_GLOBAL uint16_t *nrow = to_global(job.norms) + row * NS;
+    BGTQ_GLOBAL uint8_t *prow = to_global(prow_at);
+    BGTQ_GLOBAL uint16_t *nrow = to_global(nrow_at);
 #pragma clang loop unroll(disable)
     for (int g = 0; g < (odd ? ng : 0); ++g) {
       const int g0 = T->gstart[g], g1 = T->gend[g];
@@ -537,7 +597,7 @@ __global__ __launch_bounds__(64 * tile_waves(D), tile_waves_per_simd(D, SRC_F32)
   const BGTQ_CONST DevTables *T = to_const<DevTables>(j.t);
   const EncodeTileJob job{j.t, j.src, j.packed + j.dst_row0 * T->row_bytes, j.norms + j.dst_row0 * T->norm_stride,
                           j.src_stride, 0};
-  encode_tile_body<D, SRC_F32, false>(job, j.rows, max_codebooks, max_groups, max_row_bytes);
+  encode_tile_body<D, SRC_F32 ? BGTQ_DTYPE_F32 : BGTQ_DTYPE_F16, false>(job, j.rows, max_codebooks, max_groups, max_row_bytes);
 }
 
 // Jobs from the kernel's arguments: small calls share no device memory with
@@ -546,7 +606,19 @@ template <int D, bool SRC_F32>
 __global__ __launch_bounds__(64 * tile_waves(D), tile_waves_per_simd(D, SRC_F32)) void encode_tile_args_kernel(
     EncodeTileLaunch launch, int max_codebooks, int max_groups, int max_row_bytes) {
   const EncodeTileJob job = launch.jobs[blockIdx.y];
-  encode_tile_body<D, SRC_F32, true>(job, job.rows, max_codebooks, max_groups, max_row_bytes);
+  encode_tile_body<D, SRC_F32 ? BGTQ_DTYPE_F32 : BGTQ_DTYPE_F16, true>(job, job.rows, max_codebooks, max_groups,
+                                                                       max_row_bytes);
+}
+
+// K rows into pages, a KV head per grid y.
+template <int D, int SRC>
+__global__ __launch_bounds__(64 * tile_waves(D), tile_waves_per_simd(D, SRC == BGTQ_DTYPE_F32)) void encode_tile_paged_kernel(
+    PagedWriteParams p, int max_codebooks, int max_groups, int max_row_bytes) {
+  const int h = blockIdx.y;
+  const EncodeTileJob job{p.tables[h], static_cast<const uint8_t *>(p.k) + h * p.k_head_stride * (SRC == BGTQ_DTYPE_F32 ? 4 : 2),
+                          p.packed + h * p.packed_head_stride, p.norms + h * p.norms_head_stride, (int32_t)p.k_row_stride, 0};
+  const PagedDst place{p.slots, p.packed_page_stride, p.norms_page_stride};
+  encode_tile_body<D, SRC, true, PagedDst>(job, p.slots.rows, max_codebooks, max_groups, max_row_bytes, place);
 }
 
 template <typename K, typename J>
@@ -584,7 +656,29 @@ hipError_t launch_any(const EncodeJobDev *table, const EncodeTileLaunch *args, i
   return src_f32 ? launch_d<128, true>(table, args, grid, z, stream) : launch_d<128, false>(table, args, grid, z, stream);
 }
 
+template <int D, int SRC>
+hipError_t launch_paged(const PagedWriteParams &p, const dim3 grid, const EncodeTileSizes &z, hipStream_t stream) {
+  const int lds = tile_lds<D>(z.codebooks, z.groups, z.row_bytes).total, threads = 64 * tile_waves(D);
+  static const hipError_t ok = hipFuncSetAttribute((const void *)encode_tile_paged_kernel<D, SRC>,
+                                                   hipFuncAttributeMaxDynamicSharedMemorySize, kLdsLimit);
+  return launch_k(encode_tile_paged_kernel<D, SRC>, ok, grid, threads, lds, stream, p, z);
+}
+
 }  // namespace
+
+hipError_t launch_encode_tile_paged(const PagedWriteParams &p, int dim, int cus, const EncodeTileSizes &z,
+                                    hipStream_t stream) {
+  const int64_t wg_rows = encode_tile_wg_rows(dim), most = (p.slots.rows + wg_rows - 1) / wg_rows;
+  const int64_t resident = encode_tile_resident(dim, p.k_dtype == BGTQ_DTYPE_F32, cus, z);
+  const dim3 grid((unsigned)std::max<int64_t>(1, std::min<int64_t>(most, resident / p.kv_heads)), (unsigned)p.kv_heads);
+  auto go = [&](auto f32, auto f16, auto bf16) {
+    return p.k_dtype == BGTQ_DTYPE_F32 ? f32(p, grid, z, stream) : p.k_dtype == BGTQ_DTYPE_F16 ? f16(p, grid, z, stream)
+                                                                                               : bf16(p, grid, z, stream);
+  };
+  return dim == 64 ? go(launch_paged<64, BGTQ_DTYPE_F32>, launch_paged<64, BGTQ_DTYPE_F16>, launch_paged<64, BGTQ_DTYPE_BF16>)
+                   : go(launch_paged<128, BGTQ_DTYPE_F32>, launch_paged<128, BGTQ_DTYPE_F16>,
+                        launch_paged<128, BGTQ_DTYPE_BF16>);
+}
 
 bool encode_tile_layout(const DevTables *T) {
   const int d = T->dim;

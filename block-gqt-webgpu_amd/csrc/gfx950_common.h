@@ -204,6 +204,12 @@ __device__ __forceinline__ void ds_read_tr16_pair(const uint8_t *lds0, const uin
                : "=&v"(a), "=&v"(b)
                : "v"((uint32_t)(uintptr_t)(lds_void *)lds0), "v"((uint32_t)(uintptr_t)(lds_void *)lds1));
 }
+// One transposed read of 8-bit values (ds_read_b64_tr_b8: lane i of a 16-lane
+// group gets column i of the eight 16-byte rows whose halves the group's
+// lanes address, lanes 2 r and 2 r + 1 row r's), as ds_read_tr16_pair.
+__device__ __forceinline__ void ds_read_tr8(const uint8_t *lds, u32x2 &a) {
+  asm volatile("s_nop 7\n\tds_read_b64_tr_b8 %0, %1" : "=&v"(a) : "v"((uint32_t)(uintptr_t)(lds_void *)lds));
+}
 // Waits until at most N LDS operations of this wave are in flight; a and b
 // are tied to the wait so nothing that reads them is scheduled before it.
 // LDS operations complete in order, so with the reads of a and b issued
@@ -212,6 +218,27 @@ template <int N>
 __device__ __forceinline__ void wait_lds_tied(u32x2 &a, u32x2 &b) {
   static_assert(N >= 0 && N < 16, "lgkmcnt");
   asm volatile("s_waitcnt lgkmcnt(%2)" : "+v"(a), "+v"(b) : "n"(N));
+}
+
+template <int N>
+__device__ __forceinline__ void wait_lds_tied(u32x2 &a) {
+  static_assert(N >= 0 && N < 16, "lgkmcnt");
+  asm volatile("s_waitcnt lgkmcnt(%1)" : "+v"(a) : "n"(N));
+}
+// Wait for ds_read_tr8 read dt of DT (4 or 8) issued in order.
+template <int DT>
+__device__ __forceinline__ void wait_tr8(int dt, u32x2 &a) {
+  static_assert(DT == 4 || DT == 8, "head dim 64 or 128");
+  switch (DT - 1 - dt) {
+    case 7: return wait_lds_tied<7>(a);
+    case 6: return wait_lds_tied<6>(a);
+    case 5: return wait_lds_tied<5>(a);
+    case 4: return wait_lds_tied<4>(a);
+    case 3: return wait_lds_tied<3>(a);
+    case 2: return wait_lds_tied<2>(a);
+    case 1: return wait_lds_tied<1>(a);
+    default: return wait_lds_tied<0>(a);
+  }
 }
 
 // Wait for transposed read pair dt of DT issued in order (2 (DT - 1 - dt)

@@ -1,0 +1,339 @@
+// Causal attention over whole prompts packed one after another
+// (bgtq_prompt_attention): FP16 or BF16 rows, grouped heads, one pass over the
+// keys with a running maximum and sum (src/model/attention.wgsl:13-39 computes
+// the same in three passes with materialised scores).
+//
+// A workgroup takes kWaves x 32 query rows of one sequence and head, a wave 32
+// of them as the columns of 32x32x16 products. S^T = K Q^T leaves lane (h, q) =
+// (lane / 32, lane % 32) with query q's logits of the keys 8 (i / 4) + 4 h + i % 4
+// in registers i: a query's maximum and sum are taken in registers and over
+// one lane swap, its rescale factor is a lane's own, and the probabilities,
+// rounded to the rows' type, are the B operand of O^T += V^T P^T as they lie
+// (the product's 16 slots hold the keys in that order on both sides). V^T is
+// read from LDS by the transposing reads. Blocks of kKeys keys go HBM -> LDS by
+// DMA, 16-byte pieces XOR-swizzled by row, into two buffers: one barrier per
+// block, the next block in flight under the current one's products.
+//
+// The running maximum is raised only when a block's exceeds it by more than 8
+// in the log2 domain: probabilities then reach 2^8 at most, in range of either
+// type, and most blocks skip the rescale of O.
+#include "bgtq_internal.h"
+#include "gfx950_common.h"
+
+namespace bgtq {
+namespace {
+
+using namespace gfx;
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 half2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x32 __attribute__((ext_vector_type(32)));
+
+constexpr int kWaves = 4, kThreads = 64 * kWaves;
+constexpr int kRows = 32 * kWaves;  // query rows of a workgroup
+constexpr int kKeys = 64;           // keys of a block
+constexpr float kLazy = 8.0f;       // growth of a maximum (log2) that O is not rescaled for
+
+struct PromptParams {
+  const int32_t *offsets;
+  int32_t sequences, heads, group;  // query heads; per KV head
+  int64_t tokens;
+  const uint16_t *q, *k, *v;
+  uint16_t *out;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head;  // elements
+  float c;  // scale * log2(e)
+};
+
+// XOR of a row's 16-byte piece indexes: 16 rows' reads of one piece (K) and
+// four rows' reads of four neighbouring pieces (V) use every bank once.
+template <int D>
+__device__ __forceinline__ int swizzle(int r) {
+  return D == 64 ? ((r >> 1) & 1) << 2 | ((r >> 2) & 3) : (r & 3) << 2 | ((r >> 2) & 3);
+}
+
+template <bool BF>
+__device__ __forceinline__ f32x16 product(u32x4 a, u32x4 b, f32x16 c) {
+  if constexpr (BF)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
+}
+
+// Two values rounded to nearest even, packed.
+template <bool BF>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (BF) return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
+  else return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), half2));
+}
+
+// c plus the two values of a pair.
+template <bool BF>
+__device__ __forceinline__ float add2(uint32_t pair, float c) {
+  if constexpr (BF)
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pair), bf16x2{(__bf16)1.0f, (__bf16)1.0f}, c, false);
+  else
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(half2, pair), half2{(_Float16)1.0f, (_Float16)1.0f}, c, false);
+}
+
+template <bool BF>
+__device__ __forceinline__ float value_of(uint32_t bits) {  // the low 16 bits
+  if constexpr (BF) return __uint_as_float(bits << 16);
+  else return (float)__builtin_bit_cast(_Float16, (uint16_t)bits);
+}
+
+// The other half's value of a query's pair of lanes.
+__device__ __forceinline__ float half_max(float v) {
+  auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float half_sum(float v) {
+  auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// The sequence and its tile of kRows rows that grid slot `slot` stands for.
+// Sequence s owns the slots from offsets[s] / kRows + s on, at least as many as
+// it has tiles; the last sequence that starts at or before the slot is found
+// 64 candidates at a time (every wave by itself).
+struct Place {
+  int64_t begin;
+  int len, tile;  // tile < 0: nothing to do
+};
+__device__ __forceinline__ Place find_place(const PromptParams &p, int64_t slot) {
+  const int lane = threadIdx.x & 63;
+  auto offset = [&](int s) {
+    const int64_t o = p.offsets[s];
+    return o < 0 ? 0 : o > p.tokens ? p.tokens : o;
+  };
+  int lo = 0, n = p.sequences;
+  for (;;) {
+    const int step = (n + 63) / 64, at = lane * step;
+    const int s = lo + (at < n ? at : 0);
+    const int hits = __builtin_popcountll(__builtin_amdgcn_ballot_w64(at < n && offset(s) / kRows + s <= slot));
+    if (hits == 0) return {0, 0, -1};
+    lo += (hits - 1) * step;
+    n = min(step, n - (hits - 1) * step);
+    if (step == 1) break;
+  }
+  lo = __builtin_amdgcn_readfirstlane(lo);
+  const int64_t begin = offset(lo), end = offset(lo + 1);
+  Place r{begin, end > begin ? (int)(end - begin) : 0, 0};
+  const int64_t local = slot - (begin / kRows + lo), tiles = (r.len + kRows - 1) / kRows;
+  r.tile = local < tiles ? (int)(tiles - 1 - local) : -1;  // the longest histories first
+  return r;
+}
+
+template <int D, bool BF>
+__global__ __launch_bounds__(kThreads, 2) void prompt_kernel(PromptParams p) {
+  constexpr int PR = D / 8;                      // 16-byte pieces per row
+  constexpr int QS = D / 16;                     // 16-dimension steps of QK
+  constexpr int MT = D / 32;                     // 32-dimension tiles of O
+  constexpr int BLOCK = kKeys * D * 2;           // bytes of a block of K or V
+  constexpr int DMAS = BLOCK / 1024 / kWaves;    // DMAs per wave and operand
+  __shared__ __align__(16) uint8_t smem[4 * BLOCK];  // K, V of block 0; K, V of block 1
+  const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, qc = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t slot = blockIdx.x / (uint32_t)p.heads;
+  const int head = (int)(blockIdx.x - slot * (uint32_t)p.heads), kv = head / p.group;
+  const Place at = find_place(p, slot);
+  if (at.tile < 0) return;  // uniform for the workgroup
+  const int q0 = at.tile * kRows, row0 = q0 + 32 * wave;  // the workgroup's, this wave's first query
+  const int qi = row0 + qc;                               // this lane's query
+  const int n_blocks = (min(q0 + kRows, at.len) + kKeys - 1) / kKeys;
+
+  const uint16_t *k_base = p.k + at.begin * p.k_row + kv * p.k_head;
+  const uint16_t *v_base = p.v + at.begin * p.v_row + kv * p.v_head;
+  // Block j's rows inside the sequence; the others arrive as zeros.
+  auto issue = [&](int j) {
+    const int rest = min(kKeys, at.len - j * kKeys);
+    uint8_t *buf = smem + (j & 1) * 2 * BLOCK;
+    const __amdgpu_buffer_rsrc_t rk = rsrc(k_base + (int64_t)j * kKeys * p.k_row, (uint32_t)(((rest - 1) * p.k_row + D) * 2));
+    const __amdgpu_buffer_rsrc_t rv = rsrc(v_base + (int64_t)j * kKeys * p.v_row, (uint32_t)(((rest - 1) * p.v_row + D) * 2));
+#pragma unroll
+    for (int i = 0; i < DMAS; ++i) {
+      const int piece = (wave * DMAS + i) * 64 + lane, r = piece / PR, c = (piece % PR) ^ swizzle<D>(r);
+      dma16(rk, buf + (wave * DMAS + i) * 1024, (uint32_t)(r * (int)p.k_row * 2 + c * 16), 0);
+      dma16(rv, buf + BLOCK + (wave * DMAS + i) * 1024, (uint32_t)(r * (int)p.v_row * 2 + c * 16), 0);
+    }
+  };
+  issue(0);
+  // Q: lane (h, q) holds dimensions 16 s + 8 h + 0..7 of query q (past the
+  // sequence: its last row's, not stored).
+  u32x4 qf[QS];
+  {
+    const uint16_t *row = p.q + (at.begin + min(qi, at.len - 1)) * p.q_row + head * p.q_head;
+#pragma unroll
+    for (int s = 0; s < QS; ++s) qf[s] = *reinterpret_cast<const u32x4 *>(row + 16 * s + 8 * h);
+  }
+  f32x16 O[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) O[t][i] = 0.0f;
+  float m = -INFINITY, l = 0.0f;  // log2 domain; this lane's part of the sum
+
+  for (int j = 0; j < n_blocks; ++j) {
+    wait_vm<0>();   // this wave's part of block j has landed (and every earlier load)
+    lds_barrier();  // everyone's has, and everyone is done with the other buffer
+    if (j + 1 < n_blocks) issue(j + 1);
+    if (j * kKeys > row0 + 31) continue;  // every key of the block is past this wave's queries
+    const uint8_t *kb = smem + (j & 1) * 2 * BLOCK, *vb = kb + BLOCK;
+    f32x16 S[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) S[b][i] = 0.0f;
+#pragma unroll
+      for (int s = 0; s < QS; ++s) {
+        const int r = 32 * b + qc;  // A operand: key r
+        const u32x4 a = *reinterpret_cast<const u32x4 *>(kb + r * (2 * D) + (((2 * s + h) ^ swizzle<D>(r)) * 16));
+        S[b] = product<BF>(a, qf[s], S[b]);
+      }
+    }
+    const bool diagonal = j * kKeys + kKeys - 1 > row0;
+    if (diagonal) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          S[b][i] = j * kKeys + 32 * b + 8 * (i >> 2) + 4 * h + (i & 3) <= qi ? S[b][i] : -INFINITY;
+    }
+    float top = S[0][0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) top = fmaxf(top, S[0][i]);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) top = fmaxf(top, S[1][i]);
+    top = half_max(top) * p.c;
+    if (__builtin_amdgcn_ballot_w64(top > m + kLazy)) {  // (also the first block: m = -inf)
+      const float mn = fmaxf(m, top), a = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      l *= a;
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) O[t][i] *= a;
+    }
+    const float mu = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) S[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[b][i], p.c, -mu));
+    // The probabilities rounded to the rows' type; the sum is theirs, so a
+    // query with one key's whole weight gets that key's V exactly.
+    uint32_t P[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      P[e] = pack2<BF>(S[e >> 3][2 * (e & 7)], S[e >> 3][2 * (e & 7) + 1]);
+      l = add2<BF>(P[e], l);
+    }
+    // A key that a query does not see has probability 0, but 0 times an
+    // infinity or a NaN of its V row is not 0: such a block takes the products
+    // one key at a time, leaving out what is not seen.
+    bool plain = true;
+    if (diagonal) {
+      uint32_t bad = 0;
+      constexpr uint32_t kExp = BF ? 0x7f80u : 0x7c00u;
+#pragma unroll
+      for (int i = 0; i < PR; ++i) {
+        const u32x4 w = *reinterpret_cast<const u32x4 *>(vb + (64 * i + lane) * 16);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          bad |= (uint32_t)((w[e] & kExp) == kExp);
+          bad |= (uint32_t)((w[e] >> 16 & kExp) == kExp);
+        }
+      }
+      plain = __builtin_amdgcn_ballot_w64(bad != 0) == 0;
+    }
+    if (plain) {
+#pragma unroll
+      for (int s = 0; s < kKeys / 16; ++s) {
+        const u32x4 pf{P[4 * s], P[4 * s + 1], P[4 * s + 2], P[4 * s + 3]};
+        const int r = 16 * s + 4 * h + ((lane & 15) >> 2);
+        const int piece = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), sub = (lane & 1) * 8;
+        u32x2 va[MT][2];
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+          ds_read_tr16_pair(vb + r * (2 * D) + (((4 * t + piece) ^ swizzle<D>(r)) * 16) + sub,
+                            vb + (r + 8) * (2 * D) + (((4 * t + piece) ^ swizzle<D>(r + 8)) * 16) + sub, va[t][0], va[t][1]);
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+          wait_dt<MT>(t, va[t][0], va[t][1]);
+          O[t] = product<BF>(u32x4{va[t][0][0], va[t][0][1], va[t][1][0], va[t][1][1]}, pf, O[t]);
+        }
+      }
+    } else {
+      f32x32 all;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) all[i] = value_of<BF>(P[i >> 1] >> (16 * (i & 1)) & 0xffffu);
+#pragma clang loop unroll(disable)
+      for (int i = 0; i < 32; ++i) {
+        const float mine = all[i];
+        auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(mine), __float_as_uint(mine), false, false);
+#pragma clang loop unroll(disable)
+        for (int hh = 0; hh < 2; ++hh) {
+          const int key = 32 * (i >> 4) + 8 * ((i & 15) >> 2) + 4 * hh + (i & 3);
+          const float w = __uint_as_float(hh ? both[1] : both[0]);
+          const bool seen = j * kKeys + key <= qi;
+#pragma unroll
+          for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {  // dimensions 32 t + 8 g + 4 h + 0..3
+              const u32x2 vv = *reinterpret_cast<const u32x2 *>(vb + key * (2 * D) + (((4 * t + g) ^ swizzle<D>(key)) * 16) + 8 * h);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float x = value_of<BF>((vv[e >> 1] >> (16 * (e & 1))) & 0xffffu);
+                O[t][4 * g + e] = seen ? __builtin_fmaf(w, x, O[t][4 * g + e]) : O[t][4 * g + e];
+              }
+            }
+        }
+      }
+    }
+  }
+  l = half_sum(l);
+  if (qi >= at.len) return;
+  const float inv = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;  // (a NaN stays one)
+  uint16_t *out = p.out + (at.begin + qi) * p.out_row + head * p.out_head;
+#pragma unroll
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      *reinterpret_cast<u32x2 *>(out + 32 * t + 8 * g + 4 * h) =
+          u32x2{pack2<BF>(O[t][4 * g] * inv, O[t][4 * g + 1] * inv), pack2<BF>(O[t][4 * g + 2] * inv, O[t][4 * g + 3] * inv)};
+}
+
+template <int D, bool BF>
+hipError_t launch_d(const PromptParams &p, int64_t wgs, hipStream_t stream) {
+  hipLaunchKernelGGL((prompt_kernel<D, BF>), dim3((unsigned)wgs), dim3(kThreads), 0, stream, p);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+int64_t prompt_workgroups(const bgtq_prompt_desc &d) { return (d.tokens / kRows + d.sequences) * d.q_heads; }
+
+hipError_t launch_prompt_attention(const bgtq_prompt_desc &d, hipStream_t stream) {
+  PromptParams p{};
+  p.offsets = d.offsets;
+  p.sequences = d.sequences;
+  p.heads = d.q_heads;
+  p.group = d.q_heads / d.kv_heads;
+  p.tokens = d.tokens;
+  p.q = static_cast<const uint16_t *>(d.q);
+  p.k = static_cast<const uint16_t *>(d.k);
+  p.v = static_cast<const uint16_t *>(d.v);
+  p.out = static_cast<uint16_t *>(d.out);
+  p.q_row = d.q_row_stride, p.q_head = d.q_head_stride;
+  p.k_row = d.k_row_stride, p.k_head = d.k_head_stride;
+  p.v_row = d.v_row_stride, p.v_head = d.v_head_stride;
+  p.out_row = d.out_row_stride, p.out_head = d.out_head_stride;
+  p.c = (d.scale > 0.0f ? d.scale : (float)(1.0 / __builtin_sqrt((double)d.dim))) * kLog2e;
+  const int64_t wgs = prompt_workgroups(d);
+  if (d.dim == 64)
+    return d.dtype == BGTQ_DTYPE_BF16 ? launch_d<64, true>(p, wgs, stream) : launch_d<64, false>(p, wgs, stream);
+  return d.dtype == BGTQ_DTYPE_BF16 ? launch_d<128, true>(p, wgs, stream) : launch_d<128, false>(p, wgs, stream);
+}
+
+}  // namespace bgtq

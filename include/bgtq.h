@@ -35,6 +35,9 @@ typedef int32_t bgtq_status;
 
 #define BGTQ_DTYPE_F32 0
 #define BGTQ_DTYPE_F16 1
+/* The paged cache and the prompt attention only: */
+#define BGTQ_DTYPE_BF16 2
+#define BGTQ_DTYPE_Q8 3 /* V rows of 8-bit codes with an FP16 scale each (pages) */
 
 /* Roles of src/webgpu/buffers.ts:1 (Allocation.role). */
 #define BGTQ_ROLE_PERSISTENT_K 0
@@ -56,7 +59,8 @@ const char *bgtq_last_error(void);
  * (at least BGTQ_PREFILL_COUNTER_BYTES, 16-byte aligned, its counter prefix zeroed before the first
  * call). 5: bgtq_attention_record_timed; attention over FP32 V runs on the fused kernel. 6:
  * bgtq_prefill_append; the decode workspace holds one more partial per query head and the prefill
- * workspace the appended rows' partials (allocate what the *_workspace_size calls return). */
+ * workspace the appended rows' partials (allocate what the *_workspace_size calls return).
+ * bgtq_paged_* and bgtq_prompt_attention came later without changing any of these. */
 int32_t bgtq_abi_version(void);
 
 /* ---- context: replaces GPUDevice + GPUQueue ------------------------------ */
@@ -380,6 +384,132 @@ typedef struct {
   int64_t v_new_seq_stride, v_new_row_stride, v_new_head_stride;
 } bgtq_prefill_append_desc;
 bgtq_status bgtq_prefill_append(bgtq_context *ctx, const bgtq_prefill_desc *d, const bgtq_prefill_append_desc *a);
+
+/* ---- paged cache ----------------------------------------------------------
+ * K and V of many sequences in a pool of pages, caller-owned device memory: a
+ * page holds page_tokens tokens of every KV head, a sequence's tokens lie in
+ * the pages that its row of a page table names, in any order of the pool. No
+ * counterpart in the reference, whose stores hold one sequence each
+ * (src/runtime/packed-keys.ts:7-52): pages let sequences of any lengths share
+ * one allocation. Row r of a page (element strides for norms, FP16 K, V and
+ * the V scales):
+ *   packed[page*packed_page_stride + kv*packed_head_stride + r*row_bytes(kv)]
+ *   norms [page*norms_page_stride  + kv*norms_head_stride  + r*norm_stride(kv)]
+ *   k_f16 / v [page*page_stride + kv*head_stride + r*dim]
+ *   v_scales  [page*v_scales_page_stride + kv*v_scales_head_stride + r]
+ * K: BGTQ_KEYS_PACKED (tables[kv]; each head's own row bytes and norm stride)
+ * or BGTQ_KEYS_FP16. V: BGTQ_DTYPE_F16, or BGTQ_DTYPE_Q8: a row of int8 codes
+ * c and one FP16 scale s, standing for the FP16 values nearest s c. s is
+ * max|v| / 127 rounded up to FP16 (so no code passes 127), c = v / s rounded to
+ * the nearest integer, ties to even, of the row rounded to FP16; a row with an
+ * infinity or a NaN gets a NaN scale and reads back as NaN.
+ * dim 64 or 128; page_tokens a power of two, 32 to 4096; pages at most 2^31 - 1;
+ * q_heads / kv_heads at most 16, kv_heads at most 16; every base and page and
+ * head stride a multiple of 16 bytes (v_scales: 4), strides not negative.
+ * The packed layouts are those of bgtq_decode_append (others:
+ * BGTQ_ERR_UNSUPPORTED, nothing is queued). */
+typedef struct {
+  int32_t kv_heads, dim;
+  int32_t key_format; /* BGTQ_KEYS_PACKED or BGTQ_KEYS_FP16 */
+  int32_t v_format;   /* BGTQ_DTYPE_F16 or BGTQ_DTYPE_Q8 */
+  int32_t page_tokens;
+  int64_t pages; /* pages of the pool: indices 0 .. pages - 1 */
+  const bgtq_tables *tables[16];
+  uint8_t *packed;
+  int64_t packed_page_stride, packed_head_stride; /* bytes */
+  uint16_t *norms;
+  int64_t norms_page_stride, norms_head_stride; /* elements */
+  uint16_t *k_f16;
+  int64_t k_page_stride, k_head_stride; /* elements */
+  void *v;
+  int64_t v_page_stride, v_head_stride; /* elements (Q8: bytes) */
+  uint16_t *v_scales;
+  int64_t v_scales_page_stride, v_scales_head_stride; /* elements */
+} bgtq_pages;
+
+/* Rows of K and V outside the pool, and where they belong in it: row i of
+ * head kv at k + i*k_row_stride + kv*k_head_stride (dim elements of k_dtype:
+ * BGTQ_DTYPE_F32, _F16 or _BF16; likewise v), its place the slot slots[i] =
+ * page * page_tokens + row of the page. k and v need no alignment beyond their
+ * type's. rows: 0 .. 2^31 - 1. */
+typedef struct {
+  int64_t rows;
+  const int64_t *slots; /* device int64 [rows] */
+  void *k;
+  int32_t k_dtype;
+  int64_t k_row_stride, k_head_stride; /* elements */
+  void *v;
+  int32_t v_dtype;
+  int64_t v_row_stride, v_head_stride;
+} bgtq_paged_rows;
+/* Writes rows into the pool, K first rounded to FP16 and encoded as
+ * bgtq_encode_batched does (bit for bit), V rounded to FP16 and quantised as
+ * above: a decode step's new tokens, or a prompt's. Rows whose slot lies
+ * outside the pool (negative, or from pages * page_tokens on) are skipped: a
+ * padded batch marks its padding so. Rows of one call have different slots; a
+ * slot named twice holds a mixture of the two rows. k and v are only read. */
+bgtq_status bgtq_paged_write(bgtq_context *ctx, const bgtq_pages *pages, const bgtq_paged_rows *rows);
+/* Reads rows back: K rebuilt in the model's order of dimensions
+ * (src/reference/production_math.py:27-31) in FP32, V's FP16 values, each
+ * rounded once to k_dtype / v_dtype. Rows whose slot lies outside the pool
+ * stay as they were; a slot may be read any number of times. k or v may be
+ * NULL: only the other is read. */
+bgtq_status bgtq_paged_read(bgtq_context *ctx, const bgtq_pages *pages, const bgtq_paged_rows *rows);
+
+/* Decode attention of one layer over pages: as bgtq_decode (queries, outputs,
+ * GQA, workspace, splits and q_rotated are the same), sequence b attending to
+ * its first min(lengths[b], max_length) tokens, token t in page
+ * page_table[b*page_table_stride + t / page_tokens]. A sequence may be empty:
+ * its outputs are zero. Tokens whose table entry is not a page of the pool are
+ * left out (entries past a sequence's tokens are never used). One launch,
+ * HIP-graph capturable (lengths and page table are read on the device). */
+typedef struct {
+  int32_t batch, q_heads;
+  const float *q; /* [B, Hq, dim] FP32 contiguous, 16-byte aligned, as is out's shape */
+  float *out;
+  const uint32_t *lengths;   /* device uint32 [B] */
+  const int32_t *page_table; /* device int32 [B][page_table_stride] */
+  int64_t page_table_stride; /* elements; at least ceil(max_length / page_tokens) */
+  uint32_t max_length;       /* 1 .. 2^24 */
+  int32_t splits;            /* token splits per (sequence, KV head); 0 = choose */
+  void *workspace;           /* bgtq_paged_decode_workspace_size() bytes, as bgtq_decode's */
+  size_t workspace_bytes;
+  int32_t q_rotated;
+} bgtq_paged_decode_desc;
+bgtq_status bgtq_paged_decode_workspace_size(const bgtq_pages *pages, const bgtq_paged_decode_desc *d, size_t *bytes);
+bgtq_status bgtq_paged_decode(bgtq_context *ctx, const bgtq_pages *pages, const bgtq_paged_decode_desc *d);
+
+/* Attention over whole prompts, before their rows enter a cache: causal
+ * self-attention of `sequences` sequences of different lengths packed one
+ * after another, sequence s the rows offsets[s] .. offsets[s+1] - 1 of q, k, v
+ * and out. Query head h uses KV head h / (q_heads / kv_heads). Row i of head h
+ * at q + i*q_row_stride + h*q_head_stride (elements; likewise k, v, out; a row's
+ * dim values are adjacent). dtype: BGTQ_DTYPE_F16 or _BF16, of q, k, v and out.
+ * dim 64 or 128; any q_heads that is a multiple of kv_heads, at most 65535;
+ * sequences up to 65535, tokens (rows of each) up to 2^31 - 1. Bases 16-byte
+ * aligned, strides multiples of 8 elements and not negative; out may not overlap
+ * the inputs. offsets (device int32 [sequences + 1], nondecreasing) are clamped to
+ * 0 .. tokens; a sequence may be empty, and rows of no sequence stay as they
+ * were. scale: of the logits; 0 = 1 / sqrt(dim). Logits, softmax statistics and
+ * sums are FP32, probabilities are rounded to dtype for the product with V. One
+ * launch, no workspace, HIP-graph capturable. (The model's three attention passes
+ * over a whole prompt with uncompressed K: src/model/attention.wgsl:13-39.) */
+typedef struct {
+  int32_t q_heads, kv_heads, dim, dtype;
+  int32_t sequences;
+  int64_t tokens;
+  const int32_t *offsets;
+  const void *q;
+  int64_t q_row_stride, q_head_stride;
+  const void *k;
+  int64_t k_row_stride, k_head_stride;
+  const void *v;
+  int64_t v_row_stride, v_head_stride;
+  void *out;
+  int64_t out_row_stride, out_head_stride;
+  float scale;
+} bgtq_prompt_desc;
+bgtq_status bgtq_prompt_attention(bgtq_context *ctx, const bgtq_prompt_desc *d);
 
 /* ---- calibration-table pipeline (host only, no device needed) ------------
  * The setup that produces the tables(p) blobs bgtq_tables_create takes:

@@ -1,0 +1,208 @@
+"""Causal attention over packed prompts against 64 bits.
+
+An output may be off by the rounding of the probabilities (half a step u of the rows'
+type, relative to each: u sum p |v|), its own rounding (u |ref|) and the FP32 logits
+and sums (2^-14 of sum p |v| covers d 2^-24 times logits below 60).
+"""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+U = {"float16": 2.0 ** -11, "bfloat16": 2.0 ** -8}
+
+
+def _inputs(total, hq, hkv, dim, dtype, seed, scale=1.0):
+    import torch
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn((total, hq + 2 * hkv, dim), generator=g) * scale
+    return x.to(getattr(torch, dtype))
+
+
+def _offsets(lens, first=0):
+    import torch
+    return torch.tensor(np.concatenate([[first], first + np.cumsum(lens)]), dtype=torch.int32, device="cuda")
+
+
+def _reference(q, k, v, scale):
+    """(outputs, sum of p |v|) of one sequence [n, heads, d] in 64 bits."""
+    n, hq, d = q.shape
+    out, size = np.zeros((n, hq, d)), np.zeros((n, hq, d))
+    for h in range(hq if n else 0):
+        kv = h // (hq // k.shape[1])
+        s = np.where(np.tri(n, dtype=bool), q[:, h] @ k[:, kv].T * scale, -np.inf)
+        p = np.exp(s - s.max(-1, keepdims=True))
+        p /= p.sum(-1, keepdims=True)
+        out[:, h], size[:, h] = p @ v[:, kv], p @ np.abs(v[:, kv])
+    return out, size
+
+
+def _check(out, x, lens, hq, hkv, dtype, scale, first=0, what=""):
+    x, got, at = x.double().numpy(), out.double().cpu().numpy(), first
+    for i, n in enumerate(lens):
+        q, k, v = x[at:at + n, :hq], x[at:at + n, hq:hq + hkv], x[at:at + n, hq + hkv:]
+        ref, size = _reference(q, k, v, scale)
+        err, lim = np.abs(got[at:at + n] - ref), U[dtype] * (size + np.abs(ref)) * 1.001 + 2.0 ** -14 * size + 1e-6
+        assert np.all(err <= lim), f"{what} sequence {i} of {n}: worst {np.nanmax(err / lim):.2f} of the limit, {np.isnan(err).sum()} NaN"
+        at += n
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("hq,hkv,lens", [(1, 1, [1]), (3, 1, [2, 0, 31, 1]), (9, 3, [32, 33, 63, 64, 65, 0]), (4, 4, [127, 128, 129]),
+                                         (14, 2, [300, 1, 257]), (2, 1, [0, 0, 1000, 0]), (2, 2, [5] * 70)])
+def test_packed_prompts(device, dtype, dim, hq, hkv, lens):
+    import torch
+    from bgtq import batched
+    batched.bind_torch_stream(device)
+    print(dtype, dim, hq, hkv, lens, flush=True)
+    x = _inputs(sum(lens), hq, hkv, dim, dtype, len(lens) + hq)
+    xd = x.cuda()
+    out = torch.full((sum(lens), hq, dim), float("nan"), dtype=x.dtype, device="cuda")
+    batched.prompt_attention(device, xd[:, :hq], xd[:, hq:hq + hkv], xd[:, hq + hkv:], _offsets(lens), out)
+    torch.cuda.synchronize()
+    _check(out, x, lens, hq, hkv, dtype, 1 / np.sqrt(dim))
+
+
+@pytest.mark.parametrize("dtype,dim", [("bfloat16", 64), ("float16", 128)])
+def test_large_logits_and_scale(device, dtype, dim):
+    """Logits of a few hundred (one key takes nearly all), a given scale, and equal logits."""
+    import torch
+    from bgtq import batched
+    batched.bind_torch_stream(device)
+    lens, hq, hkv = [200, 77], 4, 2
+    for mult, scale in ((3.0, 0.25), (1.0, 1e-4), (0.0, None)):
+        x = _inputs(sum(lens), hq, hkv, dim, dtype, 3)
+        x[:, :hq] *= mult
+        xd, out = x.cuda(), torch.empty((sum(lens), hq, dim), dtype=x.dtype, device="cuda")
+        batched.prompt_attention(device, xd[:, :hq], xd[:, hq:hq + hkv], xd[:, hq + hkv:], _offsets(lens), out, scale=scale)
+        torch.cuda.synchronize()
+        _check(out, x, lens, hq, hkv, dtype, scale or 1 / np.sqrt(dim), what=f"scale {scale}")
+
+
+def test_layouts_and_rows_of_no_sequence(device):
+    """Heads-first and padded layouts; rows before the first and behind the last sequence stay as they were, whatever
+    the inputs hold there."""
+    import torch
+    from bgtq import batched
+    batched.bind_torch_stream(device)
+    dtype, dim, hq, hkv, lens, total, first = "bfloat16", 64, 4, 2, [100, 37], 180, 9
+    x = _inputs(total, hq, hkv, dim, dtype, 8)
+    x[:first], x[first + 137:] = float("nan"), float("inf")
+    q = torch.full((hq, total, dim + 8), float("nan"), dtype=x.dtype, device="cuda")
+    q[:, :, :dim] = x[:, :hq].transpose(0, 1).cuda()
+    k, v = x[:, hq:hq + hkv].transpose(0, 1).contiguous().cuda(), x[:, hq + hkv:].cuda()
+    out = torch.full((hq, total, dim), 3.0, dtype=x.dtype, device="cuda")
+    batched.prompt_attention(device, q[:, :, :dim].transpose(0, 1), k.transpose(0, 1), v, _offsets(lens, first), out.transpose(0, 1))
+    torch.cuda.synchronize()
+    _check(out.transpose(0, 1), x, lens, hq, hkv, dtype, 1 / 8, first)
+    assert bool((out[:, :first] == 3).all()) and bool((out[:, first + 137:] == 3).all())
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("bad", ["nan", "inf", "-inf"])
+def test_non_finite_rows_reach_only_what_sees_them(device, dim, bad):
+    """A K or V row with infinities or NaNs changes nothing for the queries before it, nor for other sequences."""
+    import torch
+    from bgtq import batched
+    batched.bind_torch_stream(device)
+    lens, hq, hkv, dtype = [150, 90], 2, 1, "float16"
+    x = _inputs(240, hq, hkv, dim, dtype, 4)
+    clean = x.clone()
+    x[100, hq + hkv:, 3::7] = float(bad)  # V of token 100
+    x[120, hq:hq + hkv] = float(bad)      # K of token 120
+    xd, out = x.cuda(), torch.empty((240, hq, dim), dtype=x.dtype, device="cuda")
+    batched.prompt_attention(device, xd[:, :hq], xd[:, hq:hq + hkv], xd[:, hq + hkv:], _offsets(lens), out)
+    torch.cuda.synchronize()
+    got = out.double().cpu().numpy()
+    ref, size = _reference(*(clean[:150].double().numpy()[:, a:b] for a, b in ((0, 2), (2, 3), (3, 4))), 1 / np.sqrt(dim))
+    lim = U[dtype] * (size + np.abs(ref)) * 1.001 + 2.0 ** -14 * size + 1e-6
+    assert np.all(np.abs(got[:100] - ref[:100]) <= lim[:100])
+    hit = np.zeros(dim, bool)
+    hit[3::7] = True
+    assert np.all(np.abs(got[100:120] - ref[100:120])[..., ~hit] <= lim[100:120][..., ~hit])
+    want = float(bad)
+    seen = got[100:120][..., hit]
+    assert np.all(np.isnan(seen)) if np.isnan(want) else np.all(seen == want)
+    assert np.all(~np.isfinite(got[120:150]) | np.isnan(got[120:150])) or bad == "-inf" or bad == "inf"
+    ref2, size2 = _reference(*(clean[150:].double().numpy()[:, a:b] for a, b in ((0, 2), (2, 3), (3, 4))), 1 / np.sqrt(dim))
+    assert np.all(np.abs(got[150:] - ref2) <= U[dtype] * (size2 + np.abs(ref2)) * 1.001 + 2.0 ** -14 * size2 + 1e-6)
+
+
+def test_lowest_values(device):
+    """Keys of the type's lowest and highest values: logits beyond any exponent, weights 0 and 1, no NaN."""
+    import torch
+    from bgtq import batched
+    batched.bind_torch_stream(device)
+    x = _inputs(130, 2, 1, 64, "bfloat16", 2)
+    x[:, :2] = x[:, :2].abs() + 0.1
+    x[40, 2], x[70, 2] = -3e4, 3e4
+    xd, out = x.cuda(), torch.empty((130, 2, 64), dtype=x.dtype, device="cuda")
+    batched.prompt_attention(device, xd[:, :2], xd[:, 2:3], xd[:, 3:], _offsets([130]), out)
+    torch.cuda.synchronize()
+    _check(out[:70], x[:70], [70], 2, 1, "bfloat16", 1 / 8)
+    assert torch.equal(out[70:], xd[70:71, 3:].expand(60, 2, 64))
+
+
+def test_many_sequences_and_bad_offsets(device):
+    """Thousands of short sequences (the search for a tile's sequence takes several rounds); offsets outside the rows
+    are clamped to them."""
+    import torch
+    from bgtq import batched
+    batched.bind_torch_stream(device)
+    rng = np.random.RandomState(1)
+    lens = [int(n) for n in rng.randint(0, 6, 9000)]
+    x = _inputs(sum(lens), 1, 1, 64, "float16", 1)
+    xd, out = x.cuda(), torch.empty((sum(lens), 1, 64), dtype=x.dtype, device="cuda")
+    batched.prompt_attention(device, xd[:, :1], xd[:, 1:2], xd[:, 2:], _offsets(lens), out)
+    torch.cuda.synchronize()
+    _check(out, x, lens, 1, 1, "float16", 1 / 8)
+    out2 = torch.full((300, 1, 64), 5.0, dtype=x.dtype, device="cuda")
+    y = xd[:300]
+    off = torch.tensor([-7, 100, 2 ** 30], dtype=torch.int32, device="cuda")  # sequences 0..99 and 100..299
+    batched.prompt_attention(device, y[:, :1], y[:, 1:2], y[:, 2:], off, out2)
+    torch.cuda.synchronize()
+    _check(out2, x[:300], [100, 200], 1, 1, "float16", 1 / 8)
+
+
+def test_captured_and_replayed(device):
+    """A graph of the call serves other offsets and inputs."""
+    import torch
+    from bgtq import batched
+    batched.bind_torch_stream(device)
+    hq, hkv, dim, total = 6, 2, 64, 400
+    xd = torch.zeros((total, hq + 2 * hkv, dim), dtype=torch.bfloat16, device="cuda")
+    out, off = torch.empty((total, hq, dim), dtype=torch.bfloat16, device="cuda"), _offsets([total, 0, 0])
+    args = (xd[:, :hq], xd[:, hq:hq + hkv], xd[:, hq + hkv:], off, out)
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        device.set_stream(side.cuda_stream)
+        batched.prompt_attention(device, *args)
+    batched.bind_torch_stream(device)
+    for i, lens in enumerate(([400, 0, 0], [100, 200, 100], [1, 0, 399], [133, 133, 134])):
+        x = _inputs(total, hq, hkv, dim, "bfloat16", i)
+        xd.copy_(x)
+        off.copy_(_offsets(lens))
+        graph.replay()
+        torch.cuda.synchronize()
+        _check(out, x, lens, hq, hkv, "bfloat16", 1 / 8, what=f"replay {i}")
+        replayed = out.clone()
+        batched.prompt_attention(device, *args)
+        torch.cuda.synchronize()
+        assert torch.equal(replayed, out)
+
+
+def test_wrapper_refusals(device):
+    import torch
+    import bgtq
+    from bgtq import batched
+    x = torch.zeros((8, 4, 64), dtype=torch.float16, device="cuda")
+    off = torch.tensor([0, 8], dtype=torch.int32, device="cuda")
+    ok = dict(q=x[:, :2], k=x[:, 2:3], v=x[:, 3:], offsets=off, out=x[:, :2].clone())
+    for bad in (dict(q=x[:, :2].float()), dict(k=x[:4, 2:3]), dict(v=x[:, 3:].bfloat16()), dict(offsets=off.long()), dict(scale=-1.0),
+                dict(scale=float("nan")), dict(q=x[:, :2, :32]), dict(out=x[:, :1].clone()), dict(k=x[:, :0], v=x[:, :0]),
+                dict(q=torch.zeros((8, 2, 65), dtype=torch.float16, device="cuda")[:, :, :64])):
+        with pytest.raises((bgtq.RangeError, bgtq.UnsupportedError)):
+            batched.prompt_attention(device, **{**ok, **bad})
+    batched.prompt_attention(device, x[:0, :2], x[:0, 2:3], x[:0, 3:], off[:1], x[:0, :2].clone())  # nothing to do
