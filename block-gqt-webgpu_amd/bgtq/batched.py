@@ -142,24 +142,40 @@ def prefill(device, desc) -> None:
 
 
 # ---- paged cache and packed prompts
+#
+# These wrappers check what the library cannot see (device, dtype, shape) and
+# cost a call of a few microseconds: one read of each tensor property, one
+# structure built at once.
 
-def _strides2(t):
-    """The strides of t's first two dimensions, 0 for those of one entry."""
-    return [t.stride(i) if t.shape[i] > 1 else 0 for i in (0, 1)]
-
-
-def _on(device, name, t, dtypes, dims):
-    """t checked: a tensor on the device's GPU of one of the dtypes and `dims` dimensions, its last one dense."""
-    if not t.is_cuda or (device is not None and t.device.index != device.index):
-        raise RangeError(f"{name} must lie on the context's device")
-    if str(t.dtype)[6:] not in dtypes:
-        raise RangeError(f"{name} must be of {' or '.join(dtypes)}")
-    if t.dim() != dims or (t.shape[-1] > 1 and t.stride(-1) != 1):
-        raise RangeError(f"{name} must have {dims} dimensions, the last one dense")
-    return t
+_CODES: dict = {}  # torch dtype -> BGTQ_DTYPE_* of rows outside a pool
 
 
-_ROWS = {"float32": _lib.DTYPE_F32, "float16": _lib.DTYPE_F16, "bfloat16": _lib.DTYPE_BF16}
+def _codes():
+    if not _CODES:
+        import torch
+        _CODES.update({torch.float32: _lib.DTYPE_F32, torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16})
+    return _CODES
+
+
+def _need(ok, message):
+    if not ok:
+        raise RangeError(message)
+
+
+def _dense(index, name, t, dtype, dims):
+    """t's strides, checked: a tensor on GPU `index` of the dtype (its name) with `dims` dimensions, the last one dense."""
+    if t.get_device() != index or str(t.dtype) != "torch." + dtype or t.dim() != dims:
+        raise RangeError(f"{name} must be a {dtype} tensor of {dims} dimensions on the context's device")
+    st = t.stride()
+    if st[-1] != 1 and t.shape[-1] > 1:
+        raise RangeError(f"{name}'s last dimension must be dense")
+    return st
+
+
+def _strides2(t, st):
+    """The strides of t's first two dimensions, 0 for one of a single entry."""
+    n = t.shape
+    return (st[0] if n[0] > 1 else 0, st[1] if n[1] > 1 else 0)
 
 
 class Pages:
@@ -168,6 +184,7 @@ class Pages:
     def __init__(self, struct, device_index, held):
         self.struct, self.device_index, self.held = struct, device_index, held
         self.kv_heads, self.dim = struct.kv_heads, struct.dim
+        self.ref = ctypes.byref(struct)
 
 
 def pages(*, page_tokens, v, v_scales=None, tables=None, packed=None, norms=None, k_f16=None) -> Pages:
@@ -175,68 +192,67 @@ def pages(*, page_tokens, v, v_scales=None, tables=None, packed=None, norms=None
     float16, or int8 with v_scales [.., .., page_tokens] float16; K either k_f16 [.., .., page_tokens, dim]
     float16, or packed [.., .., bytes] uint8 and norms [.., .., scales] float16 (at least page_tokens rows of
     each head's row bytes and norm stride) with the heads' tables."""
+    _need((packed is None) == (norms is None) and (packed is None) != (k_f16 is None), "K pages are packed and norms, or k_f16")
+    index = v.get_device()
+    _need(index >= 0, "pages must lie on a GPU")
+    q8 = v_scales is not None
     g = _lib.Pages()
-    _on(None, "v", v, ("float16", "int8"), 4)
+
+    def put(name, t, dtype, dims):
+        st = _dense(index, name, t, dtype, dims)
+        _need(t.shape[:2] == v.shape[:2], f"{name} must have the pool's pages and heads")
+        if dims == 4:
+            _need(t.shape == v.shape and (t.shape[2] == 1 or st[2] == t.shape[3]), f"{name} must hold page_tokens adjacent rows per page and head")
+        two = _strides2(t, st)
+        field = name if name != "k_f16" else "k"
+        setattr(g, name, t.data_ptr())
+        setattr(g, field + "_page_stride", two[0])
+        setattr(g, field + "_head_stride", two[1])
+    put("v", v, "int8" if q8 else "float16", 4)
     n, heads, rows, dim = v.shape
-    if rows != page_tokens or (rows > 1 and v.stride(2) != dim):
-        raise RangeError("v must hold page_tokens adjacent rows per page and head")
-    if (packed is None) == (k_f16 is None):
-        raise RangeError("K pages are either packed or FP16")
-    if (v.dtype.itemsize == 1) != (v_scales is not None):
-        raise RangeError("8-bit V pages have scales, FP16 V pages have none")
+    _need(rows == page_tokens, "v must hold page_tokens rows per page and head")
     g.kv_heads, g.dim, g.page_tokens, g.pages = heads, dim, page_tokens, n
-    g.v_format = _lib.DTYPE_F16 if v_scales is None else _lib.DTYPE_Q8
-    g.v, g.v_page_stride, g.v_head_stride = v.data_ptr(), *_strides2(v)
-    held = [v, v_scales, tables, packed, norms, k_f16]
-    arrays = [("v", v, v.shape)]
-    if v_scales is not None:
-        _on(None, "v_scales", v_scales, ("float16",), 3)
-        g.v_scales, g.v_scales_page_stride, g.v_scales_head_stride = v_scales.data_ptr(), *_strides2(v_scales)
-        arrays.append(("v_scales", v_scales, (n, heads, rows)))
+    g.v_format = _lib.DTYPE_Q8 if q8 else _lib.DTYPE_F16
+    if q8:
+        put("v_scales", v_scales, "float16", 3)
+        _need(v_scales.shape[2] == rows, "v_scales must hold a scale per row")
     if k_f16 is not None:
-        _on(None, "k_f16", k_f16, ("float16",), 4)
-        if k_f16.stride(2) != dim and rows > 1:
-            raise RangeError("k_f16 must hold page_tokens adjacent rows per page and head")
         g.key_format = _lib.KEYS_FP16
-        g.k_f16, g.k_page_stride, g.k_head_stride = k_f16.data_ptr(), *_strides2(k_f16)
-        arrays.append(("k_f16", k_f16, v.shape))
+        put("k_f16", k_f16, "float16", 4)
     else:
-        _on(None, "packed", packed, ("uint8",), 3)
-        _on(None, "norms", norms, ("float16",), 3)
-        if not tables or len(tables) != heads:
-            raise RangeError("packed K pages need the tables of every KV head")
+        _need(tables and len(tables) == heads, "packed K pages need the tables of every KV head")
+        g.key_format = _lib.KEYS_PACKED
+        put("packed", packed, "uint8", 3)
+        put("norms", norms, "float16", 3)
         for i, t in enumerate(tables):
             g.tables[i] = t.handle.value if hasattr(t.handle, "value") else t.handle
-        if (packed.shape[2] < rows * max(t.info["row_bytes"] for t in tables)
-                or norms.shape[2] < rows * max(t.info["norm_stride"] for t in tables)):
-            raise RangeError("packed and norms must hold page_tokens rows of every head")
-        g.key_format = _lib.KEYS_PACKED
-        g.packed, g.packed_page_stride, g.packed_head_stride = packed.data_ptr(), *_strides2(packed)
-        g.norms, g.norms_page_stride, g.norms_head_stride = norms.data_ptr(), *_strides2(norms)
-        arrays += [("packed", packed, (n, heads, packed.shape[2])), ("norms", norms, (n, heads, norms.shape[2]))]
-    for name, t, shape in arrays:
-        if tuple(t.shape) != tuple(shape) or t.device != v.device:
-            raise RangeError(f"{name} must have the pool's pages, heads and device")
-    return Pages(g, v.device.index, held)
+        _need(packed.shape[2] >= rows * max(t.info["row_bytes"] for t in tables)
+              and norms.shape[2] >= rows * max(t.info["norm_stride"] for t in tables),
+              "packed and norms must hold page_tokens rows of every head")
+    return Pages(g, index, (v, v_scales, tables, packed, norms, k_f16))
+
+
+def _row_fields(index, name, t, shape):
+    """(address, dtype, row stride, head stride) of K or V rows; zeros for none."""
+    if t is None:
+        return (None, 0, 0, 0)
+    code = _codes().get(t.dtype)
+    if code is None or t.get_device() != index or t.shape != shape:
+        raise RangeError(f"{name} must be a [rows, KV heads, dim] tensor of float32, float16 or bfloat16 on the context's device")
+    s = t.stride()
+    if s[2] != 1:
+        raise RangeError(f"{name}'s last dimension must be dense")
+    return (t.data_ptr(), code, s[0] if shape[0] > 1 else 0, s[1] if shape[1] > 1 else 0)
 
 
 def _paged_rows(device, pool, slots, k, v):
-    if pool.device_index != device.index:
+    index = device.index
+    if pool.device_index != index:
         raise RangeError("the pool must lie on the context's device")
-    _on(device, "slots", slots, ("int64",), 1)
-    r = _lib.PagedRows()
-    r.rows, r.slots = slots.shape[0], slots.data_ptr()
-    for name, t in (("k", k), ("v", v)):
-        if t is None:
-            continue
-        _on(device, name, t, tuple(_ROWS), 3)
-        if tuple(t.shape) != (slots.shape[0], pool.kv_heads, pool.dim):
-            raise RangeError(f"{name} must be [rows, KV heads, dim]")
-        setattr(r, name, t.data_ptr() or None)
-        setattr(r, name + "_dtype", _ROWS[str(t.dtype)[6:]])
-        setattr(r, name + "_row_stride", t.stride(0) if t.shape[0] > 1 else 0)
-        setattr(r, name + "_head_stride", t.stride(1) if t.shape[1] > 1 else 0)
-    return r
+    _dense(index, "slots", slots, "int64", 1)
+    n = slots.shape[0]
+    shape = (n, pool.kv_heads, pool.dim)
+    return _lib.PagedRows(n, slots.data_ptr(), *_row_fields(index, "k", k, shape), *_row_fields(index, "v", v, shape))
 
 
 def paged_write(device, pool, slots, k, v) -> None:
@@ -244,88 +260,79 @@ def paged_write(device, pool, slots, k, v) -> None:
     the slots [n] int64; slots outside the pool are skipped."""
     r = _paged_rows(device, pool, slots, k, v)
     if r.rows:
-        check(lib().bgtq_paged_write(device.handle, ctypes.byref(pool.struct), ctypes.byref(r)))
+        check(lib().bgtq_paged_write(device.handle, pool.ref, ctypes.byref(r)))
 
 
 def paged_read(device, pool, slots, k=None, v=None) -> None:
     """bgtq_paged_read: the slots' rows into k and / or v [n, Hkv, dim] (FP32, FP16 or BF16); rows of slots outside
     the pool stay as they are."""
-    if k is None and v is None:
-        raise RangeError("paged_read needs k or v")
+    _need(k is not None or v is not None, "paged_read needs k or v")
     r = _paged_rows(device, pool, slots, k, v)
     if r.rows:
-        check(lib().bgtq_paged_read(device.handle, ctypes.byref(pool.struct), ctypes.byref(r)))
+        check(lib().bgtq_paged_read(device.handle, pool.ref, ctypes.byref(r)))
 
 
 class PagedDecode:
     """A paged decode's descriptor with its pool; holds the tensors."""
 
     def __init__(self, pool, struct, held):
-        self.pool, self.struct, self.held = pool, struct, held
+        self.pool, self.struct, self.held, self.ref = pool, struct, held, ctypes.byref(struct)
 
 
 def paged_decode_desc(*, pages, q, out, lengths, page_table, max_length=None, splits=0, workspace=None,
                       q_rotated=False) -> PagedDecode:
     """bgtq_paged_decode_desc over device tensors: q, out [B, Hq, dim] FP32 contiguous, lengths [B] and
     page_table [B, pages per sequence] int32; max_length defaults to what the page table's rows hold."""
-    d = _lib.PagedDecodeDesc()
-    for name, t, types, dims in (("q", q, ("float32",), 3), ("out", out, ("float32",), 3),
-                                 ("lengths", lengths, ("int32", "uint32"), 1), ("page_table", page_table, ("int32",), 2)):
-        _on(None, name, t, types, dims)
-        if t.device.index != pages.device_index:
-            raise RangeError(f"{name} must lie on the pool's device")
-    batch, heads, dim = q.shape
-    if not q.is_contiguous() or not out.is_contiguous() or out.shape != q.shape or dim != pages.dim:
-        raise RangeError("q and out must be contiguous [B, Hq, dim]")
-    if lengths.shape[0] != batch or page_table.shape[0] != batch:
-        raise RangeError("lengths and page_table must have a row per sequence")
-    d.batch, d.q_heads, d.q, d.out = batch, heads, q.data_ptr(), out.data_ptr()
-    d.lengths, d.page_table = lengths.data_ptr(), page_table.data_ptr()
-    # (a row past the tensor's columns is none of the table's)
-    d.page_table_stride = page_table.stride(0) if batch > 1 else page_table.shape[1]
+    index = pages.device_index
+    for name, t in (("q", q), ("out", out)):
+        _dense(index, name, t, "float32", 3)
+        _need(t.is_contiguous() and t.shape == q.shape and t.shape[2] == pages.dim, "q and out must be contiguous [B, Hq, dim]")
+    batch, heads = q.shape[:2]
+    _dense(index, "lengths", lengths, "uint32" if str(lengths.dtype) == "torch.uint32" else "int32", 1)
+    st = _dense(index, "page_table", page_table, "int32", 2)
+    _need(lengths.shape[0] == batch and page_table.shape[0] == batch, "lengths and page_table must have a row per sequence")
     held_tokens = page_table.shape[1] * pages.struct.page_tokens
-    if max_length is not None and max_length > held_tokens:
-        raise RangeError("page_table rows hold fewer tokens than max_length")
-    d.max_length, d.splits, d.q_rotated = int(held_tokens if max_length is None else max_length), int(splits), int(bool(q_rotated))
-    if workspace is not None:
-        if not workspace.is_cuda or workspace.device.index != pages.device_index or not workspace.is_contiguous():
-            raise RangeError("workspace must be contiguous on the pool's device")
-        d.workspace, d.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-    return PagedDecode(pages, d, [q, out, lengths, page_table, workspace])
+    tokens = held_tokens if max_length is None else int(max_length)
+    _need(tokens <= held_tokens, "page_table rows hold fewer tokens than max_length")
+    _need(workspace is None or (workspace.get_device() == index and workspace.is_contiguous()), "workspace must be contiguous on the pool's device")
+    d = _lib.PagedDecodeDesc(batch, heads, q.data_ptr(), out.data_ptr(), lengths.data_ptr(), page_table.data_ptr(),
+                             st[0] if batch > 1 else page_table.shape[1], tokens, int(splits),
+                             None if workspace is None else workspace.data_ptr(),
+                             0 if workspace is None else workspace.numel() * workspace.element_size(), int(bool(q_rotated)))
+    return PagedDecode(pages, d, (q, out, lengths, page_table, workspace))
 
 
 def paged_decode_workspace_bytes(desc) -> int:
     n = ctypes.c_size_t(0)
-    check(lib().bgtq_paged_decode_workspace_size(ctypes.byref(desc.pool.struct), ctypes.byref(desc.struct), ctypes.byref(n)))
+    check(lib().bgtq_paged_decode_workspace_size(desc.pool.ref, desc.ref, ctypes.byref(n)))
     return n.value
 
 
 def paged_decode(device, desc) -> None:
     """bgtq_paged_decode: decode attention over the descriptor's pages."""
-    if desc.pool.device_index != device.index:
-        raise RangeError("the pool must lie on the context's device")
-    check(lib().bgtq_paged_decode(device.handle, ctypes.byref(desc.pool.struct), ctypes.byref(desc.struct)))
+    _need(desc.pool.device_index == device.index, "the pool must lie on the context's device")
+    check(lib().bgtq_paged_decode(device.handle, desc.pool.ref, desc.ref))
 
 
 def prompt_attention(device, q, k, v, offsets, out, scale=None) -> None:
     """bgtq_prompt_attention: causal attention within each of the sequences packed in q, out [tokens, Hq, dim] and
     k, v [tokens, Hkv, dim] (FP16 or BF16, any strides of the first two dimensions that are multiples of 8);
     offsets [sequences + 1] int32; scale defaults to 1 / sqrt(dim)."""
-    d = _lib.PromptDesc()
-    for name, t in (("q", q), ("k", k), ("v", v), ("out", out)):
-        _on(device, name, t, ("float16", "bfloat16"), 3)
-        if t.dtype != q.dtype or t.shape[0] != q.shape[0] or t.shape[2] != q.shape[2]:
-            raise RangeError("q, k, v and out must agree in dtype, tokens and dim")
-        setattr(d, name, t.data_ptr() or None)
-        setattr(d, name + "_row_stride", t.stride(0) if t.shape[0] > 1 else 0)
-        setattr(d, name + "_head_stride", t.stride(1) if t.shape[1] > 1 else 0)
-    _on(device, "offsets", offsets, ("int32",), 1)
-    if k.shape[1] != v.shape[1] or out.shape[1] != q.shape[1] or offsets.shape[0] < 1:
-        raise RangeError("k and v, and q and out, must agree in heads; offsets has an entry more than sequences")
-    d.q_heads, d.kv_heads, d.dim, d.dtype = q.shape[1], k.shape[1], q.shape[2], _ROWS[str(q.dtype)[6:]]
-    d.sequences, d.tokens, d.offsets = offsets.shape[0] - 1, q.shape[0], offsets.data_ptr()
-    if scale is not None:
-        if not scale > 0:
-            raise RangeError("scale must be positive")
-        d.scale = scale
+    index, dtype = device.index, q.dtype
+    code = _codes().get(dtype, _lib.DTYPE_F32)
+    _dense(index, "offsets", offsets, "int32", 1)
+    _need(code != _lib.DTYPE_F32 and q.dim() == 3 and k.dim() == 3 and offsets.shape[0] > 0,
+          "q, k, v and out must be 3-dimensional float16 or bfloat16 tensors; offsets has an entry more than sequences")
+    tokens, heads, dim = shape = q.shape
+    kv_shape = (tokens, k.shape[1], dim)
+    fields = []
+    for t, want in ((q, shape), (k, kv_shape), (v, kv_shape), (out, shape)):
+        if t.dtype != dtype or t.get_device() != index or t.shape != want:
+            raise RangeError("q and out, k and v must agree in shape, all in tokens, dim, dtype and device")
+        s = t.stride()
+        if s[2] != 1 and dim > 1:
+            raise RangeError("the last dimension of q, k, v and out must be dense")
+        fields += (t.data_ptr() or None, s[0] if tokens > 1 else 0, s[1] if want[1] > 1 else 0)
+    _need(scale is None or scale > 0, "scale must be positive")
+    d = _lib.PromptDesc(heads, kv_shape[1], dim, code, offsets.shape[0] - 1, tokens, offsets.data_ptr(), *fields, scale or 0.0)
     check(lib().bgtq_prompt_attention(device.handle, ctypes.byref(d)))

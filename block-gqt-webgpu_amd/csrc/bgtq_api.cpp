@@ -432,7 +432,8 @@ bgtq_status bgtq_tables_create(bgtq_context *ctx, const uint32_t *integer, size_
   const size_t off_rot_q = align(off_mfma + (size_t)kMfmaTableBytes * nb);
   const size_t off_gdesc = align(off_rot_q + (d % 32 == 0 ? (size_t)rot_q_bytes((int)d) : 0));
   const size_t off_glane = align(off_gdesc + sizeof(uint32_t) * d);
-  const size_t total = off_glane + (d % 32 == 0 ? sizeof(uint32_t) * kLaneRecordWords * 4 * (d / 32) : 0);
+  const size_t off_rot_k = align(off_glane + (d % 32 == 0 ? sizeof(uint32_t) * kLaneRecordWords * 4 * (d / 32) : 0));
+  const size_t total = off_rot_k + (d % 32 == 0 ? (size_t)rot_q_bytes((int)d) : 0);
   auto *t = new bgtq_tables();
   t->ctx = ctx;
   t->host.assign(total, 0);
@@ -458,6 +459,7 @@ bgtq_status bgtq_tables_create(bgtq_context *ctx, const uint32_t *integer, size_
   T->off_rot_q = (uint32_t)off_rot_q;
   T->off_gdesc = (uint32_t)off_gdesc;
   T->off_glane = (uint32_t)off_glane;
+  T->off_rot_k = (uint32_t)off_rot_k;
   T->total_bytes = (uint32_t)total;
   float cmax = 0.0f;
   for (int64_t i = 0; i < d * mc; ++i) cmax = std::max(cmax, std::fabs(cent[i]));
@@ -570,17 +572,21 @@ bgtq_status bgtq_tables_create(bgtq_context *ctx, const uint32_t *integer, size_
     std::vector<float> rq((size_t)(d * d));
     for (int64_t j = 0; j < d; ++j)
       for (int64_t i = 0; i < d; ++i) rq[j * d + perm[i]] = rot[j * d + i];
-    uint16_t *op = reinterpret_cast<uint16_t *>(h + off_rot_q);
-    for (int64_t n = 0; n < d / 16; ++n)
-      for (int64_t s = 0; s < d / 32; ++s)
-        for (int l = 0; l < 64; ++l) {
-          uint16_t *dst = op + ((n * (d / 32) + s) * 64 + l) * 16;
-          for (int jv = 0; jv < 8; ++jv) {
-            const float x = rq[(16 * n + l % 16) * d + 32 * s + 8 * (l / 16) + jv];
-            dst[jv] = f32_to_f16(x);
-            dst[8 + jv] = f32_to_f16(x - f16_to_f32(dst[jv]));
+    auto operands = [&](size_t at, auto entry) {
+      uint16_t *op = reinterpret_cast<uint16_t *>(h + at);
+      for (int64_t n = 0; n < d / 16; ++n)
+        for (int64_t s = 0; s < d / 32; ++s)
+          for (int l = 0; l < 64; ++l) {
+            uint16_t *dst = op + ((n * (d / 32) + s) * 64 + l) * 16;
+            for (int jv = 0; jv < 8; ++jv) {
+              const float x = entry(16 * n + l % 16, 32 * s + 8 * (l / 16) + jv);
+              dst[jv] = f32_to_f16(x);
+              dst[8 + jv] = f32_to_f16(x - f16_to_f32(dst[jv]));
+            }
           }
-        }
+    };
+    operands(off_rot_q, [&](int64_t row, int64_t col) { return rq[row * d + col]; });
+    operands(off_rot_k, [&](int64_t row, int64_t col) { return rq[col * d + row] * 16384.0f; });
   }
   t->tile_encode = encode_tile_layout(T);
   t->info = bgtq_tables_info{(int32_t)d, (int32_t)ng, (int32_t)rb, (int32_t)nstride, (int32_t)nib, (int32_t)mc, ncb, nb,
@@ -1708,8 +1714,10 @@ PagedWriteParams rows_params(const bgtq_pages *g, const bgtq_paged_rows *r) {
   if (g->key_format == BGTQ_KEYS_PACKED) {
     for (int h = 0; h < g->kv_heads; ++h) {
       p.tables[h] = g->tables[h]->dev();
-      p.enc_bytes[h] = (int32_t)g->tables[h]->h()->off_rot;
-      p.off_rot_t[h] = (int32_t)g->tables[h]->h()->off_rot_t;
+      const DevTables *T = g->tables[h]->h();
+      p.heads[h] = {(int32_t)T->off_rot, T->off_rot_t, T->off_rot_k, T->off_gdesc, T->off_books, (int16_t)T->row_bytes,
+                    (int16_t)T->norm_stride, (int16_t)T->max_centroids, (int16_t)T->n_books, (int16_t)T->groups,
+                    (int16_t)T->cent_exp};
     }
     p.packed = g->packed;
     p.packed_page_stride = g->packed_page_stride;
@@ -1765,7 +1773,7 @@ bgtq_status bgtq_paged_write(bgtq_context *ctx, const bgtq_pages *g, const bgtq_
       z.codebooks = std::max(z.codebooks, t.n_codebooks);
       z.groups = std::max(z.groups, t.groups);
       z.row_bytes = std::max(z.row_bytes, t.row_bytes);
-      enc = std::max(enc, p.enc_bytes[h]);
+      enc = std::max(enc, p.heads[h].enc_bytes);
     }
     tile = tile && encode_tile_lds_bytes(g->dim, z.codebooks, z.groups, z.row_bytes) <= 160 * 1024;
     const int lds = paged_write_lds_bytes(g->dim, enc);

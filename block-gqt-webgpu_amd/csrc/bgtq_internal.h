@@ -20,7 +20,7 @@ constexpr int kEncodeJobTable = 4096;     // jobs in a context's device job tabl
 struct DevTables {
   int32_t dim, groups, row_bytes, norm_stride, nibble_dims, max_centroids, n_books, n_codebooks;
   int32_t gstart[kMaxGroups], gend[kMaxGroups], gsize[kMaxGroups];  // group ranges (head-perm order)
-  uint32_t off_lut, off_books, off_rot, off_rot_t, off_mfma, off_rot_q, off_gdesc, off_glane, total_bytes;
+  uint32_t off_lut, off_books, off_rot, off_rot_t, off_mfma, off_rot_q, off_gdesc, off_glane, off_rot_k, total_bytes;
   int32_t cent_exp;  // 2^cent_exp * max|centroid| <= 2^14: fp16 hi/lo split range for MFMA operands
   // The fused decode of any packed layout: its leading pair K-steps (see
   // off_glane) and the books whose pair tables it keeps in LDS for them
@@ -47,6 +47,9 @@ struct DevTables {
   //             (hi, lo) MFMA A operands: for 16-row tile n, 32-column step
   //             s and lane l, 8 hi then 8 lo halves of
   //             Rq[16 n + l % 16][32 s + 8 (l / 16) + 0..7] (kRotQBytes).
+  // [off_rot_k] the transpose of Rq times 2^14 in the same operand form
+  //             (16-row tile n of dimensions, 32-position step s), for the
+  //             rows read back from pages: k = Rq^T (c s).
   // [off_gdesc] per head-perm position j, for the fused decode of any packed
   //             layout: uint32 byte offset in the packed row | nibble shift << 8
   //             | nibble flag << 11 | book << 12 | group << 16.
@@ -179,9 +182,14 @@ struct PagedSlots {
 struct PagedWriteParams {
   PagedSlots slots;
   int32_t kv_heads, dim;
-  const DevTables *tables[kMaxKvHeads];  // packed K, else null
-  int32_t enc_bytes[kMaxKvHeads];        // bytes of each table set's header, code LUT and books
-  int32_t off_rot_t[kMaxKvHeads];
+  // Packed K, else null; with the fields that a kernel's first loads need, so
+  // that these wait for the kernel's arguments only.
+  const DevTables *tables[kMaxKvHeads];
+  struct Head {
+    int32_t enc_bytes;  // bytes of the table set's header, code LUT and books
+    uint32_t off_rot_t, off_rot_k, off_gdesc, off_books;
+    int16_t row_bytes, norm_stride, max_centroids, books, groups, cent_exp;
+  } heads[kMaxKvHeads];
   uint8_t *packed;
   int64_t packed_page_stride, packed_head_stride;  // bytes
   uint16_t *norms;
