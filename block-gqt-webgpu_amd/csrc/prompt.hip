@@ -17,6 +17,8 @@
 // The running maximum is raised only when a block's exceeds it by more than 8
 // in the log2 domain: probabilities then reach 2^8 at most, in range of either
 // type, and most blocks skip the rescale of O.
+#include <type_traits>
+
 #include "bgtq_internal.h"
 #include "gfx950_common.h"
 
@@ -30,7 +32,6 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 half2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef float f32x32 __attribute__((ext_vector_type(32)));
 
 constexpr int kWaves = 4, kThreads = 64 * kWaves;
 constexpr int kRows = 32 * kWaves;  // query rows of a workgroup
@@ -78,11 +79,62 @@ __device__ __forceinline__ float add2(uint32_t pair, float c) {
     return __builtin_amdgcn_fdot2(__builtin_bit_cast(half2, pair), half2{(_Float16)1.0f, (_Float16)1.0f}, c, false);
 }
 
+// Infinities and NaNs among pairs of 16-bit values: the pair's magnitudes
+// (their order is the integers'), and the values of one kind (0 NaN, 1
+// infinity, 2 minus infinity) as 1, the others as 0; `finite`: the others kept.
 template <bool BF>
-__device__ __forceinline__ float value_of(uint32_t bits) {  // the low 16 bits
-  if constexpr (BF) return __uint_as_float(bits << 16);
-  else return (float)__builtin_bit_cast(_Float16, (uint16_t)bits);
+struct Odd {
+  static constexpr uint32_t kInf = BF ? 0x7f80u : 0x7c00u, kOne = BF ? 0x3f80u : 0x3c00u;
+  static __device__ __forceinline__ uint32_t finite(uint32_t w) {
+    return ((w & 0x7fffu) >= kInf ? 0u : w & 0xffffu) | ((w >> 16 & 0x7fffu) >= kInf ? 0u : w & 0xffff0000u);
+  }
+  static __device__ __forceinline__ uint32_t of_kind(uint32_t w, int kind) {
+    auto is = [&](uint32_t x) {
+      return kind == 0 ? (x & 0x7fffu) > kInf : x == (kind == 1 ? kInf : kInf | 0x8000u);
+    };
+    return (is(w & 0xffffu) ? kOne : 0u) | (is(w >> 16) ? kOne << 16 : 0u);
+  }
+};
+
+// 2 N transposed reads (ds_read_tr16_pair's) of the N rows pairs at lds[t] +
+// OFF and lds2[t] + OFF, issued together: the results are valid once waited for.
+template <int N, int OFF>
+__device__ __forceinline__ void read_v(const uint32_t (&lds)[N], const uint32_t (&lds2)[N], u32x2 (&v)[N][2]) {
+  if constexpr (N == 2) {
+    asm volatile(
+        "s_nop 7\n\tds_read_b64_tr_b16 %0, %4 offset:%8\n\tds_read_b64_tr_b16 %1, %5 offset:%8\n\t"
+        "ds_read_b64_tr_b16 %2, %6 offset:%8\n\tds_read_b64_tr_b16 %3, %7 offset:%8"
+        : "=&v"(v[0][0]), "=&v"(v[0][1]), "=&v"(v[1][0]), "=&v"(v[1][1])
+        : "v"(lds[0]), "v"(lds2[0]), "v"(lds[1]), "v"(lds2[1]), "n"(OFF));
+  } else {
+    static_assert(N == 4, "head dim 64 or 128");
+    asm volatile(
+        "s_nop 7\n\tds_read_b64_tr_b16 %0, %8 offset:%16\n\tds_read_b64_tr_b16 %1, %9 offset:%16\n\t"
+        "ds_read_b64_tr_b16 %2, %10 offset:%16\n\tds_read_b64_tr_b16 %3, %11 offset:%16\n\t"
+        "ds_read_b64_tr_b16 %4, %12 offset:%16\n\tds_read_b64_tr_b16 %5, %13 offset:%16\n\t"
+        "ds_read_b64_tr_b16 %6, %14 offset:%16\n\tds_read_b64_tr_b16 %7, %15 offset:%16"
+        : "=&v"(v[0][0]), "=&v"(v[0][1]), "=&v"(v[1][0]), "=&v"(v[1][1]), "=&v"(v[2][0]), "=&v"(v[2][1]),
+          "=&v"(v[3][0]), "=&v"(v[3][1])
+        : "v"(lds[0]), "v"(lds2[0]), "v"(lds[1]), "v"(lds2[1]), "v"(lds[2]), "v"(lds2[2]), "v"(lds[3]), "v"(lds2[3]),
+          "n"(OFF));
+  }
 }
+
+// Waits for the read pair of tile t of N when NEXT reads were issued after the
+// N pairs (t is a compile-time index after unrolling).
+template <int N, int NEXT>
+__device__ __forceinline__ void wait_newer(int t, u32x2 &a, u32x2 &b) {
+  static_assert(2 * (N - 1) + NEXT < 16, "lgkmcnt");
+  if (t == 0) wait_lds_tied<2 * (N - 1) + NEXT>(a, b);
+  else if (t == 1) wait_lds_tied<2 * (N - 2) + NEXT>(a, b);
+  else if (t == 2) wait_lds_tied<2 * (N > 2 ? N - 3 : 0) + NEXT>(a, b);
+  else wait_lds_tied<NEXT>(a, b);
+}
+
+// Ties an accumulator to its registers. After each element's update under a
+// branch: without it the update builds a second copy of the accumulator, and
+// every block of keys moves it there and back (64 moves at d=64).
+__device__ __forceinline__ void in_place(f32x16 &o) { asm volatile("" : "+v"(o)); }
 
 // The other half's value of a query's pair of lanes.
 __device__ __forceinline__ float half_max(float v) {
@@ -127,7 +179,7 @@ __device__ __forceinline__ Place find_place(const PromptParams &p, int64_t slot)
 }
 
 template <int D, bool BF>
-__global__ __launch_bounds__(kThreads, 2) void prompt_kernel(PromptParams p) {
+__global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void prompt_kernel(PromptParams p) {
   constexpr int PR = D / 8;                      // 16-byte pieces per row
   constexpr int QS = D / 16;                     // 16-dimension steps of QK
   constexpr int MT = D / 32;                     // 32-dimension tiles of O
@@ -159,7 +211,6 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_kernel(PromptParams p) {
       dma16(rv, buf + BLOCK + (wave * DMAS + i) * 1024, (uint32_t)(r * (int)p.v_row * 2 + c * 16), 0);
     }
   };
-  issue(0);
   // Q: lane (h, q) holds dimensions 16 s + 8 h + 0..7 of query q (past the
   // sequence: its last row's, not stored).
   u32x4 qf[QS];
@@ -167,7 +218,11 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_kernel(PromptParams p) {
     const uint16_t *row = p.q + (at.begin + min(qi, at.len - 1)) * p.q_row + head * p.q_head;
 #pragma unroll
     for (int s = 0; s < QS; ++s) qf[s] = *reinterpret_cast<const u32x4 *>(row + 16 * s + 8 * h);
+    // Waited for here: left to the loop, the wait would take the next block's DMAs with it.
+#pragma unroll
+    for (int s = 0; s < QS; ++s) asm volatile("" : "+v"(qf[s]));
   }
+  issue(0);
   f32x16 O[MT];
 #pragma unroll
   for (int t = 0; t < MT; ++t)
@@ -175,31 +230,44 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_kernel(PromptParams p) {
     for (int i = 0; i < 16; ++i) O[t][i] = 0.0f;
   float m = -INFINITY, l = 0.0f;  // log2 domain; this lane's part of the sum
 
-  for (int j = 0; j < n_blocks; ++j) {
+  // LDS addresses of this lane in a block: K, piece h of row qc (step s: ^ 32 s,
+  // rows 32 on: + 64 D); V, its part of rows 4 h + (lane % 16) / 4 (tile t: ^ 64 t)
+  // and 8 rows on. The swizzle of a row depends on its lane's part alone.
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void *)smem;
+  const uint32_t k_at = (uint32_t)(qc * (2 * D) + ((h ^ swizzle<D>(qc)) * 16));
+  const int vr = 4 * h + ((lane & 15) >> 2);
+  const int v_piece = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+  const uint32_t v_at = (uint32_t)(vr * (2 * D) + ((v_piece ^ swizzle<D>(vr)) * 16) + (lane & 1) * 8);
+  const uint32_t v_at8 = (uint32_t)((vr + 8) * (2 * D) + ((v_piece ^ swizzle<D>(vr + 8)) * 16) + (lane & 1) * 8);
+
+  // Every wave meets every block's barrier and loads its part of every block.
+  auto arrive = [&](int j) {
     wait_vm<0>();   // this wave's part of block j has landed (and every earlier load)
     lds_barrier();  // everyone's has, and everyone is done with the other buffer
     if (j + 1 < n_blocks) issue(j + 1);
-    if (j * kKeys > row0 + 31) continue;  // every key of the block is past this wave's queries
-    const uint8_t *kb = smem + (j & 1) * 2 * BLOCK, *vb = kb + BLOCK;
+  };
+  // Block j's keys for this wave's queries; DIAGONAL: some queries see only a part of them.
+  auto attend = [&](auto diagonal_tag, int j) {
+    constexpr bool DIAGONAL = decltype(diagonal_tag)::value;
+    const uint32_t buf = (uint32_t)(j & 1) * 2 * BLOCK;
     f32x16 S[2];
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < 2; ++b)
 #pragma unroll
       for (int i = 0; i < 16; ++i) S[b][i] = 0.0f;
 #pragma unroll
-      for (int s = 0; s < QS; ++s) {
-        const int r = 32 * b + qc;  // A operand: key r
-        const u32x4 a = *reinterpret_cast<const u32x4 *>(kb + r * (2 * D) + (((2 * s + h) ^ swizzle<D>(r)) * 16));
+    for (int s = 0; s < QS; ++s)
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {  // A operand: key 32 b + qc
+        const u32x4 a = *reinterpret_cast<const u32x4 *>(smem + ((buf + k_at) ^ (32u * s)) + 64 * D * b);
         S[b] = product<BF>(a, qf[s], S[b]);
       }
-    }
-    const bool diagonal = j * kKeys + kKeys - 1 > row0;
-    if (diagonal) {
+    if constexpr (DIAGONAL) {
+      const int d = qi - j * kKeys - 4 * h;
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          S[b][i] = j * kKeys + 32 * b + 8 * (i >> 2) + 4 * h + (i & 3) <= qi ? S[b][i] : -INFINITY;
+        for (int i = 0; i < 16; ++i) S[b][i] = 32 * b + 8 * (i >> 2) + (i & 3) <= d ? S[b][i] : -INFINITY;
     }
     float top = S[0][0];
 #pragma unroll
@@ -214,7 +282,10 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_kernel(PromptParams p) {
 #pragma unroll
       for (int t = 0; t < MT; ++t)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) O[t][i] *= a;
+        for (int i = 0; i < 16; ++i) {
+          O[t][i] *= a;
+          in_place(O[t]);
+        }
     }
     const float mu = m == -INFINITY ? 0.0f : m;
 #pragma unroll
@@ -229,69 +300,116 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_kernel(PromptParams p) {
       P[e] = pack2<BF>(S[e >> 3][2 * (e & 7)], S[e >> 3][2 * (e & 7) + 1]);
       l = add2<BF>(P[e], l);
     }
+    // O^T += V^T P^T, 16 keys a step, the next step's V on its way meanwhile.
+    uint32_t va[MT], va8[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      va[t] = (lds0 + buf + BLOCK + v_at) ^ (64u * t);
+      va8[t] = (lds0 + buf + BLOCK + v_at8) ^ (64u * t);
+    }
     // A key that a query does not see has probability 0, but 0 times an
-    // infinity or a NaN of its V row is not 0: such a block takes the products
-    // one key at a time, leaving out what is not seen.
+    // infinity or a NaN of its V row is not 0: such a block's products take
+    // the finite values, and what is seen of the others is added by itself.
     bool plain = true;
-    if (diagonal) {
-      uint32_t bad = 0;
-      constexpr uint32_t kExp = BF ? 0x7f80u : 0x7c00u;
+    if constexpr (DIAGONAL) {
+      typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+      u16x2 most{0, 0};
 #pragma unroll
       for (int i = 0; i < PR; ++i) {
-        const u32x4 w = *reinterpret_cast<const u32x4 *>(vb + (64 * i + lane) * 16);
+        const u32x4 w = *reinterpret_cast<const u32x4 *>(smem + buf + BLOCK + (64 * i + lane) * 16);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          bad |= (uint32_t)((w[e] & kExp) == kExp);
-          bad |= (uint32_t)((w[e] >> 16 & kExp) == kExp);
-        }
+        for (int e = 0; e < 4; ++e)
+          most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, w[e] & 0x7fff7fffu));
       }
-      plain = __builtin_amdgcn_ballot_w64(bad != 0) == 0;
+      plain = __builtin_amdgcn_ballot_w64(most[0] >= Odd<BF>::kInf || most[1] >= Odd<BF>::kInf) == 0;
     }
-    if (plain) {
+    if (!DIAGONAL || plain) {
+      constexpr int STEP = 16 * 2 * D;  // bytes of a step's rows
+      u32x2 v[2][MT][2];
+      read_v<MT, 0>(va, va8, v[0]);
 #pragma unroll
       for (int s = 0; s < kKeys / 16; ++s) {
+        if (s == 0) read_v<MT, STEP>(va, va8, v[1]);
+        if (s == 1) read_v<MT, 2 * STEP>(va, va8, v[0]);
+        if (s == 2) read_v<MT, 3 * STEP>(va, va8, v[1]);
         const u32x4 pf{P[4 * s], P[4 * s + 1], P[4 * s + 2], P[4 * s + 3]};
-        const int r = 16 * s + 4 * h + ((lane & 15) >> 2);
-        const int piece = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), sub = (lane & 1) * 8;
-        u32x2 va[MT][2];
-#pragma unroll
-        for (int t = 0; t < MT; ++t)
-          ds_read_tr16_pair(vb + r * (2 * D) + (((4 * t + piece) ^ swizzle<D>(r)) * 16) + sub,
-                            vb + (r + 8) * (2 * D) + (((4 * t + piece) ^ swizzle<D>(r + 8)) * 16) + sub, va[t][0], va[t][1]);
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
-          wait_dt<MT>(t, va[t][0], va[t][1]);
-          O[t] = product<BF>(u32x4{va[t][0][0], va[t][0][1], va[t][1][0], va[t][1][1]}, pf, O[t]);
+          u32x2 &a = v[s & 1][t][0], &b = v[s & 1][t][1];
+          if (s < 3) wait_newer<MT, 2 * MT>(t, a, b);  // (the next step's 2 MT reads are newer)
+          else wait_newer<MT, 0>(t, a, b);
+          O[t] = product<BF>(u32x4{a[0], a[1], b[0], b[1]}, pf, O[t]);
         }
       }
     } else {
-      f32x32 all;
+      const int d = qi - j * kKeys - 4 * h;
+      // V of dimension 32 t + qc, keys 16 s + 8 (e / 2) + 4 h + 2 (e % 2) + 0, 1 in word e.
+      auto column = [&](int s, int t) {
+        u32x4 a;
 #pragma unroll
-      for (int i = 0; i < 32; ++i) all[i] = value_of<BF>(P[i >> 1] >> (16 * (i & 1)) & 0xffffu);
+        for (int e = 0; e < 4; ++e) {
+          a[e] = 0;
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const int r = 16 * s + 8 * (e >> 1) + 4 * h + 2 * (e & 1) + x;
+            const uint8_t *at = smem + buf + BLOCK + r * (2 * D) + (((4 * t + (qc >> 3)) ^ swizzle<D>(r)) * 16) + 2 * (qc & 7);
+            a[e] |= (uint32_t)*reinterpret_cast<const uint16_t *>(at) << (16 * x);
+          }
+        }
+        return a;
+      };
+#pragma unroll
+      for (int s = 0; s < kKeys / 16; ++s)
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+          u32x4 a = column(s, t);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) a[e] = Odd<BF>::finite(a[e]);
+          O[t] = product<BF>(a, u32x4{P[4 * s], P[4 * s + 1], P[4 * s + 2], P[4 * s + 3]}, O[t]);
+        }
 #pragma clang loop unroll(disable)
-      for (int i = 0; i < 32; ++i) {
-        const float mine = all[i];
-        auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(mine), __float_as_uint(mine), false, false);
+      for (int kind = 0; kind < 3; ++kind) {
+        const float value = kind == 0 ? __builtin_nanf("") : kind == 1 ? INFINITY : -INFINITY;
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+          f32x16 n;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) n[i] = 0.0f;
 #pragma clang loop unroll(disable)
-        for (int hh = 0; hh < 2; ++hh) {
-          const int key = 32 * (i >> 4) + 8 * ((i & 15) >> 2) + 4 * hh + (i & 3);
-          const float w = __uint_as_float(hh ? both[1] : both[0]);
-          const bool seen = j * kKeys + key <= qi;
+          for (int s = 0; s < kKeys / 16; ++s) {
+            u32x4 a = column(s, t), seen;
 #pragma unroll
-          for (int t = 0; t < MT; ++t)
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {  // dimensions 32 t + 8 g + 4 h + 0..3
-              const u32x2 vv = *reinterpret_cast<const u32x2 *>(vb + key * (2 * D) + (((4 * t + g) ^ swizzle<D>(key)) * 16) + 8 * h);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float x = value_of<BF>((vv[e >> 1] >> (16 * (e & 1))) & 0xffffu);
-                O[t][4 * g + e] = seen ? __builtin_fmaf(w, x, O[t][4 * g + e]) : O[t][4 * g + e];
-              }
+            for (int e = 0; e < 4; ++e) {
+              const int k = 16 * s + 8 * (e >> 1) + 2 * (e & 1);
+              a[e] = Odd<BF>::of_kind(a[e], kind);
+              seen[e] = (k <= d ? Odd<BF>::kOne : 0u) | (k + 1 <= d ? Odd<BF>::kOne << 16 : 0u);
             }
+            n = product<BF>(a, seen, n);
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            O[t][i] = n[i] > 0.0f ? O[t][i] + value : O[t][i];
+            in_place(O[t]);
+          }
         }
       }
     }
+  };
+  // One block holds the wave's diagonal (32 rows lie within one); those after
+  // it hold no key that its queries see. Loops of their own, so that the full
+  // blocks' carries none of the diagonal's code.
+  const int jd = row0 / kKeys;
+  int j = 0;
+  for (; j < min(jd, n_blocks); ++j) {
+    arrive(j);
+    attend(std::false_type{}, j);
   }
+  if (j < n_blocks) {
+    arrive(j);
+    attend(std::true_type{}, j);
+    ++j;
+  }
+  for (; j < n_blocks; ++j) arrive(j);
   l = half_sum(l);
   if (qi >= at.len) return;
   const float inv = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;  // (a NaN stays one)
