@@ -1191,9 +1191,11 @@ static int choose_splits(int64_t units, uint32_t max_length, int32_t requested) 
 // splits win ties within 3%: 63 x 8191 36.9 (9) / 29.4 (7), 128 x 1000 16.0 (4) / 12.9 (3),
 // 129 x 8192 64.0 (4) / 56.5 (6), 128 x 32768 172 (4) / 137 (7), 512 x 8192 171 (1) / 156 (3),
 // 450 x 4096 86.8 (2) with 103 (3) 2% cheaper by this count.
-static int fused_decode_splits(int64_t units, uint32_t max_length, int extra) {
+//
+// resident: workgroups per compute unit (paged_residents).
+static int fused_decode_splits(int64_t units, uint32_t max_length, int extra, int resident = 2) {
   const int64_t max_splits = std::min<int64_t>(256, std::max<int64_t>(1, (max_length + 127) / 128));
-  const int64_t slots = 2 * (int64_t)device_cus();
+  const int64_t slots = resident * (int64_t)device_cus();
   const int64_t first = std::min(max_splits, std::max<int64_t>(1, slots / units - extra));
   const int64_t last = units > slots ? 1 : std::min(max_splits, std::max<int64_t>(first, 3 * slots / units));
   auto cost = [&](int64_t s) {
@@ -1205,7 +1207,7 @@ static int fused_decode_splits(int64_t units, uint32_t max_length, int extra) {
     const int64_t wgs = units * s, rounds = (wgs + slots - 1) / slots;
     return (double)wgs / (double)(rounds * slots);
   };
-  const int64_t up = choose_splits(units, max_length, 0), over = units * up - slots;
+  const int64_t up = std::min(max_splits, (slots + units - 1) / units), over = units * up - slots;
   if (!extra && (up == 2 || up == 3) && over > 0 && over <= slots / 50 && max_length >= 3000) return (int)up;
   int64_t best = first;
   for (int64_t s = first + 1; s <= last; ++s)
@@ -1639,7 +1641,8 @@ bool pool_layout(const DecodeParams &p, const bgtq_pages *g, FastLayout *fl, int
   return general_layout(p, g->tables, fl);
 }
 
-bgtq_status check_pages(const bgtq_pages *g) {
+// nn (may be null): pool_layout's.
+bgtq_status check_pages(const bgtq_pages *g, int *nn_out = nullptr) {
   if (!g) return fail(BGTQ_ERR_RANGE, "null pages");
   if (g->kv_heads < 1 || g->kv_heads > kMaxKvHeads) return fail(BGTQ_ERR_RANGE, "pages: kv_heads must be in 1..%d", kMaxKvHeads);
   if (g->dim != 64 && g->dim != 128) return fail(BGTQ_ERR_UNSUPPORTED, "pages hold heads of dim 64 or 128 (got %d)", g->dim);
@@ -1681,6 +1684,7 @@ bgtq_status check_pages(const bgtq_pages *g) {
   int nn = 0, sg = 0;
   if (!pool_layout(pool_params(g), g, &fl, &nn, &sg))
     return fail(BGTQ_ERR_UNSUPPORTED, "pages hold the packed layouts of the fused decode");
+  if (nn_out) *nn_out = nn;
   return BGTQ_OK;
 }
 
@@ -1800,9 +1804,20 @@ bgtq_status bgtq_paged_read(bgtq_context *ctx, const bgtq_pages *g, const bgtq_p
   return BGTQ_OK;
 }
 
+// Workgroups of the paged decode that share a compute unit. 8-bit V at d=64 leaves
+// room for three (40 KB of LDS and 125 registers at layout B), and three hide
+// more of the loads' latency: 128 units x 32768 tokens 104.9 us with two (4
+// splits) / 100.6 (6), 96 units of none to 16384 tokens 43.6 (5) / 35.3 (8), 200
+// units x 8000 51 / 46; FP16 K, 96 x 16384 51.3 / 52.4. The per-position layouts'
+// lookups are bound by LDS (96 units x 16384 60.3 / 67.3); the other forms fit twice.
+static int paged_residents(const bgtq_pages *g, int nn) {
+  return g->dim == 64 && g->v_format == BGTQ_DTYPE_Q8 && nn >= 0 ? 3 : 2;
+}
+
 // Splits of a paged decode: the fused kernel's own choice, or the caller's.
 static bgtq_status plan_paged_decode(const bgtq_pages *g, const bgtq_paged_decode_desc *d, int *splits) {
-  if (bgtq_status s = check_pages(g)) return s;
+  int nn = 0;
+  if (bgtq_status s = check_pages(g, &nn)) return s;
   if (!d) return fail(BGTQ_ERR_RANGE, "null descriptor");
   if (d->batch < 1 || d->q_heads < g->kv_heads || d->q_heads % g->kv_heads || d->q_heads / g->kv_heads > 16)
     return fail(BGTQ_ERR_RANGE, "invalid head geometry");
@@ -1819,7 +1834,18 @@ static bgtq_status plan_paged_decode(const bgtq_pages *g, const bgtq_paged_decod
   if (d->q_rotated != 0 && d->q_rotated != 1) return fail(BGTQ_ERR_RANGE, "q_rotated must be 0 or 1");
   if (d->q_rotated && g->key_format != BGTQ_KEYS_PACKED) return fail(BGTQ_ERR_RANGE, "q_rotated needs packed K");
   const int64_t units = (int64_t)d->batch * g->kv_heads;
-  *splits = d->splits > 0 ? choose_splits(units, d->max_length, d->splits) : fused_decode_splits(units, d->max_length, 0);
+  if (d->splits > 0) {
+    *splits = choose_splits(units, d->max_length, d->splits);
+    return BGTQ_OK;
+  }
+  // Few units: past the splits that merge in one round of loads every further
+  // one costs its unit's merge 0.22 us (and the change 6 us), a step of 128 tokens 1.1 us of
+  // the workgroup that takes it: sqrt(5 steps) balances the two. us, the rule
+  // without it / 40 splits: layout B, 2 units x 32768 tokens 62.1 (256) / 17.9,
+  // 8 units 34.1 (96) / 21.0, d=128, 4 units 40.6 (128) / 22.7.
+  const double steps = d->max_length / 128.0;
+  const int most = std::max(kDecodeMergeOneRound, (int)std::sqrt(5.0 * steps));
+  *splits = std::min(fused_decode_splits(units, d->max_length, 0, paged_residents(g, nn)), most);
   return BGTQ_OK;
 }
 

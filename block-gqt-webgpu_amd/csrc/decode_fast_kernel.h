@@ -56,6 +56,9 @@ constexpr int kThreads = 64 * kWaves;
 constexpr int kChunk = 32;  // tokens per wave iteration: two 16-token MFMA tiles
 constexpr int kRing = 2;    // LDS chunk buffers per wave: compute one, the next in flight
 constexpr bool kInterleaved = true;
+// Pages: queries are scaled up by at most 2^100, which FP32 holds (smaller ones
+// than 2^-86 keep fewer bits of logits that are nothing to a softmax).
+constexpr int kMaxQueryExp = 100;
 constexpr int kMergeOneRound = kDecodeMergeOneRound;
 
 // Kinds of launch of the fused kernel. Each kind's instances can sit in a
@@ -1025,7 +1028,7 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
       for (int s = 0; s < KS; ++s)
 #pragma unroll
         for (int jv = 0; jv < 8; ++jv) qmax = fmaxf(qmax, fabsf(qv[s][jv]));
-      const int e0 = split_exp(col_max(qmax));
+      const int e0 = PG ? min(split_exp(col_max(qmax)), kMaxQueryExp) : split_exp(col_max(qmax));
       half8 bh[KS], bl[KS];
 #pragma unroll
       for (int s = 0; s < KS; ++s) split_scaled(qv[s], __builtin_ldexpf(1.0f, e0), bh[s], bl[s]);
@@ -1063,6 +1066,9 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
   // B operand of QK: lane holds qr[head = col][32 s + 8 gq + 0..7], split hi/lo
   // after scaling the head's row so its largest entry is near 2^14.
   // F32: the FP32 values themselves.
+  // LATE (pages, packed K): a logit's factor kq goes into the softmax's
+  // multiply-adds instead of a multiplication of its own.
+  constexpr bool LATE = PG && KF >= 1;
   half8 qhi[KS], qlo[KS];
   float qf[F32 ? KS : 1][8];
   float kq = 1.0f;  // logit = (sum_g s_g acc_g) * kq
@@ -1082,7 +1088,8 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
         qmax = fmaxf(qmax, fabsf(v));
       }
     qmax = col_max(qmax);
-    const int eq = qmax > 0.0f ? 14 - (int)ceilf(__builtin_log2f(qmax)) : 0;
+    int eq = qmax > 0.0f ? 14 - (int)ceilf(__builtin_log2f(qmax)) : 0;
+    if constexpr (PG) eq = min(eq, kMaxQueryExp);
     const float qsc = __builtin_ldexpf(1.0f, eq);
 #pragma unroll
     for (int s = 0; s < KS; ++s)
@@ -1093,6 +1100,34 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
         qlo[s][jv] = (_Float16)(x - (float)qhi[s][jv]);
       }
     kq = __builtin_ldexpf(NAT ? 1.0f : kLog2e, -(eq + ec));
+    if constexpr (LATE) kq = fmaxf(kq, 0x1p-126f);  // (it meets masked logits: not 0)
+  }
+  // Pages, structured layouts: a code's table entry is its value's (hi, lo)
+  // pair, and the operands keep them together, each query part once for both:
+  // (hi + lo) qhi + (hi + lo) qlo in four products of 16 dimensions instead of
+  // hi qhi + lo qhi + hi qlo in three of 32, and no instruction sorts the
+  // entries (32 of 268 per chunk; the matrix cores have the room).
+  constexpr bool PAIRED = PG && KF == 1;
+  half8 qhd[PAIRED ? KS : 1][2], qld[PAIRED ? KS : 1][2];
+  if constexpr (PAIRED) {
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const u32x4 h = __builtin_bit_cast(u32x4, qhi[s]), l = __builtin_bit_cast(u32x4, qlo[s]);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        u32x4 hd, ld;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          // nibble steps: entry of two dimensions, hi pair then lo pair; byte steps: of one, hi | lo << 16
+          const uint32_t hw = h[2 * e + (k >> 1)], lw = l[2 * e + (k >> 1)];
+          const uint32_t sel = k & 1 ? 0x03020302u : 0x01000100u;
+          hd[k] = s < NN ? hw : __builtin_amdgcn_perm(hw, hw, sel);
+          ld[k] = s < NN ? lw : __builtin_amdgcn_perm(lw, lw, sel);
+        }
+        qhd[s][e] = __builtin_bit_cast(half8, hd);
+        qld[s][e] = __builtin_bit_cast(half8, ld);
+      }
+    }
   }
   // The q staging (a ring slot's, whose chunk comes later) is dead; row-wise
   // prefill's own staging area is never written again, so it needs no
@@ -1463,7 +1498,7 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
           if (s < NN) wn[u][s] = *reinterpret_cast<const uint32_t *>(row + 16 * s + 4 * gq);
           else wb[u][s] = *reinterpret_cast<const u32x2 *>(row + 16 * NN + 32 * (s - NN) + 8 * gq);
         }
-      u32x4 hi[2][KS], lo[2][KS];
+      u32x4 hi[2][KS], lo[2][KS];  // PAIRED: entries 0..1 (0..3), 2..3 (4..7)
       float af[2][F32 ? KS : 1][8];
 #pragma unroll
       for (int u = 0; u < 2; ++u)
@@ -1481,8 +1516,13 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               const u32x2 v = t64[(wn[u][s] >> (8 * k)) & 255u];
-              hi[u][s][k] = v[0];
-              lo[u][s][k] = v[1];
+              if constexpr (PAIRED) {
+                (k < 2 ? hi : lo)[u][s][2 * (k & 1)] = v[0];
+                (k < 2 ? hi : lo)[u][s][2 * (k & 1) + 1] = v[1];
+              } else {
+                hi[u][s][k] = v[0];
+                lo[u][s][k] = v[1];
+              }
             }
           } else {
             const uint32_t *t32 = tn + s * 512;  // [code]: hi | lo << 16
@@ -1490,8 +1530,13 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
             for (int k = 0; k < 4; ++k) {
               const uint32_t c0 = t32[(wb[u][s][k >> 1] >> (16 * (k & 1))) & 255u];
               const uint32_t c1 = t32[(wb[u][s][k >> 1] >> (16 * (k & 1) + 8)) & 255u];
-              hi[u][s][k] = __builtin_amdgcn_perm(c1, c0, 0x05040100u);  // c0.hi, c1.hi
-              lo[u][s][k] = __builtin_amdgcn_perm(c1, c0, 0x07060302u);  // c0.lo, c1.lo
+              if constexpr (PAIRED) {
+                (k < 2 ? hi : lo)[u][s][2 * (k & 1)] = c0;
+                (k < 2 ? hi : lo)[u][s][2 * (k & 1) + 1] = c1;
+              } else {
+                hi[u][s][k] = __builtin_amdgcn_perm(c1, c0, 0x05040100u);  // c0.hi, c1.hi
+                lo[u][s][k] = __builtin_amdgcn_perm(c1, c0, 0x07060302u);  // c0.lo, c1.lo
+              }
             }
           }
         }
@@ -1507,9 +1552,16 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
             continue;
           }
           const half8 ah = __builtin_bit_cast(half8, hi[u][s]), al = __builtin_bit_cast(half8, lo[u][s]);
-          acc[u][g] = mfma(ah, qhi[s], acc[u][g]);
-          acc[u][g] = mfma(al, qhi[s], acc[u][g]);
-          acc[u][g] = mfma(ah, qlo[s], acc[u][g]);
+          if constexpr (PAIRED) {
+            acc[u][g] = mfma(ah, qhd[s][0], acc[u][g]);
+            acc[u][g] = mfma(al, qhd[s][1], acc[u][g]);
+            acc[u][g] = mfma(ah, qld[s][0], acc[u][g]);
+            acc[u][g] = mfma(al, qld[s][1], acc[u][g]);
+          } else {
+            acc[u][g] = mfma(ah, qhi[s], acc[u][g]);
+            acc[u][g] = mfma(al, qhi[s], acc[u][g]);
+            acc[u][g] = mfma(ah, qlo[s], acc[u][g]);
+          }
         }
     }
     // FP16 K rows: swizzled 16-byte pieces.
@@ -1528,7 +1580,7 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
 #pragma unroll
     for (int u = 0; u < 2 && KF == 2; ++u) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) x[4 * u + r] = x2[u][r] * kq;
+      for (int r = 0; r < 4; ++r) x[4 * u + r] = LATE ? x2[u][r] : x2[u][r] * kq;
     }
 #pragma unroll
     for (int u = 0; u < (KF == 2 ? 0 : 2); ++u) {
@@ -1549,7 +1601,7 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
         } else {
           v = acc[u][0][r];
         }
-        x[4 * u + r] = v * kq;
+        x[4 * u + r] = LATE ? v : v * kq;
       }
     }
     if (c0 + kChunk > lim_min || !in_pool) {
@@ -1582,8 +1634,12 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
       const int r8 = col >> 1, vrow = 16 * (r8 >> 2) + 4 * gq + (r8 & 3);
       u32x2 vc[DT];
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-        ds_read_tr8(sb + vrow * D + ((dt ^ swz8<D>(vrow)) * 16) + 8 * (col & 1), vc[dt]);
+      for (int dt = 0; dt < DT; dt += 4) {
+        const uint8_t *at[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) at[i] = sb + vrow * D + (((dt + i) ^ swz8<D>(vrow)) * 16) + 8 * (col & 1);
+        ds_read_tr8(at, &vc[dt]);
+      }
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
         wait_tr8<DT>(dt, vc[dt]);
@@ -1697,6 +1753,8 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
     }
   } else {
     int raw_next = raw1;           // pages: the table entry of chunk i + 1
+    float one = 1.0f;
+    if constexpr (PG) asm("" : "+s"(one));  // (split2_mix)
     bool in_pool = page0 >= 0, in_pool_next = true;
     for (int i = 0; i < n_chunks; ++i) {
       const int c0 = first + i * stride;
@@ -1741,13 +1799,13 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
       }
       // online softmax (log2 domain; FP32 V: natural units) for head col
       float mloc = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-      const float m_new = fmaxf(m_run, col_max(mloc));
+      const float m_new = fmaxf(m_run, LATE ? col_max_logit(x) * kq : PG ? col_max_logit(x) : col_max(mloc));
       const float alpha = m_new == -INFINITY ? 1.0f : exp_of<NAT>(m_run - m_new);
       const float mb = (m_new == -INFINITY ? 0.0f : m_new) - kPShift;
       float pr[8], psum = 0.0f;
   #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        pr[j] = exp_of<NAT>(x[j] - mb);
+        pr[j] = LATE ? exp_of<NAT>(__builtin_fmaf(x[j], kq, -mb)) : exp_of<NAT>(x[j] - mb);
         psum += pr[j];
       }
       l_run = __builtin_fmaf(l_run, alpha, psum);
@@ -1756,7 +1814,8 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
   #pragma unroll
       for (int k = 0; k < (VF32 ? 0 : 4); ++k) {
         uint32_t h, l;
-        split2(pr[2 * k], pr[2 * k + 1], h, l);
+        if constexpr (PG) split2_mix(pr[2 * k], pr[2 * k + 1], one, h, l);
+        else split2(pr[2 * k], pr[2 * k + 1], h, l);
         ph[k] = h;
         pl[k] = l;
       }
@@ -1950,7 +2009,7 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
   }
   // More splits: every load of a stage in flight at once: (m, l) of all
   // heads and splits, then per-head normalised weights, then the o rows in
-  // groups of eight splits.
+  // groups of eight splits (pages: 32, a round trip each).
   float *wgt = reinterpret_cast<float *>(smem);  // [16 heads][S] (reuses the ring)
   float *mrow = wgt + 16 * S;                     // [16 heads][S] split maxima
   for (int e = tid; e < ncol * S; e += kThreads) {
@@ -1983,18 +2042,19 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
     const int64_t head = out_row(g);
     float *pp = p.part + (pbase + g) * S * (D + 2) + 2 + dm;
     float Ov = 0.0f;
-    for (int s0 = 0; s0 < S; s0 += 8) {
-      // Unconditional loads (past S: split S - 1, weighted zero), all eight in
-      // flight together; loads under a branch would go one after another.
-      float o[8], w8[8];
+    constexpr int MG = PG ? 32 : 8;
+    for (int s0 = 0; s0 < S; s0 += MG) {
+      // Unconditional loads (past S: split S - 1, weighted zero), all of a
+      // group in flight together; loads under a branch would go one after another.
+      float o[MG], w8[MG];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
+      for (int k = 0; k < MG; ++k) {
         const int sk = min(s0 + k, S - 1);
         o[k] = coherent_load(pp + sk * (D + 2));
         w8[k] = wgt[g * S + sk];
       }
 #pragma unroll
-      for (int k = 0; k < 8; ++k) Ov = __builtin_fmaf(o[k], s0 + k < S ? w8[k] : 0.0f, Ov);
+      for (int k = 0; k < MG; ++k) Ov = __builtin_fmaf(o[k], s0 + k < S ? w8[k] : 0.0f, Ov);
     }
     p.out[head * D + dm] = Ov;
   }

@@ -51,6 +51,25 @@ __device__ __forceinline__ float col_max(float v) {
   auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
+// The same of eight values per lane that come from arithmetic, not straight
+// from a matrix-core instruction (whose wait states the compiler does not
+// count for asm): fmaxf makes every operand canonical first, 13 more of 20
+// instructions.
+__device__ __forceinline__ float col_max_logit(const float (&x)[8]) {
+  auto max3 = [](float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+  };
+  float inf = INFINITY;
+  asm("" : "+s"(inf));  // (known, the median with it becomes fmaxf)
+  auto max2 = [inf](float a, float b) { return __builtin_amdgcn_fmed3f(a, b, inf); };
+  float v = max2(max3(max3(x[0], x[1], x[2]), x[3], x[4]), max3(x[5], x[6], x[7]));
+  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = max2(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return max2(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
 __device__ __forceinline__ float col_sum(float v) {
   auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
@@ -207,8 +226,13 @@ __device__ __forceinline__ void ds_read_tr16_pair(const uint8_t *lds0, const uin
 // One transposed read of 8-bit values (ds_read_b64_tr_b8: lane i of a 16-lane
 // group gets column i of the eight 16-byte rows whose halves the group's
 // lanes address, lanes 2 r and 2 r + 1 row r's), as ds_read_tr16_pair.
-__device__ __forceinline__ void ds_read_tr8(const uint8_t *lds, u32x2 &a) {
-  asm volatile("s_nop 7\n\tds_read_b64_tr_b8 %0, %1" : "=&v"(a) : "v"((uint32_t)(uintptr_t)(lds_void *)lds));
+__device__ __forceinline__ void ds_read_tr8(const uint8_t *const (&lds)[4], u32x2 *a) {
+  asm volatile(
+      "s_nop 7\n\tds_read_b64_tr_b8 %0, %4\n\tds_read_b64_tr_b8 %1, %5\n\t"
+      "ds_read_b64_tr_b8 %2, %6\n\tds_read_b64_tr_b8 %3, %7"
+      : "=&v"(a[0]), "=&v"(a[1]), "=&v"(a[2]), "=&v"(a[3])
+      : "v"((uint32_t)(uintptr_t)(lds_void *)lds[0]), "v"((uint32_t)(uintptr_t)(lds_void *)lds[1]),
+        "v"((uint32_t)(uintptr_t)(lds_void *)lds[2]), "v"((uint32_t)(uintptr_t)(lds_void *)lds[3]));
 }
 // Waits until at most N LDS operations of this wave are in flight; a and b
 // are tied to the wait so nothing that reads them is scheduled before it.

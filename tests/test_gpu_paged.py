@@ -405,9 +405,23 @@ def test_decode_long(device, oracle):
         pool.destroy()
 
 
+@pytest.mark.parametrize("layout,dim", [("S", 64), ("B", 64), ("B", 128), ("f16", 64)])
+def test_decode_of_tiny_queries(device, oracle, layout, dim):
+    """Queries down to the smallest FP32 numbers give all but equal weights, and none NaN; zeros the mean."""
+    pool = Pool(device, layout, "q8", dim, 2, 12, 32)
+    _fill(pool, 4)
+    table = _table(pool, [70, 200], np.random.RandomState(0))
+    for size in (0.0, 1e-45, 1e-39, 1e-36, 1e-30, 1e-20):
+        print(layout, dim, size, flush=True)
+        q = (_rows(2, 6, dim, "float32", 9) * size).cuda()
+        _check(_decode(pool, q, [70, 200], table), _reference(pool, oracle, q * 0, [70, 200], table), f"{layout} {dim} {size}")
+    pool.destroy()
+
+
 def test_decode_equals_dense(device):
-    """The same rows in one contiguous cache per sequence: bgtq_decode's outputs bit for bit; and 8-bit V equal to
-    FP16 V pages of the values it stands for."""
+    """8-bit V equals FP16 V pages of the values it stands for, bit for bit. And the same rows in one contiguous cache
+    per sequence: bgtq_decode sorts a code's high and low parts into products of their own and multiplies the
+    logits' factor in by itself, so the two agree as two results that are each within the tolerance of 64 bits."""
     import torch
     from bgtq import batched
     for layout, dim, heads in (("B", 64, 2), ("S", 64, 3), ("B", 128, 2)):
@@ -447,7 +461,8 @@ def test_decode_equals_dense(device):
         ws = torch.zeros(batched.workspace_bytes(batched.decode_desc(**kw)), dtype=torch.uint8, device="cuda")
         batched.decode(device, batched.decode_desc(workspace=ws, **kw))
         torch.cuda.synchronize()
-        assert torch.equal(dense, out), (layout, dim)
+        off = (dense - out).abs()
+        assert (off <= 2 * (ATOL + RTOL * dense.abs())).all(), (layout, dim, off.max().item())
         pool.destroy()
         plain.destroy()
 
