@@ -147,9 +147,16 @@ __device__ __forceinline__ float half_sum(float v) {
 }
 
 // The sequence and its tile of kRows rows that grid slot `slot` stands for.
-// Sequence s owns the slots from offsets[s] / kRows + s on, at least as many as
-// it has tiles; the last sequence that starts at or before the slot is found
-// 64 candidates at a time (every wave by itself).
+// Workgroups start in the order of their slots, and a tile's work is its
+// history: the longest histories of all sequences come first, or a long
+// sequence's would be left running alone at the end (11 prompts of 568 to 2777
+// tokens SORTED us, sequence by sequence INORDER). Tiles i of all the sequences that have
+// one make level i; with C(i) the tiles of levels i and up, the slot's level
+// is the last one with C(i) > slot, found bit by bit, a lane per sequence.
+// More than 64 sequences: sequence by sequence, sequence s owning the slots from
+// offsets[s] / kRows + s on, at least as many as it has tiles; the last
+// sequence that starts at or before the slot is found 64 candidates at a time.
+// Every wave finds the place by itself.
 struct Place {
   int64_t begin;
   int len, tile;  // tile < 0: nothing to do
@@ -160,6 +167,25 @@ __device__ __forceinline__ Place find_place(const PromptParams &p, int64_t slot)
     const int64_t o = p.offsets[s];
     return o < 0 ? 0 : o > p.tokens ? p.tokens : o;
   };
+  if (p.sequences <= 64) {
+    const int64_t begin = offset(min(lane, p.sequences)), end = offset(min(lane + 1, p.sequences));
+    const int len = end > begin ? (int)(end - begin) : 0, tiles = (int)(((int64_t)len + kRows - 1) / kRows);
+    auto tiles_from = [&](int level) { return wave_sum(max(tiles - level, 0)); };
+    int level = 0, below = 0;  // below: C(level + 1)
+    for (int bit = 1 << (31 - __builtin_clz((int)(p.tokens / kRows) + 1)); bit; bit >>= 1) {
+      const int c = tiles_from(level + bit);
+      if (c > slot) level += bit;
+      else below = c;
+    }
+    const bool here = tiles > level;
+    const uint64_t row = __builtin_amdgcn_ballot_w64(here);
+    const int rank = (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(row >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)row, 0u));
+    const uint64_t mine = __builtin_amdgcn_ballot_w64(here && rank == (int)slot - below);
+    if (mine == 0) return {0, 0, -1};
+    const int at = __builtin_ctzll(mine);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)begin, at);
+    return {(int64_t)lo, __builtin_amdgcn_readlane(len, at), level};
+  }
   int lo = 0, n = p.sequences;
   for (;;) {
     const int step = (n + 63) / 64, at = lane * step;
