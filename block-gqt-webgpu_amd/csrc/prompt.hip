@@ -150,7 +150,7 @@ __device__ __forceinline__ float half_sum(float v) {
 // Workgroups start in the order of their slots, and a tile's work is its
 // history: the longest histories of all sequences come first, or a long
 // sequence's would be left running alone at the end (11 prompts of 568 to 2777
-// tokens SORTED us, sequence by sequence INORDER). Tiles i of all the sequences that have
+// tokens 92 us, sequence by sequence 100). Tiles i of all the sequences that have
 // one make level i; with C(i) the tiles of levels i and up, the slot's level
 // is the last one with C(i) > slot, found bit by bit, a lane per sequence.
 // More than 64 sequences: sequence by sequence, sequence s owning the slots from
@@ -173,7 +173,7 @@ __device__ __forceinline__ Place find_place(const PromptParams &p, int64_t slot)
     auto tiles_from = [&](int level) { return wave_sum(max(tiles - level, 0)); };
     int level = 0, below = 0;  // below: C(level + 1)
     for (int bit = 1 << (31 - __builtin_clz((int)(p.tokens / kRows) + 1)); bit; bit >>= 1) {
-      const int c = tiles_from(level + bit);
+      const int c = __builtin_amdgcn_readfirstlane(tiles_from(level + bit));
       if (c > slot) level += bit;
       else below = c;
     }
@@ -205,7 +205,7 @@ __device__ __forceinline__ Place find_place(const PromptParams &p, int64_t slot)
 }
 
 template <int D, bool BF>
-__global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void prompt_kernel(PromptParams p) {
+__global__ __launch_bounds__(kThreads, D == 64 ? 4 : 2) void prompt_kernel(PromptParams p) {
   constexpr int PR = D / 8;                      // 16-byte pieces per row
   constexpr int QS = D / 16;                     // 16-dimension steps of QK
   constexpr int MT = D / 32;                     // 32-dimension tiles of O
@@ -272,6 +272,18 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void prompt_kernel(Promp
     lds_barrier();  // everyone's has, and everyone is done with the other buffer
     if (j + 1 < n_blocks) issue(j + 1);
   };
+  // d=128: the two waves of a SIMD issue their softmax ahead of each other's
+  // products, which need an issue slot every 32 cycles only (one prompt of 8192
+  // tokens 257 us; without 276, products first 288). d=64's four waves fill the
+  // vector unit without (11 prompts 87 us, 89 with).
+  auto softmax_first = [](int on) {
+    if constexpr (D == 128) {
+      __builtin_amdgcn_sched_barrier(0);
+      if (on) __builtin_amdgcn_s_setprio(1);
+      else __builtin_amdgcn_s_setprio(0);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
   // Block j's keys for this wave's queries; DIAGONAL: some queries see only a part of them.
   auto attend = [&](auto diagonal_tag, int j) {
     constexpr bool DIAGONAL = decltype(diagonal_tag)::value;
@@ -295,6 +307,7 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void prompt_kernel(Promp
 #pragma unroll
         for (int i = 0; i < 16; ++i) S[b][i] = 32 * b + 8 * (i >> 2) + (i & 3) <= d ? S[b][i] : -INFINITY;
     }
+    softmax_first(1);
     float top = S[0][0];
 #pragma unroll
     for (int i = 1; i < 16; ++i) top = fmaxf(top, S[0][i]);
@@ -326,6 +339,7 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void prompt_kernel(Promp
       P[e] = pack2<BF>(S[e >> 3][2 * (e & 7)], S[e >> 3][2 * (e & 7) + 1]);
       l = add2<BF>(P[e], l);
     }
+    softmax_first(0);
     // O^T += V^T P^T, 16 keys a step, the next step's V on its way meanwhile.
     uint32_t va[MT], va8[MT];
 #pragma unroll
