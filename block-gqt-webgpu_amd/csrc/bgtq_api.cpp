@@ -1766,8 +1766,8 @@ bgtq_status bgtq_paged_write(bgtq_context *ctx, const bgtq_pages *g, const bgtq_
   if (bgtq_status s = ctx->use()) return s;
   const PagedWriteParams p = rows_params(g, r);
   if (g->key_format == BGTQ_KEYS_PACKED) {
-    // Few rows: a wave per row, V in the same launch; many: the tile encoder,
-    // as for dense rows (bgtq_encode_batched).
+    // Few rows: a wave per row; many: the tile encoder, as for dense rows
+    // (bgtq_encode_batched). V goes in the same launch.
     EncodeTileSizes z{};
     bool tile = r->k_row_stride <= kTileMaxStride;
     int enc = 0;
@@ -1788,6 +1788,7 @@ bgtq_status bgtq_paged_write(bgtq_context *ctx, const bgtq_pages *g, const bgtq_
       return BGTQ_OK;
     }
     HIP_TRY(launch_encode_tile_paged(p, g->dim, device_cus(), z, ctx->stream), "paged encode launch");
+    return BGTQ_OK;
   }
   HIP_TRY(launch_paged_write(p, false, 0, device_cus(), ctx->stream), "paged write launch");
   return BGTQ_OK;
