@@ -1593,6 +1593,15 @@ struct DeviceScope {
   }
 };
 
+// Whether n0 x n1 pieces of `len` at strides s0 and s1 lie apart: the pieces
+// of either index, each with all of the other's, one after another.
+bool apart(int64_t n0, int64_t s0, int64_t n1, int64_t s1, int64_t len) {
+  auto nested = [len](__int128 outer, __int128 so, __int128 inner, __int128 si) {
+    return (inner <= 1 || si >= len) && (outer <= 1 || so >= (inner - 1) * si + len);
+  };
+  return nested(n0, s0, n1, s1) || nested(n1, s1, n0, s0);
+}
+
 // One array of a pool: its base and strides in bytes, and the bytes of a page's rows of one head.
 bgtq_status check_pool_array(const char *what, const void *base, int64_t page_stride, int64_t head_stride, int64_t rows,
                              int64_t align, int64_t pages, int32_t heads) {
@@ -1600,8 +1609,8 @@ bgtq_status check_pool_array(const char *what, const void *base, int64_t page_st
   if (page_stride < 0 || head_stride < 0) return fail(BGTQ_ERR_RANGE, "pages: negative %s stride", what);
   if (reinterpret_cast<uintptr_t>(base) % (uintptr_t)align || page_stride % align || head_stride % align)
     return fail(BGTQ_ERR_RANGE, "pages: %s base and strides must be multiples of %d bytes", what, (int)align);
-  if ((pages > 1 && page_stride < rows) || (heads > 1 && head_stride < rows))
-    return fail(BGTQ_ERR_RANGE, "pages: %s stride below the rows of a page", what);
+  if (!apart(pages, page_stride, heads, head_stride, rows))
+    return fail(BGTQ_ERR_RANGE, "pages: %s strides let a page's rows overlap", what);
   return BGTQ_OK;
 }
 
@@ -1688,10 +1697,11 @@ bgtq_status check_pages(const bgtq_pages *g, int *nn_out = nullptr) {
   return BGTQ_OK;
 }
 
-bgtq_status check_rows(const bgtq_paged_rows *r, bool both) {
+// write: both are given, and only read; else either, and written.
+bgtq_status check_rows(const bgtq_paged_rows *r, const bgtq_pages *g, bool write) {
   if (!r) return fail(BGTQ_ERR_RANGE, "null rows");
   if (r->rows < 0 || r->rows > INT32_MAX) return fail(BGTQ_ERR_RANGE, "rows must be in 0..2^31 - 1");
-  if (both ? !r->k || !r->v : !r->k && !r->v) return fail(BGTQ_ERR_RANGE, "null K or V rows");
+  if (write ? !r->k || !r->v : !r->k && !r->v) return fail(BGTQ_ERR_RANGE, "null K or V rows");
   struct {
     const void *p;
     int32_t dtype;
@@ -1704,6 +1714,7 @@ bgtq_status check_rows(const bgtq_paged_rows *r, bool both) {
     if (a.row < 0 || a.head < 0) return fail(BGTQ_ERR_RANGE, "negative rows stride");
     if (reinterpret_cast<uintptr_t>(a.p) % (a.dtype == BGTQ_DTYPE_F32 ? 4 : 2))
       return fail(BGTQ_ERR_RANGE, "rows must be aligned to their type");
+    if (!write && !apart(r->rows, a.row, g->kv_heads, a.head, g->dim)) return fail(BGTQ_ERR_RANGE, "overlapping rows to read into");
   }
   if (r->rows && !r->slots) return fail(BGTQ_ERR_RANGE, "null slots");
   if (reinterpret_cast<uintptr_t>(r->slots) % 8) return fail(BGTQ_ERR_RANGE, "slots must be 8-byte aligned");
@@ -1759,7 +1770,7 @@ extern "C" {
 
 bgtq_status bgtq_paged_write(bgtq_context *ctx, const bgtq_pages *g, const bgtq_paged_rows *r) {
   if (bgtq_status s = check_pages(g)) return s;
-  if (bgtq_status s = check_rows(r, true)) return s;
+  if (bgtq_status s = check_rows(r, g, true)) return s;
   if (!ctx) return fail(BGTQ_ERR_RANGE, "null context");
   if (!r->rows) return BGTQ_OK;
   DeviceScope scope;
@@ -1796,7 +1807,7 @@ bgtq_status bgtq_paged_write(bgtq_context *ctx, const bgtq_pages *g, const bgtq_
 
 bgtq_status bgtq_paged_read(bgtq_context *ctx, const bgtq_pages *g, const bgtq_paged_rows *r) {
   if (bgtq_status s = check_pages(g)) return s;
-  if (bgtq_status s = check_rows(r, false)) return s;
+  if (bgtq_status s = check_rows(r, g, false)) return s;
   if (!ctx) return fail(BGTQ_ERR_RANGE, "null context");
   if (!r->rows) return BGTQ_OK;
   DeviceScope scope;
@@ -1922,9 +1933,10 @@ bgtq_status bgtq_prompt_attention(bgtq_context *ctx, const bgtq_prompt_desc *d) 
       return fail(BGTQ_ERR_RANGE, "q/k/v/out: 16-byte aligned bases, strides multiples of 8 elements and not negative");
     if (a.row > kPromptMaxStride) return fail(BGTQ_ERR_RANGE, "q/k/v/out: row strides up to %lld elements", (long long)kPromptMaxStride);
   }
-  if ((d->tokens > 1 && d->out_row_stride < d->dim) || (d->q_heads > 1 && d->out_head_stride < d->dim))
-    return fail(BGTQ_ERR_RANGE, "out: strides below dim");
-  if (prompt_workgroups(*d) > INT32_MAX) return fail(BGTQ_ERR_UNSUPPORTED, "prompt attention: too many (row, head) pairs for one call");
+  if (!apart(d->tokens, d->out_row_stride, d->q_heads, d->out_head_stride, d->dim))
+    return fail(BGTQ_ERR_RANGE, "out: overlapping rows");
+  // (a launch counts its work-items in 32 bits)
+  if (prompt_workgroups(*d) > UINT32_MAX / kPromptThreads) return fail(BGTQ_ERR_UNSUPPORTED, "prompt attention: too many (row, head) pairs for one call");
   if (!ctx) return fail(BGTQ_ERR_RANGE, "null context");
   if (none) return BGTQ_OK;
   DeviceScope scope;

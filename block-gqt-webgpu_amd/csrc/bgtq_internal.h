@@ -491,6 +491,7 @@ hipError_t launch_paged_write(const PagedWriteParams &p, bool with_k, int lds_by
 hipError_t launch_paged_read(const PagedWriteParams &p, int cus, hipStream_t stream);
 // Causal attention over packed prompts (prompt.hip), and its workgroups.
 int64_t prompt_workgroups(const bgtq_prompt_desc &d);
+constexpr int kPromptThreads = 256;  // of a workgroup
 constexpr int64_t kPromptMaxStride = 1 << 22;  // elements: a block's byte offsets stay below 2^31
 hipError_t launch_prompt_attention(const bgtq_prompt_desc &d, hipStream_t stream);
 hipError_t launch_rotate_q(const DecodeParams &p, const float *q, float *qr, hipStream_t stream);

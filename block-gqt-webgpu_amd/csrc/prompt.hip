@@ -33,7 +33,7 @@ typedef _Float16 half2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-constexpr int kWaves = 4, kThreads = 64 * kWaves;
+constexpr int kThreads = kPromptThreads, kWaves = kThreads / 64;
 constexpr int kRows = 32 * kWaves;  // query rows of a workgroup
 constexpr int kKeys = 64;           // keys of a block
 constexpr float kLazy = 8.0f;       // growth of a maximum (log2) that O is not rescaled for

@@ -407,7 +407,8 @@ bgtq_status bgtq_prefill_append(bgtq_context *ctx, const bgtq_prefill_desc *d, c
  * q_heads / kv_heads at most 16, kv_heads at most 16; every base and page and
  * head stride a multiple of 16 bytes (v_scales: 4), strides not negative.
  * The packed layouts are those of bgtq_decode_append (others:
- * BGTQ_ERR_UNSUPPORTED, nothing is queued). */
+ * BGTQ_ERR_UNSUPPORTED, nothing is queued). The rows of the pages and heads do not
+ * overlap: pages outermost, each with all heads, or heads outermost (refused otherwise). */
 typedef struct {
   int32_t kv_heads, dim;
   int32_t key_format; /* BGTQ_KEYS_PACKED or BGTQ_KEYS_FP16 */
@@ -453,7 +454,7 @@ bgtq_status bgtq_paged_write(bgtq_context *ctx, const bgtq_pages *pages, const b
  * (src/reference/production_math.py:27-31) in FP32, V's FP16 values, each
  * rounded once to k_dtype / v_dtype. Rows whose slot lies outside the pool
  * stay as they were; a slot may be read any number of times. k or v may be
- * NULL: only the other is read. */
+ * NULL: only the other is read. The rows read into do not overlap (rows outermost or heads). */
 bgtq_status bgtq_paged_read(bgtq_context *ctx, const bgtq_pages *pages, const bgtq_paged_rows *rows);
 
 /* Decode attention of one layer over pages: as bgtq_decode (queries, outputs,
@@ -486,9 +487,10 @@ bgtq_status bgtq_paged_decode(bgtq_context *ctx, const bgtq_pages *pages, const 
  * at q + i*q_row_stride + h*q_head_stride (elements; likewise k, v, out; a row's
  * dim values are adjacent). dtype: BGTQ_DTYPE_F16 or _BF16, of q, k, v and out.
  * dim 64 or 128; any q_heads that is a multiple of kv_heads, at most 65535;
- * sequences up to 65535, tokens (rows of each) up to 2^31 - 1. Bases 16-byte
- * aligned, strides multiples of 8 elements and not negative; out may not overlap
- * the inputs. offsets (device int32 [sequences + 1], nondecreasing) are clamped to
+ * sequences up to 65535, tokens (rows of each) up to 2^31 - 1, (tokens / 128 +
+ * sequences) * q_heads below 2^24. Bases 16-byte aligned, strides multiples of 8
+ * elements, not negative and row strides at most 2^22; out overlaps neither the
+ * inputs nor itself (rows outermost or heads). offsets (device int32 [sequences + 1], nondecreasing) are clamped to
  * 0 .. tokens; a sequence may be empty, and rows of no sequence stay as they
  * were. scale: of the logits; 0 = 1 / sqrt(dim). Logits, softmax statistics and
  * sums are FP32, probabilities are rounded to dtype for the product with V. One

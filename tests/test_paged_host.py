@@ -51,7 +51,9 @@ BAD_PAGES = [dict(kv_heads=0), dict(kv_heads=17), dict(dim=96), dict(page_tokens
              dict(page_tokens=-64), dict(pages=0), dict(pages=1 << 31), dict(key_format=2), dict(v_format=_lib.DTYPE_F32), dict(k_f16=None),
              dict(v=None), dict(v_scales=None), dict(k_f16=A + 8), dict(v=A + 4), dict(v_scales=A + 2), dict(k_page_stride=-8),
              dict(k_page_stride=2 * 64 * 64 + 4), dict(v_head_stride=64 * 64 - 16), dict(v_scales_page_stride=63), dict(k_head_stride=0),
-             dict(key_format=_lib.KEYS_PACKED)]
+             dict(key_format=_lib.KEYS_PACKED),
+             dict(k_page_stride=64 * 64), dict(v_page_stride=64 * 64, v_head_stride=9 * 64 * 64),
+             dict(v_scales_page_stride=1 << 62, v_scales_head_stride=1 << 61, kv_heads=16, pages=1 << 30)]
 
 
 @pytest.mark.parametrize("bad", BAD_PAGES, ids=str)
@@ -72,6 +74,35 @@ def test_bad_rows(bad):
     for call in (L.bgtq_paged_write, L.bgtq_paged_read):
         assert call(None, ctypes.byref(_pages()), ctypes.byref(_rows(**bad))) == _lib.ERR_RANGE
         assert b"context" not in L.bgtq_last_error()
+
+
+def test_overlaps():
+    """Rows that are written lie apart, pages or rows outermost or heads; rows that are only read may not."""
+    L, S = _lib.lib(), 64 * 64
+    for page, head, good in ((2 * S, S, True), (S, 10 * S, True), (S, 9 * S, False), (S, S, False), (2 * S - 64, S, False)):
+        g = _pages(k_page_stride=page, k_head_stride=head)
+        assert L.bgtq_paged_read(None, ctypes.byref(g), ctypes.byref(_rows())) == _lib.ERR_RANGE
+        assert (L.bgtq_last_error() == b"null context") == good, (page, head)
+    for row, head, good in ((128, 64, True), (64, 320, True), (64, 256, False), (0, 0, False), (64, 64, False), (120, 64, False)):
+        r = _rows(k_row_stride=row, k_head_stride=head)
+        assert L.bgtq_paged_read(None, ctypes.byref(_pages()), ctypes.byref(r)) == _lib.ERR_RANGE
+        assert (L.bgtq_last_error() == b"null context") == good, (row, head)
+        assert L.bgtq_paged_write(None, ctypes.byref(_pages()), ctypes.byref(r)) == _lib.ERR_RANGE
+        assert L.bgtq_last_error() == b"null context"
+    for row, head, good in ((384, 64, True), (64, 6400, True), (64, 6392, False), (376, 64, False), (64, 64, False)):
+        d = _prompt(out_row_stride=row, out_head_stride=head)
+        assert L.bgtq_prompt_attention(None, ctypes.byref(d)) == _lib.ERR_RANGE
+        assert (L.bgtq_last_error() == b"null context") == good, (row, head)
+
+
+def test_most_prompt_rows():
+    """A launch holds 2^32 work-items, 256 per 128 rows of a head and sequence."""
+    L = _lib.lib()
+    for tokens, sequences, heads, good in (((1 << 24) * 128 // 16 - 256, 1, 16, True), ((1 << 24) * 128 // 16, 1, 16, False),
+                                           ((1 << 31) - 1, 1, 2, False), ((1 << 31) - 256, 1, 1, True)):
+        d = _prompt(tokens=tokens, sequences=sequences, q_heads=heads, kv_heads=1, out_row_stride=64 * heads)
+        assert L.bgtq_prompt_attention(None, ctypes.byref(d)) in (_lib.ERR_RANGE, _lib.ERR_UNSUPPORTED)
+        assert (L.bgtq_last_error() == b"null context") == good, (tokens, heads)
 
 
 def test_rows_that_are_missing():
