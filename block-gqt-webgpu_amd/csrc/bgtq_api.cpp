@@ -433,7 +433,8 @@ bgtq_status bgtq_tables_create(bgtq_context *ctx, const uint32_t *integer, size_
   const size_t off_gdesc = align(off_rot_q + (d % 32 == 0 ? (size_t)rot_q_bytes((int)d) : 0));
   const size_t off_glane = align(off_gdesc + sizeof(uint32_t) * d);
   const size_t off_rot_k = align(off_glane + (d % 32 == 0 ? sizeof(uint32_t) * kLaneRecordWords * 4 * (d / 32) : 0));
-  const size_t total = off_rot_k + (d % 32 == 0 ? (size_t)rot_q_bytes((int)d) : 0);
+  const size_t off_rot_a = align(off_rot_k + (d % 32 == 0 ? (size_t)rot_q_bytes((int)d) : 0));
+  const size_t total = off_rot_a + (d == 64 || d == 128 ? sizeof(float) * d * d : 0);
   auto *t = new bgtq_tables();
   t->ctx = ctx;
   t->host.assign(total, 0);
@@ -460,6 +461,7 @@ bgtq_status bgtq_tables_create(bgtq_context *ctx, const uint32_t *integer, size_
   T->off_gdesc = (uint32_t)off_gdesc;
   T->off_glane = (uint32_t)off_glane;
   T->off_rot_k = (uint32_t)off_rot_k;
+  T->off_rot_a = (uint32_t)off_rot_a;
   T->total_bytes = (uint32_t)total;
   float cmax = 0.0f;
   for (int64_t i = 0; i < d * mc; ++i) cmax = std::max(cmax, std::fabs(cent[i]));
@@ -587,6 +589,17 @@ bgtq_status bgtq_tables_create(bgtq_context *ctx, const uint32_t *integer, size_
     };
     operands(off_rot_q, [&](int64_t row, int64_t col) { return rq[row * d + col]; });
     operands(off_rot_k, [&](int64_t row, int64_t col) { return rq[col * d + row] * 16384.0f; });
+    if (d == 64 || d == 128) {
+      // Row j = 16 t + 4 r + q is operand row m = 4 q + r of tile t; column
+      // 16 n + 4 i + k is k of step i of columns n.
+      const float *R = reinterpret_cast<const float *>(h + off_rot);
+      float *a = reinterpret_cast<float *>(h + off_rot_a);
+      for (int64_t j = 0; j < d; ++j)
+        for (int64_t c = 0; c < d; ++c) {
+          const int64_t t = j / 16, m = 4 * (j & 3) + ((j >> 2) & 3), i = c % 16 / 4, k = c & 3;
+          a[((t * (d / 16) + c / 16) * 64 + 16 * k + m) * 4 + i] = R[j * d + c];
+        }
+    }
   }
   t->tile_encode = encode_tile_layout(T);
   t->info = bgtq_tables_info{(int32_t)d, (int32_t)ng, (int32_t)rb, (int32_t)nstride, (int32_t)nib, (int32_t)mc, ncb, nb,

@@ -20,7 +20,7 @@ constexpr int kEncodeJobTable = 4096;     // jobs in a context's device job tabl
 struct DevTables {
   int32_t dim, groups, row_bytes, norm_stride, nibble_dims, max_centroids, n_books, n_codebooks;
   int32_t gstart[kMaxGroups], gend[kMaxGroups], gsize[kMaxGroups];  // group ranges (head-perm order)
-  uint32_t off_lut, off_books, off_rot, off_rot_t, off_mfma, off_rot_q, off_gdesc, off_glane, off_rot_k, total_bytes;
+  uint32_t off_lut, off_books, off_rot, off_rot_t, off_mfma, off_rot_q, off_gdesc, off_glane, off_rot_k, off_rot_a, total_bytes;
   int32_t cent_exp;  // 2^cent_exp * max|centroid| <= 2^14: fp16 hi/lo split range for MFMA operands
   // The fused decode of any packed layout: its leading pair K-steps (see
   // off_glane) and the books whose pair tables it keeps in LDS for them
@@ -47,6 +47,8 @@ struct DevTables {
   //             (hi, lo) MFMA A operands: for 16-row tile n, 32-column step
   //             s and lane l, 8 hi then 8 lo halves of
   //             Rq[16 n + l % 16][32 s + 8 (l / 16) + 0..7] (kRotQBytes).
+  // [off_rot_a] (dim 64, 128) R as the tile encoder's FP32 A operands
+  //             ([16-row tile][16 columns][lane][4]), as they lie in its LDS.
   // [off_rot_k] the transpose of Rq times 2^14 in the same operand form
   //             (16-row tile n of dimensions, 32-position step s), for the
   //             rows read back from pages: k = Rq^T (c s).

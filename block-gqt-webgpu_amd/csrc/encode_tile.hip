@@ -209,6 +209,9 @@ __device__ __forceinline__ void encode_tile_body(const EncodeTileJob &job, const
   // ---- the workgroup's tables ----
   const uint8_t *Tg = reinterpret_cast<const uint8_t *>(job.t);
   {
+    const __amdgpu_buffer_rsrc_t ra = rsrc(Tg + T->off_rot_a, D * D * 4);
+#pragma unroll
+    for (int k = wave; k < D * D * 4 / 1024; k += W) dma16(ra, smem + k * 1024, k * 1024 + lane * 16, 0);
     const uint8_t *perm = Tg + offsetof(DevTables, perm), *grp = Tg + offsetof(DevTables, group_of),
                   *pcb = Tg + offsetof(DevTables, pos_cb), *pbk = Tg + offsetof(DevTables, pos_book);
     const float *loff = reinterpret_cast<const float *>(Tg + offsetof(DevTables, lut_off)),
@@ -232,15 +235,6 @@ __device__ __forceinline__ void encode_tile_body(const EncodeTileJob &job, const
       const int p = f0 ? __builtin_ctzll(f0) : f1 ? 64 + __builtin_ctzll(f1) : 0;
       const float c = books[(int)pbk[p] * mc + (int)code];
       reinterpret_cast<u32x2 *>(smem + L.tab)[e] = u32x2{__float_as_uint(c * c), code};
-    }
-    const float *R = reinterpret_cast<const float *>(Tg + T->off_rot);
-    for (int e = tid; e < D * D / 4; e += TH) {
-      // Row j = 16 t + 4 r + q (operand row m = 4 q + r of tile t), columns
-      // i .. i + 3 (k = 0..3 of step i / 4).
-      const int j = e / (D / 4), i = 4 * (e % (D / 4)), t = j / 16, m = 4 * (j & 3) + ((j >> 2) & 3);
-      const f32x4 v = *reinterpret_cast<const f32x4 *>(R + j * D + i);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) a_op[((t * NT + i / 16) * 64 + 16 * k + m) * 4 + (i % 16) / 4] = v[k];
     }
     // Group masks (1 or 0): of the tree's leaves, as lane 4 b + i of the 4x4
     // blocks (16 lanes per gq) holds group i's; of the positions, as the A
@@ -266,6 +260,7 @@ __device__ __forceinline__ void encode_tile_body(const EncodeTileJob &job, const
         cnt[2 * e + 1] = c > 3 ? 1.0f : 0.0f;
       }
     }
+    wait_vm<0>();  // the rotation's DMAs
     __syncthreads();
   }
   // The 4-wide steps each tile of 16 positions needs, in groups of four.
