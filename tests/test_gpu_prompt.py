@@ -144,6 +144,23 @@ def test_lowest_values(device):
     assert torch.equal(out[70:], xd[70:71, 3:].expand(60, 2, 64))
 
 
+@pytest.mark.parametrize("sequences", [2, 63, 64, 65, 129])
+def test_every_tile_of_mixed_sequences(device, sequences):
+    """Lengths from none to many tiles of 128 rows, in any order: each row of each sequence is written once, whatever
+    order the tiles start in."""
+    import torch
+    from bgtq import batched
+    batched.bind_torch_stream(device)
+    dtype, dim, hq, hkv = "float16", 64, 2, 1
+    lens = [int(n) for n in np.random.RandomState(sequences).permutation([(37 * i * i) % 700 if i % 5 else 0 for i in range(sequences)])]
+    lens[sequences // 2] = 1300
+    x = _inputs(sum(lens), hq, hkv, dim, dtype, sequences)
+    xd, out = x.cuda(), torch.full((sum(lens), hq, dim), float("nan"), dtype=x.dtype, device="cuda")
+    batched.prompt_attention(device, xd[:, :hq], xd[:, hq:hq + hkv], xd[:, hq + hkv:], _offsets(lens), out)
+    torch.cuda.synchronize()
+    _check(out, x, lens, hq, hkv, dtype, 1 / 8, what=f"{sequences} sequences")
+
+
 def test_many_sequences_and_bad_offsets(device):
     """Thousands of short sequences (the search for a tile's sequence takes several rounds); offsets outside the rows
     are clamped to them."""
