@@ -1829,18 +1829,29 @@ bgtq_status bgtq_paged_read(bgtq_context *ctx, const bgtq_pages *g, const bgtq_p
   return BGTQ_OK;
 }
 
-// Workgroups of the paged decode that share a compute unit. 8-bit V at d=64 leaves
-// room for three (40 KB of LDS and 125 registers at layout B), and three hide
-// more of the loads' latency: 128 units x 32768 tokens 104.9 us with two (4
-// splits) / 100.6 (6), 96 units of none to 16384 tokens 43.6 (5) / 35.3 (8), 200
-// units x 8000 51 / 46; FP16 K, 96 x 16384 51.3 / 52.4. The per-position layouts'
-// lookups are bound by LDS (96 units x 16384 60.3 / 67.3); the other forms fit twice.
+// Workgroups of the paged decode that share a compute unit, by their LDS (d=64:
+// 40 KB at layout B with 8-bit V, 55 to 66 with FP16 V; d=128: 69 KB, and 86 to 131
+// of the other forms) and, per-position layouts, registers. us per call with
+// one more or fewer: d=64, 8-bit V, 128 units x 32768 tokens 100.6 (3) / 104.9 (2), 96
+// units of none to 16384 tokens 35.3 / 43.6; per-position 96 x 16384 60.3 (2) / 67.3
+// (3); d=128, FP16 V 64 x 8000 39.4 (1) / 45.6 (2), with FP16 K 48.4 / 51.7, FP16 K with
+// 8-bit V 38.5 / 42.8.
 static int paged_residents(const bgtq_pages *g, int nn) {
-  return g->dim == 64 && g->v_format == BGTQ_DTYPE_Q8 && nn >= 0 ? 3 : 2;
+  const bool q8 = g->v_format == BGTQ_DTYPE_Q8 && nn >= 0;
+  if (g->dim == 128) return q8 && g->key_format == BGTQ_KEYS_PACKED ? 2 : 1;
+  return q8 ? 3 : 2;
 }
 
 // Splits of a paged decode: the fused kernel's own choice, or the caller's.
-static bgtq_status plan_paged_decode(const bgtq_pages *g, const bgtq_paged_decode_desc *d, int *splits) {
+struct PagedSplits {
+  int splits;  // of a sequence; with a target, were all max_length long
+  int most;    // of a sequence at most
+  int target;  // workgroups per KV head, shared by the lengths; 0: `splits` of every sequence
+  // Partials per sequence and query head that the workspace has room for.
+  int room(int batch) const { return target ? (target + batch - 1) / batch : splits; }
+};
+
+static bgtq_status plan_paged_decode(const bgtq_pages *g, const bgtq_paged_decode_desc *d, PagedSplits *plan) {
   int nn = 0;
   if (bgtq_status s = check_pages(g, &nn)) return s;
   if (!d) return fail(BGTQ_ERR_RANGE, "null descriptor");
@@ -1860,7 +1871,8 @@ static bgtq_status plan_paged_decode(const bgtq_pages *g, const bgtq_paged_decod
   if (d->q_rotated && g->key_format != BGTQ_KEYS_PACKED) return fail(BGTQ_ERR_RANGE, "q_rotated needs packed K");
   const int64_t units = (int64_t)d->batch * g->kv_heads;
   if (d->splits > 0) {
-    *splits = choose_splits(units, d->max_length, d->splits);
+    const int s = choose_splits(units, d->max_length, d->splits);
+    *plan = {s, s, 0};
     return BGTQ_OK;
   }
   // Few units: past the splits that merge in one round of loads every further
@@ -1869,23 +1881,32 @@ static bgtq_status plan_paged_decode(const bgtq_pages *g, const bgtq_paged_decod
   // without it / 40 splits: layout B, 2 units x 32768 tokens 62.1 (256) / 17.9,
   // 8 units 34.1 (96) / 21.0, d=128, 4 units 40.6 (128) / 22.7.
   const double steps = d->max_length / 128.0;
-  const int most = std::max(kDecodeMergeOneRound, (int)std::sqrt(5.0 * steps));
-  *splits = std::min(fused_decode_splits(units, d->max_length, 0, paged_residents(g, nn)), most);
+  const int most = std::min(256, std::max(kDecodeMergeOneRound, (int)std::sqrt(5.0 * steps)));
+  const int resident = paged_residents(g, nn);
+  *plan = {std::min(fused_decode_splits(units, d->max_length, 0, resident), most), most, 0};
+  // Up to 64 sequences (a lane each) share those workgroups by their lengths.
+  // us, the same splits for all / by length: lengths from none up, 32 sequences of
+  // up to 16384 tokens (SmolLM2 heads) 58.5 / 40.3, 48 (layout B) 37.4 / 30.8, d=128 7
+  // of up to 16001 37.5 / 32.4; equal lengths 64 x 32768 105.0 / 105.6, 64 x 1000 13.2 / 13.1.
+  if (d->batch > 1 && d->batch <= 64 && plan->splits > 1) {
+    const int64_t slots = resident * (int64_t)device_cus(), rounds = (units * plan->splits + slots - 1) / slots;
+    plan->target = (int)(rounds * slots / g->kv_heads);
+  }
   return BGTQ_OK;
 }
 
 bgtq_status bgtq_paged_decode_workspace_size(const bgtq_pages *g, const bgtq_paged_decode_desc *d, size_t *bytes) {
-  int splits = 1;
-  if (bgtq_status s = plan_paged_decode(g, d, &splits)) return s;
+  PagedSplits plan;
+  if (bgtq_status s = plan_paged_decode(g, d, &plan)) return s;
   if (!bytes) return fail(BGTQ_ERR_RANGE, "null output");
-  *bytes = decode_ws((int64_t)d->batch * g->kv_heads, (int64_t)d->batch * d->q_heads, g->dim, splits).total;
+  *bytes = decode_ws((int64_t)d->batch * g->kv_heads, (int64_t)d->batch * d->q_heads, g->dim, plan.room(d->batch)).total;
   return BGTQ_OK;
 }
 
 bgtq_status bgtq_paged_decode(bgtq_context *ctx, const bgtq_pages *g, const bgtq_paged_decode_desc *d) {
-  int splits = 1;
-  if (bgtq_status s = plan_paged_decode(g, d, &splits)) return s;
-  const DecodeWorkspace w = decode_ws((int64_t)d->batch * g->kv_heads, (int64_t)d->batch * d->q_heads, g->dim, splits);
+  PagedSplits plan;
+  if (bgtq_status s = plan_paged_decode(g, d, &plan)) return s;
+  const DecodeWorkspace w = decode_ws((int64_t)d->batch * g->kv_heads, (int64_t)d->batch * d->q_heads, g->dim, plan.room(d->batch));
   if (!d->workspace || d->workspace_bytes < w.total) return fail(BGTQ_ERR_RANGE, "workspace of %zu bytes required", w.total);
   if (reinterpret_cast<uintptr_t>(d->workspace) % 16) return fail(BGTQ_ERR_RANGE, "workspace must be 16-byte aligned");
   if (!ctx) return fail(BGTQ_ERR_RANGE, "null context");
@@ -1907,7 +1928,7 @@ bgtq_status bgtq_paged_decode(bgtq_context *ctx, const bgtq_pages *g, const bgtq
   p.lengths = d->lengths;
   p.q_rotated = d->q_rotated;
   p.max_length = (int32_t)d->max_length;
-  p.splits = splits;
+  p.splits = plan.splits;
   p.splits_forced = d->splits > 0;
   p.inv_sqrt_d = (float)(1.0 / std::sqrt((double)g->dim));
   p.out = d->out;
@@ -1915,6 +1936,8 @@ bgtq_status bgtq_paged_decode(bgtq_context *ctx, const bgtq_pages *g, const bgtq
   int nn = 0, sg = 0;
   if (!pool_layout(p, g, &fl, &nn, &sg)) return fail(BGTQ_ERR_UNSUPPORTED, "pages hold the packed layouts of the fused decode");
   choose_waves(p, nn);
+  p.split_target = plan.target;
+  if (plan.target) p.splits = plan.most;
   HIP_TRY(launch_decode_fast(p, fl, nn, sg, ctx->stream), "paged decode launch");
   return BGTQ_OK;
 }

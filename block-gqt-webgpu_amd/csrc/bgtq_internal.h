@@ -278,6 +278,9 @@ struct DecodeParams {
   int32_t page_shift, table_pages, pages;
   const uint16_t *v_scales;
   int64_t v_scales_page_stride, v_scales_head_stride;  // elements
+  // Pages: workgroups per KV head that up to 64 sequences share by their
+  // lengths, `splits` of a sequence at most; 0: `splits` of every sequence.
+  int32_t split_target;
   // Workgroups per (sequence, KV head) or row-wise unit that take the
   // appended rows (packed K: decode 1; row-wise prefill one row per wave),
   // after the splits in the split dimension; each leaves one partial.

@@ -175,10 +175,11 @@ __device__ __forceinline__ float exp_of(float d) {
   return __builtin_amdgcn_exp2f(NAT ? d * kLog2e : d);
 }
 
+// part0: the first head's partial rows, S per head one after another.
 // PG: a head none of whose splits met a token gets zeros.
 template <int D, int SMAX, int NW, bool NAT, bool PG>
-__device__ __forceinline__ void merge_one_round(float *part, float *out, float *stats, int64_t head0, int G, int S,
-                                             int wave, int lane) {
+__device__ __forceinline__ void merge_one_round(float *part, float *out, float *stats, int64_t head0, int64_t part0, int G,
+                                             int S, int wave, int lane) {
   constexpr int kWaves = NW;
   static_assert(SMAX <= 64, "one split per lane");
   constexpr int DL = D / 64;  // dimensions per lane
@@ -191,7 +192,7 @@ __device__ __forceinline__ void merge_one_round(float *part, float *out, float *
       ms[h] = -INFINITY;
       ls[h] = 0.0f;
       if (g >= G) continue;
-      float *pp = part + (head0 + g) * S * (D + 2);
+      float *pp = part + (part0 + (int64_t)g * S) * (D + 2);
       if (lane < S) {
         ms[h] = coherent_load(pp + lane * (D + 2));
         ls[h] = coherent_load(pp + lane * (D + 2) + 1);
@@ -386,6 +387,43 @@ __device__ __forceinline__ void merge_rows(float *part, float *out, const MergeR
   "s"((int)fl.gnb[kv]), "s"((int)fl.gbstride[kv]), "s"((int)fl.gbnib[kv]), "s"(fl.gpair[kv]),                  \
   "s"((int)fl.grb[kv]), "s"((int)fl.gns[kv]));
 
+// Pages, p.split_target set: which sequence and split of it grid y stands
+// for. A workgroup's unit of work is a step, the 2^SHIFT tokens that its
+// waves take at a time. With t steps to a workgroup, sequence b takes
+// n_b = ceil(steps_b / t) of them (one if it is empty); t is raised from the
+// sum's share in proportion to the excess, three times at most, until they
+// are at most p.split_target. They are at most split_target + batch in any
+// case, the grid: sum ceil(x) < sum x + batch. Every workgroup finds the same
+// from all the lengths, a lane per sequence.
+struct PagedPlace {
+  int b, split, first, splits;  // splits 0: nothing to do; first: the sequence's first y
+};
+template <int SHIFT>
+__device__ __forceinline__ PagedPlace paged_place(const DecodeParams &p, int y) {
+  const int lane = threadIdx.x & 63;
+  const uint32_t len = p.lengths[min(lane, p.batch - 1)];
+  const int steps = lane < p.batch ? (int)((min(len, (uint32_t)p.max_length) + (1u << SHIFT) - 1) >> SHIFT) : 0;
+  const float target = (float)p.split_target;
+  float t = fmaxf(1.0f, ceilf((float)wave_sum(steps) / target));
+  // (the thousandth: a quotient that is whole stays so through the reciprocal)
+  auto splits = [&] {
+    const int n = (int)ceilf((float)steps * __builtin_amdgcn_rcpf(t) - 1e-3f);
+    return lane < p.batch ? max(1, min(n, p.splits)) : 0;
+  };
+  int n = splits();
+  for (int k = 0; k < 3; ++k) {
+    const float all = (float)wave_sum(n);
+    if (all <= target) break;
+    t = fmaxf(t + 1.0f, ceilf(t * all / target));
+    n = splits();
+  }
+  const int end = wave_prefix(n);
+  const uint64_t at = __builtin_amdgcn_ballot_w64(y >= end - n && y < end);
+  if (at == 0) return {0, 0, 0, 0};
+  const int b = __builtin_ctzll(at), s = __builtin_amdgcn_readlane(n, b), first = __builtin_amdgcn_readlane(end, b) - s;
+  return {b, y - first, first, s};
+}
+
 // AP: what a launch does beside attention, compiled in only where used: 0
 // nothing, 1 the appended rows (decode or prefill append), 2 materialised
 // logits (inspect()), 3 K and V in pages (decode; a sequence may be empty).
@@ -428,8 +466,15 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
   // every history has, spread over all XCDs (split fastest put every unit's
   // split 0 on one XCD), and an XCD's units share one KV head's history.
   // qrow: the sequence (PF: b * qgroups + query group).
-  const int split = PF ? blockIdx.z : blockIdx.x, kv = PF ? blockIdx.x : blockIdx.y,
-            qrow = PF ? blockIdx.y : blockIdx.z;
+  // Pages: with p.split_target (KV head, y), see paged_place.
+  const int kv = PF || (PG && p.split_target) ? blockIdx.x : blockIdx.y;
+  PagedPlace pg_at{(int)blockIdx.z, (int)blockIdx.x, 0, p.splits};
+  if constexpr (PG)
+    if (p.split_target) {
+      pg_at = paged_place<(NW == 8 ? 8 : 7)>(p, blockIdx.y);
+      if (pg_at.splits == 0) return;
+    }
+  const int split = PF ? blockIdx.z : PG ? pg_at.split : blockIdx.x, qrow = PF ? blockIdx.y : PG ? pg_at.b : blockIdx.z;
   // Every kernel argument the set-up reads, in one round trip (with the
   // role chosen by the kernel, already loaded there).
   BGTQ_LOAD_ARGS
@@ -525,7 +570,7 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
   // Pages: chunk i's page from the sequence's table, looked up two chunks
   // ahead (chunks past the table's end read its last entry and stream
   // nothing). A vector load, older than the loads of the chunk before its own.
-  const int first_pg = (split * kWaves + wave) * kChunk, stride_pg = p.splits * kWaves * kChunk;
+  const int first_pg = (split * kWaves + wave) * kChunk, stride_pg = pg_at.splits * kWaves * kChunk;
   auto load_page = [&](int i) -> int {
     const int at = min((first_pg + i * stride_pg) >> p.page_shift, p.table_pages - 1);
     return p.page_table[(int64_t)b * p.page_table_stride + at];
@@ -677,7 +722,8 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
   const int part = split - p.splits;
   const bool app_wg = RL == 2 || (RL == 0 && app && part >= 0);
   const int sf = p.split_floor;
-  const int S_hist = !rowwise ? p.splits
+  const int S_hist = PG         ? pg_at.splits
+                     : !rowwise ? p.splits
                      : app    ? min(p.splits, (start_c + sf - 1) / sf)
                               : min(p.splits, max(1, (T_b + sf - 1) / sf));
   if (rowwise && !app_wg && split >= S_hist) {
@@ -689,6 +735,9 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
   // launch use different split counts; each column's rows start at the same
   // stride, so units never share rows).
   const int SP = p.splits + (app ? p.app_parts : 0);
+  // Decode: this unit's partial rows (S per head); pages, in the order of grid y.
+  const int64_t part0 = PG && p.split_target ? ((int64_t)kv * gridDim.y + pg_at.first) * p.G
+                                             : ((int64_t)qrow * p.q_heads + kv * p.G) * S;
   const int pslot = app_wg ? S_hist + part : split;  // this workgroup's partial
   // Prefill append workgroup: its rows r_a .. r_a + n_a - 1 of the chunk.
   // (ER rows per wave: a wave encodes them side by side)
@@ -1907,7 +1956,7 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
       } else {
         // Device-coherent (write-through) stores: the merging workgroup may run
         // on another XCD, whose L2 does not see this one's.
-        float *pp = p.part + (head * S + pslot) * (D + 2);
+        float *pp = p.part + (part0 + (int64_t)g * S + pslot) * (D + 2);
         coherent_store(pp + 2 + dm, Ov);
         if (dm == 0) {
           coherent_store(pp, M);
@@ -2003,10 +2052,11 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
     return;
   }
   if (S <= kMergeOneRound) {
-    if (S <= 8) merge_one_round<D, 8, NW, NAT, PG>(p.part, p.out, p.stats, (int64_t)qrow * Hq + hq0, G, S, wave, lane);
-    else if (S <= 16) merge_one_round<D, 16, NW, NAT, PG>(p.part, p.out, p.stats, (int64_t)qrow * Hq + hq0, G, S, wave, lane);
-    else if (S <= 24) merge_one_round<D, 24, NW, NAT, PG>(p.part, p.out, p.stats, (int64_t)qrow * Hq + hq0, G, S, wave, lane);
-    else merge_one_round<D, kMergeOneRound, NW, NAT, PG>(p.part, p.out, p.stats, (int64_t)qrow * Hq + hq0, G, S, wave, lane);
+    const int64_t head0 = (int64_t)qrow * Hq + hq0;
+    if (S <= 8) merge_one_round<D, 8, NW, NAT, PG>(p.part, p.out, p.stats, head0, part0, G, S, wave, lane);
+    else if (S <= 16) merge_one_round<D, 16, NW, NAT, PG>(p.part, p.out, p.stats, head0, part0, G, S, wave, lane);
+    else if (S <= 24) merge_one_round<D, 24, NW, NAT, PG>(p.part, p.out, p.stats, head0, part0, G, S, wave, lane);
+    else merge_one_round<D, kMergeOneRound, NW, NAT, PG>(p.part, p.out, p.stats, head0, part0, G, S, wave, lane);
     if (tid == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     return;
   }
@@ -2017,7 +2067,7 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
   float *mrow = wgt + 16 * S;                     // [16 heads][S] split maxima
   for (int e = tid; e < ncol * S; e += kThreads) {
     const int g = e / S, s = e - g * S;
-    float *pp = p.part + ((pbase + g) * S + s) * (D + 2);
+    float *pp = p.part + (part0 + g * S + s) * (D + 2);
     mrow[g * S + s] = coherent_load(pp);
     wgt[g * S + s] = coherent_load(pp + 1);
   }
@@ -2043,7 +2093,7 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
   for (int e = tid; e < ncol * D; e += kThreads) {
     const int g = e / D, dm = e - g * D;
     const int64_t head = out_row(g);
-    float *pp = p.part + (pbase + g) * S * (D + 2) + 2 + dm;
+    float *pp = p.part + (part0 + (int64_t)g * S) * (D + 2) + 2 + dm;
     float Ov = 0.0f;
     constexpr int MG = PG ? 32 : 8;
     for (int s0 = 0; s0 < S; s0 += MG) {
@@ -2101,7 +2151,9 @@ hipError_t launch_mode(const DecodeParams &p, const FastLayout &fl, hipStream_t 
   // head) or unit for them.
   const unsigned app = KF >= 1 && p.k_new ? (unsigned)p.app_parts : 0u;
   const dim3 grid = PF ? dim3((unsigned)p.kv_heads, (unsigned)(p.batch * p.qgroups), (unsigned)p.splits + app)
-                       : dim3((unsigned)p.splits + app, (unsigned)p.kv_heads, (unsigned)p.batch);
+                    : AP == 3 && p.split_target
+                        ? dim3((unsigned)p.kv_heads, (unsigned)(p.split_target + p.batch))
+                        : dim3((unsigned)p.splits + app, (unsigned)p.kv_heads, (unsigned)p.batch);
   hipLaunchKernelGGL((decode_fast_kernel<D, KF, NN, SG, PK, PF, VF, NW, AP>), grid, dim3(64 * NW), lds, stream, p, fl);
   return hipGetLastError();
 }

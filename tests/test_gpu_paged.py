@@ -405,6 +405,32 @@ def test_decode_long(device, oracle):
         pool.destroy()
 
 
+@pytest.mark.parametrize("layout,v,dim,heads", [("B", "q8", 64, 2), ("f16", "f16", 128, 1), ("S", "q8", 64, 3)])
+@pytest.mark.parametrize("batch", [2, 31, 64, 65])
+def test_decode_workgroups_shared_by_length(device, oracle, layout, v, dim, heads, batch):
+    """Sequences share the workgroups by their lengths: one long among short ones, mixed, equal, and none at all,
+    in one workspace; lengths beyond max_length count as it."""
+    import torch
+    rng = np.random.RandomState(batch)
+    longest = 6000 if batch == 2 else 2500
+    kinds = {"one long": [longest] + [int(n) for n in rng.randint(0, 40, batch - 1)],
+             "mixed": [int(longest * (i / batch) ** 3) for i in range(batch)],
+             "equal": [700] * batch, "short": [1] * batch, "none": [0] * batch}
+    need = max(sum(-(-n // 128) for n in lens) for lens in kinds.values())
+    pool = Pool(device, layout, v, dim, heads, need + 1, 128)
+    _fill(pool, batch)
+    q = _rows(batch, heads * 3, dim, "float32", batch, scale=1.5).cuda()
+    for kind, lens in kinds.items():
+        lens = [int(n) for n in rng.permutation(lens)]
+        print(layout, dim, batch, kind, flush=True)
+        table = _table(pool, lens, rng, spare=longest // 128 + 1)
+        _check(_decode(pool, q, lens, table, max_length=longest), _reference(pool, oracle, q, lens, table), kind)
+    short = [min(n, 300) for n in kinds["mixed"]]
+    table = _table(pool, kinds["mixed"], rng)
+    _check(_decode(pool, q, kinds["mixed"], table, max_length=300), _reference(pool, oracle, q, short, table), "clamped")
+    pool.destroy()
+
+
 @pytest.mark.parametrize("layout,dim", [("S", 64), ("B", 64), ("B", 128), ("f16", 64)])
 def test_decode_of_tiny_queries(device, oracle, layout, dim):
     """Queries down to the smallest FP32 numbers give all but equal weights, and none NaN; zeros the mean."""
