@@ -32,6 +32,14 @@
 //             its (sequence, KV head) to arrive (a device-scope counter)
 //             merges them by log-sum-exp and resets the counter to zero.
 //
+// Pages (AP 3, 8-bit V VF 3; instances in decode_paged_*.hip): a chunk's page
+// comes from the sequence's table two chunks ahead, up to 64 sequences share
+// the workgroups by their lengths (paged_place), and the loop takes fewer
+// vector instructions (PAIRED, LATE). 64 x 32768 tokens, 14 / 2 heads of layout B
+// with 8-bit V, 99 to 104 us (495 MB, 4.8 to 5.0 TB/s): vector instructions (64% of
+// the SIMDs' time) and the lookups' LDS traffic (57%, a third of it bank
+// conflicts) beside the stream.
+//
 // The arithmetic is that of src/reference/attention.py:5-22 on the
 // reconstructed K of src/reference/production_math.py:27-31: with
 // k = ((c*s) @ R)[inv_perm], q.k = sum_g s_g sum_{j in g} c_j[code_j] (R q[perm])_j.

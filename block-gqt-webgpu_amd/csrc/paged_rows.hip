@@ -11,7 +11,10 @@
 // with both operands split into FP16 hi and lo parts (three products, 2^-22
 // relative). A lane rebuilds the eight consecutive positions that it feeds the
 // product and ends with four consecutive dimensions of its row. The rotation's
-// operands lie in LDS, once per workgroup.
+// operands lie in LDS, once per workgroup. HBM's writes bound it: 131,072 rows x 2
+// heads of layout B with 8-bit V to FP32 39.9 us (166 MB, 4.2 TB/s; a copy reaches
+// 5.0); 4001 rows x 3 heads of the SmolLM2 tables 6.6 us, the chain of one tile.
+// A write of one row x 3 heads takes 4.4 us, of 16,384 x 2 (tile encoder) 13.
 #include <hip/hip_fp16.h>
 
 #include <type_traits>

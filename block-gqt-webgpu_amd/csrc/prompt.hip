@@ -17,6 +17,13 @@
 // The running maximum is raised only when a block's exceeds it by more than 8
 // in the log2 domain: probabilities then reach 2^8 at most, in range of either
 // type, and most blocks skip the rescale of O.
+//
+// Measured: 11 prompts of 568 to 2777 tokens, 14 / 2 heads of d=64, 85 us (760
+// TFLOP/s), one of 8192 tokens, 16 / 4 heads of d=128, 258 us (1065 TFLOP/s; a bf16
+// product of 8192^3 reaches 1249). A wave's block is 512 cycles of products and
+// 870 of softmax at d=64 (1024 at d=128), of which 512 are exponentials (a quarter
+// of the vector rate): the vector unit bounds d=64 (72% busy), the matrix cores
+// d=128 (53%), and what the waves of a SIMD do not overlap of the two.
 #include <type_traits>
 
 #include "bgtq_internal.h"
