@@ -1,6 +1,7 @@
 // Rows of V and FP16 K into a pool of pages: D / 8 lanes per row, eight values
 // each, so a row is one coalesced access and its maximum takes three or four
-// lane rotations. 8-bit V: s = max|v| / 127 rounded up to FP16 and c = v / s
+// lane rotations. 8-bit V: s = max|v| / 127 rounded up to FP16, at most 515.5 (the
+// largest whose 127-fold is an FP16 value), and c = v / s
 // rounded to the nearest integer, ties to even. v and s have 11 significant
 // bits, so a quotient that is no tie lies at least 2^-12 from every tie: the
 // correctly rounded FP32 quotient decides as the exact one does. That quotient
@@ -61,6 +62,8 @@ __device__ __forceinline__ void load8_half(const void *src, int dtype, bool vec,
   }
 }
 
+constexpr uint16_t kMaxScale = 0x6007u;  // 515.5 in FP16
+
 // Maximum over the L = 8 or 16 lanes that share a row.
 template <int L>
 __device__ __forceinline__ int lanes_max(int v) {
@@ -104,10 +107,13 @@ __device__ __forceinline__ void write_rows(const PagedWriteParams &p, int only, 
 #pragma unroll
     for (int k = 0; k < 8; ++k) top = max(top, (int)(h[k] & 0x7fffu));  // FP16 magnitudes order as their bits do
     top = lanes_max<L>(top);
-    // s: rounded to nearest, then up where 127 s would fall short of the maximum.
+    // s: rounded to nearest, then up where 127 s would fall short of the maximum;
+    // 515.5 at most (maxima of 65472 and 65504: 127 times 516 would round to an
+    // infinity, and 65504 / 515.5 still rounds to 127).
     const float most = f16_bits_to_f32((uint16_t)top);
     uint16_t s = f32_to_f16_bits(most / 127.0f);
     if (f16_bits_to_f32(s) * 127.0f < most) ++s;
+    s = s < kMaxScale ? s : kMaxScale;
     const bool finite = top < 0x7c00;
     const float sf = f16_bits_to_f32(s), rcp = s ? 1.0f / sf : 0.0f;
     uint32_t w[2] = {0u, 0u};

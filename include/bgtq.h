@@ -400,7 +400,8 @@ bgtq_status bgtq_prefill_append(bgtq_context *ctx, const bgtq_prefill_desc *d, c
  * K: BGTQ_KEYS_PACKED (tables[kv]; each head's own row bytes and norm stride)
  * or BGTQ_KEYS_FP16. V: BGTQ_DTYPE_F16, or BGTQ_DTYPE_Q8: a row of int8 codes
  * c and one FP16 scale s, standing for the FP16 values nearest s c. s is
- * max|v| / 127 rounded up to FP16 (so no code passes 127), c = v / s rounded to
+ * max|v| / 127 rounded up to FP16, at most 515.5 (so no code passes 127 and no
+ * finite value reads back as an infinity), c = v / s rounded to
  * the nearest integer, ties to even, of the row rounded to FP16; a row with an
  * infinity or a NaN gets a NaN scale and reads back as NaN.
  * dim 64 or 128; page_tokens a power of two, 32 to 4096; pages at most 2^31 - 1;

@@ -699,3 +699,54 @@ def test_prompts_to_pages_to_steps(device, oracle):
         torch.cuda.synchronize()
         _check(o, _reference(pool, oracle, q, lengths, table), f"step {step}")
     pool.destroy()
+
+
+@pytest.mark.parametrize("layout,dim,heads", [("B", 64, 2), ("B", 128, 2), ("f16", 64, 3)])
+@pytest.mark.parametrize("rows,dtype", [(20, "float32"), (6000, "float16"), (6001, "float32")])
+def test_largest_values_in_8_bits_stay_finite(device, oracle, layout, dim, heads, rows, dtype):
+    """Rows up to FP16's largest value: the scale is at most 515.5 (516 times 127 rounds to an infinity), codes pass no
+    127, every value comes back finite and within half a scale (and its FP16 rounding), and the decode over them is finite."""
+    import torch
+    from bgtq import batched
+    print(layout, dim, rows, dtype, flush=True)
+    pages = -(-rows // 32) + 1
+    pool = Pool(device, layout, "q8", dim, heads, pages, 32)
+    k, v = _rows(rows, heads, dim, dtype, 1), _rows(rows, heads, dim, dtype, 2).clamp(-4, 4) * 15000.0
+    tops = [65504.0, -65504.0, 65472.0, -65472.0, 65440.0, 65408.0, 32752.0]
+    tops += [65519.0, 65488.0, 65456.0] if dtype == "float32" else []  # these round to FP16's last values
+    for i in range(0, rows, 2):
+        v[i, i % heads, i % dim] = tops[i // 2 % len(tops)]
+    slots = torch.arange(rows, device="cuda")
+    batched.paged_write(device, pool.handle, slots, k.cuda(), v.cuda())
+    torch.cuda.synchronize()
+    v16 = v.half().numpy()
+    assert np.all(np.isfinite(v16))
+    pg, at = np.divmod(np.arange(rows), 32)
+    got = {}
+    for out in ("float32", "float16", "bfloat16"):
+        got[out] = torch.empty((rows, heads, dim), dtype=getattr(torch, out), device="cuda")
+        batched.paged_read(device, pool.handle, slots, v=got[out])
+    torch.cuda.synchronize()
+    for h in range(heads):
+        _, s = _quantise(v16[:, h])
+        s = np.minimum(s, np.float16(515.5)).astype(np.float64)
+        codes = np.rint(v16[:, h].astype(np.float64) / s[:, None])
+        assert np.abs(codes).max() == 127
+        assert np.array_equal(pool.v_scales[:, h].cpu().numpy()[pg, at].astype(np.float64), s)
+        assert np.array_equal(pool.v[:, h].cpu().numpy()[pg, at].astype(np.float64), codes)
+        value = (codes * s[:, None]).astype(np.float16)
+        assert np.all(np.isfinite(value))
+        for out, x in got.items():
+            assert torch.equal(x[:, h].cpu(), torch.from_numpy(value).to(x.dtype)), f"{out} V of head {h}"
+        err = np.abs(value.astype(np.float64) - v16[:, h].astype(np.float64))
+        assert np.all(err <= s[:, None] / 2 + np.abs(value.astype(np.float64)) * 2.0 ** -11)
+    table = torch.arange(pages, dtype=torch.int32, device="cuda")[None]
+    q = _rows(1, heads * 3, dim, "float32", 4).cuda()
+    out = _decode(pool, q, [rows], table)
+    torch.cuda.synchronize()
+    ref = _reference(pool, oracle, q, [rows], table)
+    assert np.all(np.isfinite(ref))
+    # values up to 2^16 of either sign cancel: the tolerance is relative to what is summed
+    err = np.abs(out.double().cpu().numpy() - ref)
+    assert np.all(err <= ATOL + RTOL * 65504.0), f"max err {err.max():.3e}"
+    pool.destroy()
