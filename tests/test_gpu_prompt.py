@@ -223,3 +223,48 @@ def test_wrapper_refusals(device):
         with pytest.raises((bgtq.RangeError, bgtq.UnsupportedError)):
             batched.prompt_attention(device, **{**ok, **bad})
     batched.prompt_attention(device, x[:0, :2], x[:0, 2:3], x[:0, 3:], off[:1], x[:0, :2].clone())  # nothing to do
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("sink,n", [(0, 9000), (4500, 9000), (17, 300), (None, 4096)])
+def test_many_small_weights_beside_a_large_one(device, dtype, dim, sink, n):
+    """A key whose weight is 2^15 to 2^30 times every other's and whose V is zero: the others are the output. (None:
+    logits that rise by 3.5 in the log2 domain from block to block of 64 keys, V random.)
+
+    A weight p (of a sum of 1) is off by half a step u p of its type, an FP16 one below 2^-25 of the largest by 2^-36:
+    u (sum p |v| + |ref|) + 2^-36 (sum |v| + n |ref|) with the sum's; the logits (below 32) and sums in FP32 by
+    2^-14 of the same; the output's own rounding is u |ref|, FP16 2^-25 where it is subnormal."""
+    import torch
+    from bgtq import batched
+    batched.bind_torch_stream(device)
+    print(dtype, dim, sink, n, flush=True)
+    gaps = [15.0, 20.5, 21.5, 25.0, 28.0, 30.0]
+    hq, typ, g = len(gaps), getattr(torch, dtype), torch.Generator().manual_seed(n + dim)
+    q, k, v = (torch.zeros((n, h, dim)) for h in (hq, 1, 1))
+    q[:, :, 0] = torch.tensor(gaps) * np.log(2.0) / 4
+    k[:, 0, 0] = 0.02 * torch.randn(n, generator=g)
+    if sink is None:
+        q[:, :, 0] = 3.5 * np.log(2.0) * torch.linspace(0.4, 1, hq)
+        k[:, 0, 0] = (torch.arange(n) // 64) % 8
+        v.normal_(generator=g)
+    else:
+        v[:, 0] = 1 + 0.25 * torch.rand((n, dim), generator=g)
+        k[sink, 0, 0], v[sink] = 4, 0
+    q, k, v = q.to(typ), k.to(typ), v.to(typ)
+    out = torch.empty((n, hq, dim), dtype=typ, device="cuda")
+    batched.prompt_attention(device, q.cuda(), k.cuda(), v.cuda(), _offsets([n]), out, scale=1.0)
+    torch.cuda.synchronize()
+    q, k, v, got = (x.double().cpu().numpy() for x in (q, k, v, out))
+    u = U[dtype]
+    for row in sorted({0, 1, 16, 17, 18, 63, 64, 128, n // 2 - 1, n // 2, n // 2 + 1, 3 * n // 4, n - 1}):
+        s = q[row, :, 0, None] * k[None, :row + 1, 0, 0]
+        p = np.exp(s - s.max(-1, keepdims=True))
+        p /= p.sum(-1, keepdims=True)
+        x = v[:row + 1, 0]
+        ref, size = p @ x, p @ np.abs(x)
+        lim = (u + 2.0 ** -14) * (size + np.abs(ref)) + u * np.abs(ref) * 1.001
+        if dtype == "float16":
+            lim += 2.0 ** -36 * (np.abs(x).sum(0) + (row + 1) * np.abs(ref)) + 2.0 ** -25
+        err = np.abs(got[row] - ref)
+        assert np.all(err <= lim), f"row {row}: {np.max(err / lim):.1f} of the limit, heads {np.max(err / lim, -1).round(2)}"
