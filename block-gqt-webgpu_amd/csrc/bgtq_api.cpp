@@ -466,6 +466,9 @@ bgtq_status bgtq_tables_create(bgtq_context *ctx, const uint32_t *integer, size_
   float cmax = 0.0f;
   for (int64_t i = 0; i < d * mc; ++i) cmax = std::max(cmax, std::fabs(cent[i]));
   T->cent_exp = cmax > 0.0f ? 14 - (int32_t)std::ceil(std::log2(cmax)) : 0;
+  float rmax = 1.0f;  // (of an orthogonal rotation at most; no table has to hold one)
+  for (int64_t i = 0; i < d * d; ++i) rmax = std::max(rmax, std::fabs(rot[i]));
+  T->rot_exp = 14 - (int32_t)std::ceil(std::log2(rmax));
   for (int64_t j = 0; j < d; ++j) {
     T->perm[j] = (uint8_t)perm[j];
     T->group_of[j] = (uint8_t)group_of[j];
@@ -588,7 +591,7 @@ bgtq_status bgtq_tables_create(bgtq_context *ctx, const uint32_t *integer, size_
           }
     };
     operands(off_rot_q, [&](int64_t row, int64_t col) { return rq[row * d + col]; });
-    operands(off_rot_k, [&](int64_t row, int64_t col) { return rq[col * d + row] * 16384.0f; });
+    operands(off_rot_k, [&](int64_t row, int64_t col) { return std::ldexp(rq[col * d + row], T->rot_exp); });
     if (d == 64 || d == 128) {
       // Row j = 16 t + 4 r + q is operand row m = 4 q + r of tile t; column
       // 16 n + 4 i + k is k of step i of columns n.
@@ -1745,7 +1748,7 @@ PagedWriteParams rows_params(const bgtq_pages *g, const bgtq_paged_rows *r) {
       const DevTables *T = g->tables[h]->h();
       p.heads[h] = {(int32_t)T->off_rot, T->off_rot_t, T->off_rot_k, T->off_gdesc, T->off_books, (int16_t)T->row_bytes,
                     (int16_t)T->norm_stride, (int16_t)T->max_centroids, (int16_t)T->n_books, (int16_t)T->groups,
-                    (int16_t)T->cent_exp};
+                    (int16_t)T->cent_exp, (int16_t)T->rot_exp};
     }
     p.packed = g->packed;
     p.packed_page_stride = g->packed_page_stride;

@@ -22,6 +22,7 @@ struct DevTables {
   int32_t gstart[kMaxGroups], gend[kMaxGroups], gsize[kMaxGroups];  // group ranges (head-perm order)
   uint32_t off_lut, off_books, off_rot, off_rot_t, off_mfma, off_rot_q, off_gdesc, off_glane, off_rot_k, off_rot_a, total_bytes;
   int32_t cent_exp;  // 2^cent_exp * max|centroid| <= 2^14: fp16 hi/lo split range for MFMA operands
+  int32_t rot_exp;   // the same of the rotation's entries for off_rot_k, at most 14
   // The fused decode of any packed layout: its leading pair K-steps (see
   // off_glane) and the books whose pair tables it keeps in LDS for them
   // (byte i = book of pair slot i, 0xff = unused).
@@ -49,7 +50,7 @@ struct DevTables {
   //             Rq[16 n + l % 16][32 s + 8 (l / 16) + 0..7] (kRotQBytes).
   // [off_rot_a] (dim 64, 128) R as the tile encoder's FP32 A operands
   //             ([16-row tile][16 columns][lane][4]), as they lie in its LDS.
-  // [off_rot_k] the transpose of Rq times 2^14 in the same operand form
+  // [off_rot_k] the transpose of Rq times 2^rot_exp in the same operand form
   //             (16-row tile n of dimensions, 32-position step s), for the
   //             rows read back from pages: k = Rq^T (c s).
   // [off_gdesc] per head-perm position j, for the fused decode of any packed
@@ -190,7 +191,7 @@ struct PagedWriteParams {
   struct Head {
     int32_t enc_bytes;  // bytes of the table set's header, code LUT and books
     uint32_t off_rot_t, off_rot_k, off_gdesc, off_books;
-    int16_t row_bytes, norm_stride, max_centroids, books, groups, cent_exp;
+    int16_t row_bytes, norm_stride, max_centroids, books, groups, cent_exp, rot_exp;
   } heads[kMaxKvHeads];
   uint8_t *packed;
   int64_t packed_page_stride, packed_head_stride;  // bytes

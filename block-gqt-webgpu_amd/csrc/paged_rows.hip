@@ -430,7 +430,7 @@ __global__ __launch_bounds__(64 * Read<D>::W, D == 64 ? 3 : 2) void paged_read_p
       }
       split8_mix(cs, one, bh[s], bl[s]);
     }
-    const float unscale = __builtin_ldexpf(1.0f, -ex - 14);
+    const float unscale = __builtin_ldexpf(1.0f, -ex - H.rot_exp);
     // The products of a 128-byte piece of every row, through LDS to whole lines.
     constexpr int N = Out<D, OUT>::kN, TP = 8 * N / 16;  // column tiles of a piece
 #pragma unroll

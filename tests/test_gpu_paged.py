@@ -750,3 +750,37 @@ def test_largest_values_in_8_bits_stay_finite(device, oracle, layout, dim, heads
     err = np.abs(out.double().cpu().numpy() - ref)
     assert np.all(err <= ATOL + RTOL * 65504.0), f"max err {err.max():.3e}"
     pool.destroy()
+
+
+@pytest.mark.parametrize("layout,dim", [("B", 64), ("A", 64), ("B", 128)])
+@pytest.mark.parametrize("factor", [1.0, 3.7, 6.0, 300.0, 0.02])
+def test_rotations_that_are_not_orthogonal(device, oracle, layout, dim, factor):
+    """Tables take any finite transform: rows under a scaled one are written, read back and attended to as the
+    definition has them, entries of any size."""
+    import dataclasses
+    import torch
+    import bgtq
+    from bgtq import batched
+    print(layout, dim, factor, flush=True)
+    pool = Pool(device, layout, "q8", dim, 2, 9, 32)
+    pool.destroy()
+    p = dataclasses.replace(pool.params[0], rotation=(np.asarray(pool.params[0].rotation) * np.float32(factor)).astype(np.float32))
+    pool.params, pool.tables = [p, p], [bgtq.Tables(device, p) for _ in range(2)]
+    pool.handle = batched.pages(page_tokens=32, tables=pool.tables, packed=pool.packed, norms=pool.norms, v=pool.v, v_scales=pool.v_scales)
+    n = 9 * 32
+    slots = np.arange(n)
+    k, v = _rows(n, 2, dim, "float16", 5), _rows(n, 2, dim, "float16", 6)
+    batched.paged_write(device, pool.handle, torch.arange(n, device="cuda"), k.cuda(), v.cuda())
+    torch.cuda.synchronize()
+    _check_write(pool, oracle, slots, k, v)
+    for out in ("float32", "bfloat16"):
+        ko, vo = (torch.empty((n, 2, dim), dtype=getattr(torch, out), device="cuda") for _ in range(2))
+        batched.paged_read(device, pool.handle, torch.arange(n, device="cuda"), ko, vo)
+        torch.cuda.synchronize()
+        _check_read(pool, oracle, slots, ko, vo)
+    q = (_rows(1, 6, dim, "float32", 7) / max(1.0, factor)).cuda()  # (logits of a few units)
+    table = torch.arange(9, dtype=torch.int32, device="cuda")[None]
+    out = _decode(pool, q, [270], table)
+    torch.cuda.synchronize()
+    _check(out, _reference(pool, oracle, q, [270], table))
+    pool.destroy()
