@@ -64,9 +64,6 @@ constexpr int kThreads = 64 * kWaves;
 constexpr int kChunk = 32;  // tokens per wave iteration: two 16-token MFMA tiles
 constexpr int kRing = 2;    // LDS chunk buffers per wave: compute one, the next in flight
 constexpr bool kInterleaved = true;
-// Pages: queries are scaled up by at most 2^100, which FP32 holds (smaller ones
-// than 2^-86 keep fewer bits of logits that are nothing to a softmax).
-constexpr int kMaxQueryExp = 100;
 constexpr int kMergeOneRound = kDecodeMergeOneRound;
 
 // Kinds of launch of the fused kernel. Each kind's instances can sit in a
@@ -1085,7 +1082,7 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
       for (int s = 0; s < KS; ++s)
 #pragma unroll
         for (int jv = 0; jv < 8; ++jv) qmax = fmaxf(qmax, fabsf(qv[s][jv]));
-      const int e0 = PG ? min(split_exp(col_max(qmax)), kMaxQueryExp) : split_exp(col_max(qmax));
+      const int e0 = split_exp(col_max(qmax));
       half8 bh[KS], bl[KS];
 #pragma unroll
       for (int s = 0; s < KS; ++s) split_scaled(qv[s], __builtin_ldexpf(1.0f, e0), bh[s], bl[s]);
@@ -1145,8 +1142,7 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
         qmax = fmaxf(qmax, fabsf(v));
       }
     qmax = col_max(qmax);
-    int eq = qmax > 0.0f ? 14 - (int)ceilf(__builtin_log2f(qmax)) : 0;
-    if constexpr (PG) eq = min(eq, kMaxQueryExp);
+    const int eq = split_exp(qmax);
     const float qsc = __builtin_ldexpf(1.0f, eq);
 #pragma unroll
     for (int s = 0; s < KS; ++s)

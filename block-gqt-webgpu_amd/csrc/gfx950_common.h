@@ -193,7 +193,12 @@ __device__ __forceinline__ void split_scaled(const float *x, float sc, half8 &hi
 }
 
 // Exponent e with max * 2^e near 2^14 (fp16 hi/lo split range); 0 for max 0.
-__device__ __forceinline__ int split_exp(float mx) { return mx > 0.0f ? 14 - (int)ceilf(__builtin_log2f(mx)) : 0; }
+// At most 100, so that FP32 holds 2^e: queries below 2^-86 keep fewer bits of
+// logits that are nothing to a softmax.
+constexpr int kMaxSplitExp = 100;
+__device__ __forceinline__ int split_exp(float mx) {
+  return mx > 0.0f ? min(14 - (int)ceilf(__builtin_log2f(mx)), kMaxSplitExp) : 0;
+}
 
 // Relaxed atomics at device scope: on gfx950 they go to the device-coherent
 // level (system-coherent bit) instead of this XCD's L2.

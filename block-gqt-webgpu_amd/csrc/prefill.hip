@@ -520,7 +520,7 @@ prefill_kernel(PrefillParams p, FastLayout fl) {
       }
     }
 #pragma unroll
-    for (int cb = 0; cb < NCB; ++cb) eqs[cb] = eq[cb] + ec;
+    for (int cb = 0; cb < NCB; ++cb) eqs[cb] = min(eq[cb] + ec, kMaxSplitExp);  // (the factor of a masked logit: not 2^-150, which is 0)
     if constexpr (D != 64) {
 #pragma unroll
       for (int i = 0; i < AHEAD; ++i)
