@@ -445,7 +445,8 @@ typedef struct {
   int64_t v_row_stride, v_head_stride;
 } bgtq_paged_rows;
 /* Writes rows into the pool, K first rounded to FP16 and encoded as
- * bgtq_encode_batched does (bit for bit), V rounded to FP16 and quantised as
+ * bgtq_encode_batched does (bit for bit; a row with an infinity or a NaN as in
+ * its calls of fewer than 16384 rows), V rounded to FP16 and quantised as
  * above: a decode step's new tokens, or a prompt's. Rows whose slot lies
  * outside the pool (negative, or from pages * page_tokens on) are skipped: a
  * padded batch marks its padding so. Rows of one call have different slots; a

@@ -784,3 +784,55 @@ def test_rotations_that_are_not_orthogonal(device, oracle, layout, dim, factor):
     torch.cuda.synchronize()
     _check(out, _reference(pool, oracle, q, [270], table))
     pool.destroy()
+
+
+@pytest.mark.parametrize("layout,v,dim,heads,page", [("S", "q8", 64, 3, 64), ("B", "q8", 64, 2, 32), ("A", "f16", 64, 2, 256),
+                                                     ("B", "f16", 128, 2, 64), ("A", "q8", 128, 1, 32)])
+@pytest.mark.parametrize("rows,scattered", [(39, False), (40, True), (9003, False), (8200, True)])
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+def test_non_finite_keys(device, oracle, layout, v, dim, heads, page, rows, scattered, dtype):
+    """K rows with infinities and NaNs (and FP32 and BF16 values that FP16 does not hold) among others: a wave's
+    row, and the tile encoder's second pass, whose blocks have skipped slots and end inside a tile. Each keeps to its
+    groups as in an encode call of few rows; no other slot changes."""
+    import torch
+    from bgtq import batched
+    from test_gpu_encode import _encode_nonfinite
+    print(layout, dim, rows, scattered, dtype, flush=True)
+    pages = -(-rows // page) + 2
+    pool = Pool(device, layout, v, dim, heads, pages, page, gap=16)
+    rng = np.random.RandomState(rows + dim)
+    slots = (rng.permutation(pages * page)[:rows] if scattered else np.arange(rows) + 5).astype(np.int64)
+    k, val = _rows(rows, heads, dim, dtype, rows, 1, 2.0), _rows(rows, heads, dim, dtype, rows, 2)
+    odd = np.unique(np.concatenate([rng.choice(rows, min(rows, 50), replace=False)[:max(8, rows // 200)], [0, rows - 1, rows - 2]]))
+    kinds = [float("inf"), -float("inf"), float("nan")] + ([1e6, -70000.0] if dtype != "float16" else [])
+    for r in odd:
+        for h in range(heads):
+            for c in rng.choice(dim, rng.choice([0, 1, 1, 2, dim // 3]), replace=False):
+                k[r, h, c] = kinds[rng.randint(len(kinds))]
+    k[odd[1]] = float("inf")
+    given = slots.copy()
+    skipped = np.unique(np.concatenate([odd[::4] if rows > 100 else odd[3:5], odd[2:3] + 1])) % rows
+    given[skipped] = rng.choice([-1, pages * page, 2 ** 40], len(skipped))
+    kept = np.ones(rows, bool)
+    kept[skipped] = False
+    before = pool.snapshot()
+    batched.paged_write(device, pool.handle, torch.from_numpy(given).cuda(), k.cuda(), val.cuda())
+    torch.cuda.synchronize()
+    k16 = k.half().numpy()
+    for h, p in enumerate(pool.params):
+        got_p, got_n = pool.k_bytes(h, slots[kept])
+        want_p, want_n = _encode_nonfinite(oracle, p, np.ascontiguousarray(k16[kept, h]).view(np.uint16), True)
+        got_n, want_n = got_n.view(np.uint16), np.asarray(want_n).view(np.uint16)
+        same = (got_n == want_n) | (np.isnan(got_n.view(np.float16)) & np.isnan(want_n.view(np.float16)))
+        bad = np.nonzero(np.any(got_p != want_p, 1) | ~same.all(1))[0]
+        assert bad.size == 0, f"head {h}: {bad.size} rows differ, first {np.nonzero(kept)[0][bad[:5]]}"
+    mask = torch.zeros(pages * page, dtype=torch.bool)
+    mask[slots[kept]] = True
+    keep = ~mask.view(pages, page).cuda()
+    now = pool.snapshot()
+    for h, p in enumerate(pool.params):
+        for x, y, w in ((before[2], now[2], p.rowBytes), (before[3], now[3], p.normStride)):
+            x, y = (a[:, h, :page * w].reshape(pages, page, w)[keep] for a in (x, y))
+            assert _same_bits(x, y)
+        assert _same_bits(before[0][:, h][keep], now[0][:, h][keep])
+    pool.destroy()
