@@ -268,3 +268,57 @@ def test_many_small_weights_beside_a_large_one(device, dtype, dim, sink, n):
             lim += 2.0 ** -36 * (np.abs(x).sum(0) + (row + 1) * np.abs(ref)) + 2.0 ** -25
         err = np.abs(got[row] - ref)
         assert np.all(err <= lim), f"row {row}: {np.max(err / lim):.1f} of the limit, heads {np.max(err / lim, -1).round(2)}"
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("bad", ["nan", "inf", "-inf"])
+@pytest.mark.parametrize("where", ["k", "v", "both"])
+def test_non_finite_rows_in_64_bits(device, dtype, dim, bad, where):
+    """K and V rows with infinities or NaNs, seen in a diagonal block and in whole ones: NaNs, infinities and finite
+    values are where the formula in 64 bits has them. Head 0's queries are positive, so that an infinite K row has
+    infinite logits (minus infinity: weight 0); the other head's signs are mixed, its logits NaN."""
+    import torch
+    from bgtq import batched
+    batched.bind_torch_stream(device)
+    print(dtype, dim, bad, where, flush=True)
+    n, hq, value = 330, 2, float(bad)
+    x = _inputs(n, hq, 1, dim, dtype, 6)
+    x[:, 0] = x[:, 0].abs() * 0.25 + 0.01
+    if where != "k":
+        x[10, 3, 3::7], x[140, 3, 5::11] = value, value
+    if where != "v":
+        x[200, 2] = value
+    xd, out = x.cuda(), torch.empty((n, hq, dim), dtype=x.dtype, device="cuda")
+    batched.prompt_attention(device, xd[:, :hq], xd[:, 2:3], xd[:, 3:], _offsets([n]), out)
+    torch.cuda.synchronize()
+    got, y = out.double().cpu().numpy(), x.double().numpy()
+    for h in range(hq):
+        for i in range(n):
+            with np.errstate(invalid="ignore"):
+                s = (y[i, h] * y[:i + 1, 2]).sum(-1) / np.sqrt(dim)
+                p = np.exp(s - s.max())
+                p /= p.sum()
+                live = ~(p == 0)  # (a key of weight 0 adds nothing, whatever its V)
+                ref, size = (p[live, None] * y[:i + 1, 3][live]).sum(0), (p[live, None] * np.abs(y[:i + 1, 3][live])).sum(0)
+            assert np.array_equal(np.isnan(got[i, h]), np.isnan(ref)), f"head {h} query {i}"
+            assert np.array_equal(np.isinf(got[i, h]), np.isinf(ref)), f"head {h} query {i}"
+            f = np.isfinite(ref)
+            assert np.array_equal(got[i, h][np.isinf(ref)], ref[np.isinf(ref)])
+            lim = U[dtype] * (size[f] + 2 * np.abs(ref[f])) * 1.001 + 2.0 ** -14 * size[f] + 1e-6
+            assert np.all(np.abs(got[i, h][f] - ref[f]) <= lim), f"head {h} query {i}"
+
+
+def test_two_calls_give_the_same_bits(device):
+    """No order of workgroups shows in the result."""
+    import torch
+    from bgtq import batched
+    batched.bind_torch_stream(device)
+    lens = [700, 33, 1, 257]
+    for dtype, dim in (("float16", 64), ("bfloat16", 64), ("bfloat16", 128)):
+        x = _inputs(sum(lens), 9, 3, dim, dtype, 2).cuda()
+        outs = [torch.full((sum(lens), 9, dim), float(i), dtype=x.dtype, device="cuda") for i in range(4)]
+        for o in outs:
+            batched.prompt_attention(device, x[:, :9], x[:, 9:12], x[:, 12:], _offsets(lens), o)
+        torch.cuda.synchronize()
+        assert all(torch.equal(outs[0], o) for o in outs[1:])
