@@ -333,6 +333,6 @@ def prompt_attention(device, q, k, v, offsets, out, scale=None) -> None:
         if s[2] != 1 and dim > 1:
             raise RangeError("the last dimension of q, k, v and out must be dense")
         fields += (t.data_ptr() or None, s[0] if tokens > 1 else 0, s[1] if want[1] > 1 else 0)
-    _need(scale is None or scale > 0, "scale must be positive")
+    _need(scale is None or ctypes.c_float(scale).value > 0, "scale must be positive in FP32")  # (0 stands for the default)
     d = _lib.PromptDesc(heads, kv_shape[1], dim, code, offsets.shape[0] - 1, tokens, offsets.data_ptr(), *fields, scale or 0.0)
     check(lib().bgtq_prompt_attention(device.handle, ctypes.byref(d)))

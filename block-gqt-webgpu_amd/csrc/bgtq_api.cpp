@@ -1955,7 +1955,8 @@ bgtq_status bgtq_prompt_attention(bgtq_context *ctx, const bgtq_prompt_desc *d) 
   if (d->dtype != BGTQ_DTYPE_F16 && d->dtype != BGTQ_DTYPE_BF16) return fail(BGTQ_ERR_RANGE, "invalid dtype");
   if (d->sequences < 0 || d->sequences > 65535) return fail(BGTQ_ERR_RANGE, "sequences must be in 0..65535");
   if (d->tokens < 0 || d->tokens > INT32_MAX) return fail(BGTQ_ERR_RANGE, "tokens must be in 0..2^31 - 1");
-  if (!(d->scale >= 0.0f && d->scale <= 3.0e38f)) return fail(BGTQ_ERR_RANGE, "scale must be finite and not negative");
+  // (the kernel takes scale * log2(e) in FP32)
+  if (!(d->scale >= 0.0f && d->scale <= 2.0e38f)) return fail(BGTQ_ERR_RANGE, "scale must be in 0..2e38");
   const bool none = !d->sequences || !d->tokens;
   if (!none && (!d->offsets || !d->q || !d->k || !d->v || !d->out)) return fail(BGTQ_ERR_RANGE, "null offsets/q/k/v/out");
   if (reinterpret_cast<uintptr_t>(d->offsets) % 4) return fail(BGTQ_ERR_RANGE, "offsets must be 4-byte aligned");

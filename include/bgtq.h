@@ -494,7 +494,7 @@ bgtq_status bgtq_paged_decode(bgtq_context *ctx, const bgtq_pages *pages, const 
  * elements, not negative and row strides at most 2^22; out overlaps neither the
  * inputs nor itself (rows outermost or heads). offsets (device int32 [sequences + 1], nondecreasing) are clamped to
  * 0 .. tokens; a sequence may be empty, and rows of no sequence stay as they
- * were. scale: of the logits; 0 = 1 / sqrt(dim). Logits, softmax statistics and
+ * were. scale: of the logits, at most 2e38; 0 = 1 / sqrt(dim). Logits, softmax statistics and
  * sums are FP32, probabilities are rounded to dtype for the product with V (FP16:
  * 11 bits down to 2^-25 of the largest, absolute 2^-36 of it below). One
  * launch, no workspace, HIP-graph capturable. (The model's three attention passes

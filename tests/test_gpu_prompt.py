@@ -322,3 +322,20 @@ def test_two_calls_give_the_same_bits(device):
             batched.prompt_attention(device, x[:, :9], x[:, 9:12], x[:, 12:], _offsets(lens), o)
         torch.cuda.synchronize()
         assert all(torch.equal(outs[0], o) for o in outs[1:])
+
+
+def test_scales_that_fp32_does_not_hold(device):
+    """A scale that is 0 in FP32 is refused: it would stand for the default. The smallest that is none gives equal weights."""
+    import torch
+    import bgtq
+    from bgtq import batched
+    batched.bind_torch_stream(device)
+    x = _inputs(70, 1, 1, 64, "bfloat16", 1).cuda()
+    out = torch.empty((70, 1, 64), dtype=x.dtype, device="cuda")
+    args = (x[:, :1], x[:, 1:2], x[:, 2:], _offsets([70]), out)
+    for scale in (1e-46, 1e-300, 0.0, 1e39, 2.5e38):
+        with pytest.raises(bgtq.RangeError):
+            batched.prompt_attention(device, *args, scale=scale)
+    batched.prompt_attention(device, *args, scale=1e-45)
+    torch.cuda.synchronize()
+    _check(out, x.cpu() * torch.tensor([0, 1, 1], dtype=x.dtype)[:, None], [70], 1, 1, "bfloat16", 1.0)

@@ -159,3 +159,11 @@ def test_wrappers_want_gpu_tensors():
     x = torch.zeros((4, 2, 32, 64), dtype=torch.float16)
     with pytest.raises(bgtq.RangeError):
         batched.pages(page_tokens=32, v=x, k_f16=x)
+
+
+def test_prompt_scales():
+    """Every accepted scale times log2(e) is finite in FP32."""
+    L = _lib.lib()
+    for scale, good in ((0.0, True), (1e-45, True), (2.0e38, True), (2.5e38, False), (3.0e38, False), (3.4e38, False)):
+        assert L.bgtq_prompt_attention(None, ctypes.byref(_prompt(scale=scale))) == _lib.ERR_RANGE
+        assert (L.bgtq_last_error() == b"null context") == good, scale
