@@ -1688,14 +1688,13 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
       u32x2 vc[DT];
 #pragma unroll
       for (int dt = 0; dt < DT; dt += 4) {
-        const uint8_t *at[4];
+        uint32_t at[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) at[i] = sb + vrow * D + (((dt + i) ^ swz8<D>(vrow)) * 16) + 8 * (col & 1);
+        for (int i = 0; i < 4; ++i) at[i] = lds_at(sb) + vrow * D + (((dt + i) ^ swz8<D>(vrow)) * 16) + 8 * (col & 1);
         ds_read_tr8(at, &vc[dt]);
       }
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
-        wait_tr8<DT>(dt, vc[dt]);
         u32x4 vb;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -1725,16 +1724,16 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
         for (int dt = 0; dt < DT; ++dt) O[dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(pr[j], v[j][dt], O[dt], 0, 0, 0);
     } else {
       u32x2 vt[DT][2];
+      uint32_t at[DT], at16[DT];
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
         const int piece = 2 * dt + tpiece;
-        ds_read_tr16_pair(sb + trow * (2 * D) + ((piece ^ swz<D>(trow)) * 16) + thalf,
-                          sb + (16 + trow) * (2 * D) + ((piece ^ swz<D>(16 + trow)) * 16) + thalf, vt[dt][0],
-                          vt[dt][1]);
+        at[dt] = lds_at(sb) + trow * (2 * D) + ((piece ^ swz<D>(trow)) * 16) + thalf;
+        at16[dt] = lds_at(sb) + (16 + trow) * (2 * D) + ((piece ^ swz<D>(16 + trow)) * 16) + thalf;
       }
+      ds_read_tr16(at, at16, vt);
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
-        wait_dt<DT>(dt, vt[dt][0], vt[dt][1]);
         const half8 vb = __builtin_bit_cast(half8, u32x4{vt[dt][0][0], vt[dt][0][1], vt[dt][1][0], vt[dt][1][1]});
         O[dt] = mfma(pha, vb, O[dt]);
         O[dt] = mfma(pla, vb, O[dt]);

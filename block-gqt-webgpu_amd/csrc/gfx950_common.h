@@ -238,86 +238,68 @@ __device__ __forceinline__ void lds_barrier() {
   asm volatile("" ::: "memory");
 }
 
-// Two transposed FP16 reads (ds_read_b64_tr_b16: lane i of a 16-lane group
-// gets column i of the four rows the group addresses) issued from inline asm.
-// The builtin form makes the compiler wait for every vector-memory load in
-// flight first (it may alias an LDS DMA), which drains a DMA ring; the caller
+// Transposed FP16 reads (ds_read_b64_tr_b16: lane i of a 16-lane group gets
+// column i of the four rows the group addresses) of N pairs of rows, at LDS
+// addresses lds[i] + OFF and lds2[i] + OFF, from inline asm that waits for them
+// itself. The builtin form makes the compiler wait for every vector-memory load
+// in flight first (it may alias an LDS DMA), which drains a DMA ring; the caller
 // has waited for the DMA that wrote these rows. The compiler's hazard
 // recognizer does not look into asm: the s_nop 7 covers the wait states a
 // matrix-core instruction that read the destination registers as its
-// accumulator input needs before they are written (8-pass XDL). The results
-// are not valid until a wait_lds_tied on them.
-__device__ __forceinline__ void ds_read_tr16_pair(const uint8_t *lds0, const uint8_t *lds1, u32x2 &a, u32x2 &b) {
-  asm volatile("s_nop 7\n\tds_read_b64_tr_b16 %0, %2\n\tds_read_b64_tr_b16 %1, %3"
-               : "=&v"(a), "=&v"(b)
-               : "v"((uint32_t)(uintptr_t)(lds_void *)lds0), "v"((uint32_t)(uintptr_t)(lds_void *)lds1));
+// accumulator input needs before they are written (8-pass XDL).
+template <int N, int OFF = 0>
+__device__ __forceinline__ void ds_read_tr16(const uint32_t (&lds)[N], const uint32_t (&lds2)[N], u32x2 (&v)[N][2]) {
+  static_assert(N == 2 || N == 4 || N == 8, "pairs");
+  if constexpr (N == 2)
+    asm volatile(
+          "s_nop 7\n\t"
+          "ds_read_b64_tr_b16 %0, %4 offset:%8\n\tds_read_b64_tr_b16 %1, %5 offset:%8\n\t"
+          "ds_read_b64_tr_b16 %2, %6 offset:%8\n\tds_read_b64_tr_b16 %3, %7 offset:%8\n\t"
+          "s_waitcnt lgkmcnt(0)"
+        : "=&v"(v[0][0]), "=&v"(v[0][1]), "=&v"(v[1][0]), "=&v"(v[1][1])
+        : "v"(lds[0]), "v"(lds2[0]), "v"(lds[1]), "v"(lds2[1]), "n"(OFF));
+  else if constexpr (N == 4)
+    asm volatile(
+          "s_nop 7\n\t"
+          "ds_read_b64_tr_b16 %0, %8 offset:%16\n\tds_read_b64_tr_b16 %1, %9 offset:%16\n\t"
+          "ds_read_b64_tr_b16 %2, %10 offset:%16\n\tds_read_b64_tr_b16 %3, %11 offset:%16\n\t"
+          "ds_read_b64_tr_b16 %4, %12 offset:%16\n\tds_read_b64_tr_b16 %5, %13 offset:%16\n\t"
+          "ds_read_b64_tr_b16 %6, %14 offset:%16\n\tds_read_b64_tr_b16 %7, %15 offset:%16\n\t"
+          "s_waitcnt lgkmcnt(0)"
+        : "=&v"(v[0][0]), "=&v"(v[0][1]), "=&v"(v[1][0]), "=&v"(v[1][1]), "=&v"(v[2][0]), "=&v"(v[2][1]),
+          "=&v"(v[3][0]), "=&v"(v[3][1])
+        : "v"(lds[0]), "v"(lds2[0]), "v"(lds[1]), "v"(lds2[1]), "v"(lds[2]), "v"(lds2[2]), "v"(lds[3]), "v"(lds2[3]),
+          "n"(OFF));
+  else
+    asm volatile(
+          "s_nop 7\n\t"
+          "ds_read_b64_tr_b16 %0, %16 offset:%32\n\tds_read_b64_tr_b16 %1, %17 offset:%32\n\t"
+          "ds_read_b64_tr_b16 %2, %18 offset:%32\n\tds_read_b64_tr_b16 %3, %19 offset:%32\n\t"
+          "ds_read_b64_tr_b16 %4, %20 offset:%32\n\tds_read_b64_tr_b16 %5, %21 offset:%32\n\t"
+          "ds_read_b64_tr_b16 %6, %22 offset:%32\n\tds_read_b64_tr_b16 %7, %23 offset:%32\n\t"
+          "ds_read_b64_tr_b16 %8, %24 offset:%32\n\tds_read_b64_tr_b16 %9, %25 offset:%32\n\t"
+          "ds_read_b64_tr_b16 %10, %26 offset:%32\n\tds_read_b64_tr_b16 %11, %27 offset:%32\n\t"
+          "ds_read_b64_tr_b16 %12, %28 offset:%32\n\tds_read_b64_tr_b16 %13, %29 offset:%32\n\t"
+          "ds_read_b64_tr_b16 %14, %30 offset:%32\n\tds_read_b64_tr_b16 %15, %31 offset:%32\n\t"
+          "s_waitcnt lgkmcnt(0)"
+        : "=&v"(v[0][0]), "=&v"(v[0][1]), "=&v"(v[1][0]), "=&v"(v[1][1]), "=&v"(v[2][0]), "=&v"(v[2][1]),
+          "=&v"(v[3][0]), "=&v"(v[3][1]), "=&v"(v[4][0]), "=&v"(v[4][1]), "=&v"(v[5][0]), "=&v"(v[5][1]),
+          "=&v"(v[6][0]), "=&v"(v[6][1]), "=&v"(v[7][0]), "=&v"(v[7][1])
+        : "v"(lds[0]), "v"(lds2[0]), "v"(lds[1]), "v"(lds2[1]), "v"(lds[2]), "v"(lds2[2]), "v"(lds[3]), "v"(lds2[3]),
+          "v"(lds[4]), "v"(lds2[4]), "v"(lds[5]), "v"(lds2[5]), "v"(lds[6]), "v"(lds2[6]), "v"(lds[7]), "v"(lds2[7]),
+          "n"(OFF));
 }
-// One transposed read of 8-bit values (ds_read_b64_tr_b8: lane i of a 16-lane
+// The LDS address of a generic pointer into it.
+__device__ __forceinline__ uint32_t lds_at(const uint8_t *p) { return (uint32_t)(uintptr_t)(lds_void *)p; }
+// Four transposed reads of 8-bit values (ds_read_b64_tr_b8: lane i of a 16-lane
 // group gets column i of the eight 16-byte rows whose halves the group's
-// lanes address, lanes 2 r and 2 r + 1 row r's), as ds_read_tr16_pair.
-__device__ __forceinline__ void ds_read_tr8(const uint8_t *const (&lds)[4], u32x2 *a) {
+// lanes address, lanes 2 r and 2 r + 1 row r's), as ds_read_tr16.
+__device__ __forceinline__ void ds_read_tr8(const uint32_t (&lds)[4], u32x2 *a) {
   asm volatile(
       "s_nop 7\n\tds_read_b64_tr_b8 %0, %4\n\tds_read_b64_tr_b8 %1, %5\n\t"
-      "ds_read_b64_tr_b8 %2, %6\n\tds_read_b64_tr_b8 %3, %7"
+      "ds_read_b64_tr_b8 %2, %6\n\tds_read_b64_tr_b8 %3, %7\n\ts_waitcnt lgkmcnt(0)"
       : "=&v"(a[0]), "=&v"(a[1]), "=&v"(a[2]), "=&v"(a[3])
-      : "v"((uint32_t)(uintptr_t)(lds_void *)lds[0]), "v"((uint32_t)(uintptr_t)(lds_void *)lds[1]),
-        "v"((uint32_t)(uintptr_t)(lds_void *)lds[2]), "v"((uint32_t)(uintptr_t)(lds_void *)lds[3]));
-}
-// Waits until at most N LDS operations of this wave are in flight; a and b
-// are tied to the wait so nothing that reads them is scheduled before it.
-// LDS operations complete in order, so with the reads of a and b issued
-// before the N newest, they have landed.
-template <int N>
-__device__ __forceinline__ void wait_lds_tied(u32x2 &a, u32x2 &b) {
-  static_assert(N >= 0 && N < 16, "lgkmcnt");
-  asm volatile("s_waitcnt lgkmcnt(%2)" : "+v"(a), "+v"(b) : "n"(N));
-}
-
-template <int N>
-__device__ __forceinline__ void wait_lds_tied(u32x2 &a) {
-  static_assert(N >= 0 && N < 16, "lgkmcnt");
-  asm volatile("s_waitcnt lgkmcnt(%1)" : "+v"(a) : "n"(N));
-}
-// Wait for ds_read_tr8 read dt of DT (4 or 8) issued in order.
-template <int DT>
-__device__ __forceinline__ void wait_tr8(int dt, u32x2 &a) {
-  static_assert(DT == 4 || DT == 8, "head dim 64 or 128");
-  switch (DT - 1 - dt) {
-    case 7: return wait_lds_tied<7>(a);
-    case 6: return wait_lds_tied<6>(a);
-    case 5: return wait_lds_tied<5>(a);
-    case 4: return wait_lds_tied<4>(a);
-    case 3: return wait_lds_tied<3>(a);
-    case 2: return wait_lds_tied<2>(a);
-    case 1: return wait_lds_tied<1>(a);
-    default: return wait_lds_tied<0>(a);
-  }
-}
-
-// Wait for transposed read pair dt of DT issued in order (2 (DT - 1 - dt)
-// newer reads may still be in flight); dt is a compile-time index after
-// unrolling.
-template <int DT>
-__device__ __forceinline__ void wait_dt(int dt, u32x2 &a, u32x2 &b) {
-  if constexpr (DT == 2) {
-    if (dt == 0) wait_lds_tied<2>(a, b);
-    else wait_lds_tied<0>(a, b);
-  } else if constexpr (DT == 4) {
-    if (dt == 0) wait_lds_tied<6>(a, b);
-    else if (dt == 1) wait_lds_tied<4>(a, b);
-    else if (dt == 2) wait_lds_tied<2>(a, b);
-    else wait_lds_tied<0>(a, b);
-  } else {
-    static_assert(DT == 8, "head dim 32, 64 or 128");
-    if (dt == 0) wait_lds_tied<14>(a, b);
-    else if (dt == 1) wait_lds_tied<12>(a, b);
-    else if (dt == 2) wait_lds_tied<10>(a, b);
-    else if (dt == 3) wait_lds_tied<8>(a, b);
-    else if (dt == 4) wait_lds_tied<6>(a, b);
-    else if (dt == 5) wait_lds_tied<4>(a, b);
-    else if (dt == 6) wait_lds_tied<2>(a, b);
-    else wait_lds_tied<0>(a, b);
-  }
+      : "v"(lds[0]), "v"(lds[1]), "v"(lds[2]), "v"(lds[3]));
 }
 
 // 16-byte piece swizzle of an FP16 row of D values in LDS: conflict-free

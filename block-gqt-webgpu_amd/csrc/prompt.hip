@@ -27,7 +27,11 @@
 // product of 8192^3 reaches 1249). A wave's block is 512 cycles of products and
 // 870 of softmax at d=64 (1024 at d=128), of which 512 are exponentials (a quarter
 // of the vector rate): the vector unit bounds d=64 (72% busy), the matrix cores
-// d=128 (53%), and what the waves of a SIMD do not overlap of the two.
+// d=128 (53%), and what the waves of a SIMD do not overlap of the two. A step's V
+// arrives behind the step before's products, waited for where it is read (one
+// prompt of 8192 tokens 1.2% slower than with each read waited for at its use).
+// At d=64 the 128 registers of four waves per SIMD leave 16 or 32 bytes of scratch
+// to the branch for V rows with infinities or NaNs, none to the others.
 #include <type_traits>
 
 #include "bgtq_internal.h"
@@ -111,41 +115,6 @@ struct Odd {
     return (is(w & 0xffffu) ? kOne : 0u) | (is(w >> 16) ? kOne << 16 : 0u);
   }
 };
-
-// 2 N transposed reads (ds_read_tr16_pair's) of the N rows pairs at lds[t] +
-// OFF and lds2[t] + OFF, issued together: the results are valid once waited for.
-template <int N, int OFF>
-__device__ __forceinline__ void read_v(const uint32_t (&lds)[N], const uint32_t (&lds2)[N], u32x2 (&v)[N][2]) {
-  if constexpr (N == 2) {
-    asm volatile(
-        "s_nop 7\n\tds_read_b64_tr_b16 %0, %4 offset:%8\n\tds_read_b64_tr_b16 %1, %5 offset:%8\n\t"
-        "ds_read_b64_tr_b16 %2, %6 offset:%8\n\tds_read_b64_tr_b16 %3, %7 offset:%8"
-        : "=&v"(v[0][0]), "=&v"(v[0][1]), "=&v"(v[1][0]), "=&v"(v[1][1])
-        : "v"(lds[0]), "v"(lds2[0]), "v"(lds[1]), "v"(lds2[1]), "n"(OFF));
-  } else {
-    static_assert(N == 4, "head dim 64 or 128");
-    asm volatile(
-        "s_nop 7\n\tds_read_b64_tr_b16 %0, %8 offset:%16\n\tds_read_b64_tr_b16 %1, %9 offset:%16\n\t"
-        "ds_read_b64_tr_b16 %2, %10 offset:%16\n\tds_read_b64_tr_b16 %3, %11 offset:%16\n\t"
-        "ds_read_b64_tr_b16 %4, %12 offset:%16\n\tds_read_b64_tr_b16 %5, %13 offset:%16\n\t"
-        "ds_read_b64_tr_b16 %6, %14 offset:%16\n\tds_read_b64_tr_b16 %7, %15 offset:%16"
-        : "=&v"(v[0][0]), "=&v"(v[0][1]), "=&v"(v[1][0]), "=&v"(v[1][1]), "=&v"(v[2][0]), "=&v"(v[2][1]),
-          "=&v"(v[3][0]), "=&v"(v[3][1])
-        : "v"(lds[0]), "v"(lds2[0]), "v"(lds[1]), "v"(lds2[1]), "v"(lds[2]), "v"(lds2[2]), "v"(lds[3]), "v"(lds2[3]),
-          "n"(OFF));
-  }
-}
-
-// Waits for the read pair of tile t of N when NEXT reads were issued after the
-// N pairs (t is a compile-time index after unrolling).
-template <int N, int NEXT>
-__device__ __forceinline__ void wait_newer(int t, u32x2 &a, u32x2 &b) {
-  static_assert(2 * (N - 1) + NEXT < 16, "lgkmcnt");
-  if (t == 0) wait_lds_tied<2 * (N - 1) + NEXT>(a, b);
-  else if (t == 1) wait_lds_tied<2 * (N - 2) + NEXT>(a, b);
-  else if (t == 2) wait_lds_tied<2 * (N > 2 ? N - 3 : 0) + NEXT>(a, b);
-  else wait_lds_tied<NEXT>(a, b);
-}
 
 // Ties an accumulator to its registers. After each element's update under a
 // branch: without it the update builds a second copy of the accumulator, and
@@ -382,20 +351,18 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 4 : 2) void prompt_kernel(Promp
     if (!DIAGONAL || plain) {
       constexpr int STEP = 16 * 2 * D;  // bytes of a step's rows
       u32x2 v[2][MT][2];
-      read_v<MT, 0>(va, va8, v[0]);
+      ds_read_tr16<MT, 0>(va, va8, v[0]);
 #pragma unroll
       for (int s = 0; s < kKeys / 16; ++s) {
-        if (s == 0) read_v<MT, STEP>(va, va8, v[1]);
-        if (s == 1) read_v<MT, 2 * STEP>(va, va8, v[0]);
-        if (s == 2) read_v<MT, 3 * STEP>(va, va8, v[1]);
         const u32x4 pf{P[4 * s], P[4 * s + 1], P[4 * s + 2], P[4 * s + 3]};
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
-          u32x2 &a = v[s & 1][t][0], &b = v[s & 1][t][1];
-          if (s < 3) wait_newer<MT, 2 * MT>(t, a, b);  // (the next step's 2 MT reads are newer)
-          else wait_newer<MT, 0>(t, a, b);
+          const u32x2 a = v[s & 1][t][0], b = v[s & 1][t][1];
           O[t] = product<BF>(u32x4{a[0], a[1], b[0], b[1]}, pf, O[t]);
         }
+        if (s == 0) ds_read_tr16<MT, STEP>(va, va8, v[1]);
+        if (s == 1) ds_read_tr16<MT, 2 * STEP>(va, va8, v[0]);
+        if (s == 2) ds_read_tr16<MT, 3 * STEP>(va, va8, v[1]);
       }
     } else {
       const int d = qi - j * kKeys - 4 * h;
