@@ -1314,8 +1314,9 @@ bgtq_status bgtq_decode_workspace_size(const bgtq_decode_desc *d, size_t *bytes)
   return BGTQ_OK;
 }
 
-// Whether the fused kernel reads p's V: FP16 rows, or FP32 rows in a decode
-// without an appended token; 16-byte aligned base and strides.
+// Whether the fused kernel reads p's V: FP16 rows, 8-bit rows of pages, or
+// FP32 rows in a contiguous decode without an appended token; 16-byte aligned
+// base and strides.
 static bool fused_v(const DecodeParams &p) {
   const bool f32 = p.v_dtype == BGTQ_DTYPE_F32, q8 = p.v_dtype == BGTQ_DTYPE_Q8;  // (Q8: pages only)
   if (f32 ? p.k_new || p.starts || p.page_shift : p.v_dtype != BGTQ_DTYPE_F16 && !q8) return false;
@@ -1382,7 +1383,7 @@ static bool fast_layout(const DecodeParams &p, const bgtq_tables *const *tables,
 }
 
 // Whether the fused kernel's per-position code lookup serves a packed layout
-// the structured check (fast_layout) refused: FP16 V; 16-byte aligned packed
+// the structured check (fast_layout) refused: V as fused_v; 16-byte aligned packed
 // and scale bases and strides; per KV head up to 8 books of up to 256
 // centroids whose code tables fit the kernel's LDS, each book's positions
 // all nibble or all byte codes, norm stride up to 8, groups in ascending

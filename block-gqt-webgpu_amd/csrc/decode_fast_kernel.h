@@ -36,9 +36,9 @@
 // comes from the sequence's table two chunks ahead, up to 64 sequences share
 // the workgroups by their lengths (paged_place), and the loop takes fewer
 // vector instructions (PAIRED, LATE). 64 x 32768 tokens, 14 / 2 heads of layout B
-// with 8-bit V, 99 to 104 us (495 MB, 4.8 to 5.0 TB/s): vector instructions (64% of
-// the SIMDs' time) and the lookups' LDS traffic (57%, a third of it bank
-// conflicts) beside the stream.
+// with 8-bit V, 99 to 104 us (495 MB, 4.8 to 5.0 TB/s): vector instructions (61% of
+// the SIMDs' time) and the lookups' LDS traffic (54%, more than half of it bank
+// conflicts) beside the stream; with FP16 V 122 us (755 MB, 6.2 TB/s).
 //
 // The arithmetic is that of src/reference/attention.py:5-22 on the
 // reconstructed K of src/reference/production_math.py:27-31: with

@@ -22,14 +22,17 @@
 // output (below, they are subnormal, off by 2^-36 of the maximum at most).
 // 8192 tokens of d=128 in FP16 276 us with a threshold of 4, 301 with 1.
 //
-// Measured: 11 prompts of 568 to 2777 tokens, 14 / 2 heads of d=64, 85 us (760
-// TFLOP/s), one of 8192 tokens, 16 / 4 heads of d=128, 258 us (1065 TFLOP/s; a bf16
-// product of 8192^3 reaches 1249). A wave's block is 512 cycles of products and
+// Measured (several boxes): 11 prompts of 568 to 2777 tokens, 14 / 2 heads of d=64,
+// 85 to 92 us (700 to 760 TFLOP/s), one of 8192 tokens, 16 / 4 heads of d=128, 258 to 268 us
+// (1025 to 1065 TFLOP/s; a bf16 product of 8192^3 reaches 1249). A wave's block is 512 cycles of products and
 // 870 of softmax at d=64 (1024 at d=128), of which 512 are exponentials (a quarter
-// of the vector rate): the vector unit bounds d=64 (72% busy), the matrix cores
-// d=128 (53%), and what the waves of a SIMD do not overlap of the two. A step's V
+// of the vector rate): the vector unit bounds d=64 (70% busy), the matrix cores
+// d=128 (52%), and what the waves of a SIMD do not overlap of the two. A step's V
 // arrives behind the step before's products, waited for where it is read (one
 // prompt of 8192 tokens 1.2% slower than with each read waited for at its use).
+// Nothing splits the keys: a tile's history is one workgroup's chain, and few
+// tiles and heads leave compute units idle (4096 tokens on 4 heads of d=128 88 us,
+// where their products take 14).
 // At d=64 the 128 registers of four waves per SIMD leave 16 or 32 bytes of scratch
 // to the branch for V rows with infinities or NaNs, none to the others.
 #include <type_traits>
