@@ -836,3 +836,159 @@ def test_non_finite_keys(device, oracle, layout, v, dim, heads, page, rows, scat
             assert _same_bits(x, y)
         assert _same_bits(before[0][:, h][keep], now[0][:, h][keep])
     pool.destroy()
+
+
+def _relay(pool, heads_first):
+    """The pool's arrays in other storage: heads outermost, or pages with other pages between them."""
+    import torch
+    from bgtq import batched
+
+    def again(t):
+        if t is None:
+            return None
+        if heads_first:
+            return torch.empty((t.shape[1], t.shape[0], *t.shape[2:]), dtype=t.dtype, device="cuda").transpose(0, 1).copy_(t)
+        n = (int(np.prod(t.shape[2:])) * t.element_size() + 15) // 16 * 16 // t.element_size()
+        flat = torch.empty((t.shape[0], 3, t.shape[1], n), dtype=t.dtype, device="cuda")[:, 1, :, :int(np.prod(t.shape[2:]))]
+        return flat.unflatten(2, t.shape[2:]).copy_(t)
+    pool.v, pool.v_scales, pool.packed, pool.norms, pool.k = (again(t) for t in (pool.v, pool.v_scales, pool.packed, pool.norms, pool.k))
+    pool.handle = batched.pages(page_tokens=pool.page, tables=pool.tables or None, packed=pool.packed, norms=pool.norms,
+                                k_f16=pool.k, v=pool.v, v_scales=pool.v_scales)
+
+
+@pytest.mark.parametrize("layout,v,dim,heads,page", [("S", "q8", 64, 3, 64), ("B", "q8", 64, 16, 32), ("B", "f16", 128, 2, 4096), ("f16", "q8", 64, 2, 32),
+                                                     ("f16", "f16", 128, 3, 128)])
+@pytest.mark.parametrize("heads_first", [True, False])
+def test_other_pool_strides(device, oracle, layout, v, dim, heads, page, heads_first):
+    """Heads outermost, or a pool inside a larger one; few and many rows; a page table inside a wider one, lengths of
+    uint32; 16 KV heads of 16 query heads."""
+    import torch
+    from bgtq import batched
+    print(layout, v, dim, heads, page, heads_first, flush=True)
+    pages = 4 if page == 4096 else 12000 // page // heads + 3
+    pool = Pool(device, layout, v, dim, heads, pages, page)
+    _relay(pool, heads_first)
+    n, rng = pages * page, np.random.RandomState(1)
+    k, val = _rows(n, heads, dim, "bfloat16", 1), _rows(n, heads, dim, "float32", 2)
+    slots = rng.permutation(n)
+    few = 37
+    for part in (slice(0, few), slice(few, n)):
+        batched.paged_write(device, pool.handle, torch.from_numpy(slots[part].copy()).cuda(), k[part].cuda(), val[part].cuda())
+    torch.cuda.synchronize()
+    _check_write(pool, oracle, slots, k, val)
+    sd = torch.from_numpy(slots).cuda()
+    ko, vo = torch.empty((n, heads, dim), device="cuda"), torch.empty((n, heads, dim), device="cuda")
+    batched.paged_read(device, pool.handle, sd, ko, vo)
+    torch.cuda.synchronize()
+    _check_read(pool, oracle, slots, ko, vo)
+    G = 16 if heads == 16 else 3
+    lengths = [min(page * 2 - 5, 300), 0, page + 1]
+    wide = torch.full((3, 9), 2 ** 31 - 1, dtype=torch.int32)
+    wide[0, 2:4], wide[2, 2:4] = torch.tensor([1, 3]), torch.tensor([2, 0])
+    table = wide.cuda()[:, 2:5]
+    q = _rows(3, heads * G, dim, "float32", 3).cuda()
+    out = torch.full_like(q, float("nan"))
+    args = dict(pages=pool.handle, q=q, out=out, lengths=torch.tensor(lengths, dtype=torch.uint32, device="cuda"), page_table=table)
+    ws = torch.zeros(batched.paged_decode_workspace_bytes(batched.paged_decode_desc(**args)), dtype=torch.uint8, device="cuda")
+    batched.paged_decode(device, batched.paged_decode_desc(workspace=ws, **args))
+    torch.cuda.synchronize()
+    _check(out, _reference(pool, oracle, q, lengths, table))
+    pool.destroy()
+
+
+@pytest.mark.parametrize("batch", [200, 1100])
+def test_decode_of_many_sequences(device, oracle, batch):
+    """More sequences than share workgroups by their lengths, and more (sequence, head) units than the counters' prefix
+    holds, twice in one workspace."""
+    import torch
+    from bgtq import batched
+    rng = np.random.RandomState(batch)
+    pool = Pool(device, "B", "q8", 64, 1, 64, 32)
+    _fill(pool, 2)
+    table = torch.from_numpy(rng.randint(0, 64, (batch, 24)).astype(np.int32)).cuda()
+    lengths = [int(x) for x in rng.randint(0, 24 * 32 + 1, batch)]
+    q = _rows(batch, 2, 64, "float32", 3).cuda()
+    outs = [_decode(pool, q, lengths, table) for _ in range(2)]
+    torch.cuda.synchronize()
+    assert torch.equal(*outs)
+    some = [0, 1, batch // 2, batch - 1] + [int(x) for x in rng.randint(0, batch, 40)]
+    ref = _reference(pool, oracle, q[some], [lengths[i] for i in some], table[some])
+    _check(outs[0][some], ref)
+    assert bool((outs[0][[i for i, n in enumerate(lengths) if n == 0]] == 0).all())
+    pool.destroy()
+
+
+def test_two_contexts_at_once(device, oracle):
+    """Two contexts on two streams write different rows of one pool, neighbours in memory among them, while one of
+    them decodes; neither touches the other's rows."""
+    import torch
+    import bgtq
+    from bgtq import batched
+    pool = Pool(device, "S", "q8", 64, 3, 130, 64)
+    other = bgtq.Device(0)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    n = 130 * 64
+    k, v = _rows(n, 3, 64, "float16", 1), _rows(n, 3, 64, "float16", 2)
+    kd, vd = k.cuda(), v.cuda()
+    slots = torch.arange(n, device="cuda")
+    table = torch.arange(128, dtype=torch.int32, device="cuda").view(4, 32)
+    q = _rows(4, 9, 64, "float32", 3).cuda()
+    torch.cuda.synchronize()
+    pool2 = batched.pages(page_tokens=64, tables=pool.tables, packed=pool.packed, norms=pool.norms, v=pool.v, v_scales=pool.v_scales)
+    odd = [torch.arange(n, device="cuda")[i::2] for i in range(2)]
+    parts = [(slots[o], kd[o].contiguous(), vd[o].contiguous()) for o in odd]
+    torch.cuda.synchronize()
+    for dev, s in zip((device, other), streams):
+        dev.set_stream(s.cuda_stream)
+    for dev, handle, (at, kk, vv) in zip((device, other), (pool.handle, pool2), parts):
+        batched.paged_write(dev, handle, at, kk, vv)
+    torch.cuda.synchronize()
+    _check_write(pool, oracle, np.arange(n), k, v)
+    outs = [torch.empty_like(q) for _ in range(2)]
+    descs = []
+    for handle, o in zip((pool.handle, pool2), outs):
+        args = dict(pages=handle, q=q, out=o, lengths=torch.tensor([2048, 100, 0, 1999], dtype=torch.int32, device="cuda"), page_table=table)
+        ws = torch.zeros(batched.paged_decode_workspace_bytes(batched.paged_decode_desc(**args)), dtype=torch.uint8, device="cuda")
+        descs.append(batched.paged_decode_desc(workspace=ws, **args))
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for dev, d in zip((device, other), descs):
+            batched.paged_decode(dev, d)
+    torch.cuda.synchronize()
+    assert torch.equal(*outs)
+    _check(outs[0], _reference(pool, oracle, q, [2048, 100, 0, 1999], table))
+    batched.bind_torch_stream(device)
+    other.destroy()
+    pool.destroy()
+
+
+@pytest.mark.parametrize("layout,v,rows", [("S", "q8", 6000), ("f16", "f16", 500), ("B", "q8", 3)])
+def test_write_and_read_captured(device, oracle, layout, v, rows):
+    """A graph of a write and the read back, replayed with other rows and slots."""
+    import torch
+    from bgtq import batched
+    heads = 3 if layout == "S" else 2
+    pool = Pool(device, layout, v, 64, heads, rows // 64 + 3, 64)
+    n = (rows // 64 + 3) * 64
+    slots = torch.zeros(rows, dtype=torch.int64, device="cuda")
+    k, val, ko, vo = (torch.empty((rows, heads, 64), device="cuda") for _ in range(4))
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        device.set_stream(side.cuda_stream)
+        batched.paged_write(device, pool.handle, slots, k, val)
+        batched.paged_read(device, pool.handle, slots, ko, vo)
+    batched.bind_torch_stream(device)
+    for step in range(4):
+        s = np.random.RandomState(step).permutation(n)[:rows]
+        nk, nv = _rows(rows, heads, 64, "float32", step, 1), _rows(rows, heads, 64, "float32", step, 2)
+        slots.copy_(torch.from_numpy(s)), k.copy_(nk), val.copy_(nv)
+        graph.replay()
+        torch.cuda.synchronize()
+        _check_write(pool, oracle, s, nk, nv)
+        _check_read(pool, oracle, s, ko, vo)
+        again = [torch.empty_like(ko), torch.empty_like(vo)]
+        batched.paged_read(device, pool.handle, slots, *again)
+        torch.cuda.synchronize()
+        assert torch.equal(again[0], ko) and torch.equal(again[1], vo)
+    pool.destroy()

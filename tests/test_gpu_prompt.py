@@ -339,3 +339,53 @@ def test_scales_that_fp32_does_not_hold(device):
     batched.prompt_attention(device, *args, scale=1e-45)
     torch.cuda.synchronize()
     _check(out, x.cpu() * torch.tensor([0, 1, 1], dtype=x.dtype)[:, None], [70], 1, 1, "bfloat16", 1.0)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_rows_far_apart(device, dim):
+    """The largest row stride: offsets past 2^32 bytes, rows of q, k, v and out side by side in one buffer."""
+    import torch
+    from bgtq import batched
+    batched.bind_torch_stream(device)
+    lens, hq, hkv, stride, dtype = [300, 1, 339], 2, 1, 1 << 22, "bfloat16"
+    total = sum(lens)
+    x = _inputs(total, hq, hkv, dim, dtype, 3)
+    buf = torch.empty((total, stride), dtype=x.dtype, device="cuda")
+    part = buf[:, :(2 * hq + 2 * hkv) * dim].unflatten(1, (2 * hq + 2 * hkv, dim))
+    part[:, :hq + 2 * hkv] = x.cuda()
+    out = part[:, hq + 2 * hkv:]
+    out.fill_(float("nan"))
+    batched.prompt_attention(device, part[:, :hq], part[:, hq:hq + hkv], part[:, hq + hkv:hq + 2 * hkv], _offsets(lens), out)
+    torch.cuda.synchronize()
+    _check(out, x, lens, hq, hkv, dtype, 1 / np.sqrt(dim))
+
+
+@pytest.mark.parametrize("sequences", [64, 65, 200])
+def test_many_sequences_captured(device, sequences):
+    """A graph over many sequences serves other lengths, empty ones among them; rows of none stay as they were."""
+    import torch
+    from bgtq import batched
+    batched.bind_torch_stream(device)
+    hq, hkv, dim, total, dtype = 3, 1, 64, 5000, "float16"
+    xd = torch.zeros((total, hq + 2 * hkv, dim), dtype=torch.float16, device="cuda")
+    out, off = torch.empty((total, hq, dim), dtype=torch.float16, device="cuda"), torch.zeros(sequences + 1, dtype=torch.int32, device="cuda")
+    args = (xd[:, :hq], xd[:, hq:hq + hkv], xd[:, hq + hkv:], off, out)
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        device.set_stream(side.cuda_stream)
+        batched.prompt_attention(device, *args)
+    batched.bind_torch_stream(device)
+    for step in range(3):
+        rng = np.random.RandomState(step)
+        lens = [int(n) for n in rng.multinomial(total - 100, rng.dirichlet(np.full(sequences, 0.2)))]
+        x = _inputs(total, hq, hkv, dim, dtype, step)
+        xd.copy_(x), off.copy_(_offsets(lens, 60)), out.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        _check(out, x, lens, hq, hkv, dtype, 1 / 8, 60, f"replay {step}")
+        assert bool((out[:60] == 7).all()) and bool((out[-40:] == 7).all())
+        replayed = out.clone()
+        batched.prompt_attention(device, *args)
+        torch.cuda.synchronize()
+        assert torch.equal(replayed, out)
