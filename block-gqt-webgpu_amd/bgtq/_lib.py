@@ -127,6 +127,17 @@ class PromptDesc(ctypes.Structure):
                 ("out_head_stride", ctypes.c_int64), ("scale", ctypes.c_float)]
 
 
+class RotationDesc(ctypes.Structure):
+    _fields_ = [("table", ctypes.c_void_p), ("table_rows", ctypes.c_int64), ("q_norm", ctypes.c_void_p),
+                ("k_norm", ctypes.c_void_p), ("eps", ctypes.c_double)]
+
+
+class HeadRows(ctypes.Structure):
+    _fields_ = [("src", ctypes.c_void_p), ("dst", ctypes.c_void_p), ("heads", ctypes.c_int32), ("dtype", ctypes.c_int32),
+                ("src_row_stride", ctypes.c_int64), ("src_head_stride", ctypes.c_int64),
+                ("dst_row_stride", ctypes.c_int64), ("dst_head_stride", ctypes.c_int64)]
+
+
 class Binding(ctypes.Structure):
     _fields_ = [("ptr", ctypes.c_void_p), ("bytes", ctypes.c_size_t), ("tables", ctypes.c_void_p)]
 
@@ -202,6 +213,10 @@ SIGNATURES = {
                                                 ctypes.POINTER(ctypes.c_size_t)]),
     "bgtq_paged_decode": (_I32, [_VP, ctypes.POINTER(Pages), ctypes.POINTER(PagedDecodeDesc)]),
     "bgtq_prompt_attention": (_I32, [_VP, ctypes.POINTER(PromptDesc)]),
+    "bgtq_rotate": (_I32, [_VP, ctypes.POINTER(RotationDesc), _I32, ctypes.c_int64, _VP, ctypes.POINTER(HeadRows),
+                           ctypes.POINTER(HeadRows)]),
+    "bgtq_paged_append": (_I32, [_VP, ctypes.POINTER(Pages), ctypes.POINTER(PagedRows), ctypes.POINTER(RotationDesc), _VP,
+                                 ctypes.POINTER(HeadRows)]),
     "bgtq_model_submit": (_I32, [_VP, ctypes.POINTER(ModelDispatch), _SZ]),
     "bgtq_allocate_bits": (_I32, [_VP, _SZ, ctypes.c_int64, _I32, _I32, _VP]),
     "bgtq_layout_groups": (_I32, [_VP, _SZ, _VP, _VP, _VP]),

@@ -272,6 +272,92 @@ def paged_read(device, pool, slots, k=None, v=None) -> None:
         check(lib().bgtq_paged_read(device.handle, pool.ref, ctypes.byref(r)))
 
 
+# ---- head norms and position rotation
+
+def rope_table(positions: int, dim: int, base: float, device="cuda"):
+    """The rotation table [positions, dim] float32 of angles p base^(-2 i / dim) (src/model/kernels.wgsl's rope), from
+    angles in 64 bits: a row's dim / 2 cosines, then as many sines."""
+    import torch
+    freq = float(base) ** (-torch.arange(0, dim, 2, dtype=torch.float64, device=device) / dim)
+    angle = torch.arange(positions, dtype=torch.float64, device=device)[:, None] * freq
+    return torch.cat([angle.cos(), angle.sin()], 1).float()
+
+
+class Rope:
+    """A rotation (bgtq_rotation) over device tensors; holds them."""
+
+    def __init__(self, struct, dim, device_index, held):
+        self.struct, self.dim, self.device_index, self.held = struct, dim, device_index, held
+        self.ref = ctypes.byref(struct)
+
+
+def rope(*, table, q_norm=None, k_norm=None, eps=1e-6) -> Rope:
+    """A rotation: table [positions, dim] float32 (see rope_table), and float32 [dim] weights of the norms of each head
+    of the queries and of the keys (None: no norm)."""
+    index = table.get_device()
+    _need(index >= 0, "the table must lie on a GPU")
+    _dense(index, "table", table, "float32", 2)
+    _need(table.is_contiguous(), "the table must be contiguous")
+    dim = table.shape[1]
+    for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
+        if w is not None:
+            _dense(index, name, w, "float32", 1)
+            _need(w.shape[0] == dim, f"{name} must hold a weight per dimension")
+    return Rope(_lib.RotationDesc(_addr(table), table.shape[0], _addr(q_norm), _addr(k_norm), float(eps)), dim, index,
+                (table, q_norm, k_norm))
+
+
+def _head_rows(index, name, t, out, rows, dim):
+    """bgtq_head_rows of t [rows, heads, dim] and where it goes (None: in place)."""
+    out = t if out is None else out
+    code = _codes().get(t.dtype)
+    if code is None or t.dim() != 3 or t.shape[0] != rows or t.shape[2] != dim or t.get_device() != index:
+        raise RangeError(f"{name} must be a [rows, heads, dim] tensor of float32, float16 or bfloat16 on the context's device")
+    if out.dtype != t.dtype or out.shape != t.shape or out.get_device() != index:
+        raise RangeError(f"{name} and its output must agree in shape, dtype and device")
+    s, o = t.stride(), out.stride()
+    if s[2] != 1 or o[2] != 1:
+        raise RangeError(f"{name}'s last dimension must be dense")
+    several, heads = rows > 1, t.shape[1]
+    return _lib.HeadRows(t.data_ptr(), out.data_ptr(), heads, code, s[0] if several else 0, s[1] if heads > 1 else 0,
+                         o[0] if several else 0, o[1] if heads > 1 else 0)
+
+
+def _positions(device, rope, positions):
+    """The number of rows, checked."""
+    index = device.index
+    _need(rope.device_index == index, "the rotation must lie on the context's device")
+    _dense(index, "positions", positions, "int64", 1)
+    _need(positions.is_contiguous(), "positions must be contiguous")
+    return positions.shape[0]
+
+
+def rotate(device, rope, positions, q=None, k=None, q_out=None, k_out=None) -> None:
+    """bgtq_rotate: rows q [n, Hq, dim] and k [n, Hkv, dim] (FP32, FP16 or BF16, any strides of the first two
+    dimensions) at positions [n] int64 normed and rotated into q_out and k_out (None: in place); rows whose position
+    is none of the table's are left out."""
+    n = _positions(device, rope, positions)
+    _need(q is not None or k is not None, "rotate needs q or k")
+    rows = [None if t is None else ctypes.byref(_head_rows(device.index, name, t, out, n, rope.dim))
+            for name, t, out in (("q", q, q_out), ("k", k, k_out))]
+    if n:
+        check(lib().bgtq_rotate(device.handle, rope.ref, rope.dim, n, _addr(positions), *rows))
+
+
+def paged_append(device, pool, slots, rope, positions, k, v, q=None, q_out=None) -> None:
+    """bgtq_paged_append: rows k, v [n, Hkv, dim] of a step into the slots [n] int64, k normed and rotated to positions
+    [n] int64 on the way, and the step's queries q [n, Hq, dim] (None: none) into q_out (None: in place). Rows of
+    slots outside the pool, or of positions outside the table, are not written."""
+    n = _positions(device, rope, positions)
+    _need(pool.dim == rope.dim, "the pool's heads and the rotation must agree in dim")
+    _need(k is not None and v is not None, "paged_append needs k and v")
+    r = _paged_rows(device, pool, slots, k, v)
+    _need(r.rows == n, "slots and positions must have an entry per row")
+    queries = None if q is None else ctypes.byref(_head_rows(device.index, "q", q, q_out, n, rope.dim))
+    if n:
+        check(lib().bgtq_paged_append(device.handle, pool.ref, ctypes.byref(r), rope.ref, _addr(positions), queries))
+
+
 class PagedDecode:
     """A paged decode's descriptor with its pool; holds the tensors."""
 

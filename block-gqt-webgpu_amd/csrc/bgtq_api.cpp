@@ -19,6 +19,7 @@
 
 #include "../../include/bgtq.h"
 #include "bgtq_internal.h"
+#include "rotate.h"
 
 using namespace bgtq;
 
@@ -1785,11 +1786,8 @@ PagedWriteParams rows_params(const bgtq_pages *g, const bgtq_paged_rows *r) {
 
 extern "C" {
 
-bgtq_status bgtq_paged_write(bgtq_context *ctx, const bgtq_pages *g, const bgtq_paged_rows *r) {
-  if (bgtq_status s = check_pages(g)) return s;
-  if (bgtq_status s = check_rows(r, g, true)) return s;
-  if (!ctx) return fail(BGTQ_ERR_RANGE, "null context");
-  if (!r->rows) return BGTQ_OK;
+// Rows into pages; rotation (null: none): K's on the way, and the queries'.
+static bgtq_status write_pages(bgtq_context *ctx, const bgtq_pages *g, const bgtq_paged_rows *r, const Rotation *rotation) {
   DeviceScope scope;
   if (bgtq_status s = ctx->use()) return s;
   const PagedWriteParams p = rows_params(g, r);
@@ -1812,14 +1810,106 @@ bgtq_status bgtq_paged_write(bgtq_context *ctx, const bgtq_pages *g, const bgtq_
     const bool wave = lds <= 160 * 1024;
     if (!tile && !wave) return fail(BGTQ_ERR_UNSUPPORTED, "paged write needs %d bytes of LDS (limit 163840)", lds);
     if (!tile || (wave && r->rows * g->kv_heads < encode_wave_max_rows(g->dim, true))) {
-      HIP_TRY(launch_paged_write(p, true, lds, device_cus(), ctx->stream), "paged write launch");
+      HIP_TRY(launch_paged_write(p, rotation, true, lds, device_cus(), ctx->stream), "paged write launch");
       return BGTQ_OK;
     }
-    HIP_TRY(launch_encode_tile_paged(p, g->dim, device_cus(), z, ctx->stream), "paged encode launch");
+    HIP_TRY(launch_encode_tile_paged(p, rotation, g->dim, device_cus(), z, ctx->stream), "paged encode launch");
     return BGTQ_OK;
   }
-  HIP_TRY(launch_paged_write(p, false, 0, device_cus(), ctx->stream), "paged write launch");
+  HIP_TRY(launch_paged_write(p, rotation, false, 0, device_cus(), ctx->stream), "paged write launch");
   return BGTQ_OK;
+}
+
+bgtq_status bgtq_paged_write(bgtq_context *ctx, const bgtq_pages *g, const bgtq_paged_rows *r) {
+  if (bgtq_status s = check_pages(g)) return s;
+  if (bgtq_status s = check_rows(r, g, true)) return s;
+  if (!ctx) return fail(BGTQ_ERR_RANGE, "null context");
+  if (!r->rows) return BGTQ_OK;
+  return write_pages(ctx, g, r, nullptr);
+}
+
+static bgtq_status check_rotation(const bgtq_rotation *r, int64_t rows, const int64_t *positions) {
+  if (!r) return fail(BGTQ_ERR_RANGE, "null rotation");
+  if (!r->table || r->table_rows < 1) return fail(BGTQ_ERR_RANGE, "rotation: a table of at least one row is required");
+  if (reinterpret_cast<uintptr_t>(r->table) % 16) return fail(BGTQ_ERR_RANGE, "rotation: the table must be 16-byte aligned");
+  if (reinterpret_cast<uintptr_t>(r->q_norm) % 4 || reinterpret_cast<uintptr_t>(r->k_norm) % 4)
+    return fail(BGTQ_ERR_RANGE, "rotation: norm weights must be 4-byte aligned");
+  if (!(r->eps >= 0.0) || !std::isfinite(r->eps)) return fail(BGTQ_ERR_RANGE, "rotation: eps must be finite and not negative");
+  if (rows && !positions) return fail(BGTQ_ERR_RANGE, "null positions");
+  if (reinterpret_cast<uintptr_t>(positions) % 8) return fail(BGTQ_ERR_RANGE, "positions must be 8-byte aligned");
+  return BGTQ_OK;
+}
+
+static bgtq_status check_head_rows(const bgtq_head_rows *h, int64_t rows, int32_t dim) {
+  if (h->heads < 1 || h->heads > 65535) return fail(BGTQ_ERR_RANGE, "rotation: heads must be in 1..65535");
+  if (h->dtype != BGTQ_DTYPE_F32 && h->dtype != BGTQ_DTYPE_F16 && h->dtype != BGTQ_DTYPE_BF16)
+    return fail(BGTQ_ERR_RANGE, "invalid rows dtype");
+  if (rows && (!h->src || !h->dst)) return fail(BGTQ_ERR_RANGE, "rotation: null rows");
+  if (h->src_row_stride < 0 || h->src_head_stride < 0 || h->dst_row_stride < 0 || h->dst_head_stride < 0)
+    return fail(BGTQ_ERR_RANGE, "negative rows stride");
+  const uintptr_t align = h->dtype == BGTQ_DTYPE_F32 ? 4 : 2;
+  if (reinterpret_cast<uintptr_t>(h->src) % align || reinterpret_cast<uintptr_t>(h->dst) % align)
+    return fail(BGTQ_ERR_RANGE, "rows must be aligned to their type");
+  if (!apart(rows, h->dst_row_stride, h->heads, h->dst_head_stride, dim)) return fail(BGTQ_ERR_RANGE, "overlapping rotated rows");
+  if (h->src == h->dst && ((rows > 1 && h->src_row_stride != h->dst_row_stride) ||
+                           (h->heads > 1 && h->src_head_stride != h->dst_head_stride)))
+    return fail(BGTQ_ERR_RANGE, "rows rotated in place must keep their strides");
+  return BGTQ_OK;
+}
+
+// The rotation of a call's rows; h (may be null): the rows it rotates itself, with `norm`.
+static Rotation rotation_of(const bgtq_rotation *r, const int64_t *positions, const bgtq_head_rows *h, const float *norm) {
+  Rotation x{};
+  x.table = r->table;
+  x.table_rows = r->table_rows;
+  x.positions = positions;
+  x.q_norm = norm;
+  x.k_norm = r->k_norm;
+  x.eps = r->eps;
+  if (h) {
+    x.q = h->src;
+    x.q_out = h->dst;
+    x.q_heads = h->heads;
+    x.q_dtype = h->dtype;
+    x.q_row_stride = h->src_row_stride;
+    x.q_head_stride = h->src_head_stride;
+    x.q_out_row_stride = h->dst_row_stride;
+    x.q_out_head_stride = h->dst_head_stride;
+  }
+  return x;
+}
+
+bgtq_status bgtq_rotate(bgtq_context *ctx, const bgtq_rotation *r, int32_t dim, int64_t rows, const int64_t *positions,
+                        const bgtq_head_rows *q, const bgtq_head_rows *k) {
+  if (dim != 64 && dim != 128) return fail(BGTQ_ERR_UNSUPPORTED, "heads of dim 64 or 128 are rotated (got %d)", dim);
+  if (rows < 0 || rows > INT32_MAX) return fail(BGTQ_ERR_RANGE, "rows must be in 0..2^31 - 1");
+  if (bgtq_status s = check_rotation(r, rows, positions)) return s;
+  if (!q && !k) return fail(BGTQ_ERR_RANGE, "null q and k");
+  if (q)
+    if (bgtq_status s = check_head_rows(q, rows, dim)) return s;
+  if (k)
+    if (bgtq_status s = check_head_rows(k, rows, dim)) return s;
+  if (!ctx) return fail(BGTQ_ERR_RANGE, "null context");
+  if (!rows) return BGTQ_OK;
+  DeviceScope scope;
+  if (bgtq_status s = ctx->use()) return s;
+  HIP_TRY(launch_rotate(rotation_of(r, positions, q, r->q_norm), rotation_of(r, positions, k, r->k_norm), rows, dim,
+                        device_cus(), ctx->stream),
+          "rotation launch");
+  return BGTQ_OK;
+}
+
+bgtq_status bgtq_paged_append(bgtq_context *ctx, const bgtq_pages *g, const bgtq_paged_rows *rows, const bgtq_rotation *r,
+                              const int64_t *positions, const bgtq_head_rows *q) {
+  if (bgtq_status s = check_pages(g)) return s;
+  if (bgtq_status s = check_rows(rows, g, true)) return s;
+  if (bgtq_status s = check_rotation(r, rows->rows, positions)) return s;
+  if (q)
+    if (bgtq_status s = check_head_rows(q, rows->rows, g->dim)) return s;
+  if (!ctx) return fail(BGTQ_ERR_RANGE, "null context");
+  if (!rows->rows) return BGTQ_OK;
+  const Rotation rotation = rotation_of(r, positions, q, r->q_norm);
+  return write_pages(ctx, g, rows, &rotation);
 }
 
 bgtq_status bgtq_paged_read(bgtq_context *ctx, const bgtq_pages *g, const bgtq_paged_rows *r) {

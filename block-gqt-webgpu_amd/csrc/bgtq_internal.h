@@ -488,12 +488,18 @@ hipError_t launch_encode_tile(const EncodeJobDev *jobs, int n_jobs, int dim, int
                               const EncodeTileSizes &z, hipStream_t stream);
 hipError_t launch_encode_tile_args(const EncodeTileLaunch &launch, int dim, int src_f32, int64_t max_rows, int cus,
                                    const EncodeTileSizes &z, hipStream_t stream);
-hipError_t launch_encode_tile_paged(const PagedWriteParams &p, int dim, int cus, const EncodeTileSizes &z,
-                                    hipStream_t stream);
+// rotation (null: none): K rows normed and rotated on the way, and the call's queries.
+struct Rotation;
+hipError_t launch_encode_tile_paged(const PagedWriteParams &p, const Rotation *rotation, int dim, int cus,
+                                    const EncodeTileSizes &z, hipStream_t stream);
 // Paged rows (paged_rows.hip). Write: packed K with a wave per row and, in
 // the same launch, V; or FP16 K and V alone (packed null). Read: both back.
 int paged_write_lds_bytes(int dim, int enc_bytes);
-hipError_t launch_paged_write(const PagedWriteParams &p, bool with_k, int lds_bytes, int cus, hipStream_t stream);
+hipError_t launch_paged_write(const PagedWriteParams &p, const Rotation *rotation, bool with_k, int lds_bytes, int cus,
+                              hipStream_t stream);
+// Rows of two sets of heads normed and rotated (rotate.hip): q, and k in a
+// rotation's query fields (its q null: none).
+hipError_t launch_rotate(const Rotation &q, const Rotation &k, int64_t rows, int dim, int cus, hipStream_t stream);
 hipError_t launch_paged_read(const PagedWriteParams &p, int cus, hipStream_t stream);
 // Causal attention over packed prompts (prompt.hip), and its workgroups.
 int64_t prompt_workgroups(const bgtq_prompt_desc &d);

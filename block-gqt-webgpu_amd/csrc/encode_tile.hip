@@ -105,14 +105,24 @@ __host__ __device__ inline TileLds tile_lds(int n_codebooks, int groups, int row
 struct DenseDst {
   static constexpr bool kPaged = false;
 };
+template <typename Rot = NoRotation>
 struct PagedDst {
   static constexpr bool kPaged = true;
   PagedSlots slots;
   int64_t packed_page_stride, norms_page_stride;  // bytes, elements
+  Rot rotation;
+  __device__ __forceinline__ bool find(int64_t row, int64_t &page, int &at) const {
+    const bool in = slots.find(row, page, at);
+    if constexpr (Rot::kOn) return rotation.kept(row) && in;
+    return in;
+  }
 };
 
-// Waves per SIMD that the register budget leaves room for.
-constexpr int tile_waves_per_simd(int D, bool src_f32) { return D != 64 ? 2 : src_f32 ? 3 : 4; }
+// Waves per SIMD that the register budget leaves room for (rotated rows: the
+// table row's 2 x D / 4 values are held too).
+constexpr int tile_waves_per_simd(int D, bool src_f32, bool rotated = false) {
+  return D != 64 || rotated ? 2 : src_f32 ? 3 : 4;
+}
 
 // One job: its packed and norms already point at its first destination row.
 //
@@ -123,9 +133,10 @@ constexpr int tile_waves_per_simd(int D, bool src_f32) { return D != 64 ? 2 : sr
 // chain meets a non-finite input. The chain runs over the 8-wide blocks that
 // touch the group (encode.hip; whole groups in encode_bulk.hip), or with
 // WHOLE_ROWS over the row (the wave encoder, for smaller calls).
-template <int D, int SRC, bool WHOLE_ROWS, typename Dst = DenseDst>
+template <int D, int SRC, bool WHOLE_ROWS, typename Dst = DenseDst, typename Rot = NoRotation>
 __device__ __forceinline__ void encode_tile_body(const EncodeTileJob &job, const int64_t rows, int max_codebooks,
-                                                 int max_groups, int max_row_bytes, const Dst &place = Dst{}) {
+                                                 int max_groups, int max_row_bytes, const Dst &place = Dst{},
+                                                 const Rot &rotation = Rot{}) {
   using S = Tile<D>;
   constexpr bool SRC_F32 = SRC == BGTQ_DTYPE_F32, SRC_BF16 = SRC == BGTQ_DTYPE_BF16;
   constexpr int KS = S::KS, NT = S::NT, NV = S::NV, W = tile_waves(D), TH = 64 * W;
@@ -154,7 +165,19 @@ __device__ __forceinline__ void encode_tile_body(const EncodeTileJob &job, const
   constexpr int kElem = SRC_F32 ? 4 : 2, NP = KS * kElem / 16;  // 16-byte pieces per lane
   const bool vec = reinterpret_cast<uintptr_t>(job.src) % 16 == 0 && (job.src_stride * kElem) % 16 == 0;  // uniform
   u32x4 raw[NP];
+  // Rotated rows: the cosines and sines of this lane's values KS gq + 0 .. KS - 1.
+  f32x4 turn_c[Rot::kOn ? KS / 4 : 1], turn_s[Rot::kOn ? KS / 4 : 1];
   auto load_rows = [&](int64_t b, int gq, int col) {
+    if constexpr (Rot::kOn) {
+      const float *cs;
+      rotation.find(min(b * kTileRows + col, rows - 1), cs, D);
+      const f32x4 *c4 = reinterpret_cast<const f32x4 *>(cs + KS * (gq & 1)), *s4 = reinterpret_cast<const f32x4 *>(cs + D / 2 + KS * (gq & 1));
+#pragma unroll
+      for (int k = 0; k < KS / 4; ++k) {
+        turn_c[k] = c4[k];
+        turn_s[k] = s4[k];
+      }
+    }
     const int nr = (int)min((int64_t)kTileRows, rows - b * kTileRows);
     const uint8_t *base = static_cast<const uint8_t *>(job.src) + b * kTileRows * (int64_t)job.src_stride * kElem;
     const __amdgpu_buffer_rsrc_t r =
@@ -180,6 +203,45 @@ __device__ __forceinline__ void encode_tile_body(const EncodeTileJob &job, const
   // holds an infinity or a NaN (FP16 squares sum to at most 3e11).
   auto stage_rows = [&](int gq, int col) {
     float squares = 0.0f;
+    if constexpr (Rot::kOn) {
+      // Normed and rotated in FP32 (rotate.h): a value's pair is the same one
+      // of the lane 32 away, a row's sum over the four lanes of its column.
+      float x[KS];
+#pragma unroll
+      for (int i = 0; i < KS; ++i) {
+        if (SRC_F32) x[i] = __uint_as_float(raw[i / 4][i % 4]);
+        else {
+          const uint32_t u = raw[i / 8][(i / 2) % 4] >> (16 * (i & 1)) & 0xffffu;
+          x[i] = SRC_BF16 ? __uint_as_float(u << 16) : f16_bits_to_f32((uint16_t)u);
+        }
+      }
+      if (rotation.k_norm) {
+        double sum = 0.0;
+#pragma unroll
+        for (int i = 0; i < KS; ++i) sum += rot::square(x[i]);
+        const float f = rot::factor(rot::col_sum(sum), D, rotation.eps);
+        const float *w = rotation.k_norm + KS * gq;
+#pragma unroll
+        for (int i = 0; i < KS; ++i) x[i] = (x[i] * f) * w[i];
+      }
+#pragma unroll
+      for (int k = 0; k < KS / 4; ++k) {
+        uint32_t v[2];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t u = __float_as_uint(x[4 * k + e]);
+          const auto both = __builtin_amdgcn_permlane32_swap(u, u, false, false);  // the lower lane's, the upper's
+          const uint32_t h = f32_to_f16_bits(rot::turn(x[4 * k + e], __uint_as_float(gq < 2 ? both[1] : both[0]), turn_c[k][e],
+                                                       turn_s[k][e], gq >= 2));
+          v[e >> 1] = e & 1 ? v[e >> 1] | h << 16 : h;
+        }
+        typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+        squares = __builtin_amdgcn_fdot2(__builtin_bit_cast(half2_t, v[0]), __builtin_bit_cast(half2_t, v[0]), squares, false);
+        squares = __builtin_amdgcn_fdot2(__builtin_bit_cast(half2_t, v[1]), __builtin_bit_cast(half2_t, v[1]), squares, false);
+        *reinterpret_cast<u32x2 *>(wv + col * S::XROW + 2 * KS * gq + 8 * k) = u32x2{v[0], v[1]};
+      }
+      return __builtin_amdgcn_ballot_w64(!(squares < INFINITY));
+    }
 #pragma unroll
     for (int k = 0; k < KS / 4; ++k) {
       uint32_t v[2];
@@ -310,7 +372,7 @@ __device__ __forceinline__ void encode_tile_body(const EncodeTileJob &job, const
       const int nb = (int)min((int64_t)kTileRows, rows - b * kTileRows);
       int64_t page;
       int at;
-      if (col < nb && place.slots.find(b * kTileRows + col, page, at)) {
+      if (col < nb && place.find(b * kTileRows + col, page, at)) {
         prow_pg = job.packed + page * place.packed_page_stride + (int64_t)at * RB;
         nrow_pg = job.norms + page * place.norms_page_stride + (int64_t)at * NS;
       }
@@ -539,7 +601,7 @@ __device__ __forceinline__ void encode_tile_body(const EncodeTileJob &job, const
     if constexpr (Dst::kPaged) {
       int64_t page = 0;
       int at = 0;
-      stored = stored && place.slots.find(row, page, at);
+      stored = stored && place.find(row, page, at);
       prow_at = job.packed + page * place.packed_page_stride + (int64_t)at * RB;
       nrow_at = job.norms + page * place.norms_page_stride + (int64_t)at * NS;
     }
@@ -609,27 +671,30 @@ __global__ __launch_bounds__(64 * tile_waves(D), tile_waves_per_simd(D, SRC_F32)
 // K rows into pages, a KV head per grid y; the workgroups share the head's V
 // rows too (16384 rows x 2 heads written and read back 20.6 us, with V in a launch
 // of its own 21.6).
-template <int D, int SRC>
-__global__ __launch_bounds__(64 * tile_waves(D), tile_waves_per_simd(D, SRC == BGTQ_DTYPE_F32)) void encode_tile_paged_kernel(
-    PagedWriteParams p, int max_codebooks, int max_groups, int max_row_bytes) {
+// Rot on: K rows are normed and rotated first; the workgroups share the queries too.
+template <int D, int SRC, typename Rot>
+__global__ __launch_bounds__(64 * tile_waves(D), tile_waves_per_simd(D, SRC == BGTQ_DTYPE_F32, Rot::kOn)) void encode_tile_paged_kernel(
+    PagedWriteParams p, Rot rotation, int max_codebooks, int max_groups, int max_row_bytes) {
   const int h = blockIdx.y;
   const EncodeTileJob job{p.tables[h], static_cast<const uint8_t *>(p.k) + h * p.k_head_stride * (SRC == BGTQ_DTYPE_F32 ? 4 : 2),
                           p.packed + h * p.packed_head_stride, p.norms + h * p.norms_head_stride, (int32_t)p.k_row_stride, 0};
-  const PagedDst place{p.slots, p.packed_page_stride, p.norms_page_stride};
+  const PagedDst<Rot> place{p.slots, p.packed_page_stride, p.norms_page_stride, rotation};
   constexpr int kThreads = 64 * tile_waves(D), kLanes = D / 8;
   write_rows<D, false>(p, h, (int64_t)blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes,
-                       (int64_t)gridDim.x * (kThreads / kLanes));
-  encode_tile_body<D, SRC, true, PagedDst>(job, p.slots.rows, max_codebooks, max_groups, max_row_bytes, place);
+                       (int64_t)gridDim.x * (kThreads / kLanes), rotation);
+  if constexpr (Rot::kOn)
+    rot::rotate_queries<D, kThreads>(rotation, p.slots.rows, (int64_t)h * gridDim.x + blockIdx.x, (int64_t)gridDim.x * gridDim.y);
+  encode_tile_body<D, SRC, true, PagedDst<Rot>>(job, p.slots.rows, max_codebooks, max_groups, max_row_bytes, place, rotation);
 }
 
-template <typename K, typename J>
+template <typename K, typename... J>
 hipError_t launch_k(K kernel, const hipError_t allowed, const dim3 grid, int threads, int lds, hipStream_t stream,
-                    const J &jobs, const EncodeTileSizes &z) {
+                    const EncodeTileSizes &z, const J &...jobs) {
   if (allowed != hipSuccess) {
     (void)hipGetLastError();
     return allowed;
   }
-  hipLaunchKernelGGL(kernel, grid, dim3((unsigned)threads), lds, stream, jobs, z.codebooks, z.groups, z.row_bytes);
+  hipLaunchKernelGGL(kernel, grid, dim3((unsigned)threads), lds, stream, jobs..., z.codebooks, z.groups, z.row_bytes);
   return hipGetLastError();
 }
 
@@ -640,11 +705,11 @@ hipError_t launch_d(const EncodeJobDev *table, const EncodeTileLaunch *args, con
   if (table) {
     static const hipError_t ok = hipFuncSetAttribute((const void *)encode_tile_kernel<D, SRC_F32>,
                                                      hipFuncAttributeMaxDynamicSharedMemorySize, kLdsLimit);
-    return launch_k(encode_tile_kernel<D, SRC_F32>, ok, grid, threads, lds, stream, table, z);
+    return launch_k(encode_tile_kernel<D, SRC_F32>, ok, grid, threads, lds, stream, z, table);
   }
   static const hipError_t ok = hipFuncSetAttribute((const void *)encode_tile_args_kernel<D, SRC_F32>,
                                                    hipFuncAttributeMaxDynamicSharedMemorySize, kLdsLimit);
-  return launch_k(encode_tile_args_kernel<D, SRC_F32>, ok, grid, threads, lds, stream, *args, z);
+  return launch_k(encode_tile_args_kernel<D, SRC_F32>, ok, grid, threads, lds, stream, z, *args);
 }
 
 hipError_t launch_any(const EncodeJobDev *table, const EncodeTileLaunch *args, int n_jobs, int dim, int src_f32,
@@ -657,28 +722,40 @@ hipError_t launch_any(const EncodeJobDev *table, const EncodeTileLaunch *args, i
   return src_f32 ? launch_d<128, true>(table, args, grid, z, stream) : launch_d<128, false>(table, args, grid, z, stream);
 }
 
-template <int D, int SRC>
-hipError_t launch_paged(const PagedWriteParams &p, const dim3 grid, const EncodeTileSizes &z, hipStream_t stream) {
+template <int D, int SRC, typename Rot>
+hipError_t launch_paged(const PagedWriteParams &p, const Rot &rotation, const dim3 grid, const EncodeTileSizes &z,
+                        hipStream_t stream) {
   const int lds = tile_lds<D>(z.codebooks, z.groups, z.row_bytes).total, threads = 64 * tile_waves(D);
-  static const hipError_t ok = hipFuncSetAttribute((const void *)encode_tile_paged_kernel<D, SRC>,
+  static const hipError_t ok = hipFuncSetAttribute((const void *)encode_tile_paged_kernel<D, SRC, Rot>,
                                                    hipFuncAttributeMaxDynamicSharedMemorySize, kLdsLimit);
-  return launch_k(encode_tile_paged_kernel<D, SRC>, ok, grid, threads, lds, stream, p, z);
+  return launch_k(encode_tile_paged_kernel<D, SRC, Rot>, ok, grid, threads, lds, stream, z, p, rotation);
+}
+
+template <int D, typename Rot>
+hipError_t launch_paged_src(const PagedWriteParams &p, const Rot &rotation, const dim3 grid, const EncodeTileSizes &z,
+                            hipStream_t stream) {
+  return p.k_dtype == BGTQ_DTYPE_F32   ? launch_paged<D, BGTQ_DTYPE_F32>(p, rotation, grid, z, stream)
+         : p.k_dtype == BGTQ_DTYPE_F16 ? launch_paged<D, BGTQ_DTYPE_F16>(p, rotation, grid, z, stream)
+                                       : launch_paged<D, BGTQ_DTYPE_BF16>(p, rotation, grid, z, stream);
+}
+
+// Workgroups that the chip holds at once (encode_tile_resident).
+int64_t resident_of(int dim, int waves_per_simd, int cus, const EncodeTileSizes &z) {
+  const int lds = encode_tile_lds_bytes(dim, z.codebooks, z.groups, z.row_bytes);
+  return (int64_t)cus * std::max(1, std::min(4 * waves_per_simd / tile_waves(dim), kLdsLimit / lds));
 }
 
 }  // namespace
 
-hipError_t launch_encode_tile_paged(const PagedWriteParams &p, int dim, int cus, const EncodeTileSizes &z,
-                                    hipStream_t stream) {
+hipError_t launch_encode_tile_paged(const PagedWriteParams &p, const Rotation *rotation, int dim, int cus,
+                                    const EncodeTileSizes &z, hipStream_t stream) {
   const int64_t wg_rows = encode_tile_wg_rows(dim), most = (p.slots.rows + wg_rows - 1) / wg_rows;
-  const int64_t resident = encode_tile_resident(dim, p.k_dtype == BGTQ_DTYPE_F32, cus, z);
+  const int64_t resident = resident_of(dim, tile_waves_per_simd(dim, p.k_dtype == BGTQ_DTYPE_F32, rotation != nullptr), cus, z);
   const dim3 grid((unsigned)std::max<int64_t>(1, std::min<int64_t>(most, resident / p.kv_heads)), (unsigned)p.kv_heads);
-  auto go = [&](auto f32, auto f16, auto bf16) {
-    return p.k_dtype == BGTQ_DTYPE_F32 ? f32(p, grid, z, stream) : p.k_dtype == BGTQ_DTYPE_F16 ? f16(p, grid, z, stream)
-                                                                                               : bf16(p, grid, z, stream);
-  };
-  return dim == 64 ? go(launch_paged<64, BGTQ_DTYPE_F32>, launch_paged<64, BGTQ_DTYPE_F16>, launch_paged<64, BGTQ_DTYPE_BF16>)
-                   : go(launch_paged<128, BGTQ_DTYPE_F32>, launch_paged<128, BGTQ_DTYPE_F16>,
-                        launch_paged<128, BGTQ_DTYPE_BF16>);
+  if (rotation)
+    return dim == 64 ? launch_paged_src<64>(p, *rotation, grid, z, stream) : launch_paged_src<128>(p, *rotation, grid, z, stream);
+  return dim == 64 ? launch_paged_src<64>(p, NoRotation{}, grid, z, stream)
+                   : launch_paged_src<128>(p, NoRotation{}, grid, z, stream);
 }
 
 bool encode_tile_layout(const DevTables *T) {
@@ -707,8 +784,7 @@ int encode_tile_wg_rows(int dim) { return kTileRows * tile_waves(dim); }
 // them) shared by the jobs, rounded down: a few more than fit take a second
 // round as long as the first. A wave walks its job's blocks with that stride.
 int64_t encode_tile_resident(int dim, int src_f32, int cus, const EncodeTileSizes &z) {
-  const int lds = encode_tile_lds_bytes(dim, z.codebooks, z.groups, z.row_bytes);
-  return (int64_t)cus * std::max(1, std::min(4 * tile_waves_per_simd(dim, src_f32) / tile_waves(dim), kLdsLimit / lds));
+  return resident_of(dim, tile_waves_per_simd(dim, src_f32), cus, z);
 }
 
 hipError_t launch_encode_tile(const EncodeJobDev *jobs, int n_jobs, int dim, int src_f32, int64_t max_rows, int cus,

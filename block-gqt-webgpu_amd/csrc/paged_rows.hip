@@ -45,17 +45,25 @@ __host__ __device__ inline WriteLds write_lds(int enc_bytes) {
   return L;
 }
 
-template <int D, bool WITH_K>
-__global__ __launch_bounds__(kThreads) void paged_write_kernel(PagedWriteParams p) {
+// Rot on: K rows are normed and rotated first, and one more slice of grid y
+// takes the queries.
+template <int D, bool WITH_K, typename Rot>
+__global__ __launch_bounds__(kThreads) void paged_write_kernel(PagedWriteParams p, Rot rotation) {
   constexpr int JL = row_enc::Lane<D>::JL, L8 = D / 8;
   extern __shared__ __align__(16) uint8_t smem[];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int head = blockIdx.y;
+  if constexpr (Rot::kOn) {
+    if (head == (WITH_K ? p.kv_heads + 1 : p.k_f16 ? 2 : 1)) {
+      rot::rotate_queries<D, kThreads>(rotation, p.slots.rows, blockIdx.x, gridDim.x);
+      return;
+    }
+  }
   if (!WITH_K || head == p.kv_heads) {
     const int64_t first = (int64_t)blockIdx.x * (kThreads / L8) + tid / L8, step = (int64_t)gridDim.x * (kThreads / L8);
-    if (!WITH_K && head == 1) write_rows<D, true>(p, -1, first, step);
-    else write_rows<D, false>(p, -1, first, step);
+    if (!WITH_K && head == 1) write_rows<D, true>(p, -1, first, step, rotation);
+    else write_rows<D, false>(p, -1, first, step, rotation);
     return;
   }
   const DevTables *Tg = p.tables[head];
@@ -75,8 +83,34 @@ __global__ __launch_bounds__(kThreads) void paged_write_kernel(PagedWriteParams 
   }
   auto load_row = [&](int64_t r, float (&v)[JL]) {  // (a row past the call's reads row 0)
     const int64_t at = (r < p.slots.rows ? r : 0) * p.k_row_stride + head * p.k_head_stride + lane;
+    if constexpr (Rot::kOn) {
+      // A value pairs with the one 32 lanes away (d=64) or the lane's other one.
+      const float *cs;
+      rotation.find(r < p.slots.rows ? r : 0, cs, D);
+      const float c = cs[lane & (D / 2 - 1)], s = cs[D / 2 + (lane & (D / 2 - 1))];
+      float x[JL];
 #pragma unroll
-    for (int jl = 0; jl < JL; ++jl) v[jl] = f16_bits_to_f32(f32_to_f16_bits(load_one(p.k, p.k_dtype, at + 64 * jl)));
+      for (int jl = 0; jl < JL; ++jl) x[jl] = load_one(p.k, p.k_dtype, at + 64 * jl);
+      if (rotation.k_norm) {
+        double sum = rot::square(x[0]);
+        if (JL > 1) sum += rot::square(x[JL - 1]);
+        const float f = rot::factor(rot::col_sum(rot::lanes_sum<16>(sum)), D, rotation.eps);
+#pragma unroll
+        for (int jl = 0; jl < JL; ++jl) x[jl] = (x[jl] * f) * rotation.k_norm[lane + 64 * jl];
+      }
+      float y[JL];
+      if constexpr (JL == 1) {
+        y[0] = rot::turn(x[0], __shfl_xor(x[0], 32, 64), c, s, lane >= 32);
+      } else {
+        y[0] = rot::turn(x[0], x[1], c, s, false);
+        y[1] = rot::turn(x[1], x[0], c, s, true);
+      }
+#pragma unroll
+      for (int jl = 0; jl < JL; ++jl) v[jl] = f16_bits_to_f32(f32_to_f16_bits(y[jl]));
+    } else {
+#pragma unroll
+      for (int jl = 0; jl < JL; ++jl) v[jl] = f16_bits_to_f32(f32_to_f16_bits(load_one(p.k, p.k_dtype, at + 64 * jl)));
+    }
   };
   int64_t row = (int64_t)blockIdx.x * kWaves + wave;
   float xn[JL];
@@ -106,7 +140,9 @@ __global__ __launch_bounds__(kThreads) void paged_write_kernel(PagedWriteParams 
         T, c, x, [&](int i, int jl) { return rot_t[i * D + lane + 64 * jl]; }, lut, books, scr, lane);
     int64_t page;
     int at;
-    if (p.slots.find(row, page, at)) {  // (uniform)
+    bool kept = p.slots.find(row, page, at);
+    if constexpr (Rot::kOn) kept = kept && rotation.kept(row);
+    if (kept) {  // (uniform)
       uint8_t *prow = p.packed + page * p.packed_page_stride + head * p.packed_head_stride + (int64_t)at * RB;
       uint16_t *nrow = p.norms + page * p.norms_page_stride + head * p.norms_head_stride + (int64_t)at * NS;
       for (int o = lane; o < RB; o += 64) prow[o] = row_enc::packed_byte(scr.codes, o, nib, logical);
@@ -480,24 +516,28 @@ __global__ __launch_bounds__(64 * Read<D>::W, D == 64 ? 3 : 2) void paged_read_p
   }
 }
 
-template <int D>
-hipError_t launch_write_d(const PagedWriteParams &p, bool with_k, int lds, int cus, hipStream_t stream) {
+template <int D, typename Rot>
+hipError_t launch_write_d(const PagedWriteParams &p, const Rot &rotation, bool with_k, int lds, int cus, hipStream_t stream) {
   const int64_t heads = p.kv_heads, per_wg = kThreads / (D / 8);
+  unsigned queries = 0;
+  if constexpr (Rot::kOn) queries = rotation.q != nullptr;
   // About 16 waves per compute unit, as the row encoder of dense rows.
   const int64_t most = 4 * (int64_t)cus;
   if (!with_k) {
     const int64_t wgs = std::min<int64_t>((p.slots.rows * heads + per_wg - 1) / per_wg, 2 * most);
-    hipLaunchKernelGGL((paged_write_kernel<D, false>), dim3((unsigned)wgs, p.k_f16 ? 2u : 1u), dim3(kThreads), 0, stream, p);
+    hipLaunchKernelGGL((paged_write_kernel<D, false, Rot>), dim3((unsigned)wgs, (p.k_f16 ? 2u : 1u) + queries), dim3(kThreads), 0,
+                       stream, p, rotation);
     return hipGetLastError();
   }
-  static const hipError_t ok = hipFuncSetAttribute((const void *)paged_write_kernel<D, true>,
+  static const hipError_t ok = hipFuncSetAttribute((const void *)paged_write_kernel<D, true, Rot>,
                                                    hipFuncAttributeMaxDynamicSharedMemorySize, kLdsLimit);
   if (ok != hipSuccess) {
     (void)hipGetLastError();
     return ok;
   }
   const int64_t wgs = std::min<int64_t>((p.slots.rows + kWaves - 1) / kWaves, std::max<int64_t>(1, most / heads));
-  hipLaunchKernelGGL((paged_write_kernel<D, true>), dim3((unsigned)wgs, (unsigned)heads + 1), dim3(kThreads), lds, stream, p);
+  hipLaunchKernelGGL((paged_write_kernel<D, true, Rot>), dim3((unsigned)wgs, (unsigned)heads + 1 + queries), dim3(kThreads), lds,
+                     stream, p, rotation);
   return hipGetLastError();
 }
 
@@ -544,9 +584,13 @@ int paged_write_lds_bytes(int dim, int enc_bytes) {
   return dim == 64 ? write_lds<64>(enc_bytes).total : write_lds<128>(enc_bytes).total;
 }
 
-hipError_t launch_paged_write(const PagedWriteParams &p, bool with_k, int lds_bytes, int cus, hipStream_t stream) {
-  return p.dim == 64 ? launch_write_d<64>(p, with_k, lds_bytes, cus, stream)
-                     : launch_write_d<128>(p, with_k, lds_bytes, cus, stream);
+hipError_t launch_paged_write(const PagedWriteParams &p, const Rotation *rotation, bool with_k, int lds_bytes, int cus,
+                              hipStream_t stream) {
+  if (rotation)
+    return p.dim == 64 ? launch_write_d<64>(p, *rotation, with_k, lds_bytes, cus, stream)
+                       : launch_write_d<128>(p, *rotation, with_k, lds_bytes, cus, stream);
+  return p.dim == 64 ? launch_write_d<64>(p, NoRotation{}, with_k, lds_bytes, cus, stream)
+                     : launch_write_d<128>(p, NoRotation{}, with_k, lds_bytes, cus, stream);
 }
 
 hipError_t launch_paged_read(const PagedWriteParams &p, int cus, hipStream_t stream) {

@@ -12,6 +12,7 @@
 #include "bgtq_internal.h"
 #include "encode_row.h"
 #include "gfx950_common.h"
+#include "rotate_rows.h"
 
 namespace bgtq {
 namespace {
@@ -62,6 +63,58 @@ __device__ __forceinline__ void load8_half(const void *src, int dtype, bool vec,
   }
 }
 
+// Eight values from element `at` on, as FP32.
+__device__ __forceinline__ void load8_float(const void *src, int dtype, bool vec, int64_t at, float (&x)[8]) {
+  if (!vec) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = load_one(src, dtype, at + k);
+    return;
+  }
+  if (dtype == BGTQ_DTYPE_F32) {
+    const f32x4 *p = reinterpret_cast<const f32x4 *>(static_cast<const float *>(src) + at);
+    const f32x4 a = p[0], b = p[1];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = k < 4 ? a[k & 3] : b[k & 3];
+    return;
+  }
+  const u32x4 w = *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(src) + at);
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const uint32_t u = k & 1 ? w[k >> 1] >> 16 : w[k >> 1] & 0xffffu;
+    x[k] = dtype == BGTQ_DTYPE_F16 ? f16_bits_to_f32((uint16_t)u) : __uint_as_float(u << 16);
+  }
+}
+// The same of a row normed and rotated (rotate.h), rounded to FP16: lane `sub`
+// of the row's D / 8 has values 8 sub on, those they pair with half a row away.
+template <int D>
+__device__ __forceinline__ void load8_rotated(const void *src, int dtype, bool vec, int64_t row_at, int sub, const Rotation &r,
+                                              const float *cs, uint16_t (&h)[8]) {
+  constexpr int L = D / 8;
+  const int mine = 8 * sub, other = 8 * (sub ^ (L / 2)), pair = 8 * (sub & (L / 2 - 1));
+  float x[8], y[8];
+  load8_float(src, dtype, vec, row_at + mine, x);
+  load8_float(src, dtype, vec, row_at + other, y);
+  float c[8], s[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    c[k] = cs[pair + k];
+    s[k] = cs[D / 2 + pair + k];
+  }
+  if (r.k_norm) {
+    double sum = 0.0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) sum += rot::square(x[k]);
+    const float f = rot::factor(rot::lanes_sum<L>(sum), D, r.eps);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      x[k] = (x[k] * f) * r.k_norm[mine + k];
+      y[k] = (y[k] * f) * r.k_norm[other + k];
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 8; ++k) h[k] = f32_to_f16_bits(rot::turn(x[k], y[k], c[k], s[k], sub >= L / 2));
+}
+
 constexpr uint16_t kMaxScale = 0x6007u;  // 515.5 in FP16
 
 // Maximum over the L = 8 or 16 lanes that share a row.
@@ -76,8 +129,9 @@ __device__ __forceinline__ int lanes_max(int v) {
 
 // V, or FP16 K (of_k), of the call to the pool: rows first, first + step, ...
 // of KV head `only`; only < 0: of all heads, row i of head h numbered i * heads + h.
-template <int D, bool of_k>
-__device__ __forceinline__ void write_rows(const PagedWriteParams &p, int only, int64_t first, int64_t step) {
+template <int D, bool of_k, typename Rot = NoRotation>
+__device__ __forceinline__ void write_rows(const PagedWriteParams &p, int only, int64_t first, int64_t step,
+                                           const Rot &rotation = Rot{}) {
   constexpr int L = D / 8;
   const int lane = threadIdx.x & 63, sub = lane % L;
   const void *src = of_k ? p.k : p.v;
@@ -90,9 +144,16 @@ __device__ __forceinline__ void write_rows(const PagedWriteParams &p, int only, 
     const int head = only < 0 ? (int)(r - row * p.kv_heads) : only;
     int64_t page;
     int at;
-    const bool kept = p.slots.find(row, page, at);
+    bool kept = p.slots.find(row, page, at);
     uint16_t h[8];
-    load8_half(src, dtype, vec, row * rs + head * hs + 8 * sub, h);
+    if constexpr (Rot::kOn) {
+      const float *cs;
+      kept = rotation.find(row, cs, D) && kept;
+      if constexpr (of_k) load8_rotated<D>(src, dtype, vec, row * rs + head * hs, sub, rotation, cs, h);
+      else load8_half(src, dtype, vec, row * rs + head * hs + 8 * sub, h);
+    } else {
+      load8_half(src, dtype, vec, row * rs + head * hs + 8 * sub, h);
+    }
     if (!kept) continue;  // (the lanes of a row agree)
     if (!q8) {
       uint16_t *dst = of_k ? p.k_f16 + page * p.kp_page_stride + head * p.kp_head_stride

@@ -1,0 +1,29 @@
+// Head norms and position rotation of query and key rows in one pass
+// (bgtq_rotate): rotate_rows.h has the arithmetic, a workgroup a run of whole
+// rows, so that the heads of a row share its table row in the L1 cache; grid y
+// is the queries, then the keys.
+#include "rotate_rows.h"
+
+namespace bgtq {
+namespace {
+
+constexpr int kThreads = 256;
+
+template <int D>
+__global__ __launch_bounds__(kThreads) void rotate_kernel(Rotation q, Rotation k, int64_t rows) {
+  if (blockIdx.y == 0) rot::rotate_queries<D, kThreads>(q, rows, blockIdx.x, gridDim.x);
+  else rot::rotate_queries<D, kThreads>(k, rows, blockIdx.x, gridDim.x);
+}
+
+}  // namespace
+
+hipError_t launch_rotate(const Rotation &q, const Rotation &k, int64_t rows, int dim, int cus, hipStream_t stream) {
+  const int64_t lanes = rows * std::max(q.q ? q.q_heads : 0, k.q ? k.q_heads : 0) * (dim / 8);
+  const int64_t wgs = std::max<int64_t>(1, std::min<int64_t>({rows, (lanes + kThreads - 1) / kThreads, 8 * (int64_t)cus}));
+  const dim3 grid((unsigned)wgs, k.q ? 2u : 1u);
+  if (dim == 64) hipLaunchKernelGGL(rotate_kernel<64>, grid, dim3(kThreads), 0, stream, q, k, rows);
+  else hipLaunchKernelGGL(rotate_kernel<128>, grid, dim3(kThreads), 0, stream, q, k, rows);
+  return hipGetLastError();
+}
+
+}  // namespace bgtq

@@ -60,7 +60,8 @@ const char *bgtq_last_error(void);
  * call). 5: bgtq_attention_record_timed; attention over FP32 V runs on the fused kernel. 6:
  * bgtq_prefill_append; the decode workspace holds one more partial per query head and the prefill
  * workspace the appended rows' partials (allocate what the *_workspace_size calls return).
- * bgtq_paged_* and bgtq_prompt_attention came later without changing any of these. */
+ * bgtq_paged_*, bgtq_prompt_attention, bgtq_rotate and the *_window forms came later without
+ * changing any of these. */
 int32_t bgtq_abi_version(void);
 
 /* ---- context: replaces GPUDevice + GPUQueue ------------------------------ */
@@ -458,6 +459,45 @@ bgtq_status bgtq_paged_write(bgtq_context *ctx, const bgtq_pages *pages, const b
  * stay as they were; a slot may be read any number of times. k or v may be
  * NULL: only the other is read. The rows read into do not overlap (rows outermost or heads). */
 bgtq_status bgtq_paged_read(bgtq_context *ctx, const bgtq_pages *pages, const bgtq_paged_rows *rows);
+
+/* Head norms and position rotation of a step's rows (the model's rope pass,
+ * src/model/kernels.wgsl:11-54, with a norm per head where a model has one):
+ *   norm (weights given): x' = fl(fl(x r) w), r = FP32 of 1 / sqrt(mean(x^2) + eps)
+ *   rotation: the pairs (i, i + dim/2), y1 = fma(x1, c, -fl(x2 s)), y2 = fma(x2, c, fl(x1 s))
+ * in FP32, rounded once to the rows' type. table: device FP32
+ * [table_rows][dim], row p the cosines of position p's dim/2 angles, then the
+ * sines; 16-byte aligned. positions: device int64 [rows]; a row whose position
+ * is none of the table's (negative, or from table_rows on) is left out: nothing of
+ * it is written. */
+typedef struct {
+  const float *table;
+  int64_t table_rows;
+  const float *q_norm, *k_norm; /* device FP32 [dim] weights, NULL: no norm */
+  double eps;                   /* finite, not negative */
+} bgtq_rotation;
+/* Row i of head h at src + i*row_stride + h*head_stride (dim elements of dtype
+ * BGTQ_DTYPE_F32, _F16 or _BF16, aligned to their type; 16-byte aligned rows are
+ * faster), its result likewise at dst. dst is src (the same strides: in place) or
+ * overlaps no row that the call reads; its rows lie apart. heads: 1 .. 65535. */
+typedef struct {
+  const void *src;
+  void *dst;
+  int32_t heads, dtype;
+  int64_t src_row_stride, src_head_stride, dst_row_stride, dst_head_stride; /* elements */
+} bgtq_head_rows;
+/* Rotates rows of q (norm q_norm) and of k (norm k_norm); either may be NULL.
+ * dim 64 or 128, rows 0 .. 2^31 - 1. One launch, HIP-graph capturable. */
+bgtq_status bgtq_rotate(bgtq_context *ctx, const bgtq_rotation *r, int32_t dim, int64_t rows, const int64_t *positions,
+                        const bgtq_head_rows *q, const bgtq_head_rows *k);
+/* bgtq_paged_write of a step's rows before their rotation: K is normed and
+ * rotated as bgtq_rotate does in FP32, rounded to FP16 and encoded, V written as it
+ * is; rows whose position is none of the table's are skipped as those of slots
+ * outside the pool are. The same pool bit for bit as bgtq_rotate of K into FP32
+ * rows and bgtq_paged_write of them. q (may be NULL): queries of the same rows,
+ * rotated as bgtq_rotate does, also those whose slot lies outside the pool. One
+ * launch, HIP-graph capturable. */
+bgtq_status bgtq_paged_append(bgtq_context *ctx, const bgtq_pages *pages, const bgtq_paged_rows *rows, const bgtq_rotation *r,
+                              const int64_t *positions, const bgtq_head_rows *q);
 
 /* Decode attention of one layer over pages: as bgtq_decode (queries, outputs,
  * GQA, workspace, splits and q_rotated are the same), sequence b attending to
