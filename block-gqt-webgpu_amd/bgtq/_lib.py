@@ -127,6 +127,10 @@ class PromptDesc(ctypes.Structure):
                 ("out_head_stride", ctypes.c_int64), ("scale", ctypes.c_float)]
 
 
+class Window(ctypes.Structure):
+    _fields_ = [("window", ctypes.c_int32), ("sinks", ctypes.c_int32)]
+
+
 class RotationDesc(ctypes.Structure):
     _fields_ = [("table", ctypes.c_void_p), ("table_rows", ctypes.c_int64), ("q_norm", ctypes.c_void_p),
                 ("k_norm", ctypes.c_void_p), ("eps", ctypes.c_double)]
@@ -213,6 +217,10 @@ SIGNATURES = {
                                                 ctypes.POINTER(ctypes.c_size_t)]),
     "bgtq_paged_decode": (_I32, [_VP, ctypes.POINTER(Pages), ctypes.POINTER(PagedDecodeDesc)]),
     "bgtq_prompt_attention": (_I32, [_VP, ctypes.POINTER(PromptDesc)]),
+    "bgtq_prompt_attention_window": (_I32, [_VP, ctypes.POINTER(PromptDesc), ctypes.POINTER(Window)]),
+    "bgtq_paged_decode_window_workspace_size": (_I32, [ctypes.POINTER(Pages), ctypes.POINTER(PagedDecodeDesc),
+                                                       ctypes.POINTER(Window), ctypes.POINTER(ctypes.c_size_t)]),
+    "bgtq_paged_decode_window": (_I32, [_VP, ctypes.POINTER(Pages), ctypes.POINTER(PagedDecodeDesc), ctypes.POINTER(Window)]),
     "bgtq_rotate": (_I32, [_VP, ctypes.POINTER(RotationDesc), _I32, ctypes.c_int64, _VP, ctypes.POINTER(HeadRows),
                            ctypes.POINTER(HeadRows)]),
     "bgtq_paged_append": (_I32, [_VP, ctypes.POINTER(Pages), ctypes.POINTER(PagedRows), ctypes.POINTER(RotationDesc), _VP,

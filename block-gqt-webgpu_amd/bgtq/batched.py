@@ -358,17 +358,28 @@ def paged_append(device, pool, slots, rope, positions, k, v, q=None, q_out=None)
         check(lib().bgtq_paged_append(device.handle, pool.ref, ctypes.byref(r), rope.ref, _addr(positions), queries))
 
 
-class PagedDecode:
-    """A paged decode's descriptor with its pool; holds the tensors."""
+def _window(window, sinks):
+    """bgtq_window of a window's tokens and sinks; None for no window (None or 0)."""
+    if not window:
+        _need(not sinks, "sinks need a window")
+        return None
+    _need(0 < window < 1 << 31 and 0 <= sinks <= 1 << 30, "window must be in 1..2^31 - 1, sinks in 0..2^30")
+    return _lib.Window(int(window), int(sinks))
 
-    def __init__(self, pool, struct, held):
+
+class PagedDecode:
+    """A paged decode's descriptor with its pool and window; holds the tensors."""
+
+    def __init__(self, pool, struct, held, window=None):
         self.pool, self.struct, self.held, self.ref = pool, struct, held, ctypes.byref(struct)
+        self.window = None if window is None else ctypes.byref(window)
 
 
 def paged_decode_desc(*, pages, q, out, lengths, page_table, max_length=None, splits=0, workspace=None,
-                      q_rotated=False) -> PagedDecode:
+                      q_rotated=False, window=None, sinks=0) -> PagedDecode:
     """bgtq_paged_decode_desc over device tensors: q, out [B, Hq, dim] FP32 contiguous, lengths [B] and
-    page_table [B, pages per sequence] int32; max_length defaults to what the page table's rows hold."""
+    page_table [B, pages per sequence] int32; max_length defaults to what the page table's rows hold. window (None
+    or 0: none): the query sees its sequence's last `window` tokens and the first `sinks`."""
     index = pages.device_index
     for name, t in (("q", q), ("out", out)):
         _dense(index, name, t, "float32", 3)
@@ -385,25 +396,32 @@ def paged_decode_desc(*, pages, q, out, lengths, page_table, max_length=None, sp
                              st[0] if batch > 1 else page_table.shape[1], tokens, int(splits),
                              None if workspace is None else workspace.data_ptr(),
                              0 if workspace is None else workspace.numel() * workspace.element_size(), int(bool(q_rotated)))
-    return PagedDecode(pages, d, (q, out, lengths, page_table, workspace))
+    return PagedDecode(pages, d, (q, out, lengths, page_table, workspace), _window(window, sinks))
 
 
 def paged_decode_workspace_bytes(desc) -> int:
     n = ctypes.c_size_t(0)
-    check(lib().bgtq_paged_decode_workspace_size(desc.pool.ref, desc.ref, ctypes.byref(n)))
+    if desc.window is None:
+        check(lib().bgtq_paged_decode_workspace_size(desc.pool.ref, desc.ref, ctypes.byref(n)))
+    else:
+        check(lib().bgtq_paged_decode_window_workspace_size(desc.pool.ref, desc.ref, desc.window, ctypes.byref(n)))
     return n.value
 
 
 def paged_decode(device, desc) -> None:
-    """bgtq_paged_decode: decode attention over the descriptor's pages."""
+    """bgtq_paged_decode, or with a window bgtq_paged_decode_window: decode attention over the descriptor's pages."""
     _need(desc.pool.device_index == device.index, "the pool must lie on the context's device")
-    check(lib().bgtq_paged_decode(device.handle, desc.pool.ref, desc.ref))
+    if desc.window is None:
+        check(lib().bgtq_paged_decode(device.handle, desc.pool.ref, desc.ref))
+    else:
+        check(lib().bgtq_paged_decode_window(device.handle, desc.pool.ref, desc.ref, desc.window))
 
 
-def prompt_attention(device, q, k, v, offsets, out, scale=None) -> None:
+def prompt_attention(device, q, k, v, offsets, out, scale=None, window=None, sinks=0) -> None:
     """bgtq_prompt_attention: causal attention within each of the sequences packed in q, out [tokens, Hq, dim] and
     k, v [tokens, Hkv, dim] (FP16 or BF16, any strides of the first two dimensions that are multiples of 8);
-    offsets [sequences + 1] int32; scale defaults to 1 / sqrt(dim)."""
+    offsets [sequences + 1] int32; scale defaults to 1 / sqrt(dim). window (None or 0: none): a position sees the last
+    `window` ones, its own among them, and its sequence's first `sinks` (bgtq_prompt_attention_window)."""
     index, dtype = device.index, q.dtype
     code = _codes().get(dtype, _lib.DTYPE_F32)
     _dense(index, "offsets", offsets, "int32", 1)
@@ -421,4 +439,8 @@ def prompt_attention(device, q, k, v, offsets, out, scale=None) -> None:
         fields += (t.data_ptr() or None, s[0] if tokens > 1 else 0, s[1] if want[1] > 1 else 0)
     _need(scale is None or ctypes.c_float(scale).value > 0, "scale must be positive in FP32")  # (0 stands for the default)
     d = _lib.PromptDesc(heads, kv_shape[1], dim, code, offsets.shape[0] - 1, tokens, offsets.data_ptr(), *fields, scale or 0.0)
-    check(lib().bgtq_prompt_attention(device.handle, ctypes.byref(d)))
+    w = _window(window, sinks)
+    if w is None:
+        check(lib().bgtq_prompt_attention(device.handle, ctypes.byref(d)))
+    else:
+        check(lib().bgtq_prompt_attention_window(device.handle, ctypes.byref(d), ctypes.byref(w)))

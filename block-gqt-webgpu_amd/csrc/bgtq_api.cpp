@@ -1945,7 +1945,16 @@ struct PagedSplits {
   int room(int batch) const { return target ? (target + batch - 1) / batch : splits; }
 };
 
-static bgtq_status plan_paged_decode(const bgtq_pages *g, const bgtq_paged_decode_desc *d, PagedSplits *plan) {
+// A window of the windowed entry points: window 1 .. 2^31 - 1, sinks 0 .. 2^30.
+static bgtq_status check_window(const bgtq_window *w) {
+  if (!w) return fail(BGTQ_ERR_RANGE, "null window");
+  if (w->window < 1) return fail(BGTQ_ERR_RANGE, "window must be at least 1");
+  if (w->sinks < 0 || w->sinks > (1 << 30)) return fail(BGTQ_ERR_RANGE, "sinks must be in 0..2^30");
+  return BGTQ_OK;
+}
+
+// w (null: none): a window, which bounds what a sequence streams.
+static bgtq_status plan_paged_decode(const bgtq_pages *g, const bgtq_paged_decode_desc *d, const bgtq_window *w, PagedSplits *plan) {
   int nn = 0;
   if (bgtq_status s = check_pages(g, &nn)) return s;
   if (!d) return fail(BGTQ_ERR_RANGE, "null descriptor");
@@ -1964,8 +1973,10 @@ static bgtq_status plan_paged_decode(const bgtq_pages *g, const bgtq_paged_decod
   if (d->q_rotated != 0 && d->q_rotated != 1) return fail(BGTQ_ERR_RANGE, "q_rotated must be 0 or 1");
   if (d->q_rotated && g->key_format != BGTQ_KEYS_PACKED) return fail(BGTQ_ERR_RANGE, "q_rotated needs packed K");
   const int64_t units = (int64_t)d->batch * g->kv_heads;
+  // Tokens that a sequence streams at most: the window's and the sinks' whole chunks.
+  const uint32_t longest = (uint32_t)std::min<int64_t>(d->max_length, w ? (int64_t)w->window + w->sinks + 62 : INT64_MAX);
   if (d->splits > 0) {
-    const int s = choose_splits(units, d->max_length, d->splits);
+    const int s = choose_splits(units, longest, d->splits);
     *plan = {s, s, 0};
     return BGTQ_OK;
   }
@@ -1974,10 +1985,10 @@ static bgtq_status plan_paged_decode(const bgtq_pages *g, const bgtq_paged_decod
   // the workgroup that takes it: sqrt(5 steps) balances the two. us, the rule
   // without it / 40 splits: layout B, 2 units x 32768 tokens 62.1 (256) / 17.9,
   // 8 units 34.1 (96) / 21.0, d=128, 4 units 40.6 (128) / 22.7.
-  const double steps = d->max_length / 128.0;
+  const double steps = longest / 128.0;
   const int most = std::min(256, std::max(kDecodeMergeOneRound, (int)std::sqrt(5.0 * steps)));
   const int resident = paged_residents(g, nn);
-  *plan = {std::min(fused_decode_splits(units, d->max_length, 0, resident), most), most, 0};
+  *plan = {std::min(fused_decode_splits(units, longest, 0, resident), most), most, 0};
   // Up to 64 sequences (a lane each) share those workgroups by their lengths.
   // us, the same splits for all / by length: lengths from none up, 32 sequences of
   // up to 16384 tokens (SmolLM2 heads) 58.5 / 40.3, 48 (layout B) 37.4 / 30.8, d=128 7
@@ -1989,17 +2000,17 @@ static bgtq_status plan_paged_decode(const bgtq_pages *g, const bgtq_paged_decod
   return BGTQ_OK;
 }
 
-bgtq_status bgtq_paged_decode_workspace_size(const bgtq_pages *g, const bgtq_paged_decode_desc *d, size_t *bytes) {
+static bgtq_status paged_decode_workspace(const bgtq_pages *g, const bgtq_paged_decode_desc *d, const bgtq_window *w, size_t *bytes) {
   PagedSplits plan;
-  if (bgtq_status s = plan_paged_decode(g, d, &plan)) return s;
+  if (bgtq_status s = plan_paged_decode(g, d, w, &plan)) return s;
   if (!bytes) return fail(BGTQ_ERR_RANGE, "null output");
   *bytes = decode_ws((int64_t)d->batch * g->kv_heads, (int64_t)d->batch * d->q_heads, g->dim, plan.room(d->batch)).total;
   return BGTQ_OK;
 }
 
-bgtq_status bgtq_paged_decode(bgtq_context *ctx, const bgtq_pages *g, const bgtq_paged_decode_desc *d) {
+static bgtq_status paged_decode(bgtq_context *ctx, const bgtq_pages *g, const bgtq_paged_decode_desc *d, const bgtq_window *window) {
   PagedSplits plan;
-  if (bgtq_status s = plan_paged_decode(g, d, &plan)) return s;
+  if (bgtq_status s = plan_paged_decode(g, d, window, &plan)) return s;
   const DecodeWorkspace w = decode_ws((int64_t)d->batch * g->kv_heads, (int64_t)d->batch * d->q_heads, g->dim, plan.room(d->batch));
   if (!d->workspace || d->workspace_bytes < w.total) return fail(BGTQ_ERR_RANGE, "workspace of %zu bytes required", w.total);
   if (reinterpret_cast<uintptr_t>(d->workspace) % 16) return fail(BGTQ_ERR_RANGE, "workspace must be 16-byte aligned");
@@ -2026,6 +2037,7 @@ bgtq_status bgtq_paged_decode(bgtq_context *ctx, const bgtq_pages *g, const bgtq
   p.splits_forced = d->splits > 0;
   p.inv_sqrt_d = (float)(1.0 / std::sqrt((double)g->dim));
   p.out = d->out;
+  if (window) p.window = window->window, p.sinks = window->sinks;
   FastLayout fl{};
   int nn = 0, sg = 0;
   if (!pool_layout(p, g, &fl, &nn, &sg)) return fail(BGTQ_ERR_UNSUPPORTED, "pages hold the packed layouts of the fused decode");
@@ -2036,8 +2048,24 @@ bgtq_status bgtq_paged_decode(bgtq_context *ctx, const bgtq_pages *g, const bgtq
   return BGTQ_OK;
 }
 
+bgtq_status bgtq_paged_decode_workspace_size(const bgtq_pages *g, const bgtq_paged_decode_desc *d, size_t *bytes) {
+  return paged_decode_workspace(g, d, nullptr, bytes);
+}
+bgtq_status bgtq_paged_decode(bgtq_context *ctx, const bgtq_pages *g, const bgtq_paged_decode_desc *d) {
+  return paged_decode(ctx, g, d, nullptr);
+}
+bgtq_status bgtq_paged_decode_window_workspace_size(const bgtq_pages *g, const bgtq_paged_decode_desc *d, const bgtq_window *w,
+                                                    size_t *bytes) {
+  if (bgtq_status s = check_window(w)) return s;
+  return paged_decode_workspace(g, d, w, bytes);
+}
+bgtq_status bgtq_paged_decode_window(bgtq_context *ctx, const bgtq_pages *g, const bgtq_paged_decode_desc *d, const bgtq_window *w) {
+  if (bgtq_status s = check_window(w)) return s;
+  return paged_decode(ctx, g, d, w);
+}
+
 // ---------------------------------------------------------------- attention over packed prompts
-bgtq_status bgtq_prompt_attention(bgtq_context *ctx, const bgtq_prompt_desc *d) {
+static bgtq_status prompt_attention(bgtq_context *ctx, const bgtq_prompt_desc *d, const bgtq_window *w) {
   if (!d) return fail(BGTQ_ERR_RANGE, "null descriptor");
   if (d->kv_heads < 1 || d->q_heads < d->kv_heads || d->q_heads % d->kv_heads || d->q_heads > 65535)
     return fail(BGTQ_ERR_RANGE, "invalid head geometry");
@@ -2072,8 +2100,14 @@ bgtq_status bgtq_prompt_attention(bgtq_context *ctx, const bgtq_prompt_desc *d) 
   if (none) return BGTQ_OK;
   DeviceScope scope;
   if (bgtq_status s = ctx->use()) return s;
-  HIP_TRY(launch_prompt_attention(*d, ctx->stream), "prompt attention launch");
+  HIP_TRY(launch_prompt_attention(*d, w, ctx->stream), "prompt attention launch");
   return BGTQ_OK;
+}
+
+bgtq_status bgtq_prompt_attention(bgtq_context *ctx, const bgtq_prompt_desc *d) { return prompt_attention(ctx, d, nullptr); }
+bgtq_status bgtq_prompt_attention_window(bgtq_context *ctx, const bgtq_prompt_desc *d, const bgtq_window *w) {
+  if (bgtq_status s = check_window(w)) return s;
+  return prompt_attention(ctx, d, w);
 }
 
 // ---------------------------------------------------------------- chunked prefill

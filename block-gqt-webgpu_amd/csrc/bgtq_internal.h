@@ -282,6 +282,8 @@ struct DecodeParams {
   // Pages: workgroups per KV head that up to 64 sequences share by their
   // lengths, `splits` of a sequence at most; 0: `splits` of every sequence.
   int32_t split_target;
+  // Pages: the query sees its last `window` tokens (0: all) and the first `sinks`.
+  int32_t window, sinks;
   // Workgroups per (sequence, KV head) or row-wise unit that take the
   // appended rows (packed K: decode 1; row-wise prefill one row per wave),
   // after the splits in the split dimension; each leaves one partial.
@@ -505,7 +507,7 @@ hipError_t launch_paged_read(const PagedWriteParams &p, int cus, hipStream_t str
 int64_t prompt_workgroups(const bgtq_prompt_desc &d);
 constexpr int kPromptThreads = 256;  // of a workgroup
 constexpr int64_t kPromptMaxStride = 1 << 22;  // elements: a block's byte offsets stay below 2^31
-hipError_t launch_prompt_attention(const bgtq_prompt_desc &d, hipStream_t stream);
+hipError_t launch_prompt_attention(const bgtq_prompt_desc &d, const bgtq_window *w, hipStream_t stream);
 hipError_t launch_rotate_q(const DecodeParams &p, const float *q, float *qr, hipStream_t stream);
 // Device address of this device's bgtq_decode_noalloc scratch (decode_scratch.hip).
 hipError_t decode_scratch_setup(int device, hipStream_t stream, uint8_t **out);

@@ -392,6 +392,31 @@ __device__ __forceinline__ void merge_rows(float *part, float *out, const MergeR
   "s"((int)fl.gnb[kv]), "s"((int)fl.gbstride[kv]), "s"((int)fl.gbnib[kv]), "s"(fl.gpair[kv]),                  \
   "s"((int)fl.grb[kv]), "s"((int)fl.gns[kv]));
 
+// Pages: the tokens that a sequence of n tokens streams, in whole chunks. Behind
+// a window these are the sinks' chunks, then those from the window's first
+// token on (a chunk that holds both is streamed for each); without one, or
+// where it hides nothing, all. place(c): the c-th of these tokens (c a
+// multiple of kChunk), and the tokens lo .. hi - 1 that its chunk attends to.
+struct PagedSpan {
+  int sunk, shift, low, sinks, n, tokens;  // tokens: streamed, the last chunk's up to n
+  __device__ __forceinline__ PagedSpan(int n_, int window, int sinks_) : sunk(0), shift(0), low(0), sinks(0), n(n_), tokens(n_) {
+    const int first = window ? max(0, n_ - window) : 0;
+    if (first > sinks_) {
+      low = first;
+      sinks = sinks_;
+      sunk = (sinks_ + kChunk - 1) / kChunk * kChunk;
+      shift = first / kChunk * kChunk - sunk;
+      tokens = n_ - shift;
+    }
+  }
+  __device__ __forceinline__ int place(int c, int &lo, int &hi) const {
+    const bool sink = c < sunk;
+    lo = sink ? 0 : low;
+    hi = sink ? sinks : n;
+    return sink ? c : c + shift;
+  }
+};
+
 // Pages, p.split_target set: which sequence and split of it grid y stands
 // for. A workgroup's unit of work is a step, the 2^SHIFT tokens that its
 // waves take at a time. With t steps to a workgroup, sequence b takes
@@ -407,7 +432,8 @@ template <int SHIFT>
 __device__ __forceinline__ PagedPlace paged_place(const DecodeParams &p, int y) {
   const int lane = threadIdx.x & 63;
   const uint32_t len = p.lengths[min(lane, p.batch - 1)];
-  const int steps = lane < p.batch ? (int)((min(len, (uint32_t)p.max_length) + (1u << SHIFT) - 1) >> SHIFT) : 0;
+  const int tokens = PagedSpan((int)min(len, (uint32_t)p.max_length), p.window, p.sinks).tokens;
+  const int steps = lane < p.batch ? (tokens + (1 << SHIFT) - 1) >> SHIFT : 0;
   const float target = (float)p.split_target;
   float t = fmaxf(1.0f, ceilf((float)wave_sum(steps) / target));
   // (the thousandth: a quotient that is whole stays so through the reciprocal)
@@ -485,7 +511,7 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
   BGTQ_LOAD_ARGS
   if constexpr (PG)
     asm volatile("" ::"s"(p.page_table), "s"(p.page_table_stride), "s"(p.page_shift), "s"(p.table_pages), "s"(p.pages),
-                 "s"(p.v_scales));
+                 "s"(p.v_scales), "s"(p.window), "s"(p.sinks));
   __builtin_amdgcn_sched_barrier(0);
   const int unit = qrow * p.kv_heads + kv;
   uint32_t *const counter = p.counters + (int64_t)unit * (p.counter_stride > 0 ? p.counter_stride : 1);
@@ -576,8 +602,16 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
   // ahead (chunks past the table's end read its last entry and stream
   // nothing). A vector load, older than the loads of the chunk before its own.
   const int first_pg = (split * kWaves + wave) * kChunk, stride_pg = pg_at.splits * kWaves * kChunk;
+  // (Behind a window the place of a chunk takes the length, waited for here.)
+  int span_n = 0;
+  if (PG && p.window) {
+    span_n = (int)min(len_b, (uint32_t)p.max_length);
+    asm volatile("" : "+s"(span_n));  // (made a select, it would be waited for without a window too)
+  }
+  const PagedSpan span(span_n, PG ? p.window : 0, PG ? p.sinks : 0);
   auto load_page = [&](int i) -> int {
-    const int at = min((first_pg + i * stride_pg) >> p.page_shift, p.table_pages - 1);
+    int lo, hi;
+    const int at = min(span.place(first_pg + i * stride_pg, lo, hi) >> p.page_shift, p.table_pages - 1);
     return p.page_table[(int64_t)b * p.page_table_stride + at];
   };
   // The page as an index into the pool: -1 where the table names none.
@@ -752,7 +786,7 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
   // Tokens the history splits attend to; the append workgroup's range ends
   // after its rows (decode: all tokens, so the new one lies inside the causal
   // limits).
-  const int T_att = !app ? T_b : app_wg ? (rowwise ? start_c + r_a + n_a : T_b) : rowwise ? start_c : T_b - 1;
+  const int T_att = PG && p.window ? span.tokens : !app ? T_b : app_wg ? (rowwise ? start_c + r_a + n_a : T_b) : rowwise ? start_c : T_b - 1;
   // Splits of one (sequence, KV head) interleave at chunk granularity: wave w
   // of split s takes chunks (s * 4 + w) + 4 S i, so the waves working on a
   // sequence at any moment sweep adjacent memory.
@@ -769,14 +803,24 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
   // a row-wise prefill chunk's history is read by every unit of its KV head,
   // so those loads keep the default policy and the units share it in L2.
   constexpr int kPol = PF ? kCached : kStream;
+  // A chunk's first token, and (pages) the tokens lo .. hi - 1 that it attends to.
+  auto chunk_at = [&](int i, int &lo, int &hi) {
+    const int c = first + i * stride;
+    lo = 0, hi = T_att;
+    if constexpr (PG) {
+      if (p.window) return span.place(c, lo, hi);
+    }
+    return c;
+  };
   auto issue = [&](int i, int pg = 0) {
-    const int c0 = first + i * stride;
+    int lo, hi;
+    const int c0 = chunk_at(i, lo, hi);
     // Tokens of the chunk inside the sequence; none for a chunk past the end
     // (a zero-sized descriptor: the DMA only writes zeros to LDS). A history
     // split's range ends before the appended token, so its row arrives as
     // zeros; the append workgroup streams nothing.
     // Pages hold whole chunks; one of a page that is not in the pool streams nothing.
-    const int in_seq = app_wg || pg < 0 ? 0 : min(T_att - c0, kChunk);
+    const int in_seq = app_wg || pg < 0 ? 0 : min(hi - c0, kChunk);
     const uint32_t rest = __builtin_amdgcn_readfirstlane(in_seq > 0 ? in_seq : 0);  // wave-uniform: SGPR descriptor
     uint8_t *sb = slot_base(i % Sl::RING);
     const int64_t pn = PG && pg > 0 ? pg : 0;
@@ -785,8 +829,16 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
     const uint8_t *k_base_c = PG ? k_base + pn * (KF >= 1 ? p.packed_seq_stride : 2 * p.k_seq_stride) : k_base;
     const uint16_t *n_base_c = PG && KF >= 1 ? n_base + pn * p.norms_seq_stride : n_base;
     const __amdgpu_buffer_rsrc_t rV = rsrc(v_rows_c + (int64_t)r0 * D * VB, rest * (VB * D));
+    if (PG && !Q8 && c0 < lo) {
+      // The window begins inside the chunk (wave-uniform): V rows before it may
+      // hold infinities or NaNs and arrive as zeros, their offsets past the range.
 #pragma unroll
-    for (int k = 0; k < VI; ++k) dma16<kPol>(rV, sb + k * 1024, voff_rows[k], 0);
+      for (int k = 0; k < VI; ++k)
+        dma16<kPol>(rV, sb + k * 1024, (64 * k + lane) / PR < lo - c0 ? 0x7fffff00u : voff_rows[k], 0);
+    } else {
+#pragma unroll
+      for (int k = 0; k < VI; ++k) dma16<kPol>(rV, sb + k * 1024, voff_rows[k], 0);
+    }
     if constexpr (Q8) {
       // (an odd chunk's last scale comes with the next row's: chunk_pv clears that)
       const uint16_t *vs = vs_base + pn * p.v_scales_page_stride + r0;
@@ -1391,7 +1443,8 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
   // col, tokens c0 + 16 u + 4 gq + r in x[4 u + r], log2 domain, masked past
   // the causal ends.
   // in_pool (pages): the chunk's page is one of the pool's; else it is masked whole.
-  auto chunk_logits = [&](const uint8_t *sb, int c0, float (&x)[8], bool in_pool = true) {
+  // lo, hi (pages): the tokens that it attends to.
+  auto chunk_logits = [&](const uint8_t *sb, int c0, float (&x)[8], bool in_pool = true, int lo = 0, int hi = 0) {
     const uint8_t *kbuf = sb + Sl::KOFF;
     // KF 2: transpose the scale rows (every read of the wave's slot precedes
     // its writes: one wave's LDS operations complete in order).
@@ -1657,11 +1710,19 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
         x[4 * u + r] = LATE ? v : v * kq;
       }
     }
-    if (c0 + kChunk > lim_min || !in_pool) {
+    if constexpr (PG) {
+      if (c0 + kChunk > hi || c0 < lo || !in_pool) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int tok = c0 + 16 * (j >> 2) + 4 * gq + (j & 3);
+          x[j] = tok < hi && tok >= lo && in_pool ? x[j] : -INFINITY;
+        }
+      }
+    } else if (c0 + kChunk > lim_min) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int tok = c0 + 16 * (j >> 2) + 4 * gq + (j & 3);
-        x[j] = tok < lim && in_pool ? x[j] : -INFINITY;
+        x[j] = tok < lim ? x[j] : -INFINITY;
       }
     }
   };
@@ -1670,18 +1731,18 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
   // pr themselves, on the FP32 matrix cores.
   // 8-bit V: v = RN16(s c), the FP16 value that a row's code and scale stand
   // for, from the codes read transposed (as 1024 + (c + 128) in FP16, exact).
-  // rest: the chunk's tokens inside the sequence.
-  auto chunk_pv = [&](const uint8_t *sb, const half8 pha, const half8 pla, const float *pr, int rest = kChunk) {
+  // skip, rest (pages): the chunk's first token, and the one after the last, that are attended to.
+  auto chunk_pv = [&](const uint8_t *sb, const half8 pha, const half8 pla, const float *pr, int skip = 0, int rest = kChunk) {
     if constexpr (Q8) {
       typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
       const uint8_t *sc = sb + Sl::VSOFF + 8 * gq;
       const u32x2 s0 = *reinterpret_cast<const u32x2 *>(sc), s1 = *reinterpret_cast<const u32x2 *>(sc + 32);
       uint32_t s4[4] = {s0[0], s0[1], s1[0], s1[1]};  // tokens 4 gq + 0..3, 16 + 4 gq + 0..3
-      if (rest < kChunk) {  // (wave-uniform) no scale of a row past the sequence: it may hold anything
+      if (rest < kChunk || skip > 0) {  // (wave-uniform) no scale of a row that is not attended to: it may hold anything
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int tok = 16 * (j >> 1) + 4 * gq + 2 * (j & 1);
-          s4[j] = tok + 1 < rest ? s4[j] : tok < rest ? s4[j] & 0xffffu : 0u;
+          s4[j] &= (tok < rest && tok >= skip ? 0xffffu : 0u) | (tok + 1 < rest && tok + 1 >= skip ? 0xffff0000u : 0u);
         }
       }
       const int r8 = col >> 1, vrow = 16 * (r8 >> 2) + 4 * gq + (r8 & 3);
@@ -1809,7 +1870,8 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
     if constexpr (PG) asm("" : "+s"(one));  // (split2_mix)
     bool in_pool = page0 >= 0, in_pool_next = true;
     for (int i = 0; i < n_chunks; ++i) {
-      const int c0 = first + i * stride;
+      int lo, hi;
+      const int c0 = chunk_at(i, lo, hi);
       // Refill the buffer computed on last iteration with chunk i + AHEAD, then
       // wait for chunk i: its DMA is older than the (up to AHEAD) chunks issued
       // after it. With materialised logits the loop also stores, so wait for all.
@@ -1842,7 +1904,7 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
       }
 
       float x[8];
-      chunk_logits(sb, c0, x, in_pool);
+      chunk_logits(sb, c0, x, in_pool, lo, hi);
       if (lg) {  // materialised logits for inspect() (natural units)
   #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -1895,7 +1957,7 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
       // there: 64 x 32768 tokens 106.0 / 103.7, 29 ragged FP16 sequences 54.8 / 52.8).
       if (!PF && !PG) wait_vm<0>();
       const half8 pha = __builtin_bit_cast(half8, ph), pla = __builtin_bit_cast(half8, pl);
-      chunk_pv(sb, pha, pla, pr, PG ? min(T_att - c0, kChunk) : kChunk);
+      chunk_pv(sb, pha, pla, pr, PG ? lo - c0 : 0, PG ? min(hi - c0, kChunk) : kChunk);
       if constexpr (PG) in_pool = in_pool_next;
     }
   }

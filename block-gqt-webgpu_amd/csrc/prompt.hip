@@ -75,6 +75,7 @@ struct PromptParams {
   uint16_t *out;
   int64_t q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head;  // elements
   float c;  // scale * log2(e)
+  int32_t window, sinks;  // window 0: all tokens up to the query's
 };
 
 // XOR of a row's 16-byte piece indexes: 16 rows' reads of one piece (K) and
@@ -198,7 +199,8 @@ __device__ __forceinline__ Place find_place(const PromptParams &p, int64_t slot)
   return r;
 }
 
-template <int D, bool BF>
+// WIN: a query sees the `window` keys up to its own and the sequence's first `sinks`.
+template <int D, bool BF, bool WIN>
 __global__ __launch_bounds__(kThreads, D == 64 ? 4 : 2) void prompt_kernel(PromptParams p) {
   constexpr int PR = D / 8;                      // 16-byte pieces per row
   constexpr int QS = D / 16;                     // 16-dimension steps of QK
@@ -214,14 +216,21 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 4 : 2) void prompt_kernel(Promp
   if (at.tile < 0) return;  // uniform for the workgroup
   const int q0 = at.tile * kRows, row0 = q0 + 32 * wave;  // the workgroup's, this wave's first query
   const int qi = row0 + qc;                               // this lane's query
-  const int n_blocks = (min(q0 + kRows, at.len) + kKeys - 1) / kKeys;
+  const int n_all = (min(q0 + kRows, at.len) + kKeys - 1) / kKeys;
+  // Blocks that the workgroup's queries see something of: all up to its
+  // diagonal; behind a window those of the sinks, then from the first query's
+  // window on. block(i): the i-th of them.
+  const int sink_blocks = WIN ? (min(p.sinks, at.len) + kKeys - 1) / kKeys : 0;
+  const int skipped = WIN ? max(0, max(0, q0 - p.window + 1) / kKeys - sink_blocks) : 0;
+  const int n_blocks = n_all - skipped;
+  auto block = [&](int i) { return WIN && i >= sink_blocks ? i + skipped : i; };
 
   const uint16_t *k_base = p.k + at.begin * p.k_row + kv * p.k_head;
   const uint16_t *v_base = p.v + at.begin * p.v_row + kv * p.v_head;
   // Block j's rows inside the sequence; the others arrive as zeros.
-  auto issue = [&](int j) {
-    const int rest = min(kKeys, at.len - j * kKeys);
-    uint8_t *buf = smem + (j & 1) * 2 * BLOCK;
+  auto issue = [&](int i0) {
+    const int j = block(i0), rest = min(kKeys, at.len - j * kKeys);
+    uint8_t *buf = smem + (i0 & 1) * 2 * BLOCK;
     const __amdgpu_buffer_rsrc_t rk = rsrc(k_base + (int64_t)j * kKeys * p.k_row, (uint32_t)(((rest - 1) * p.k_row + D) * 2));
     const __amdgpu_buffer_rsrc_t rv = rsrc(v_base + (int64_t)j * kKeys * p.v_row, (uint32_t)(((rest - 1) * p.v_row + D) * 2));
 #pragma unroll
@@ -278,10 +287,15 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 4 : 2) void prompt_kernel(Promp
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  // Block j's keys for this wave's queries; DIAGONAL: some queries see only a part of them.
-  auto attend = [&](auto diagonal_tag, int j) {
+  // The keys of the workgroup's block i0 for this wave's queries; DIAGONAL: some queries see only a part of them.
+  auto attend = [&](auto diagonal_tag, int i0) {
     constexpr bool DIAGONAL = decltype(diagonal_tag)::value;
-    const uint32_t buf = (uint32_t)(j & 1) * 2 * BLOCK;
+    const int j = block(i0);
+    const uint32_t buf = (uint32_t)(i0 & 1) * 2 * BLOCK;
+    // Whether this lane's query sees key 4 h + k of the block.
+    const int d = qi - j * kKeys - 4 * h;
+    const int d_low = WIN ? d - p.window : 0, d_sink = WIN ? p.sinks - j * kKeys - 4 * h : 0;
+    auto sees = [&](int k) { return k <= d && (!WIN || k > d_low || k < d_sink); };
     f32x16 S[2];
 #pragma unroll
     for (int b = 0; b < 2; ++b)
@@ -295,11 +309,10 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 4 : 2) void prompt_kernel(Promp
         S[b] = product<BF>(a, qf[s], S[b]);
       }
     if constexpr (DIAGONAL) {
-      const int d = qi - j * kKeys - 4 * h;
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) S[b][i] = 32 * b + 8 * (i >> 2) + (i & 3) <= d ? S[b][i] : -INFINITY;
+        for (int i = 0; i < 16; ++i) S[b][i] = sees(32 * b + 8 * (i >> 2) + (i & 3)) ? S[b][i] : -INFINITY;
     }
     softmax_first(1);
     float top = S[0][0];
@@ -374,7 +387,6 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 4 : 2) void prompt_kernel(Promp
         if (s == 2) ds_read_tr16<MT, 3 * STEP>(va, va8, v[1]);
       }
     } else {
-      const int d = qi - j * kKeys - 4 * h;
       // V of dimension 32 t + qc, keys 16 s + 8 (e / 2) + 4 h + 2 (e % 2) + 0, 1 in word e.
       auto column = [&](int s, int t) {
         u32x4 a;
@@ -414,7 +426,7 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 4 : 2) void prompt_kernel(Promp
             for (int e = 0; e < 4; ++e) {
               const int k = 16 * s + 8 * (e >> 1) + 2 * (e & 1);
               a[e] = Odd<BF>::of_kind(a[e], kind);
-              seen[e] = (k <= d ? Odd<BF>::kOne : 0u) | (k + 1 <= d ? Odd<BF>::kOne << 16 : 0u);
+              seen[e] = (sees(k) ? Odd<BF>::kOne : 0u) | (sees(k + 1) ? Odd<BF>::kOne << 16 : 0u);
             }
             n = product<BF>(a, seen, n);
           }
@@ -430,11 +442,27 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 4 : 2) void prompt_kernel(Promp
   // One block holds the wave's diagonal (32 rows lie within one); those after
   // it hold no key that its queries see. Loops of their own, so that the full
   // blocks' carries none of the diagonal's code.
+  // Behind a window the full blocks have some before them that the queries
+  // see a part of, or nothing: the sinks' and those of the window's edge.
   const int jd = row0 / kKeys;
   int j = 0;
-  for (; j < min(jd, n_blocks); ++j) {
-    arrive(j);
-    attend(std::false_type{}, j);
+  if constexpr (WIN) {
+    const int low = row0 - p.window;  // the last key that the first query does not see
+    for (; j < n_blocks; ++j) {
+      const int k0 = block(j) * kKeys;
+      if (k0 >= jd * kKeys || k0 > low + 31) break;
+      arrive(j);
+      if (k0 < p.sinks || k0 + kKeys - 1 > low) attend(std::true_type{}, j);
+    }
+    for (; j < n_blocks && block(j) < jd; ++j) {
+      arrive(j);
+      attend(std::false_type{}, j);
+    }
+  } else {
+    for (; j < min(jd, n_blocks); ++j) {
+      arrive(j);
+      attend(std::false_type{}, j);
+    }
   }
   if (j < n_blocks) {
     arrive(j);
@@ -456,7 +484,8 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 4 : 2) void prompt_kernel(Promp
 
 template <int D, bool BF>
 hipError_t launch_d(const PromptParams &p, int64_t wgs, hipStream_t stream) {
-  hipLaunchKernelGGL((prompt_kernel<D, BF>), dim3((unsigned)wgs), dim3(kThreads), 0, stream, p);
+  if (p.window) hipLaunchKernelGGL((prompt_kernel<D, BF, true>), dim3((unsigned)wgs), dim3(kThreads), 0, stream, p);
+  else hipLaunchKernelGGL((prompt_kernel<D, BF, false>), dim3((unsigned)wgs), dim3(kThreads), 0, stream, p);
   return hipGetLastError();
 }
 
@@ -464,8 +493,10 @@ hipError_t launch_d(const PromptParams &p, int64_t wgs, hipStream_t stream) {
 
 int64_t prompt_workgroups(const bgtq_prompt_desc &d) { return (d.tokens / kRows + d.sequences) * d.q_heads; }
 
-hipError_t launch_prompt_attention(const bgtq_prompt_desc &d, hipStream_t stream) {
+hipError_t launch_prompt_attention(const bgtq_prompt_desc &d, const bgtq_window *w, hipStream_t stream) {
   PromptParams p{};
+  // (a lane compares keys with its query less the window: no wrap of 32 bits; no sequence comes near)
+  if (w) p.window = std::min(w->window, INT32_MAX - 256), p.sinks = w->sinks;
   p.offsets = d.offsets;
   p.sequences = d.sequences;
   p.heads = d.q_heads;

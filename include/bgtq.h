@@ -522,6 +522,21 @@ typedef struct {
 bgtq_status bgtq_paged_decode_workspace_size(const bgtq_pages *pages, const bgtq_paged_decode_desc *d, size_t *bytes);
 bgtq_status bgtq_paged_decode(bgtq_context *ctx, const bgtq_pages *pages, const bgtq_paged_decode_desc *d);
 
+/* A sliding window with sinks: position p sees the tokens t <= p with t > p - window
+ * (its own among them) or t < sinks. window at least 1, sinks 0 .. 2^30. The
+ * windowed calls are otherwise those without; what lies behind a window is neither
+ * read nor looked up, so its pages may be given back (a table entry of -1), but for
+ * those of the sinks and of the 32 tokens (decode) or 64 (chunks) that hold the window's
+ * first one, which are looked up and may be -1 only if none of theirs is seen. */
+typedef struct {
+  int32_t window, sinks;
+} bgtq_window;
+/* The query of sequence b at position lengths[b] - 1 (the newest token). */
+bgtq_status bgtq_paged_decode_window_workspace_size(const bgtq_pages *pages, const bgtq_paged_decode_desc *d,
+                                                    const bgtq_window *w, size_t *bytes);
+bgtq_status bgtq_paged_decode_window(bgtq_context *ctx, const bgtq_pages *pages, const bgtq_paged_decode_desc *d,
+                                     const bgtq_window *w);
+
 /* Attention over whole prompts, before their rows enter a cache: causal
  * self-attention of `sequences` sequences of different lengths packed one
  * after another, sequence s the rows offsets[s] .. offsets[s+1] - 1 of q, k, v
@@ -555,6 +570,8 @@ typedef struct {
   float scale;
 } bgtq_prompt_desc;
 bgtq_status bgtq_prompt_attention(bgtq_context *ctx, const bgtq_prompt_desc *d);
+/* The same behind a window of each sequence's own positions. */
+bgtq_status bgtq_prompt_attention_window(bgtq_context *ctx, const bgtq_prompt_desc *d, const bgtq_window *w);
 
 /* ---- calibration-table pipeline (host only, no device needed) ------------
  * The setup that produces the tables(p) blobs bgtq_tables_create takes:

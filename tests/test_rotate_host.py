@@ -1,11 +1,11 @@
-"""What the rotation's entry points refuse, without a GPU: every check precedes device work."""
+"""What the rotation's and the windowed entry points refuse, without a GPU: every check precedes device work."""
 import ctypes
 
 import pytest
 import torch  # noqa: F401  (before bgtq, so that one HIP runtime, torch's, serves both)
 
 from bgtq import _lib
-from test_paged_host import A, BAD_PAGES, _pages
+from test_paged_host import A, BAD_PAGES, _decode, _pages, _prompt
 from test_paged_host import _rows as _paged_rows
 
 
@@ -70,3 +70,30 @@ def test_other_refusals():
     # what is left once everything else holds: no context
     assert _rotate(good, q=_heads(), k=_heads()) == _append(good, q=_heads()) == _lib.ERR_RANGE
     assert b"context" in L.bgtq_last_error()
+
+
+@pytest.mark.parametrize("bad", [None, dict(window=0), dict(window=-1), dict(sinks=-1), dict(sinks=(1 << 30) + 1)], ids=str)
+def test_bad_windows(bad):
+    L, n = _lib.lib(), ctypes.c_size_t()
+    w = None if bad is None else ctypes.byref(_lib.Window(**{**dict(window=5, sinks=1), **bad}))
+    assert L.bgtq_prompt_attention_window(None, ctypes.byref(_prompt()), w) == _lib.ERR_RANGE
+    assert L.bgtq_paged_decode_window(None, ctypes.byref(_pages()), ctypes.byref(_decode()), w) == _lib.ERR_RANGE
+    assert L.bgtq_paged_decode_window_workspace_size(ctypes.byref(_pages()), ctypes.byref(_decode()), w, ctypes.byref(n)) == _lib.ERR_RANGE
+    assert b"context" not in L.bgtq_last_error()
+
+
+def test_windowed_workspace():
+    """What a window streams sizes the workspace; the other checks are those without one."""
+    L, sizes = _lib.lib(), []
+    d = _decode(max_length=1 << 20, page_table_stride=1 << 15)
+    for window in (1, 1 << 12, 1 << 20, (1 << 31) - 1):
+        n = ctypes.c_size_t()
+        assert L.bgtq_paged_decode_window_workspace_size(ctypes.byref(_pages()), ctypes.byref(d), ctypes.byref(_lib.Window(window, 1 << 30 if window > 1 << 20 else 0)),
+                                                         ctypes.byref(n)) == _lib.OK
+        sizes.append(n.value)
+    n = ctypes.c_size_t()
+    assert L.bgtq_paged_decode_workspace_size(ctypes.byref(_pages()), ctypes.byref(d), ctypes.byref(n)) == _lib.OK
+    assert sizes == sorted(sizes) and sizes[-1] == n.value
+    good = ctypes.byref(_lib.Window(5, 1))
+    assert L.bgtq_prompt_attention_window(None, ctypes.byref(_prompt(dim=96)), good) == _lib.ERR_UNSUPPORTED
+    assert L.bgtq_paged_decode_window(None, ctypes.byref(_pages()), ctypes.byref(_decode(max_length=0)), good) == _lib.ERR_RANGE
