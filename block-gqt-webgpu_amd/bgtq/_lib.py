@@ -127,6 +127,19 @@ class PromptDesc(ctypes.Structure):
                 ("out_head_stride", ctypes.c_int64), ("scale", ctypes.c_float)]
 
 
+PAGED_PREFILL_COUNTER_BYTES = 64 * 1024
+
+
+class PagedPrefillDesc(ctypes.Structure):
+    _fields_ = [("q_heads", ctypes.c_int32), ("dtype", ctypes.c_int32), ("sequences", ctypes.c_int32),
+                ("tokens", ctypes.c_int64), ("offsets", ctypes.c_void_p), ("lengths", ctypes.c_void_p),
+                ("page_table", ctypes.c_void_p), ("page_table_stride", ctypes.c_int64), ("max_length", ctypes.c_uint32),
+                ("q", ctypes.c_void_p), ("q_row_stride", ctypes.c_int64), ("q_head_stride", ctypes.c_int64),
+                ("out", ctypes.c_void_p), ("out_row_stride", ctypes.c_int64), ("out_head_stride", ctypes.c_int64),
+                ("scale", ctypes.c_float), ("window", ctypes.c_int32), ("sinks", ctypes.c_int32),
+                ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t)]
+
+
 class Window(ctypes.Structure):
     _fields_ = [("window", ctypes.c_int32), ("sinks", ctypes.c_int32)]
 
@@ -221,6 +234,9 @@ SIGNATURES = {
     "bgtq_paged_decode_window_workspace_size": (_I32, [ctypes.POINTER(Pages), ctypes.POINTER(PagedDecodeDesc),
                                                        ctypes.POINTER(Window), ctypes.POINTER(ctypes.c_size_t)]),
     "bgtq_paged_decode_window": (_I32, [_VP, ctypes.POINTER(Pages), ctypes.POINTER(PagedDecodeDesc), ctypes.POINTER(Window)]),
+    "bgtq_paged_prefill_workspace_size": (_I32, [ctypes.POINTER(Pages), ctypes.POINTER(PagedPrefillDesc),
+                                                 ctypes.POINTER(ctypes.c_size_t)]),
+    "bgtq_paged_prefill": (_I32, [_VP, ctypes.POINTER(Pages), ctypes.POINTER(PagedPrefillDesc)]),
     "bgtq_rotate": (_I32, [_VP, ctypes.POINTER(RotationDesc), _I32, ctypes.c_int64, _VP, ctypes.POINTER(HeadRows),
                            ctypes.POINTER(HeadRows)]),
     "bgtq_paged_append": (_I32, [_VP, ctypes.POINTER(Pages), ctypes.POINTER(PagedRows), ctypes.POINTER(RotationDesc), _VP,

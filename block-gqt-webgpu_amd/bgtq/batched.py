@@ -417,6 +417,62 @@ def paged_decode(device, desc) -> None:
         check(lib().bgtq_paged_decode_window(device.handle, desc.pool.ref, desc.ref, desc.window))
 
 
+class PagedPrefill:
+    """A chunk call's descriptor with its pool; holds the tensors."""
+
+    def __init__(self, pool, struct, held):
+        self.pool, self.struct, self.held, self.ref = pool, struct, held, ctypes.byref(struct)
+
+
+def paged_prefill_desc(*, pages, q, out, offsets, lengths, page_table, max_length=None, scale=None, window=None, sinks=0,
+                       workspace=None) -> PagedPrefill:
+    """bgtq_paged_prefill_desc over device tensors: q, out [tokens, Hq, dim] FP16 or BF16 (any strides of the first two
+    dimensions that are multiples of 8), the new rows of the sequences packed one after another at offsets
+    [sequences + 1] int32; lengths [sequences] int32: the tokens of each with its new ones; page_table [sequences, pages
+    per sequence] int32; max_length defaults to what its rows hold; scale to 1 / sqrt(dim); window (None or 0: none) and
+    sinks as paged_decode_desc's."""
+    index, dtype = pages.device_index, q.dtype
+    code = _codes().get(dtype, _lib.DTYPE_F32)
+    _need(code != _lib.DTYPE_F32 and q.dim() == 3 and q.shape[2] == pages.dim and offsets.shape[0] > 0,
+          "q and out must be [tokens, Hq, dim] tensors of float16 or bfloat16; offsets has an entry more than sequences")
+    fields = []
+    for name, t in (("q", q), ("out", out)):
+        if t.dtype != dtype or t.get_device() != index or t.shape != q.shape:
+            raise RangeError("q and out must agree in shape, dtype and the pool's device")
+        s = t.stride()
+        _need(s[2] == 1, f"{name}'s last dimension must be dense")
+        fields += (t.data_ptr() or None, s[0] if q.shape[0] > 1 else 0, s[1] if q.shape[1] > 1 else 0)
+    _dense(index, "offsets", offsets, "int32", 1)
+    _dense(index, "lengths", lengths, "uint32" if str(lengths.dtype) == "torch.uint32" else "int32", 1)
+    st = _dense(index, "page_table", page_table, "int32", 2)
+    sequences = offsets.shape[0] - 1
+    _need(lengths.shape[0] == sequences and page_table.shape[0] == sequences, "lengths and page_table must have a row per sequence")
+    held_tokens = page_table.shape[1] * pages.struct.page_tokens
+    most = held_tokens if max_length is None else int(max_length)
+    _need(most <= held_tokens, "page_table rows hold fewer tokens than max_length")
+    _need(workspace is None or (workspace.get_device() == index and workspace.is_contiguous()), "workspace must be contiguous on the pool's device")
+    _need(scale is None or ctypes.c_float(scale).value > 0, "scale must be positive in FP32")  # (0 stands for the default)
+    w = _window(window, sinks)
+    d = _lib.PagedPrefillDesc(q.shape[1], code, sequences, q.shape[0], offsets.data_ptr(), lengths.data_ptr(),
+                              page_table.data_ptr(), st[0] if sequences > 1 else page_table.shape[1], most, *fields, scale or 0.0,
+                              0 if w is None else w.window, 0 if w is None else w.sinks,
+                              None if workspace is None else workspace.data_ptr(),
+                              0 if workspace is None else workspace.numel() * workspace.element_size())
+    return PagedPrefill(pages, d, (q, out, offsets, lengths, page_table, workspace))
+
+
+def paged_prefill_workspace_bytes(desc) -> int:
+    n = ctypes.c_size_t(0)
+    check(lib().bgtq_paged_prefill_workspace_size(desc.pool.ref, desc.ref, ctypes.byref(n)))
+    return n.value
+
+
+def paged_prefill(device, desc) -> None:
+    """bgtq_paged_prefill: attention of the descriptor's chunks of new tokens over its pages."""
+    _need(desc.pool.device_index == device.index, "the pool must lie on the context's device")
+    check(lib().bgtq_paged_prefill(device.handle, desc.pool.ref, desc.ref))
+
+
 def prompt_attention(device, q, k, v, offsets, out, scale=None, window=None, sinks=0) -> None:
     """bgtq_prompt_attention: causal attention within each of the sequences packed in q, out [tokens, Hq, dim] and
     k, v [tokens, Hkv, dim] (FP16 or BF16, any strides of the first two dimensions that are multiples of 8);

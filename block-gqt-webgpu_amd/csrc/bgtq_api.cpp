@@ -19,6 +19,7 @@
 
 #include "../../include/bgtq.h"
 #include "bgtq_internal.h"
+#include "chunk.h"
 #include "rotate.h"
 
 using namespace bgtq;
@@ -2062,6 +2063,122 @@ bgtq_status bgtq_paged_decode_window_workspace_size(const bgtq_pages *g, const b
 bgtq_status bgtq_paged_decode_window(bgtq_context *ctx, const bgtq_pages *g, const bgtq_paged_decode_desc *d, const bgtq_window *w) {
   if (bgtq_status s = check_window(w)) return s;
   return paged_decode(ctx, g, d, w);
+}
+
+// ---------------------------------------------------------------- chunks over pages
+// The fields of a chunk call that its launch and its workspace go by.
+static bgtq_status chunk_params(const bgtq_pages *g, const bgtq_paged_prefill_desc *d, ChunkParams *out) {
+  if (bgtq_status s = check_pages(g)) return s;
+  if (!d) return fail(BGTQ_ERR_RANGE, "null descriptor");
+  if (d->q_heads < g->kv_heads || d->q_heads % g->kv_heads || d->q_heads / g->kv_heads > 16)
+    return fail(BGTQ_ERR_RANGE, "invalid head geometry");
+  if (d->dtype != BGTQ_DTYPE_F16 && d->dtype != BGTQ_DTYPE_BF16) return fail(BGTQ_ERR_RANGE, "invalid dtype");
+  if (d->sequences < 0 || d->sequences > 65535) return fail(BGTQ_ERR_RANGE, "sequences must be in 0..65535");
+  if (d->tokens < 0 || d->tokens > INT32_MAX) return fail(BGTQ_ERR_RANGE, "tokens must be in 0..2^31 - 1");
+  if (d->max_length < 1 || d->max_length > (1u << 24)) return fail(BGTQ_ERR_RANGE, "max_length must be in 1..2^24");
+  if (!(d->scale >= 0.0f && d->scale <= 2.0e38f)) return fail(BGTQ_ERR_RANGE, "scale must be in 0..2e38");
+  if (d->window < 0) return fail(BGTQ_ERR_RANGE, "window must not be negative");
+  if (d->sinks < 0 || d->sinks > (1 << 30) || (d->sinks && !d->window))
+    return fail(BGTQ_ERR_RANGE, "sinks must be in 0..2^30, and 0 without a window");
+  const int64_t need = ((int64_t)d->max_length + g->page_tokens - 1) / g->page_tokens;
+  if (d->page_table_stride < need)
+    return fail(BGTQ_ERR_RANGE, "page table rows hold fewer than the %lld pages of max_length", (long long)need);
+  ChunkParams p{};
+  p.sequences = d->sequences;
+  p.heads = d->q_heads;
+  p.kv_heads = g->kv_heads;
+  p.group = d->q_heads / g->kv_heads;
+  p.tokens = d->tokens;
+  p.max_length = (int32_t)d->max_length;
+  p.target = chunk_residents(g->dim) * device_cus();
+  if (d->tokens * p.group > INT32_MAX) return fail(BGTQ_ERR_UNSUPPORTED, "paged prefill: too many (row, head) pairs for one call");
+  // (a launch counts its work-items in 32 bits)
+  if (chunk_items(p) > UINT32_MAX / (64 * kChunkWaves))
+    return fail(BGTQ_ERR_UNSUPPORTED, "paged prefill: too many (row, head) pairs for one call");
+  p.slot_columns = (int32_t)std::min<int64_t>(kChunkColumns, (std::max<int64_t>(1, d->tokens * p.group) + 31) / 32 * 32);
+  *out = p;
+  return BGTQ_OK;
+}
+
+static size_t chunk_workspace(const ChunkParams &p, int dim) {
+  return BGTQ_PAGED_PREFILL_COUNTER_BYTES + (chunk_splits(p.max_length) ? 2 * (size_t)p.target * chunk_slot_bytes(dim, p.slot_columns) : 0);
+}
+
+bgtq_status bgtq_paged_prefill_workspace_size(const bgtq_pages *g, const bgtq_paged_prefill_desc *d, size_t *bytes) {
+  ChunkParams p;
+  if (bgtq_status s = chunk_params(g, d, &p)) return s;
+  if (!bytes) return fail(BGTQ_ERR_RANGE, "null output");
+  *bytes = chunk_workspace(p, g->dim);
+  return BGTQ_OK;
+}
+
+bgtq_status bgtq_paged_prefill(bgtq_context *ctx, const bgtq_pages *g, const bgtq_paged_prefill_desc *d) {
+  ChunkParams p;
+  if (bgtq_status s = chunk_params(g, d, &p)) return s;
+  const bool none = !d->sequences || !d->tokens;
+  if (!none && (!d->offsets || !d->lengths || !d->page_table || !d->q || !d->out))
+    return fail(BGTQ_ERR_RANGE, "null offsets/lengths/page table/q/out");
+  if (reinterpret_cast<uintptr_t>(d->offsets) % 4 || reinterpret_cast<uintptr_t>(d->lengths) % 4 ||
+      reinterpret_cast<uintptr_t>(d->page_table) % 4)
+    return fail(BGTQ_ERR_RANGE, "offsets, lengths and page table must be 4-byte aligned");
+  struct {
+    const void *p;
+    int64_t row, head;
+  } x[2] = {{d->q, d->q_row_stride, d->q_head_stride}, {d->out, d->out_row_stride, d->out_head_stride}};
+  for (auto &a : x)
+    if (a.row < 0 || a.head < 0 || a.row % 8 || a.head % 8 || reinterpret_cast<uintptr_t>(a.p) % 16)
+      return fail(BGTQ_ERR_RANGE, "q/out: 16-byte aligned bases, strides multiples of 8 elements and not negative");
+  if (!apart(d->tokens, d->out_row_stride, d->q_heads, d->out_head_stride, g->dim)) return fail(BGTQ_ERR_RANGE, "out: overlapping rows");
+  const size_t need = chunk_workspace(p, g->dim);
+  if (!d->workspace || d->workspace_bytes < need) return fail(BGTQ_ERR_RANGE, "workspace of %zu bytes required", need);
+  if (reinterpret_cast<uintptr_t>(d->workspace) % 16) return fail(BGTQ_ERR_RANGE, "workspace must be 16-byte aligned");
+  if (!ctx) return fail(BGTQ_ERR_RANGE, "null context");
+  if (none) return BGTQ_OK;
+  DeviceScope scope;
+  if (bgtq_status s = ctx->use()) return s;
+  p.offsets = d->offsets;
+  p.lengths = d->lengths;
+  p.page_table = d->page_table;
+  p.page_table_stride = d->page_table_stride;
+  p.page_shift = __builtin_ctz((unsigned)g->page_tokens);
+  p.table_pages = (int32_t)(((int64_t)d->max_length + g->page_tokens - 1) / g->page_tokens);
+  p.pages = (int32_t)g->pages;
+  p.q = static_cast<const uint16_t *>(d->q);
+  p.out = static_cast<uint16_t *>(d->out);
+  p.q_row = d->q_row_stride, p.q_head = d->q_head_stride;
+  p.out_row = d->out_row_stride, p.out_head = d->out_head_stride;
+  p.c = (d->scale > 0.0f ? d->scale : (float)(1.0 / std::sqrt((double)g->dim))) * 1.4426950408889634f;
+  p.window = std::min(d->window, 1 << 25);  // (past every position; positions less it stay within 32 bits)
+  p.sinks = std::min(d->sinks, 1 << 25);
+  const bgtq_paged_rows no_rows{};
+  const PagedWriteParams w = rows_params(g, &no_rows);
+  if (g->key_format == BGTQ_KEYS_PACKED) {
+    p.packed = g->packed;
+    p.packed_page = g->packed_page_stride, p.packed_head = g->packed_head_stride;
+    p.norms = g->norms;
+    p.norms_page = g->norms_page_stride, p.norms_head = g->norms_head_stride;
+    for (int h = 0; h < g->kv_heads; ++h) {
+      p.tables[h] = w.tables[h];
+      p.head[h] = w.heads[h];
+      p.off_rot_q[h] = g->tables[h]->h()->off_rot_q;
+    }
+  } else {
+    p.k = g->k_f16;
+    p.k_page = g->k_page_stride, p.k_head = g->k_head_stride;
+  }
+  const int64_t vb = g->v_format == BGTQ_DTYPE_Q8 ? 1 : 2;
+  p.v = static_cast<const uint8_t *>(g->v);
+  p.v_page = vb * g->v_page_stride, p.v_head = vb * g->v_head_stride;
+  if (vb == 1) {
+    p.v_scales = g->v_scales;
+    p.vs_page = g->v_scales_page_stride, p.vs_head = g->v_scales_head_stride;
+  }
+  p.counters = static_cast<uint32_t *>(d->workspace);
+  p.part = reinterpret_cast<float *>(static_cast<uint8_t *>(d->workspace) + BGTQ_PAGED_PREFILL_COUNTER_BYTES);
+  static_assert(2 * 2 * 1024 * 4 <= BGTQ_PAGED_PREFILL_COUNTER_BYTES, "a counter per slot");
+  if (2 * (size_t)p.target * 4 > BGTQ_PAGED_PREFILL_COUNTER_BYTES) return fail(BGTQ_ERR_UNSUPPORTED, "paged prefill: too many compute units");
+  HIP_TRY(launch_chunk(p, g->dim, d->dtype == BGTQ_DTYPE_BF16, ctx->stream), "paged prefill launch");
+  return BGTQ_OK;
 }
 
 // ---------------------------------------------------------------- attention over packed prompts

@@ -1,0 +1,8 @@
+// Chunk attention instances: FP16 K at d=128.
+#include "chunk_kernel.h"
+
+namespace bgtq {
+
+hipError_t launch_chunk_f16_d128(const ChunkParams &p, bool bf16, hipStream_t stream) { return launch_k<128, 0>(p, bf16, stream); }
+
+}  // namespace bgtq

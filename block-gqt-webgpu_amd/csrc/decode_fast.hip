@@ -49,11 +49,22 @@ hipError_t launch_decode_paged_any128(const DecodeParams &p, const FastLayout &f
 hipError_t launch_decode_paged_d64(const DecodeParams &p, const FastLayout &fl, int nn, int sg, hipStream_t stream);
 hipError_t launch_decode_paged_d128(const DecodeParams &p, const FastLayout &fl, int nn, int sg, hipStream_t stream);
 
+hipError_t launch_decode_paged_window_any64(const DecodeParams &p, const FastLayout &fl, hipStream_t stream);
+hipError_t launch_decode_paged_window_any128(const DecodeParams &p, const FastLayout &fl, hipStream_t stream);
+hipError_t launch_decode_paged_window_d64(const DecodeParams &p, const FastLayout &fl, int nn, int sg, hipStream_t stream);
+hipError_t launch_decode_paged_window_d128(const DecodeParams &p, const FastLayout &fl, int nn, int sg, hipStream_t stream);
+
 hipError_t launch_decode_fast(const DecodeParams &p, const FastLayout &fl, int nn, int sg, hipStream_t stream) {
   const int kind = decode_fast_launch_kind(p);
   if (kind == kKindPaged) {
     if (nn < 0) return p.dim == 64 ? launch_decode_paged_any64(p, fl, stream) : launch_decode_paged_any128(p, fl, stream);
     return p.dim == 64 ? launch_decode_paged_d64(p, fl, nn, sg, stream) : launch_decode_paged_d128(p, fl, nn, sg, stream);
+  }
+  if (kind == kKindPagedWindow) {
+    if (nn < 0)
+      return p.dim == 64 ? launch_decode_paged_window_any64(p, fl, stream) : launch_decode_paged_window_any128(p, fl, stream);
+    return p.dim == 64 ? launch_decode_paged_window_d64(p, fl, nn, sg, stream)
+                       : launch_decode_paged_window_d128(p, fl, nn, sg, stream);
   }
   if (nn < 0) {  // any packed layout
     if (p.dim != 64) return launch_decode_fast_any128(p, fl, stream);

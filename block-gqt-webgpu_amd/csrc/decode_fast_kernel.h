@@ -32,7 +32,7 @@
 //             its (sequence, KV head) to arrive (a device-scope counter)
 //             merges them by log-sum-exp and resets the counter to zero.
 //
-// Pages (AP 3, 8-bit V VF 3; instances in decode_paged_*.hip): a chunk's page
+// Pages (AP 3, behind a window 4, 8-bit V VF 3; instances in decode_paged_*.hip): a chunk's page
 // comes from the sequence's table two chunks ahead, up to 64 sequences share
 // the workgroups by their lengths (paged_place), and the loop takes fewer
 // vector instructions (PAIRED, LATE). 64 x 32768 tokens, 14 / 2 heads of layout B
@@ -74,9 +74,10 @@ constexpr int kKindAppend = 2;   // decode with an appended token (bgtq_decode_a
 constexpr int kKindPrefill = 4;  // row-wise prefill (p.starts), with or without appended rows
 constexpr int kKindAll = 7;
 constexpr int kKindPaged = 8;  // decode over pages (p.page_table), instances of their own units
+constexpr int kKindPagedWindow = 16;  // the same behind a window (p.window), likewise
 
 inline int decode_fast_launch_kind(const DecodeParams &p) {
-  return p.page_table ? kKindPaged : p.starts ? kKindPrefill : p.k_new ? kKindAppend : kKindDecode;
+  return p.page_table ? (p.window ? kKindPagedWindow : kKindPaged) : p.starts ? kKindPrefill : p.k_new ? kKindAppend : kKindDecode;
 }
 
 template <int D>
@@ -428,12 +429,13 @@ struct PagedSpan {
 struct PagedPlace {
   int b, split, first, splits;  // splits 0: nothing to do; first: the sequence's first y
 };
-template <int SHIFT>
+template <int SHIFT, bool WIN>
 __device__ __forceinline__ PagedPlace paged_place(const DecodeParams &p, int y) {
   const int lane = threadIdx.x & 63;
   const uint32_t len = p.lengths[min(lane, p.batch - 1)];
-  const int tokens = PagedSpan((int)min(len, (uint32_t)p.max_length), p.window, p.sinks).tokens;
-  const int steps = lane < p.batch ? (tokens + (1 << SHIFT) - 1) >> SHIFT : 0;
+  uint32_t tokens = min(len, (uint32_t)p.max_length);
+  if (WIN) tokens = (uint32_t)PagedSpan((int)tokens, p.window, p.sinks).tokens;
+  const int steps = lane < p.batch ? (int)((tokens + (1u << SHIFT) - 1) >> SHIFT) : 0;
   const float target = (float)p.split_target;
   float t = fmaxf(1.0f, ceilf((float)wave_sum(steps) / target));
   // (the thousandth: a quotient that is whole stays so through the reciprocal)
@@ -457,7 +459,9 @@ __device__ __forceinline__ PagedPlace paged_place(const DecodeParams &p, int y) 
 
 // AP: what a launch does beside attention, compiled in only where used: 0
 // nothing, 1 the appended rows (decode or prefill append), 2 materialised
-// logits (inspect()), 3 K and V in pages (decode; a sequence may be empty).
+// logits (inspect()), 3 K and V in pages (decode; a sequence may be empty), 4
+// the same behind a window (in one instance with 3 it cost that 2 to 3%: 64 x
+// 32768 tokens 105.4 / 107.6 us, one SmolLM2 step 10.25 / 10.56).
 // RL: the workgroup's role in a launch with appended rows and packed K, known
 // from its split index before anything else: 1 a history split, 2 an append
 // workgroup; 0 either (decided at run time). The kernel below picks it.
@@ -466,7 +470,7 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
   using Gm = Geo<D>;
   using Sl = Slot<D, KF, NN, VF, NW>;
   static_assert(VF == 0 || PF == 0, "FP32 and 8-bit V: decode only");
-  static_assert((AP == 3) >= (VF == 3) && (AP != 3 || (PF == 0 && VF != 1 && VF != 2 && Sl::AHEAD == 1)), "pages");
+  static_assert((AP >= 3) >= (VF == 3) && (AP < 3 || (PF == 0 && VF != 1 && VF != 2 && Sl::AHEAD == 1)), "pages");
   static_assert(NW == 4 || NW == 8, "waves per workgroup");
   constexpr int kWaves = NW, kThreads = 64 * NW;
   static_assert(PF == 0 || PF == 8 || PF == 16, "row-wise unit width");
@@ -475,7 +479,7 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
   constexpr int KS = Gm::KS, DT = Gm::DT, PR = Gm::PR, VI = Sl::VI, KRI = Gm::KRI;
   constexpr bool VF32 = VF == 1 || VF == 2, Q8 = VF == 3;
   constexpr int VB = VF32 ? 4 : Q8 ? 1 : 2;  // bytes per V value
-  constexpr bool PG = AP == 3;               // K and V lie in pages
+  constexpr bool PG = AP >= 3, WIN = AP == 4;  // K and V lie in pages; behind a window
   constexpr bool NAT = VF32;                 // logits in natural units, else log2 domain
   constexpr bool F32 = VF == 1 && KF >= 1;     // rotation and QK in FP32
   constexpr float kLogit = NAT ? 1.0f : kLn2;  // a logit's natural value
@@ -502,7 +506,7 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
   PagedPlace pg_at{(int)blockIdx.z, (int)blockIdx.x, 0, p.splits};
   if constexpr (PG)
     if (p.split_target) {
-      pg_at = paged_place<(NW == 8 ? 8 : 7)>(p, blockIdx.y);
+      pg_at = paged_place<(NW == 8 ? 8 : 7), WIN>(p, blockIdx.y);
       if (pg_at.splits == 0) return;
     }
   const int split = PF ? blockIdx.z : PG ? pg_at.split : blockIdx.x, qrow = PF ? blockIdx.y : PG ? pg_at.b : blockIdx.z;
@@ -511,7 +515,8 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
   BGTQ_LOAD_ARGS
   if constexpr (PG)
     asm volatile("" ::"s"(p.page_table), "s"(p.page_table_stride), "s"(p.page_shift), "s"(p.table_pages), "s"(p.pages),
-                 "s"(p.v_scales), "s"(p.window), "s"(p.sinks));
+                 "s"(p.v_scales));
+  if constexpr (WIN) asm volatile("" ::"s"(p.window), "s"(p.sinks));
   __builtin_amdgcn_sched_barrier(0);
   const int unit = qrow * p.kv_heads + kv;
   uint32_t *const counter = p.counters + (int64_t)unit * (p.counter_stride > 0 ? p.counter_stride : 1);
@@ -603,15 +608,11 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
   // nothing). A vector load, older than the loads of the chunk before its own.
   const int first_pg = (split * kWaves + wave) * kChunk, stride_pg = pg_at.splits * kWaves * kChunk;
   // (Behind a window the place of a chunk takes the length, waited for here.)
-  int span_n = 0;
-  if (PG && p.window) {
-    span_n = (int)min(len_b, (uint32_t)p.max_length);
-    asm volatile("" : "+s"(span_n));  // (made a select, it would be waited for without a window too)
-  }
-  const PagedSpan span(span_n, PG ? p.window : 0, PG ? p.sinks : 0);
+  const PagedSpan span(WIN ? (int)min(len_b, (uint32_t)p.max_length) : 0, WIN ? p.window : 0, WIN ? p.sinks : 0);
   auto load_page = [&](int i) -> int {
-    int lo, hi;
-    const int at = min(span.place(first_pg + i * stride_pg, lo, hi) >> p.page_shift, p.table_pages - 1);
+    int lo, hi, c = first_pg + i * stride_pg;
+    if constexpr (WIN) c = span.place(c, lo, hi);
+    const int at = min(c >> p.page_shift, p.table_pages - 1);
     return p.page_table[(int64_t)b * p.page_table_stride + at];
   };
   // The page as an index into the pool: -1 where the table names none.
@@ -786,7 +787,7 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
   // Tokens the history splits attend to; the append workgroup's range ends
   // after its rows (decode: all tokens, so the new one lies inside the causal
   // limits).
-  const int T_att = PG && p.window ? span.tokens : !app ? T_b : app_wg ? (rowwise ? start_c + r_a + n_a : T_b) : rowwise ? start_c : T_b - 1;
+  const int T_att = WIN ? span.tokens : !app ? T_b : app_wg ? (rowwise ? start_c + r_a + n_a : T_b) : rowwise ? start_c : T_b - 1;
   // Splits of one (sequence, KV head) interleave at chunk granularity: wave w
   // of split s takes chunks (s * 4 + w) + 4 S i, so the waves working on a
   // sequence at any moment sweep adjacent memory.
@@ -807,10 +808,7 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
   auto chunk_at = [&](int i, int &lo, int &hi) {
     const int c = first + i * stride;
     lo = 0, hi = T_att;
-    if constexpr (PG) {
-      if (p.window) return span.place(c, lo, hi);
-    }
-    return c;
+    return WIN ? span.place(c, lo, hi) : c;
   };
   auto issue = [&](int i, int pg = 0) {
     int lo, hi;
@@ -829,7 +827,7 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
     const uint8_t *k_base_c = PG ? k_base + pn * (KF >= 1 ? p.packed_seq_stride : 2 * p.k_seq_stride) : k_base;
     const uint16_t *n_base_c = PG && KF >= 1 ? n_base + pn * p.norms_seq_stride : n_base;
     const __amdgpu_buffer_rsrc_t rV = rsrc(v_rows_c + (int64_t)r0 * D * VB, rest * (VB * D));
-    if (PG && !Q8 && c0 < lo) {
+    if (WIN && !Q8 && c0 < lo) {
       // The window begins inside the chunk (wave-uniform): V rows before it may
       // hold infinities or NaNs and arrive as zeros, their offsets past the range.
 #pragma unroll
@@ -1710,7 +1708,7 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
         x[4 * u + r] = LATE ? v : v * kq;
       }
     }
-    if constexpr (PG) {
+    if constexpr (WIN) {
       if (c0 + kChunk > hi || c0 < lo || !in_pool) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -1718,11 +1716,11 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
           x[j] = tok < hi && tok >= lo && in_pool ? x[j] : -INFINITY;
         }
       }
-    } else if (c0 + kChunk > lim_min) {
+    } else if (c0 + kChunk > lim_min || !in_pool) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int tok = c0 + 16 * (j >> 2) + 4 * gq + (j & 3);
-        x[j] = tok < lim ? x[j] : -INFINITY;
+        x[j] = tok < lim && in_pool ? x[j] : -INFINITY;
       }
     }
   };
@@ -1738,11 +1736,12 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
       const uint8_t *sc = sb + Sl::VSOFF + 8 * gq;
       const u32x2 s0 = *reinterpret_cast<const u32x2 *>(sc), s1 = *reinterpret_cast<const u32x2 *>(sc + 32);
       uint32_t s4[4] = {s0[0], s0[1], s1[0], s1[1]};  // tokens 4 gq + 0..3, 16 + 4 gq + 0..3
-      if (rest < kChunk || skip > 0) {  // (wave-uniform) no scale of a row that is not attended to: it may hold anything
+      if (rest < kChunk || (WIN && skip > 0)) {  // (wave-uniform) no scale of a row that is not attended to: it may hold anything
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int tok = 16 * (j >> 1) + 4 * gq + 2 * (j & 1);
-          s4[j] &= (tok < rest && tok >= skip ? 0xffffu : 0u) | (tok + 1 < rest && tok + 1 >= skip ? 0xffff0000u : 0u);
+          if constexpr (WIN) s4[j] &= (tok < rest && tok >= skip ? 0xffffu : 0u) | (tok + 1 < rest && tok + 1 >= skip ? 0xffff0000u : 0u);
+          else s4[j] = tok + 1 < rest ? s4[j] : tok < rest ? s4[j] & 0xffffu : 0u;
         }
       }
       const int r8 = col >> 1, vrow = 16 * (r8 >> 2) + 4 * gq + (r8 & 3);
@@ -1957,7 +1956,7 @@ __device__ __forceinline__ void decode_fast_body(const DecodeParams &p, const Fa
       // there: 64 x 32768 tokens 106.0 / 103.7, 29 ragged FP16 sequences 54.8 / 52.8).
       if (!PF && !PG) wait_vm<0>();
       const half8 pha = __builtin_bit_cast(half8, ph), pla = __builtin_bit_cast(half8, pl);
-      chunk_pv(sb, pha, pla, pr, PG ? lo - c0 : 0, PG ? min(hi - c0, kChunk) : kChunk);
+      chunk_pv(sb, pha, pla, pr, WIN ? lo - c0 : 0, PG ? min(hi - c0, kChunk) : kChunk);
       if constexpr (PG) in_pool = in_pool_next;
     }
   }
@@ -2216,7 +2215,7 @@ hipError_t launch_mode(const DecodeParams &p, const FastLayout &fl, hipStream_t 
   // head) or unit for them.
   const unsigned app = KF >= 1 && p.k_new ? (unsigned)p.app_parts : 0u;
   const dim3 grid = PF ? dim3((unsigned)p.kv_heads, (unsigned)(p.batch * p.qgroups), (unsigned)p.splits + app)
-                    : AP == 3 && p.split_target
+                    : AP >= 3 && p.split_target
                         ? dim3((unsigned)p.kv_heads, (unsigned)(p.split_target + p.batch))
                         : dim3((unsigned)p.splits + app, (unsigned)p.kv_heads, (unsigned)p.batch);
   hipLaunchKernelGGL((decode_fast_kernel<D, KF, NN, SG, PK, PF, VF, NW, AP>), grid, dim3(64 * NW), lds, stream, p, fl);
@@ -2231,14 +2230,15 @@ template <int KINDS, int D, int KF, int NN, int SG, int PK = 0>
 hipError_t launch_one(const DecodeParams &p, const FastLayout &fl, hipStream_t stream) {
   const int kind = decode_fast_launch_kind(p);
   if (!(kind & KINDS)) return hipErrorInvalidValue;
-  if constexpr ((KINDS & kKindPaged) != 0) {
-    static_assert(KINDS == kKindPaged, "pages have units of their own");
+  if constexpr ((KINDS & (kKindPaged | kKindPagedWindow)) != 0) {
+    static_assert(KINDS == kKindPaged || KINDS == kKindPagedWindow, "pages have units of their own");
+    constexpr int AP = KINDS == kKindPaged ? 3 : 4;
     if constexpr (D == 64 && KF != 2)  // (the per-position path keeps four waves)
       if (p.waves == 8)
-        return p.v_scales ? launch_mode<D, KF, NN, SG, PK, 0, 3, 8, 3>(p, fl, stream)
-                          : launch_mode<D, KF, NN, SG, PK, 0, 0, 8, 3>(p, fl, stream);
-    return p.v_scales ? launch_mode<D, KF, NN, SG, PK, 0, 3, kWaves, 3>(p, fl, stream)
-                      : launch_mode<D, KF, NN, SG, PK, 0, 0, kWaves, 3>(p, fl, stream);
+        return p.v_scales ? launch_mode<D, KF, NN, SG, PK, 0, 3, 8, AP>(p, fl, stream)
+                          : launch_mode<D, KF, NN, SG, PK, 0, 0, 8, AP>(p, fl, stream);
+    return p.v_scales ? launch_mode<D, KF, NN, SG, PK, 0, 3, kWaves, AP>(p, fl, stream)
+                      : launch_mode<D, KF, NN, SG, PK, 0, 0, kWaves, AP>(p, fl, stream);
   }
   if (p.v_dtype == BGTQ_DTYPE_F32) {
     if constexpr ((KINDS & kKindDecode) != 0)

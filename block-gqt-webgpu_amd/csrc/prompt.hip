@@ -288,14 +288,21 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 4 : 2) void prompt_kernel(Promp
     }
   };
   // The keys of the workgroup's block i0 for this wave's queries; DIAGONAL: some queries see only a part of them.
-  auto attend = [&](auto diagonal_tag, int i0) {
+  // (WIN, DIAGONAL: unless `whole`.)
+  auto attend = [&](auto diagonal_tag, int i0, bool whole = false) {
     constexpr bool DIAGONAL = decltype(diagonal_tag)::value;
     const int j = block(i0);
     const uint32_t buf = (uint32_t)(i0 & 1) * 2 * BLOCK;
-    // Whether this lane's query sees key 4 h + k of the block.
+    // Whether this lane's query sees key 4 h + k of the block; behind a window
+    // from a bit for each (one comparison more per key spilled 65 registers).
     const int d = qi - j * kKeys - 4 * h;
-    const int d_low = WIN ? d - p.window : 0, d_sink = WIN ? p.sinks - j * kKeys - 4 * h : 0;
-    auto sees = [&](int k) { return k <= d && (!WIN || k > d_low || k < d_sink); };
+    uint64_t seen_bits = 0;
+    if constexpr (WIN && DIAGONAL) {
+      auto below = [](int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : ~(~0ull << n); };  // bits 0 .. n - 1
+      seen_bits = below(d + 1) & (~below(d + 1 - p.window) | below(p.sinks - j * kKeys - 4 * h));
+    }
+    const uint32_t seen_lo = (uint32_t)seen_bits, seen_hi = (uint32_t)(seen_bits >> 32);
+    auto sees = [&](int k) -> bool { return WIN ? (k < 32 ? seen_lo >> k : seen_hi >> (k - 32)) & 1u : k <= d; };
     f32x16 S[2];
 #pragma unroll
     for (int b = 0; b < 2; ++b)
@@ -308,7 +315,7 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 4 : 2) void prompt_kernel(Promp
         const u32x4 a = *reinterpret_cast<const u32x4 *>(smem + ((buf + k_at) ^ (32u * s)) + 64 * D * b);
         S[b] = product<BF>(a, qf[s], S[b]);
       }
-    if constexpr (DIAGONAL) {
+    if (DIAGONAL && !whole) {
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -358,7 +365,7 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 4 : 2) void prompt_kernel(Promp
     // infinity or a NaN of its V row is not 0: such a block's products take
     // the finite values, and what is seen of the others is added by itself.
     bool plain = true;
-    if constexpr (DIAGONAL) {
+    if (DIAGONAL && !whole) {
       typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
       u16x2 most{0, 0};
 #pragma unroll
@@ -387,6 +394,10 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 4 : 2) void prompt_kernel(Promp
         if (s == 2) ds_read_tr16<MT, 3 * STEP>(va, va8, v[1]);
       }
     } else {
+      // (through an opaque copy: or the rare branch's addresses are held across the loop)
+      int rare = lane;
+      asm volatile("" : "+v"(rare));
+      const int h = rare >> 5, qc = rare & 31;
       // V of dimension 32 t + qc, keys 16 s + 8 (e / 2) + 4 h + 2 (e % 2) + 0, 1 in word e.
       auto column = [&](int s, int t) {
         u32x4 a;
@@ -442,34 +453,31 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 4 : 2) void prompt_kernel(Promp
   // One block holds the wave's diagonal (32 rows lie within one); those after
   // it hold no key that its queries see. Loops of their own, so that the full
   // blocks' carries none of the diagonal's code.
-  // Behind a window the full blocks have some before them that the queries
-  // see a part of, or nothing: the sinks' and those of the window's edge.
+  // Behind a window the blocks before the full ones are seen in part or not at
+  // all: the sinks' and those of the window's edge.
   const int jd = row0 / kKeys;
   int j = 0;
   if constexpr (WIN) {
+    // (one body for both: with one for the full blocks and one for the others it spilled 97 registers)
     const int low = row0 - p.window;  // the last key that the first query does not see
     for (; j < n_blocks; ++j) {
       const int k0 = block(j) * kKeys;
-      if (k0 >= jd * kKeys || k0 > low + 31) break;
       arrive(j);
-      if (k0 < p.sinks || k0 + kKeys - 1 > low) attend(std::true_type{}, j);
-    }
-    for (; j < n_blocks && block(j) < jd; ++j) {
-      arrive(j);
-      attend(std::false_type{}, j);
+      const bool whole = k0 > low + 31 && k0 < jd * kKeys;
+      if (k0 <= jd * kKeys && (k0 < p.sinks || k0 + kKeys - 1 > low)) attend(std::true_type{}, j, whole);
     }
   } else {
     for (; j < min(jd, n_blocks); ++j) {
       arrive(j);
       attend(std::false_type{}, j);
     }
+    if (j < n_blocks) {
+      arrive(j);
+      attend(std::true_type{}, j);
+      ++j;
+    }
+    for (; j < n_blocks; ++j) arrive(j);
   }
-  if (j < n_blocks) {
-    arrive(j);
-    attend(std::true_type{}, j);
-    ++j;
-  }
-  for (; j < n_blocks; ++j) arrive(j);
   l = half_sum(l);
   if (qi >= at.len) return;
   const float inv = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;  // (a NaN stays one)

@@ -537,6 +537,47 @@ bgtq_status bgtq_paged_decode_window_workspace_size(const bgtq_pages *pages, con
 bgtq_status bgtq_paged_decode_window(bgtq_context *ctx, const bgtq_pages *pages, const bgtq_paged_decode_desc *d,
                                      const bgtq_window *w);
 
+/* Attention of chunks of new tokens over pages (bgtq_prefill for sequences of
+ * any lengths in pages, src/model/decoder.ts:46-56 with rows > 1): sequence s brings
+ * the rows offsets[s] .. offsets[s+1] - 1 of q and out, its last ones: row i of c has
+ * position lengths[s] - c + i and sees the tokens up to its own (behind a window,
+ * window > 0: as bgtq_window). The pages already hold the new tokens (bgtq_paged_append
+ * or _write first). A batch may mix sequences of one new token, many and none.
+ * dtype: BGTQ_DTYPE_F16 or _BF16, of q and out; layouts of both as bgtq_prompt_desc's;
+ * offsets are clamped to 0 .. tokens, lengths to max_length; rows of no sequence stay
+ * as they were, rows that see nothing (negative positions, tokens without a page)
+ * become zero. Tokens whose table entry is not a page of the pool are left out.
+ * q_heads / kv_heads at most 16; tokens * q_heads / kv_heads below 2^31. Logits, softmax
+ * statistics and sums are FP32; probabilities are rounded to FP16 (11 bits down to
+ * 2^-25 of the largest) for the product with V. Packed K is multiplied in the code
+ * domain: BF16 rows by the rotated query and K row rounded to FP16 each, FP16
+ * rows by both as pairs of FP16 values (22 bits). scale: of the logits, at most 2e38; 0 =
+ * 1 / sqrt(dim). workspace: 16-byte aligned, bgtq_paged_prefill_workspace_size()
+ * bytes (its first BGTQ_PAGED_PREFILL_COUNTER_BYTES zero before the first call on it,
+ * left zero by every call whatever its geometry; the rest needs no contents);
+ * calls sharing one must be ordered on one stream. One launch, HIP-graph capturable;
+ * out overlaps neither q nor the pool. */
+#define BGTQ_PAGED_PREFILL_COUNTER_BYTES (64u * 1024u)
+typedef struct {
+  int32_t q_heads, dtype, sequences;
+  int64_t tokens;
+  const int32_t *offsets;    /* device int32 [sequences + 1], nondecreasing */
+  const uint32_t *lengths;   /* device uint32 [sequences]: tokens with the chunk's */
+  const int32_t *page_table; /* device int32 [sequences][page_table_stride] */
+  int64_t page_table_stride; /* elements; at least ceil(max_length / page_tokens) */
+  uint32_t max_length;       /* 1 .. 2^24 */
+  const void *q;
+  int64_t q_row_stride, q_head_stride;
+  void *out;
+  int64_t out_row_stride, out_head_stride;
+  float scale;
+  int32_t window, sinks; /* 0: no window */
+  void *workspace;
+  size_t workspace_bytes;
+} bgtq_paged_prefill_desc;
+bgtq_status bgtq_paged_prefill_workspace_size(const bgtq_pages *pages, const bgtq_paged_prefill_desc *d, size_t *bytes);
+bgtq_status bgtq_paged_prefill(bgtq_context *ctx, const bgtq_pages *pages, const bgtq_paged_prefill_desc *d);
+
 /* Attention over whole prompts, before their rows enter a cache: causal
  * self-attention of `sequences` sequences of different lengths packed one
  * after another, sequence s the rows offsets[s] .. offsets[s+1] - 1 of q, k, v
