@@ -33,7 +33,7 @@ DEVICE_SOURCES = ["encode.hip", "encode_bulk.hip", "encode_tile.hip", "encode_wa
                   "decode_fast_d128.hip", "decode_paged_any64.hip", "decode_paged_any128.hip", "decode_paged_d64.hip",
                   "decode_paged_d128.hip", "decode_paged_window_any64.hip", "decode_paged_window_any128.hip",
                   "decode_paged_window_d64.hip", "decode_paged_window_d128.hip", "prefill.hip", "reconstruct.hip", "model_ops.hip", "decode_scratch.hip",
-                  "paged_rows.hip", "prompt.hip", "rotate.hip", "chunk.hip", "chunk_f16_d64.hip",
+                  "paged_rows.hip", "prompt.hip", "rotate.hip", "chunk.hip", "chunk_wide.hip", "chunk_f16_d64.hip",
                   "chunk_f16_d128.hip", "chunk_packed2_d64.hip", "chunk_packed2_d128.hip", "chunk_packed_d64.hip",
                   "chunk_packed_d128.hip"]
 HOST_SOURCES = ["bgtq_api.cpp", "calibrate.cpp"]

@@ -2067,7 +2067,7 @@ bgtq_status bgtq_paged_decode_window(bgtq_context *ctx, const bgtq_pages *g, con
 
 // ---------------------------------------------------------------- chunks over pages
 // The fields of a chunk call that its launch and its workspace go by.
-static bgtq_status chunk_params(const bgtq_pages *g, const bgtq_paged_prefill_desc *d, ChunkParams *out) {
+static bgtq_status chunk_params(const bgtq_pages *g, const bgtq_paged_prefill_desc *d, ChunkParams *out, ChunkPlan *plan) {
   if (bgtq_status s = check_pages(g)) return s;
   if (!d) return fail(BGTQ_ERR_RANGE, "null descriptor");
   if (d->q_heads < g->kv_heads || d->q_heads % g->kv_heads || d->q_heads / g->kv_heads > 16)
@@ -2085,36 +2085,38 @@ static bgtq_status chunk_params(const bgtq_pages *g, const bgtq_paged_prefill_de
     return fail(BGTQ_ERR_RANGE, "page table rows hold fewer than the %lld pages of max_length", (long long)need);
   ChunkParams p{};
   p.sequences = d->sequences;
-  p.heads = d->q_heads;
   p.kv_heads = g->kv_heads;
   p.group = d->q_heads / g->kv_heads;
   p.tokens = d->tokens;
   p.max_length = (int32_t)d->max_length;
-  p.target = chunk_residents(g->dim) * device_cus();
   if (d->tokens * p.group > INT32_MAX) return fail(BGTQ_ERR_UNSUPPORTED, "paged prefill: too many (row, head) pairs for one call");
+  *plan = plan_chunks(p, g->dim, g->key_format == BGTQ_KEYS_PACKED, g->v_format == BGTQ_DTYPE_Q8, d->dtype == BGTQ_DTYPE_BF16, device_cus());
   // (a launch counts its work-items in 32 bits)
-  if (chunk_items(p) > UINT32_MAX / (64 * kChunkWaves))
+  if (std::max(plan->narrow_items + 2 * device_cus() + kMaxKvHeads, plan->wide_items) > UINT32_MAX / (64 * kChunkWaves))
     return fail(BGTQ_ERR_UNSUPPORTED, "paged prefill: too many (row, head) pairs for one call");
-  p.slot_columns = (int32_t)std::min<int64_t>(kChunkColumns, (std::max<int64_t>(1, d->tokens * p.group) + 31) / 32 * 32);
+  if (2 * (int64_t)std::max(plan->narrow_aim, plan->wide_aim) * 4 > BGTQ_PAGED_PREFILL_COUNTER_BYTES)
+    return fail(BGTQ_ERR_UNSUPPORTED, "paged prefill: too many compute units");
   *out = p;
   return BGTQ_OK;
 }
 
-static size_t chunk_workspace(const ChunkParams &p, int dim) {
-  return BGTQ_PAGED_PREFILL_COUNTER_BYTES + (chunk_splits(p.max_length) ? 2 * (size_t)p.target * chunk_slot_bytes(dim, p.slot_columns) : 0);
+static size_t chunk_workspace(const ChunkPlan &plan) {
+  return BGTQ_PAGED_PREFILL_COUNTER_BYTES + (size_t)(plan.part_bytes + plan.rebuilt_bytes + plan.turned_bytes);
 }
 
 bgtq_status bgtq_paged_prefill_workspace_size(const bgtq_pages *g, const bgtq_paged_prefill_desc *d, size_t *bytes) {
   ChunkParams p;
-  if (bgtq_status s = chunk_params(g, d, &p)) return s;
+  ChunkPlan plan;
+  if (bgtq_status s = chunk_params(g, d, &p, &plan)) return s;
   if (!bytes) return fail(BGTQ_ERR_RANGE, "null output");
-  *bytes = chunk_workspace(p, g->dim);
+  *bytes = chunk_workspace(plan);
   return BGTQ_OK;
 }
 
 bgtq_status bgtq_paged_prefill(bgtq_context *ctx, const bgtq_pages *g, const bgtq_paged_prefill_desc *d) {
   ChunkParams p;
-  if (bgtq_status s = chunk_params(g, d, &p)) return s;
+  ChunkPlan plan;
+  if (bgtq_status s = chunk_params(g, d, &p, &plan)) return s;
   const bool none = !d->sequences || !d->tokens;
   if (!none && (!d->offsets || !d->lengths || !d->page_table || !d->q || !d->out))
     return fail(BGTQ_ERR_RANGE, "null offsets/lengths/page table/q/out");
@@ -2129,7 +2131,7 @@ bgtq_status bgtq_paged_prefill(bgtq_context *ctx, const bgtq_pages *g, const bgt
     if (a.row < 0 || a.head < 0 || a.row % 8 || a.head % 8 || reinterpret_cast<uintptr_t>(a.p) % 16)
       return fail(BGTQ_ERR_RANGE, "q/out: 16-byte aligned bases, strides multiples of 8 elements and not negative");
   if (!apart(d->tokens, d->out_row_stride, d->q_heads, d->out_head_stride, g->dim)) return fail(BGTQ_ERR_RANGE, "out: overlapping rows");
-  const size_t need = chunk_workspace(p, g->dim);
+  const size_t need = chunk_workspace(plan);
   if (!d->workspace || d->workspace_bytes < need) return fail(BGTQ_ERR_RANGE, "workspace of %zu bytes required", need);
   if (reinterpret_cast<uintptr_t>(d->workspace) % 16) return fail(BGTQ_ERR_RANGE, "workspace must be 16-byte aligned");
   if (!ctx) return fail(BGTQ_ERR_RANGE, "null context");
@@ -2173,11 +2175,22 @@ bgtq_status bgtq_paged_prefill(bgtq_context *ctx, const bgtq_pages *g, const bgt
     p.v_scales = g->v_scales;
     p.vs_page = g->v_scales_page_stride, p.vs_head = g->v_scales_head_stride;
   }
-  p.counters = static_cast<uint32_t *>(d->workspace);
-  p.part = reinterpret_cast<float *>(static_cast<uint8_t *>(d->workspace) + BGTQ_PAGED_PREFILL_COUNTER_BYTES);
-  static_assert(2 * 2 * 1024 * 4 <= BGTQ_PAGED_PREFILL_COUNTER_BYTES, "a counter per slot");
-  if (2 * (size_t)p.target * 4 > BGTQ_PAGED_PREFILL_COUNTER_BYTES) return fail(BGTQ_ERR_UNSUPPORTED, "paged prefill: too many compute units");
-  HIP_TRY(launch_chunk(p, g->dim, d->dtype == BGTQ_DTYPE_BF16, ctx->stream), "paged prefill launch");
+  uint8_t *const ws = static_cast<uint8_t *>(d->workspace);
+  p.counters = reinterpret_cast<uint32_t *>(ws);
+  p.part = reinterpret_cast<float *>(ws + BGTQ_PAGED_PREFILL_COUNTER_BYTES);
+  if (plan.rebuilt_rows) {
+    const int64_t operand = plan.rebuilt_rows * g->kv_heads * g->dim;
+    uint16_t *const at = reinterpret_cast<uint16_t *>(ws + BGTQ_PAGED_PREFILL_COUNTER_BYTES + plan.part_bytes);
+    p.rebuilt_k = at;
+    p.rebuilt_v = at + operand;
+    p.rebuilt_lo = plan.split ? at + 2 * operand : nullptr;
+    p.rebuilt_head = plan.rebuilt_rows;
+    if (plan.turned_bytes) {
+      p.turned = at + plan.rebuilt_bytes / 2;
+      p.turned_exp = reinterpret_cast<int32_t *>(p.turned + d->tokens * d->q_heads * g->dim * (plan.split ? 2 : 1));
+    }
+  }
+  HIP_TRY(launch_chunks(p, plan, g->dim, d->dtype == BGTQ_DTYPE_BF16, device_cus(), ctx->stream), "paged prefill launch");
   return BGTQ_OK;
 }
 

@@ -1,28 +1,41 @@
-// Attention of chunks of new tokens over the paged cache: launch parameters
-// (chunk_kernel.h has the kernel, chunk_*.hip its instances).
+// Attention of chunks of new tokens over the paged cache (bgtq_paged_prefill,
+// src/model/decoder.ts:46-56 with rows > 1, over pages): launch parameters.
+//
+// A sequence's chunk has rows x G query columns per KV head. Narrow ones (at
+// most 32) are attended straight from the pages (chunk_rows.h); the rows that wide
+// ones see are rebuilt once, in the same launch, and attended in a second one
+// (chunk_wide.hip), which reads FP16 pages as they lie. Units (a sequence, a KV
+// head, a tile of columns) are cut along their tokens into items where there are
+// few, whose partials are merged in their order: narrow units' by the last item
+// to end, wide ones' in a third launch.
 #pragma once
 
 #include "bgtq_internal.h"
 
 namespace bgtq {
 
-constexpr int kChunkWaves = 8;                   // of a workgroup
-constexpr int kChunkColumns = 32 * kChunkWaves;  // query columns (row x head of a KV head's group) of a tile
+constexpr int kChunkWaves = 8;                   // of a workgroup for narrow units
+constexpr int kChunkColumns = 32 * kChunkWaves;
 constexpr int kChunkKeys = 64;                   // tokens of a block
-// Workgroups that share a compute unit: a launch aims at as many items as the chip holds.
-constexpr int chunk_residents(int dim) { return dim == 64 ? 2 : 1; }
+// Wide units: waves of a workgroup, waves per SIMD by their registers, workgroups per compute unit.
+constexpr int chunk_wide_waves(int dim, bool split) { return dim == 128 && split ? 8 : 4; }
+constexpr int chunk_wide_waves_per_simd(int dim, bool split) { return dim == 64 ? split ? 3 : 4 : 2; }
+constexpr int chunk_wide_residents(int dim, bool split) {
+  return 4 * chunk_wide_waves_per_simd(dim, split) / chunk_wide_waves(dim, split);
+}
 // Costs of a unit, in eighths of a wide block: its set-up, a block of a wide
-// unit, one of a narrow unit (at most 32 columns: the waves share its blocks);
-// the least cost of an item where a unit is split.
+// unit, one of a narrow unit; the least cost of an item where a unit is split.
 constexpr int kChunkSetup = 16, kChunkWide = 8, kChunkNarrow = 3, kChunkLeast = 48;
 constexpr int kChunkMostSplits = 64;
+// Bytes of rebuilt rows at most: sequences that take more are attended in groups.
+constexpr int64_t kChunkRebuiltBytes = (int64_t)1 << 30;
 
 struct ChunkParams {
   const int32_t *offsets;
   const uint32_t *lengths;
   const int32_t *page_table;
   int64_t page_table_stride;
-  int32_t sequences, heads, kv_heads, group;  // query heads; KV heads; query heads per KV head
+  int32_t sequences, kv_heads, group;  // KV heads; query heads per KV head
   int64_t tokens;
   int32_t max_length, page_shift, table_pages, pages;
   const uint16_t *q;
@@ -44,22 +57,32 @@ struct ChunkParams {
   const DevTables *tables[kMaxKvHeads];
   PagedWriteParams::Head head[kMaxKvHeads];
   uint32_t off_rot_q[kMaxKvHeads];
-  // Items: units' splits; `target` of them are aimed at, a split unit's leave
-  // partials in slots of slot_columns columns.
-  int32_t target, slot_columns;
+  // Items: units' splits; `aim` of them are aimed at, a split unit's leave
+  // partials in slots of slot_columns columns. narrow_items: the workgroups of
+  // the first launch that attend.
+  int32_t aim, slot_columns, narrow_items, rotate_items;
   uint32_t *counters;
   float *part;
+  // Rebuilt rows, [KV head][row][dim]: K (and its low parts), V; null: pages are read as they lie.
+  uint16_t *rebuilt_k, *rebuilt_lo, *rebuilt_v;
+  int64_t rebuilt_head;  // rows of a KV head
+  // Packed K: the queries in the code domain, [row][head][dim] (BF16 rows' FP16
+  // values; FP16 rows': high parts, then low ones), and their powers of two.
+  uint16_t *turned;
+  int32_t *turned_exp;
 };
 
-// Bytes of a slot's partial results: (o[dim], m, l) of each column.
-inline int64_t chunk_slot_bytes(int dim, int columns) { return (int64_t)columns * (dim + 2) * 4; }
-// Whether a unit of so many tokens may cost more than the least item, and is then split where there are few.
-constexpr bool chunk_splits(int64_t max_length) {
-  return kChunkSetup + kChunkWide * ((max_length + kChunkKeys - 1) / kChunkKeys) > kChunkLeast;
-}
-// Items that a launch's grid has room for: its units, and as many again as it
-// aims at where units are split (the items of split units number at most 2 target).
-int64_t chunk_items(const ChunkParams &p);
-hipError_t launch_chunk(const ChunkParams &p, int dim, bool bf16, hipStream_t stream);
+// What a call launches, from what the host knows.
+struct ChunkPlan {
+  bool split;               // K and q as pairs of FP16 values
+  int64_t wide_sequences;   // that may be wide at most
+  int64_t narrow_items;     // first launch: attending workgroups
+  int32_t narrow_aim, wide_aim, wide_columns;
+  int64_t group, wide_items;  // sequences of a group; items of its launch at most
+  int64_t slots;              // of its split units at most
+  int64_t part_bytes, rebuilt_rows, rebuilt_bytes, turned_bytes;  // rows of a KV head; of all operands
+};
+ChunkPlan plan_chunks(const ChunkParams &p, int dim, bool packed, bool q8, bool bf16, int cus);
+hipError_t launch_chunks(const ChunkParams &p, const ChunkPlan &plan, int dim, bool bf16, int cus, hipStream_t stream);
 
 }  // namespace bgtq

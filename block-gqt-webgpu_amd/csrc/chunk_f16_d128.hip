@@ -1,8 +1,10 @@
-// Chunk attention instances: FP16 K at d=128.
-#include "chunk_kernel.h"
+// Chunk attention, narrow units and rebuilt rows: instances for FP16 K at d=128.
+#include "chunk_rows.h"
 
 namespace bgtq {
 
-hipError_t launch_chunk_f16_d128(const ChunkParams &p, bool bf16, hipStream_t stream) { return launch_k<128, 0>(p, bf16, stream); }
+hipError_t launch_chunk_f16_d128(const ChunkParams &p, bool bf16, int items, hipStream_t stream) {
+  return launch_k<128, 0>(p, bf16, items, stream);
+}
 
 }  // namespace bgtq

@@ -46,10 +46,13 @@ def test_bad_descriptors(bad):
 def test_limits_and_workspace():
     L, n = _lib.lib(), ctypes.c_size_t()
     size = lambda **kw: (L.bgtq_paged_prefill_workspace_size(ctypes.byref(_pages()), ctypes.byref(_desc(**kw)), ctypes.byref(n)), n.value)  # noqa: E731
-    # no history long enough to be split: the counters alone
-    assert size() == (_lib.OK, _lib.PAGED_PREFILL_COUNTER_BYTES)
-    small, large = size(max_length=1 << 20, page_table_stride=1 << 15, tokens=3), size(max_length=1 << 20, page_table_stride=1 << 15, tokens=5000)
-    assert small[0] == large[0] == _lib.OK and _lib.PAGED_PREFILL_COUNTER_BYTES < small[1] < large[1]
+    # at most ten query columns and no history long enough to be split: the counters alone
+    assert size(tokens=10) == (_lib.OK, _lib.PAGED_PREFILL_COUNTER_BYTES)
+    # partials, and the rebuilt rows of sequences that may have more than 32 columns: 1 GiB of those at most
+    long = dict(max_length=1 << 20, page_table_stride=1 << 15)
+    sizes = [size(**long, tokens=n) for n in (3, 40, 5000)] + [size(**long, tokens=5000, sequences=60000)]
+    assert all(s == _lib.OK for s, _ in sizes) and [n for _, n in sizes] == sorted({n for _, n in sizes})
+    assert sizes[-1][1] < (1 << 30) + (200 << 20)
     assert _status(tokens=(1 << 31) - 1) == _lib.ERR_UNSUPPORTED  # times the heads of a group
     assert L.bgtq_paged_prefill_workspace_size(ctypes.byref(_pages()), ctypes.byref(_desc()), None) == _lib.ERR_RANGE
     assert L.bgtq_paged_prefill(None, None, None) == L.bgtq_paged_prefill(None, ctypes.byref(_pages()), None) == _lib.ERR_RANGE
