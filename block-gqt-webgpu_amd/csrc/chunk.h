@@ -2,7 +2,7 @@
 // src/model/decoder.ts:46-56 with rows > 1, over pages): launch parameters.
 //
 // A sequence's chunk has rows x G query columns per KV head. Narrow ones (at
-// most 32) are attended straight from the pages (chunk_rows.h); the rows that wide
+// most 32, and all of a small call) are attended straight from the pages (chunk_rows.h); the rows that wide
 // ones see are rebuilt once, in the same launch, and attended in a second one
 // (chunk_wide.hip), which reads FP16 pages as they lie. Units (a sequence, a KV
 // head, a tile of columns) are cut along their tokens into items where there are
@@ -15,7 +15,6 @@
 namespace bgtq {
 
 constexpr int kChunkWaves = 8;                   // of a workgroup for narrow units
-constexpr int kChunkColumns = 32 * kChunkWaves;
 constexpr int kChunkKeys = 64;                   // tokens of a block
 // Wide units: waves of a workgroup, waves per SIMD by their registers, workgroups per compute unit.
 constexpr int chunk_wide_waves(int dim, bool split) { return dim == 128 && split ? 8 : 4; }
@@ -27,6 +26,8 @@ constexpr int chunk_wide_residents(int dim, bool split) {
 // unit, one of a narrow unit; the least cost of an item where a unit is split.
 constexpr int kChunkSetup = 16, kChunkWide = 8, kChunkNarrow = 3, kChunkLeast = 48;
 constexpr int kChunkMostSplits = 64;
+// Calls of at most this many columns attend all units as narrow ones, in tiles of 32, in their one launch.
+constexpr int kChunkSmall = 512;
 // Bytes of rebuilt rows at most: sequences that take more are attended in groups.
 constexpr int64_t kChunkRebuiltBytes = (int64_t)1 << 30;
 
@@ -60,7 +61,7 @@ struct ChunkParams {
   // Items: units' splits; `aim` of them are aimed at, a split unit's leave
   // partials in slots of slot_columns columns. narrow_items: the workgroups of
   // the first launch that attend.
-  int32_t aim, slot_columns, narrow_items, rotate_items;
+  int32_t aim, slot_columns, narrow_items, rotate_items, all_narrow;
   uint32_t *counters;
   float *part;
   // Rebuilt rows, [KV head][row][dim]: K (and its low parts), V; null: pages are read as they lie.

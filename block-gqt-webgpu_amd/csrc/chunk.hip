@@ -22,10 +22,11 @@ ChunkPlan plan_chunks(const ChunkParams &p, int dim, bool packed, bool q8, bool 
   // (units that cost no more than the least item are never split: find_item)
   const bool narrow_splits = kChunkSetup + kChunkNarrow * blocks > kChunkLeast, wide_splits = kChunkSetup + kChunkWide * blocks > kChunkLeast;
   c.narrow_aim = cus;
-  c.narrow_items = S * H + (narrow_splits ? c.narrow_aim : 0);
+  const bool all_narrow = columns <= kChunkSmall;
+  c.narrow_items = (S + (all_narrow ? columns / 32 : 0)) * H + (narrow_splits ? c.narrow_aim : 0);
   const int64_t narrow_bytes = narrow_splits ? 2 * (int64_t)c.narrow_aim * 32 * (dim + 2) * 4 : 0;
   c.part_bytes = narrow_bytes;
-  c.wide_sequences = std::min<int64_t>(S, columns / 33);
+  c.wide_sequences = all_narrow ? 0 : std::min<int64_t>(S, columns / 33);
   if (!c.wide_sequences) return c;
   c.wide_columns = 32 * chunk_wide_waves(dim, c.split);
   c.wide_aim = chunk_wide_residents(dim, c.split) * cus;
@@ -60,6 +61,7 @@ hipError_t launch_chunks(const ChunkParams &params, const ChunkPlan &plan, int d
     }
     p.aim = plan.narrow_aim;
     p.slot_columns = 32;
+    p.all_narrow = !plan.wide_sequences;
     const int items = (int)narrow + p.rotate_items + (rebuild ? (cus + p.kv_heads - 1) / p.kv_heads * p.kv_heads : 0);
     if (!p.packed) return dim == 64 ? launch_chunk_f16_d64(p, bf16, items, stream) : launch_chunk_f16_d128(p, bf16, items, stream);
     if (two) return dim == 64 ? launch_chunk_packed2_d64(p, bf16, items, stream) : launch_chunk_packed2_d128(p, bf16, items, stream);

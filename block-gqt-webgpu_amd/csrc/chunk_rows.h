@@ -33,7 +33,8 @@ template <int D, int KF>
 struct RowsLds {
   static constexpr int BOOKS = KF ? kBookBytes : 0;
   static constexpr int FLAG = BOOKS, ROWS = BOOKS + 256;  // (row pieces are XORed into addresses: whole 256 bytes)
-  static constexpr int OWN = 32 * D * 2;                  // a wave's rows
+  static constexpr int HALF = 32 * D * 2;                 // 32 rows
+  static constexpr int OWN = KF ? HALF : 2 * HALF;        // a wave's rows: K then V; FP16 K: K, V
   static constexpr int JOIN = 4 * 64 * (D / 2 + 2) * 4;   // four waves' states
   static constexpr int STAGE = most_of(32 * (D + 4) * 4, kChunkWaves * kStageBytes);  // rotated queries
   static constexpr int BYTES = ROWS + most_of(most_of(kChunkWaves * OWN, JOIN), STAGE);
@@ -120,8 +121,8 @@ struct Rows {
   // The codes of the 32 rows from row `at` of page `page` (the wave's) on. A pass's rows are added to the
   // wave's base, so that the lane's offsets are the same for all passes (held for each, they took up to 64 registers).
   __device__ __forceinline__ void load_k(int page, int at) {
-    const uint8_t *src = pk + (int64_t)page * k_page + (int64_t)at * rb;
-    const uint16_t *n = KF ? pn + (int64_t)page * n_page + (int64_t)at * ns : nullptr;
+    const uint8_t *src = scalar(pk + (int64_t)page * k_page + (int64_t)at * rb);
+    const uint16_t *n = KF ? scalar(pn + (int64_t)page * n_page + (int64_t)at * ns) : nullptr;
 #pragma unroll
     for (int k = 0; k < PASSES; ++k) {
       const uint8_t *row = src + STRIDE * k * rb;
@@ -141,8 +142,8 @@ struct Rows {
     }
   }
   __device__ __forceinline__ void load_v(int page, int at) {
-    const uint8_t *src = pv + (int64_t)page * v_page + (int64_t)at * (Q8 ? D : 2 * D);
-    const uint16_t *s = Q8 ? ps + (int64_t)page * s_page + at : nullptr;
+    const uint8_t *src = scalar(pv + (int64_t)page * v_page + (int64_t)at * (Q8 ? D : 2 * D));
+    const uint16_t *s = Q8 ? scalar(ps + (int64_t)page * s_page + at) : nullptr;
 #pragma unroll
     for (int k = 0; k < PASSES; ++k) {
       const uint8_t *row = src + STRIDE * k * (Q8 ? D : 2 * D);
@@ -231,9 +232,9 @@ __device__ __forceinline__ void narrow_item(const ChunkParams &p, uint8_t *smem)
   constexpr int B = 32, QS = D / 16, MT = D / 32, PASSES = R::PASSES;
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, qc = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  Item it = find_item(p, blockIdx.x, kNarrowUnits, kChunkColumns, p.aim);
+  const Item it = find_item(p, blockIdx.x, p.all_narrow ? kAllUnits : kNarrowUnits, 32, p.aim);
   if (it.splits == 0) return;  // uniform for the workgroup
-  const Columns cs(it, p.group, kChunkColumns);
+  const Columns cs(it, p.group, 32);
   R rows(p, it.kv, smem);
   uint8_t *const area = smem + L::ROWS;
   const uint32_t own = L::ROWS + (uint32_t)wave * L::OWN;
@@ -243,56 +244,84 @@ __device__ __forceinline__ void narrow_item(const ChunkParams &p, uint8_t *smem)
   const int first = r0 * kChunkWaves + wave, end = min(r1 * kChunkWaves, bl.count);
   const int in_page = (1 << p.page_shift) - 1;
   auto token = [&](int i) { return bl.at<B>(min(i, end - 1)); };
-  // FP16 K: the lane's part of the product's operand straight from its row.
-  u32x4 ka[KF == 0 ? QS : 1];
-  auto load_k = [&](int page, int t) {
-    if constexpr (KF == 0) {
-      const uint8_t *src = rows.pk + (int64_t)page * rows.k_page + (int64_t)(t & in_page) * (2 * D);
+  // FP16 rows go to LDS by DMA: K of the next block behind this one's product, V behind its own.
+  constexpr int DMAS = 32 * D * 2 / 1024, PR = D / 8;
+  constexpr bool DK = KF == 0, DV = DK && !Q8;
+  const uint32_t own_v = own + (DK ? L::HALF : 0);
+  auto dma = [&](const uint8_t *src, uint32_t to, int rest) {  // (rows from `rest` on arrive as zeros)
+    const __amdgpu_buffer_rsrc_t r = rsrc(scalar(src), (uint32_t)__builtin_amdgcn_readfirstlane(max(0, min(32, rest))) * 2 * D);
 #pragma unroll
-      for (int s = 0; s < QS; ++s) ka[s] = *reinterpret_cast<const u32x4 *>(src + (uint32_t)(qc * (2 * D) + 32 * s + 16 * h));
-    } else {
-      rows.load_k(page, t & in_page);
+    for (int k = 0; k < DMAS; ++k) {
+      const int piece = k * 64 + lane, row = piece / PR, c = (piece % PR) ^ swizzle<D>(row);
+      dma16(r, smem + to + k * 1024, (uint32_t)(row * (2 * D) + c * 16), 0);
     }
+  };
+  auto load_k = [&](int page, int t) {
+    const int at = t & in_page;
+    if constexpr (DK) dma(rows.pk + (int64_t)max(page, 0) * rows.k_page + (int64_t)at * (2 * D), own, page < 0 ? 0 : it.n - t);
+    else rows.load_k(max(page, 0), at);
+  };
+  auto load_v = [&](int page, int t) {
+    const int at = t & in_page;
+    if constexpr (DV) dma(rows.pv + (int64_t)max(page, 0) * rows.v_page + (int64_t)at * (2 * D), own_v, page < 0 ? 0 : it.n - t);
+    else rows.load_v(max(page, 0), at);
   };
   int page = -1, page1 = -1;
   if (first < end) {
     page = chunk_page(p, it.seq, token(first));
     page1 = chunk_page(p, it.seq, token(first + kChunkWaves));
-    load_k(max(page, 0), token(first));
-    rows.load_v(max(page, 0), token(first) & in_page);
+    if constexpr (!DK) {
+      load_k(page, token(first));
+      load_v(page, token(first));
+    }
   }
   R::books(p, it.kv, smem);
   W w;
-  if constexpr (KF != 0) w.begin(p, it, w.template load_rotated<true>(p, it, cs, 0, reinterpret_cast<float *>(area)), true);
-  else w.load_plain(p, it, cs, 0);
-  lds_barrier();  // the books, and the queries' staging done with
+  if constexpr (KF != 0) {
+    w.begin(p, it, w.template load_rotated<true>(p, it, cs, 0, reinterpret_cast<float *>(area)), true);
+    lds_barrier();  // the books, and the queries' staging done with
+  } else {
+    w.load_plain(p, it, cs, 0);
+    // (waited for here: the loop's counts are of its own loads)
+#pragma unroll
+    for (int s = 0; s < QS; ++s) asm volatile("" : "+v"(w.qh[s]));
+    if (first < end) {
+      load_k(page, token(first));
+      __builtin_amdgcn_sched_barrier(0);
+      load_v(page, token(first));
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
   for (int i = first; i < end; i += kChunkWaves) {
     const int t0 = bl.at<B>(i), t1 = token(i + kChunkWaves);
     const int page2 = chunk_page(p, it.seq, token(i + 2 * kChunkWaves));
-    auto put = [&](int k, u32x4 x) { *reinterpret_cast<u32x4 *>(smem + own + rows.place(k)) = x; };
+    auto put = [&](uint32_t to, int k, u32x4 x) { *reinterpret_cast<u32x4 *>(smem + to + rows.place(k)) = x; };
     f32x16 S[1];
 #pragma unroll
     for (int e = 0; e < 16; ++e) S[0][e] = 0.0f;
-    if constexpr (KF == 0) {
-#pragma unroll
-      for (int s = 0; s < QS; ++s) S[0] = product(ka[s], w.qh[s], S[0]);
-      load_k(max(page1, 0), t1);
+    if constexpr (DK) {
+      wait_vm<DV ? DMAS : 0>();  // K has landed; FP16 V may be on its way
+      w.qk(smem, own, S, true);
+      wait_lds();
+      __builtin_amdgcn_sched_barrier(0);
+      load_k(page1, t1);
+      __builtin_amdgcn_sched_barrier(0);
     } else {
       u32x4 lo[SPLIT ? PASSES : 1];
 #pragma unroll
       for (int k = 0; k < PASSES; ++k) {
         u32x4 hi;
         rows.make_k(k, hi, lo[SPLIT ? k : 0]);
-        put(k, hi);
+        put(own, k, hi);
         few_passes(k);
       }
-      load_k(max(page1, 0), t1);  // the next block's codes
+      load_k(page1, t1);  // the next block's codes
       wave_sync();
       w.qk(smem, own, S, true);
       if constexpr (SPLIT) {
         wave_sync();
 #pragma unroll
-        for (int k = 0; k < PASSES; ++k) put(k, lo[k]);
+        for (int k = 0; k < PASSES; ++k) put(own, k, lo[k]);
         wave_sync();
         w.qk(smem, own, S, false);
       }
@@ -302,21 +331,53 @@ __device__ __forceinline__ void narrow_item(const ChunkParams &p, uint8_t *smem)
     const uint64_t seen = masked ? w.seen_bits(t0, page < 0 ? 0ull : ~0ull) : ~0ull;
     uint32_t P[8];
     w.softmax(S, P, masked, seen);
-    wave_sync();
     float odd = 0.0f;
-    const int rest = page < 0 ? 0 : it.n - t0;
+    if constexpr (DV) {
+      wait_vm<DMAS>();  // V has landed; the next K may be on its way
+      if (masked) {
 #pragma unroll
-    for (int k = 0; k < PASSES; ++k) {
-      put(k, rows.make_v(k, rest, odd));
-      few_passes(k);
+        for (int k = 0; k < DMAS; ++k) {
+          const u32x4 v = *reinterpret_cast<const u32x4 *>(smem + own_v + (64 * k + lane) * 16);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) odd = odd2(v[e], odd);
+        }
+      }
+    } else {
+      const int rest = page < 0 ? 0 : it.n - t0;
+      wave_sync();
+#pragma unroll
+      for (int k = 0; k < PASSES; ++k) {
+        put(own_v, k, rows.make_v(k, rest, odd));
+        few_passes(k);
+      }
+      if constexpr (!DK) load_v(page1, t1);
+      wave_sync();
     }
-    rows.load_v(max(page1, 0), t1 & in_page);
-    wave_sync();
-    w.template pv<1>(smem, own, P, masked && __builtin_amdgcn_ballot_w64(odd != 0.0f) != 0, seen);
-    wave_sync();
+    if (masked && __builtin_amdgcn_ballot_w64(odd != 0.0f) != 0) {
+      w.template add_odd<1>(smem, own_v, seen);
+      // (the rows are this wave's own: their infinities and NaNs become zeros)
+      wave_sync();
+#pragma clang loop unroll(disable)
+      for (int k = 0; k < 32 * D * 2 / 1024; ++k) {
+        u32x4 &v = *reinterpret_cast<u32x4 *>(smem + own_v + (64 * k + lane) * 16);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = finite16(v[e]);
+      }
+      wave_sync();
+    }
+    w.template pv<1, false>(smem, own_v, P, false);
+    if constexpr (DK) {
+      wait_lds();
+      __builtin_amdgcn_sched_barrier(0);
+      load_v(page1, t1);
+      __builtin_amdgcn_sched_barrier(0);
+    } else {
+      wave_sync();
+    }
     page = page1;
     page1 = page2;
   }
+  if constexpr (DK) wait_vm<0>();  // (the last block's loads, once more, are still on their way to LDS)
   // The waves' states of the same columns, halved three times; wave 0 ends with the sum.
   float *const join = reinterpret_cast<float *>(area);
   constexpr int STATE = D / 2 + 2;  // floats of a lane
@@ -379,7 +440,7 @@ __device__ __forceinline__ void rebuild_rows(const ChunkParams &p, uint8_t *smem
   R::books(p, kv, smem);
   lds_barrier();
   for (int s0 = 0; s0 < p.sequences; s0 += 64) {
-    const SequencePlan q = plan_of(p, s0 + lane, kWideUnits, kChunkColumns);
+    const SequencePlan q = plan_of(p, s0 + lane, kWideUnits, 32);
     const int count = rebuilt_rows(q) / 32, end = wave_prefix(count), all = __builtin_amdgcn_readlane(end, 63);
     for (; at < base + all; at += stride) {
       const int local = (int)(at - base);

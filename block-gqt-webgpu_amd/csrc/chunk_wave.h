@@ -70,6 +70,14 @@ __device__ __forceinline__ uint32_t of_kind16(uint32_t w, int kind) {
   return (is(w & 0xffffu) ? kOne16 : 0u) | (is(w >> 16) ? kOne16 << 16 : 0u);
 }
 
+// A pointer of the wave's in scalar registers (left to the compiler, a DMA's descriptor became a loop over lanes).
+template <typename T>
+__device__ __forceinline__ const T *scalar(const T *ptr) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(ptr);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)a), hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(a >> 32));
+  return reinterpret_cast<const T *>((uintptr_t)lo | (uintptr_t)hi << 32);
+}
+
 // The tokens that a tile's rows, at positions first .. last, see something of, in
 // blocks of B: all up to the last; behind a window the sinks' blocks, then
 // those from the first position's window on. at(i): the i-th block's first token.
@@ -97,8 +105,8 @@ struct Item {
   int64_t base;                // the sequence's first row among the rebuilt ones
 };
 
-// What a launch does: every unit; the narrow ones (and the rebuilding of the
-// wide ones' K and V); the wide ones.
+// The units of a launch: all of them, as narrow ones; the narrow ones (beside the rebuilding
+// of the wide ones' K and V); the wide ones.
 enum { kAllUnits, kNarrowUnits, kWideUnits };
 
 // A sequence's units and what each costs; a lane per sequence.
@@ -127,7 +135,7 @@ __device__ __forceinline__ SequencePlan plan_of(const ChunkParams &p, int s, int
     blocks = (int)min((int64_t)blocks, seen / kChunkKeys + 3);
   }
   return {begin, rows, n, tiles * p.kv_heads, wide,
-          (float)(kChunkSetup + (wide ? kChunkWide : kChunkNarrow) * (int64_t)blocks)};
+          (float)(kChunkSetup + (wide && which != kAllUnits ? kChunkWide : kChunkNarrow) * (int64_t)blocks)};
 }
 __device__ __forceinline__ int splits_of(const SequencePlan &q, float share) {
   // (the thousandth: a quotient that is whole stays so through the reciprocal)
@@ -203,12 +211,10 @@ __device__ __forceinline__ Item find_item(const ChunkParams &p, int item, int wh
 // An item's columns: the tile's rows x heads, row-major.
 struct Columns {
   int col0, count, before, first, last;  // before: the first row's position (negative: such rows see nothing); the tile's first and last
-  bool narrow;                           // of a unit that all waves share
   __device__ __forceinline__ Columns(const Item &it, int G, int tile) {
     const int64_t columns = (int64_t)it.rows * G;
     col0 = it.tile * tile;  // (rows x G below 2^31: checked on the host)
     count = (int)min(columns - col0, (int64_t)tile);
-    narrow = columns <= 32;
     before = it.n - it.rows;
     first = before + col0 / G;
     last = before + (col0 + count - 1) / G;
@@ -478,69 +484,65 @@ struct Wave {
       l = add2(P[e], l);
     }
   }
-  // O^T += V^T P^T of the V rows at LDS offset `at`. odd: some queries see a part of the rows only, and
-  // some hold infinities or NaNs: the products take the finite values, and what is
-  // seen of the others is added by itself.
-  template <int NB>
-  __device__ __forceinline__ void pv(uint8_t *smem, uint32_t at, const uint32_t (&P)[8 * NB], bool odd, uint64_t seen) {
+  // O^T += V^T P^T of the V rows at LDS offset `at`; odd: of their finite values.
+  template <int NB, bool MAYBE_ODD>
+  __device__ __forceinline__ void pv(uint8_t *smem, uint32_t at, const uint32_t (&P)[8 * NB], bool odd) {
     constexpr int STEP = 16 * 2 * D;  // bytes of a step's rows
     const int lane = threadIdx.x & 63;
-    if (!odd) {
-      const int h = lane >> 5, vr = 4 * h + ((lane & 15) >> 2), piece = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-      const uint32_t lds0 = lds_at(smem) + at;
-      const uint32_t v_at = (uint32_t)(vr * (2 * D) + ((piece ^ swizzle<D>(vr)) * 16) + (lane & 1) * 8);
-      const uint32_t v_at8 = (uint32_t)((vr + 8) * (2 * D) + ((piece ^ swizzle<D>(vr + 8)) * 16) + (lane & 1) * 8);
-      uint32_t va[MT], va8[MT];
+    const int h = lane >> 5, vr = 4 * h + ((lane & 15) >> 2), piece = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+    const uint32_t lds0 = lds_at(smem) + at;
+    const uint32_t v_at = (uint32_t)(vr * (2 * D) + ((piece ^ swizzle<D>(vr)) * 16) + (lane & 1) * 8);
+    const uint32_t v_at8 = (uint32_t)((vr + 8) * (2 * D) + ((piece ^ swizzle<D>(vr + 8)) * 16) + (lane & 1) * 8);
+    uint32_t va[MT], va8[MT];
 #pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        va[t] = (lds0 + v_at) ^ (64u * t);
-        va8[t] = (lds0 + v_at8) ^ (64u * t);
-      }
-      u32x2 v[2][MT][2];
-      ds_read_tr16<MT, 0>(va, va8, v[0]);
-#pragma unroll
-      for (int s = 0; s < 2 * NB; ++s) {
-        const u32x4 pf{P[4 * s], P[4 * s + 1], P[4 * s + 2], P[4 * s + 3]};
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {
-          const u32x2 a = v[s & 1][t][0], b = v[s & 1][t][1];
-          O[t] = product(u32x4{a[0], a[1], b[0], b[1]}, pf, O[t]);
-        }
-        if (s == 0) ds_read_tr16<MT, STEP>(va, va8, v[1]);
-        if constexpr (NB == 2) {
-          if (s == 1) ds_read_tr16<MT, 2 * STEP>(va, va8, v[0]);
-          if (s == 2) ds_read_tr16<MT, 3 * STEP>(va, va8, v[1]);
-        }
-      }
-      return;
+    for (int t = 0; t < MT; ++t) {
+      va[t] = (lds0 + v_at) ^ (64u * t);
+      va8[t] = (lds0 + v_at8) ^ (64u * t);
     }
-    int rare = lane;
-    asm volatile("" : "+v"(rare));  // (the rare branch's addresses are not held across the loop)
-    const int h = rare >> 5, qc = rare & 31;
-    // V of dimension 32 t + qc, tokens 16 s + 8 (e / 2) + 4 h + 2 (e % 2) + 0, 1 in word e.
-    auto column = [&](int s, int t) {
-      u32x4 a;
+    u32x2 v[2][MT][2];
+    ds_read_tr16<MT, 0>(va, va8, v[0]);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        a[e] = 0;
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const int r = 16 * s + 8 * (e >> 1) + 4 * h + 2 * (e & 1) + x;
-          const uint8_t *from = smem + at + r * (2 * D) + (((4 * t + (qc >> 3)) ^ swizzle<D>(r)) * 16) + 2 * (qc & 7);
-          a[e] |= (uint32_t)*reinterpret_cast<const uint16_t *>(from) << (16 * x);
-        }
-      }
-      return a;
-    };
-#pragma unroll
-    for (int s = 0; s < 2 * NB; ++s)
+    for (int s = 0; s < 2 * NB; ++s) {
+      const u32x4 pf{P[4 * s], P[4 * s + 1], P[4 * s + 2], P[4 * s + 3]};
 #pragma unroll
       for (int t = 0; t < MT; ++t) {
-        u32x4 a = column(s, t);
+        u32x4 a{v[s & 1][t][0][0], v[s & 1][t][0][1], v[s & 1][t][1][0], v[s & 1][t][1][1]};
+        if (MAYBE_ODD && odd) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) a[e] = finite16(a[e]);
-        O[t] = product(a, u32x4{P[4 * s], P[4 * s + 1], P[4 * s + 2], P[4 * s + 3]}, O[t]);
+          for (int e = 0; e < 4; ++e) a[e] = finite16(a[e]);
+        }
+        O[t] = product(a, pf, O[t]);
       }
+      if (s == 0) ds_read_tr16<MT, STEP>(va, va8, v[1]);
+      if constexpr (NB == 2) {
+        if (s == 1) ds_read_tr16<MT, 2 * STEP>(va, va8, v[0]);
+        if (s == 2) ds_read_tr16<MT, 3 * STEP>(va, va8, v[1]);
+      }
+    }
+  }
+  // V of dimension 32 t + (rare & 31), tokens 16 s + 8 (e / 2) + 4 (rare / 32) + 2 (e % 2) + 0, 1 in word e.
+  __device__ __forceinline__ static u32x4 v_column(const uint8_t *smem, uint32_t at, int rare, int s, int t) {
+    const int h = rare >> 5, qc = rare & 31;
+    u32x4 a;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      a[e] = 0;
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int r = 16 * s + 8 * (e >> 1) + 4 * h + 2 * (e & 1) + x;
+        const uint8_t *from = smem + at + r * (2 * D) + (((4 * t + (qc >> 3)) ^ swizzle<D>(r)) * 16) + 2 * (qc & 7);
+        a[e] |= (uint32_t)*reinterpret_cast<const uint16_t *>(from) << (16 * x);
+      }
+    }
+    return a;
+  }
+  // Some queries see a part of the rows only, and some rows hold infinities
+  // or NaNs: what is seen of those is added to O by itself, and the products
+  // take the finite values.
+  template <int NB>
+  __device__ __forceinline__ void add_odd(const uint8_t *smem, uint32_t at, uint64_t seen) {
+    int rare = threadIdx.x & 63;
+    asm volatile("" : "+v"(rare));  // (this branch's addresses are not held across the loop)
 #pragma clang loop unroll(disable)
     for (int kind = 0; kind < 3; ++kind) {
       const float value = kind == 0 ? __builtin_nanf("") : kind == 1 ? INFINITY : -INFINITY;
@@ -551,7 +553,7 @@ struct Wave {
         for (int i = 0; i < 16; ++i) n[i] = 0.0f;
 #pragma clang loop unroll(disable)
         for (int s = 0; s < 2 * NB; ++s) {
-          u32x4 a = column(s, t), sees;
+          u32x4 a = v_column(smem, at, rare, s, t), sees;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int k = 16 * s + 8 * (e >> 1) + 2 * (e & 1);
@@ -565,6 +567,7 @@ struct Wave {
           O[t][i] = n[i] > 0.0f ? O[t][i] + value : O[t][i];
           in_place(O[t]);
         }
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
   }

@@ -59,22 +59,22 @@ __global__ __launch_bounds__((64 * Wide<D, SRC, BF>::W), (Wide<D, SRC, BF>::PER_
         const bool ok = (uint32_t)pg < (uint32_t)p.pages;
         const int in = ok ? min(32, max(0, it.n - th)) : 0;
         const int64_t at = ok ? pg : 0;
-        const __amdgpu_buffer_rsrc_t rk = rsrc(p.k + kv * p.k_head + at * p.k_page + (int64_t)(th & in_page) * D, (uint32_t)in * 2 * D);
-        const __amdgpu_buffer_rsrc_t rv = rsrc(p.v + kv * p.v_head + at * p.v_page + (int64_t)(th & in_page) * D * 2, (uint32_t)in * 2 * D);
+        const __amdgpu_buffer_rsrc_t rk = rsrc(scalar(p.k + kv * p.k_head + at * p.k_page + (int64_t)(th & in_page) * D), (uint32_t)__builtin_amdgcn_readfirstlane(in) * 2 * D);
+        const __amdgpu_buffer_rsrc_t rv = rsrc(scalar(p.v + kv * p.v_head + at * p.v_page + (int64_t)(th & in_page) * D * 2), (uint32_t)__builtin_amdgcn_readfirstlane(in) * 2 * D);
         const uint32_t o = (uint32_t)((r & 31) * (2 * D) + c * 16);
         dma16(rk, buf + d * 1024, o, 0);
         dma16(rv, buf + TILE + d * 1024, o, 0);
       }
     } else {
       const int64_t at = (kv * p.rebuilt_head + it.base + t0) * D;
-      const __amdgpu_buffer_rsrc_t rk = rsrc(p.rebuilt_k + at, TILE), rv = rsrc(p.rebuilt_v + at, TILE);
+      const __amdgpu_buffer_rsrc_t rk = rsrc(scalar(p.rebuilt_k + at), TILE), rv = rsrc(scalar(p.rebuilt_v + at), TILE);
 #pragma unroll
       for (int k = 0; k < DMAS; ++k) {
         const int d = wave * DMAS + k, piece = d * 64 + lane, r = piece / PR, c = (piece % PR) ^ swizzle<D>(r);
         const uint32_t o = (uint32_t)(r * (2 * D) + c * 16);
         dma16(rk, buf + d * 1024, o, 0);
         dma16(rv, buf + TILE + d * 1024, o, 0);
-        if constexpr (SPLIT) dma16(rsrc(p.rebuilt_lo + at, TILE), buf + 2 * TILE + d * 1024, o, 0);
+        if constexpr (SPLIT) dma16(rsrc(scalar(p.rebuilt_lo + at), TILE), buf + 2 * TILE + d * 1024, o, 0);
       }
     }
   };
@@ -93,7 +93,8 @@ __global__ __launch_bounds__((64 * Wide<D, SRC, BF>::W), (Wide<D, SRC, BF>::PER_
   const bool any = 32 * wave < cs.count;
   const int lo = cs.before + (cs.col0 + min(32 * wave, cs.count - 1)) / p.group,
             hi = cs.before + (cs.col0 + min(32 * wave + 31, cs.count - 1)) / p.group;
-  for (int i = b0; i < b1; ++i) {
+  // The next block: it has landed, and the one after it is on its way.
+  auto arrive = [&](int i) -> uint64_t {
     wait_vm<0>();   // this wave's part of block i has landed
     lds_barrier();  // everyone's has, and everyone is done with the other buffer
     const uint64_t there = in_pool(e0);
@@ -103,9 +104,10 @@ __global__ __launch_bounds__((64 * Wide<D, SRC, BF>::W), (Wide<D, SRC, BF>::PER_
       __builtin_amdgcn_sched_barrier(0);  // (ahead of the DMAs: its wait leaves them in flight)
       issue(i + 1, e0);
     }
-    const int t0 = bl.at<kChunkKeys>(i);
-    const int part = any ? w.sight(t0, kChunkKeys, lo, hi) : 0;
-    if (part == 0) continue;
+    return there;
+  };
+  auto attend = [&](auto masked_tag, int i, uint64_t there) {
+    constexpr bool MASKED = decltype(masked_tag)::value;
     const uint32_t buf = (uint32_t)(i & 1) * X::BUFFER;
     f32x16 S[2];
 #pragma unroll
@@ -114,11 +116,10 @@ __global__ __launch_bounds__((64 * Wide<D, SRC, BF>::W), (Wide<D, SRC, BF>::PER_
       for (int e = 0; e < 16; ++e) S[b][e] = 0.0f;
     w.qk(smem, buf, S, true);
     if constexpr (SPLIT) w.qk(smem, buf + 2 * TILE, S, false);
-    const bool masked = part == 1 || there != ~0ull;  // (entries behind the sequence's may be none: masked in any case)
     uint64_t seen = ~0ull;
     bool odd = false;
-    if (masked) {
-      seen = w.seen_bits(t0, there);
+    if constexpr (MASKED) {
+      seen = w.seen_bits(bl.at<kChunkKeys>(i), there);
       // A token that a query does not see has probability 0, but 0 times an infinity or a NaN of its V row is not 0.
       float z = 0.0f;
 #pragma unroll
@@ -130,8 +131,21 @@ __global__ __launch_bounds__((64 * Wide<D, SRC, BF>::W), (Wide<D, SRC, BF>::PER_
       odd = __builtin_amdgcn_ballot_w64(z != 0.0f) != 0;
     }
     uint32_t P[16];
-    w.softmax(S, P, masked, seen);
-    w.template pv<2>(smem, buf + TILE, P, odd, seen);
+    w.softmax(S, P, MASKED, seen);
+    if (MASKED && odd) w.template add_odd<2>(smem, buf + TILE, seen);
+    w.template pv<2, MASKED>(smem, buf + TILE, P, odd);
+  };
+  // Runs of blocks that all queries see whole in a loop of their own, which
+  // carries none of the masks' code. (Entries behind the sequence's may name no page: such blocks are seen in part anyway.)
+  for (int i = b0; i < b1; ++i) {
+    uint64_t there;
+    for (;;) {
+      there = arrive(i);
+      if (there != ~0ull || !any || w.sight(bl.at<kChunkKeys>(i), kChunkKeys, lo, hi) != 2) break;
+      attend(std::false_type{}, i, there);
+      if (++i == b1) break;
+    }
+    if (i < b1 && any && w.sight(bl.at<kChunkKeys>(i), kChunkKeys, lo, hi) != 0) attend(std::true_type{}, i, there);
   }
   w.template store<false>(p, it, cs, 32 * wave, cs.count);
 }

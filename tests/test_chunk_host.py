@@ -46,13 +46,16 @@ def test_bad_descriptors(bad):
 def test_limits_and_workspace():
     L, n = _lib.lib(), ctypes.c_size_t()
     size = lambda **kw: (L.bgtq_paged_prefill_workspace_size(ctypes.byref(_pages()), ctypes.byref(_desc(**kw)), ctypes.byref(n)), n.value)  # noqa: E731
-    # at most ten query columns and no history long enough to be split: the counters alone
+    # no history long enough to be split and few query columns: the counters alone
     assert size(tokens=10) == (_lib.OK, _lib.PAGED_PREFILL_COUNTER_BYTES)
-    # partials, and the rebuilt rows of sequences that may have more than 32 columns: 1 GiB of those at most
+    # partials, and in larger calls the rebuilt rows of sequences that may have more than 32 columns: 1 GiB of those at most
     long = dict(max_length=1 << 20, page_table_stride=1 << 15)
-    sizes = [size(**long, tokens=n) for n in (3, 40, 5000)] + [size(**long, tokens=5000, sequences=60000)]
-    assert all(s == _lib.OK for s, _ in sizes) and [n for _, n in sizes] == sorted({n for _, n in sizes})
-    assert sizes[-1][1] < (1 << 30) + (200 << 20)
+    few, few_more = size(**long, tokens=3), size(**long, tokens=40)
+    assert few == few_more and few[1] > _lib.PAGED_PREFILL_COUNTER_BYTES
+    more = size(**long, tokens=700)
+    assert more[0] == _lib.OK and more[1] > few[1] + (1 << 28)
+    most = size(**long, tokens=5000, sequences=60000)
+    assert most[0] == _lib.OK and more[1] <= most[1] < (1 << 30) + (200 << 20)
     assert _status(tokens=(1 << 31) - 1) == _lib.ERR_UNSUPPORTED  # times the heads of a group
     assert L.bgtq_paged_prefill_workspace_size(ctypes.byref(_pages()), ctypes.byref(_desc()), None) == _lib.ERR_RANGE
     assert L.bgtq_paged_prefill(None, None, None) == L.bgtq_paged_prefill(None, ctypes.byref(_pages()), None) == _lib.ERR_RANGE
