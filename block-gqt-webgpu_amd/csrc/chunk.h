@@ -17,14 +17,18 @@ namespace bgtq {
 constexpr int kChunkWaves = 8;                   // of a workgroup for narrow units
 constexpr int kChunkKeys = 64;                   // tokens of a block
 // Wide units: waves of a workgroup, waves per SIMD by their registers, workgroups per compute unit.
-constexpr int chunk_wide_waves(int dim, bool split) { return dim == 128 && split ? 8 : 4; }
+// (Eight waves instead of four share a block's DMAs and barrier, in coarser units: d=64 by single
+// products 326 -> 316 us of 2048 rows behind 32768 tokens, d=128 65 -> 67 us of 2 x 1000 behind a window.)
+constexpr int chunk_wide_waves(int dim, bool split) { return (dim == 128) == split ? 8 : 4; }
 constexpr int chunk_wide_waves_per_simd(int dim, bool split) { return dim == 64 ? split ? 3 : 4 : 2; }
 constexpr int chunk_wide_residents(int dim, bool split) {
   return 4 * chunk_wide_waves_per_simd(dim, split) / chunk_wide_waves(dim, split);
 }
 // Costs of a unit, in eighths of a wide block: its set-up, a block of a wide
-// unit, one of a narrow unit; the least cost of an item where a unit is split.
-constexpr int kChunkSetup = 16, kChunkWide = 8, kChunkNarrow = 3, kChunkLeast = 48;
+// unit, one of a narrow unit; the least cost of a wide and of a narrow item where a unit is split.
+constexpr int kChunkSetup = 16, kChunkWide = 8, kChunkNarrow = 3, kChunkLeast = 48, kChunkLeastNarrow = 32;
+// A second round of wide items costs this much more; none is made of calls whose items may cost kChunkLong at most.
+constexpr int kChunkRound = 64, kChunkLong = 384;
 constexpr int kChunkMostSplits = 64;
 // Calls of at most this many columns attend all units as narrow ones, in tiles of 32, in their one launch.
 constexpr int kChunkSmall = 512;
@@ -61,7 +65,7 @@ struct ChunkParams {
   // Items: units' splits; `aim` of them are aimed at, a split unit's leave
   // partials in slots of slot_columns columns. narrow_items: the workgroups of
   // the first launch that attend.
-  int32_t aim, slot_columns, narrow_items, rotate_items, all_narrow;
+  int32_t aim, slot_columns, narrow_items, rotate_items, all_narrow, two_rounds;
   uint32_t *counters;
   float *part;
   // Rebuilt rows, [KV head][row][dim]: K (and its low parts), V; null: pages are read as they lie.
@@ -78,7 +82,7 @@ struct ChunkPlan {
   bool split;               // K and q as pairs of FP16 values
   int64_t wide_sequences;   // that may be wide at most
   int64_t narrow_items;     // first launch: attending workgroups
-  int32_t narrow_aim, wide_aim, wide_columns;
+  int32_t narrow_aim, wide_aim, wide_columns, two_rounds;
   int64_t group, wide_items;  // sequences of a group; items of its launch at most
   int64_t slots;              // of its split units at most
   int64_t part_bytes, rebuilt_rows, rebuilt_bytes, turned_bytes;  // rows of a KV head; of all operands

@@ -20,7 +20,7 @@ ChunkPlan plan_chunks(const ChunkParams &p, int dim, bool packed, bool q8, bool 
   const int64_t columns = p.tokens * p.group, S = p.sequences, H = p.kv_heads;
   const int64_t blocks = (p.max_length + kChunkKeys - 1) / kChunkKeys;
   // (units that cost no more than the least item are never split: find_item)
-  const bool narrow_splits = kChunkSetup + kChunkNarrow * blocks > kChunkLeast, wide_splits = kChunkSetup + kChunkWide * blocks > kChunkLeast;
+  const bool narrow_splits = kChunkSetup + kChunkNarrow * blocks > kChunkLeastNarrow, wide_splits = kChunkSetup + kChunkWide * blocks > kChunkLeast;
   c.narrow_aim = cus;
   const bool all_narrow = columns <= kChunkSmall;
   c.narrow_items = (S + (all_narrow ? columns / 32 : 0)) * H + (narrow_splits ? c.narrow_aim : 0);
@@ -40,7 +40,9 @@ ChunkPlan plan_chunks(const ChunkParams &p, int dim, bool packed, bool q8, bool 
     c.rebuilt_bytes = most * bytes;
     if (packed) c.turned_bytes = columns * H * (dim * (c.split ? 4 : 2) + 4);
   }
-  c.wide_items = (columns / c.wide_columns + std::min(c.group, c.wide_sequences)) * H + (wide_splits ? c.wide_aim : 0);
+  const int64_t units = (columns / c.wide_columns + std::min(c.group, c.wide_sequences)) * H;
+  c.two_rounds = wide_splits && c.group <= 64 && units * (kChunkSetup + kChunkWide * blocks) > (int64_t)kChunkLong * c.wide_aim;
+  c.wide_items = units + (wide_splits ? (c.two_rounds + 1) * c.wide_aim : 0);
   const int64_t slot_columns = std::min<int64_t>(c.wide_columns, (columns + 31) / 32 * 32);
   c.slots = wide_splits ? 2 * c.wide_aim : 0;
   c.part_bytes = std::max(narrow_bytes, c.slots * slot_columns * (dim + 2) * 4);
@@ -69,6 +71,7 @@ hipError_t launch_chunks(const ChunkParams &params, const ChunkPlan &plan, int d
   };
   auto wide = [&]() -> hipError_t {
     p.aim = plan.wide_aim;
+    p.two_rounds = plan.two_rounds;
     p.slot_columns = (int32_t)std::min<int64_t>(plan.wide_columns, (p.tokens * p.group + 31) / 32 * 32);
     if (hipError_t e = launch_chunk_wide(p, dim, bf16, (int)plan.wide_items, stream)) return e;
     return plan.slots ? launch_chunk_merge(p, dim, bf16, plan.wide_columns, (int)plan.slots, stream) : hipSuccess;

@@ -35,7 +35,8 @@ struct RowsLds {
   static constexpr int FLAG = BOOKS, ROWS = BOOKS + 256;  // (row pieces are XORed into addresses: whole 256 bytes)
   static constexpr int HALF = 32 * D * 2;                 // 32 rows
   static constexpr int OWN = KF ? HALF : 2 * HALF;        // a wave's rows: K then V; FP16 K: K, V
-  static constexpr int JOIN = 4 * 64 * (D / 2 + 2) * 4;   // four waves' states
+  static constexpr int STATE = D / 8 * 64 * 16;           // a wave's O; (m, l) of its columns lie behind all of them
+  static constexpr int JOIN = kChunkWaves * (STATE + 32 * 8);
   static constexpr int STAGE = most_of(32 * (D + 4) * 4, kChunkWaves * kStageBytes);  // rotated queries
   static constexpr int BYTES = ROWS + most_of(most_of(kChunkWaves * OWN, JOIN), STAGE);
 };
@@ -230,7 +231,7 @@ __device__ __forceinline__ void narrow_item(const ChunkParams &p, uint8_t *smem)
   using W = Wave<D, SPLIT, BF>;
   using R = Rows<D, KF, Q8, SPLIT>;
   constexpr int B = 32, QS = D / 16, MT = D / 32, PASSES = R::PASSES;
-  const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, qc = lane & 31;
+  const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const Item it = find_item(p, blockIdx.x, p.all_narrow ? kAllUnits : kNarrowUnits, 32, p.aim);
   if (it.splits == 0) return;  // uniform for the workgroup
@@ -281,16 +282,16 @@ __device__ __forceinline__ void narrow_item(const ChunkParams &p, uint8_t *smem)
     w.begin(p, it, w.template load_rotated<true>(p, it, cs, 0, reinterpret_cast<float *>(area)), true);
     lds_barrier();  // the books, and the queries' staging done with
   } else {
-    w.load_plain(p, it, cs, 0);
-    // (waited for here: the loop's counts are of its own loads)
-#pragma unroll
-    for (int s = 0; s < QS; ++s) asm volatile("" : "+v"(w.qh[s]));
     if (first < end) {
       load_k(page, token(first));
       __builtin_amdgcn_sched_barrier(0);
       load_v(page, token(first));
       __builtin_amdgcn_sched_barrier(0);
     }
+    w.load_plain(p, it, cs, 0);
+    // (waited for here: the loop's counts are of its own loads)
+#pragma unroll
+    for (int s = 0; s < QS; ++s) asm volatile("" : "+v"(w.qh[s]));
   }
   for (int i = first; i < end; i += kChunkWaves) {
     const int t0 = bl.at<B>(i), t1 = token(i + kChunkWaves);
@@ -378,39 +379,41 @@ __device__ __forceinline__ void narrow_item(const ChunkParams &p, uint8_t *smem)
     page1 = page2;
   }
   if constexpr (DK) wait_vm<0>();  // (the last block's loads, once more, are still on their way to LDS)
-  // The waves' states of the same columns, halved three times; wave 0 ends with the sum.
-  float *const join = reinterpret_cast<float *>(area);
-  constexpr int STATE = D / 2 + 2;  // floats of a lane
+  // The waves' states of the same columns, summed by all threads: four dimensions of a column each.
+  constexpr int STATE = L::STATE;
+  w.l = half_sum(w.l);
+  __syncthreads();
+  if ((lane & 31) < cs.count) {
+    u32x4 *const to = reinterpret_cast<u32x4 *>(area + wave * STATE) + lane;
 #pragma unroll
-  for (int half = kChunkWaves / 2; half >= 1; half >>= 1) {
-    __syncthreads();
-    if (wave >= half && wave < 2 * half) {
-      float *to = join + (wave - half) * 64 * STATE + lane;
-      to[0] = w.m;
-      to[64] = w.l;
+    for (int t = 0; t < MT; ++t)
 #pragma unroll
-      for (int t = 0; t < MT; ++t)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) to[64 * (2 + 16 * t + i)] = w.O[t][i];
-    }
-    __syncthreads();
-    if (wave < half) {
-      const float *from = join + wave * 64 * STATE + lane;
-      const float m2 = from[0], l2 = from[64], mn = fmaxf(w.m, m2);
-      // (a state that saw nothing is all zeros)
-      const float a = w.m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(w.m - mn), b = m2 == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m2 - mn);
-      w.m = mn;
-      w.l = w.l * a + l2 * b;
-#pragma unroll
-      for (int t = 0; t < MT; ++t)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          w.O[t][i] = w.O[t][i] * a + from[64 * (2 + 16 * t + i)] * b;
-          if (i == 15) __builtin_amdgcn_sched_barrier(0);  // (a tile's reads at a time)
-        }
-    }
+      for (int g = 0; g < 4; ++g)
+        to[(4 * t + g) * 64] = __builtin_bit_cast(u32x4, (f32x4{w.O[t][4 * g], w.O[t][4 * g + 1], w.O[t][4 * g + 2], w.O[t][4 * g + 3]}));
+    if (lane < 32) *reinterpret_cast<u32x2 *>(area + kChunkWaves * STATE + (wave * 32 + lane) * 8) = u32x2{__float_as_uint(w.m), __float_as_uint(w.l)};
   }
-  w.template store<true>(p, it, cs, 0, wave == 0 ? cs.count : 0);
+  __syncthreads();
+  for (int e = tid; e < cs.count * (D / 4); e += kThreads) {
+    const int piece = e / cs.count, c = e - piece * cs.count;
+    float m[kChunkWaves], l[kChunkWaves], M = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kChunkWaves; ++k) {
+      const u32x2 ml = *reinterpret_cast<const u32x2 *>(area + kChunkWaves * STATE + (k * 32 + c) * 8);
+      m[k] = __uint_as_float(ml[0]), l[k] = __uint_as_float(ml[1]);
+      M = fmaxf(M, m[k]);
+    }
+    f32x4 o{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int k = 0; k < kChunkWaves; ++k) {
+      // (a state that saw nothing is all zeros)
+      const float a = m[k] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[k] - M);
+      const f32x4 x = *(reinterpret_cast<const f32x4 *>(area + k * STATE) + (piece >> 1) * 64 + 32 * (piece & 1) + c);
+      sum = __builtin_fmaf(l[k], a, sum);
+#pragma unroll
+      for (int d = 0; d < 4; ++d) o[d] = __builtin_fmaf(x[d], a, o[d]);
+    }
+    store_piece<D, BF>(p, it, cs, piece, c, o, M, sum);
+  }
   if (it.splits == 1) return;
   // The last item of the unit to arrive merges.
   int *const flag = reinterpret_cast<int *>(smem + L::FLAG);

@@ -142,9 +142,15 @@ __device__ __forceinline__ int splits_of(const SequencePlan &q, float share) {
   return q.units ? max(1, min((int)ceilf(q.cost * __builtin_amdgcn_rcpf(share) - 1e-3f), kChunkMostSplits)) : 0;
 }
 __device__ __forceinline__ float wave_sum_f(float v) {
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m, 64);
-  return v;
+  auto turned = [](float x, auto by) { return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), decltype(by)::value, 0xf, 0xf, false)); };
+  v += turned(v, std::integral_constant<int, 0x128>{});
+  v += turned(v, std::integral_constant<int, 0x124>{});
+  v += turned(v, std::integral_constant<int, 0x122>{});
+  v += turned(v, std::integral_constant<int, 0x121>{});
+  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  // (the lanes' orders differ: one's sum for all)
+  return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(half_sum(v))));
 }
 // Rows that a wide sequence's tokens take among the rebuilt ones: whole blocks.
 __device__ __forceinline__ int rebuilt_rows(const SequencePlan &q) { return q.wide ? (q.n + kChunkKeys - 1) / kChunkKeys * kChunkKeys : 0; }
@@ -154,25 +160,37 @@ __device__ __forceinline__ int rebuilt_rows(const SequencePlan &q) { return q.wi
 // longest tile's blocks; an item's share t of cost is the sum's by `aim`, at
 // least kChunkLeast, and a sequence's units are split into ceil(cost / t). Of up to
 // 64 sequences t is raised until the items are at most `aim`, or as few as
-// there are units. Items of split units number at most 2 sum / t <= 2 aim: their
-// partials' slots. BY_SLOT: the item that has slot `item`.
+// there are units. Where units hardly outnumber the workgroups the GPU holds, whole
+// splits leave some of those idle (224 units on 1024: 4 each, 896): wide units
+// then take two rounds of items, of a share t2, where 2 t2 is less. Items of split units
+// number at most 2 sum / t <= 2 aim: their partials' slots. BY_SLOT: the item
+// that has slot `item`.
 template <bool BY_SLOT = false>
 __device__ __forceinline__ Item find_item(const ChunkParams &p, int item, int which, int tile, int aim) {
   const int lane = threadIdx.x & 63;
-  const float target = (float)aim;
   float all = 0.0f;
   SequencePlan q{};
   for (int s0 = 0; s0 < p.sequences; s0 += 64) {
     q = plan_of(p, s0 + lane, which, tile);
     all += wave_sum_f((float)q.units * q.cost);
   }
-  float share = fmaxf((float)kChunkLeast, ceilf(all / target));
+  const float least = which == kWideUnits ? kChunkLeast : kChunkLeastNarrow;
+  float share = fmaxf(least, ceilf(all / (float)aim));
   if (p.sequences <= 64) {
     const float units = (float)wave_sum(q.units);
-    for (int k = 0; k < 3; ++k) {
-      const float items = (float)wave_sum(splits_of(q, share) * q.units);
-      if (items <= fmaxf(target, units)) break;
-      share = fmaxf(share + 1.0f, ceilf(share * items / target));
+    // The share from t on that makes at most `target` items, or one of each unit (negative: more).
+    auto fit = [&](float t, float target) {
+      for (int k = 0;; ++k) {
+        const float items = (float)wave_sum(splits_of(q, t) * q.units);
+        if (items <= fmaxf(target, units)) return t;
+        if (k == 3) return -t;
+        t = fmaxf(t + 1.0f, ceilf(t * items / target));
+      }
+    };
+    share = fabsf(fit(share, (float)aim));
+    if (which == kWideUnits && p.two_rounds) {
+      const float half = fit(fmaxf(least, ceilf(all / (float)(2 * aim))), (float)(2 * aim));
+      if (half > 0.0f && 2.0f * half + kChunkRound < share) share = half;
     }
   }
   int first = 0, slots = 0;
@@ -228,6 +246,39 @@ __device__ __forceinline__ uint16_t *out_of(const ChunkParams &p, const Item &it
 }
 __device__ __forceinline__ float inverse_sum(float sum) { return sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum; }  // (a NaN stays one)
 
+// A split unit's partial: o in pieces of four dimensions, [piece][column], then (m, l) of each column. POLICY
+// kPolicySc1: for a reader in the same launch, which may run on another XCD.
+template <int D, int POLICY>
+struct Partial {
+  __amdgpu_buffer_rsrc_t r;
+  int SC;
+  __device__ __forceinline__ Partial(const ChunkParams &p, const Item &it, int split) {
+    SC = p.slot_columns;
+    const uint32_t slot_bytes = (uint32_t)SC * (D + 2) * 4;
+    r = rsrc(reinterpret_cast<uint8_t *>(p.part) + (int64_t)(it.slot0 + split) * slot_bytes, slot_bytes);
+  }
+  __device__ __forceinline__ void put(int piece, int column, f32x4 o) const {
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), r, (piece * SC + column) * 16, 0, POLICY);
+  }
+  __device__ __forceinline__ void put(int column, float m, float l) const {
+    __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(m), __float_as_uint(l)}, r, D * SC * 4 + column * 8, 0, POLICY);
+  }
+  __device__ __forceinline__ u32x4 o(int piece, int column) const { return __builtin_amdgcn_raw_buffer_load_b128(r, (piece * SC + column) * 16, 0, POLICY); }
+  __device__ __forceinline__ u32x2 ml(int column) const { return __builtin_amdgcn_raw_buffer_load_b64(r, D * SC * 4 + column * 8, 0, POLICY); }
+};
+// Four dimensions of a column, final or a split unit's partial for the same launch.
+template <int D, bool BF>
+__device__ __forceinline__ void store_piece(const ChunkParams &p, const Item &it, const Columns &cs, int piece, int c, f32x4 o, float m, float l) {
+  if (it.splits == 1) {
+    const float inv = inverse_sum(l);
+    *reinterpret_cast<u32x2 *>(out_of(p, it, cs, c) + 4 * piece) = u32x2{pack_out<BF>(o[0] * inv, o[1] * inv), pack_out<BF>(o[2] * inv, o[3] * inv)};
+  } else {
+    const Partial<D, kPolicySc1> to(p, it, it.split);
+    to.put(piece, c, o);
+    if (piece == 0) to.put(c, m, l);
+  }
+}
+
 constexpr int kStageRow = 20, kStageBytes = 32 * kStageRow * 4;  // of a wave
 // A wave's 32 columns: lane (h, q) = (lane / 32, lane % 32) has query q's part.
 // SPLIT: K and q as pairs of FP16 values.
@@ -240,6 +291,7 @@ struct Wave {
   float cl;    // a product's factor: scale log2(e) over the powers of two
   int pos;     // this lane's query's position
   int window, sinks;
+  uint32_t lane_at;  // this lane's bytes in a tile of K rows, and 65536 times those in one of V rows
 
   // Column c's row of the chunk and head (past the tile's: its last column's).
   __device__ __forceinline__ static void column(const ChunkParams &p, const Item &it, const Columns &cs, int c, int &row, int &head) {
@@ -283,6 +335,10 @@ struct Wave {
   // Nothing seen yet. eq: the queries' power of two; K rows in the code domain (`coded`) carry the books', 2^(cent_exp - 14).
   __device__ __forceinline__ void begin(const ChunkParams &p, const Item &it, int eq, bool coded) {
     window = p.window, sinks = p.sinks;
+    const int lane = threadIdx.x & 63, h = lane >> 5, qc = lane & 31, vr = 4 * h + ((lane & 15) >> 2);
+    const int piece = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+    lane_at = (uint32_t)(qc * (2 * D) + ((h ^ swizzle<D>(qc)) * 16)) |
+              (uint32_t)(vr * (2 * D) + ((piece ^ swizzle<D>(vr)) * 16) + (lane & 1) * 8) << 16;
     // (it meets masked logits: not 0)
     cl = fmaxf(__builtin_ldexpf(p.c, -eq - (coded ? p.head[it.kv].cent_exp - 14 : 0)), 0x1p-126f);
 #pragma unroll
@@ -418,8 +474,9 @@ struct Wave {
   // S += K Q^T of the NB x 32 K rows at LDS offset `at`; low: the queries' low parts too.
   template <int NB>
   __device__ __forceinline__ void qk(uint8_t *smem, uint32_t at, f32x16 (&S)[NB], bool low) const {
-    const int lane = threadIdx.x & 63, h = lane >> 5, qc = lane & 31;
-    const uint32_t k_at = (uint32_t)(qc * (2 * D) + ((h ^ swizzle<D>(qc)) * 16));
+    uint32_t k_at = lane_at;
+    if constexpr (D == 64) asm volatile("" : "+v"(k_at));  // (parted here: each held across the loop, one was spilled, and its reload waited for the DMAs)
+    k_at &= 0xffffu;
 #pragma unroll
     for (int s = 0; s < QS; ++s)
 #pragma unroll
@@ -439,7 +496,9 @@ struct Wave {
   // Whether this lane's query sees token 4 h + k of a block from t0 on (bit k), of those in `there`.
   __device__ __forceinline__ uint64_t seen_bits(int t0, uint64_t there) const {
     auto below = [](int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : ~(~0ull << n); };  // bits 0 .. n - 1
-    const int h = (threadIdx.x & 63) >> 5, d = pos - t0 - 4 * h;
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));  // (made here: what is held across the loop spills)
+    const int h = lane >> 5, d = pos - t0 - 4 * h;
     uint64_t bits = below(d + 1);
     if (window) bits &= ~below(d + 1 - window) | below(sinks - t0 - 4 * h);
     return bits & (there >> (4 * h));
@@ -488,16 +547,14 @@ struct Wave {
   template <int NB, bool MAYBE_ODD>
   __device__ __forceinline__ void pv(uint8_t *smem, uint32_t at, const uint32_t (&P)[8 * NB], bool odd) {
     constexpr int STEP = 16 * 2 * D;  // bytes of a step's rows
-    const int lane = threadIdx.x & 63;
-    const int h = lane >> 5, vr = 4 * h + ((lane & 15) >> 2), piece = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-    const uint32_t lds0 = lds_at(smem) + at;
-    const uint32_t v_at = (uint32_t)(vr * (2 * D) + ((piece ^ swizzle<D>(vr)) * 16) + (lane & 1) * 8);
-    const uint32_t v_at8 = (uint32_t)((vr + 8) * (2 * D) + ((piece ^ swizzle<D>(vr + 8)) * 16) + (lane & 1) * 8);
+    uint32_t v_at = lane_at;
+    if constexpr (D == 64) asm volatile("" : "+v"(v_at));
+    v_at = lds_at(smem) + at + (v_at >> 16);
     uint32_t va[MT], va8[MT];
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
-      va[t] = (lds0 + v_at) ^ (64u * t);
-      va8[t] = (lds0 + v_at8) ^ (64u * t);
+      va[t] = v_at ^ (64u * t);
+      va8[t] = ((v_at ^ 32u) + 16 * D) ^ (64u * t);  // (swizzle(vr + 8) = swizzle(vr) ^ 2)
     }
     u32x2 v[2][MT][2];
     ds_read_tr16<MT, 0>(va, va8, v[0]);
@@ -573,9 +630,7 @@ struct Wave {
   }
 
   // The item's results, of this wave's columns first_column on (below `stored` of the tile's): to out, or, of a split
-  // unit, as a partial: o in pieces of four dimensions, [piece][column], then (m, l) of each column. COHERENT: for a reader in the same launch,
-  // which may run on another XCD.
-  template <bool COHERENT>
+  // unit, as a partial (Partial).
   __device__ __forceinline__ void store(const ChunkParams &p, const Item &it, const Columns &cs, int first_column, int stored) {
     const int lane = threadIdx.x & 63, h = lane >> 5, mine = first_column + (lane & 31);
     l = half_sum(l);
@@ -591,30 +646,21 @@ struct Wave {
               u32x2{pack_out<BF>(O[t][4 * g] * inv, O[t][4 * g + 1] * inv), pack_out<BF>(O[t][4 * g + 2] * inv, O[t][4 * g + 3] * inv)};
       return;
     }
-    constexpr int kPolicy = COHERENT ? kPolicySc1 : kCached;
-    const int SC = p.slot_columns;
-    const uint32_t slot_bytes = (uint32_t)SC * (D + 2) * 4;
-    const __amdgpu_buffer_rsrc_t r = rsrc(reinterpret_cast<uint8_t *>(p.part) + (int64_t)(it.slot0 + it.split) * slot_bytes, slot_bytes);
+    const Partial<D, kCached> to(p, it, it.split);
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll
       for (int g = 0; g < 4; ++g)
-        __builtin_amdgcn_raw_buffer_store_b128(
-            __builtin_bit_cast(u32x4, (f32x4{O[t][4 * g], O[t][4 * g + 1], O[t][4 * g + 2], O[t][4 * g + 3]})), r,
-            (int)(((8 * t + 2 * g + h) * SC + mine) * 16), 0, kPolicy);
-    if (h == 0)
-      __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(m), __float_as_uint(l)}, r, (int)(D * SC * 4 + mine * 8), 0, kPolicy);
+        to.put(8 * t + 2 * g + h, mine, f32x4{O[t][4 * g], O[t][4 * g + 1], O[t][4 * g + 2], O[t][4 * g + 3]});
+    if (h == 0) to.put(mine, m, l);
   }
 };
 
 // Pieces e0, e0 + step, ... below e1 of a unit's columns, merged from its items' partials in their order.
 template <int D, bool BF, bool COHERENT>
 __device__ __forceinline__ void merge_pieces(const ChunkParams &p, const Item &it, const Columns &cs, int e0, int e1, int step) {
-  const int SC = p.slot_columns;
-  const uint32_t slot_bytes = (uint32_t)SC * (D + 2) * 4;
   for (int e = e0; e < e1; e += step) {
     const int piece = e / cs.count, c = e - piece * cs.count;
-    auto slot = [&](int s) { return rsrc(reinterpret_cast<uint8_t *>(p.part) + (int64_t)(it.slot0 + s) * slot_bytes, slot_bytes); };
     float M = -INFINITY, sum = 0.0f;
     f32x4 o{0.0f, 0.0f, 0.0f, 0.0f};
     constexpr int N = 8, kPolicy = COHERENT ? kPolicySc1 : kCached;  // splits whose loads are in flight together
@@ -623,9 +669,9 @@ __device__ __forceinline__ void merge_pieces(const ChunkParams &p, const Item &i
       f32x4 x[N];
 #pragma unroll
       for (int k = 0; k < N; ++k) {
-        const __amdgpu_buffer_rsrc_t r = slot(min(s0 + k, it.splits - 1));
-        ml[k] = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, D * SC * 4 + c * 8, 0, kPolicy));
-        x[k] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (piece * SC + c) * 16, 0, kPolicy));
+        const Partial<D, kPolicy> from(p, it, min(s0 + k, it.splits - 1));
+        ml[k] = from.ml(c);
+        x[k] = __builtin_bit_cast(f32x4, from.o(piece, c));
       }
       float top = M;
 #pragma unroll
@@ -637,8 +683,8 @@ __device__ __forceinline__ void merge_pieces(const ChunkParams &p, const Item &i
 #pragma unroll
       for (int k = 0; k < N; ++k) {
         const float mk = __uint_as_float(ml[k][0]);
-        const bool live = s0 + k < it.splits && mk != -INFINITY;
-        const float w = live ? __builtin_amdgcn_exp2f(mk - M) : 0.0f;
+        const bool live = s0 + k < it.splits;
+        const float w = mk == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mk - M);  // (a state that saw nothing is all zeros)
         sum = live ? __builtin_fmaf(__uint_as_float(ml[k][1]), w, sum) : sum;
 #pragma unroll
         for (int d = 0; d < 4; ++d) o[d] = live ? __builtin_fmaf(x[k][d], w, o[d]) : o[d];

@@ -37,13 +37,14 @@ __global__ __launch_bounds__((64 * Wide<D, SRC, BF>::W), (Wide<D, SRC, BF>::PER_
   const Blocks bl = Blocks::of<kChunkKeys>(cs.first, min(cs.last, it.n - 1), p.window, p.sinks);
   const int b0 = (int)((int64_t)bl.count * it.split / it.splits), b1 = (int)((int64_t)bl.count * (it.split + 1) / it.splits);
   const int kv = it.kv;
-  // The table's entry of a block's half, a lane's: looked up with a block's
-  // DMAs, a block ahead (pages: two, since the DMAs need it), for the whole block's test.
+  // The table's entry of a block's half, and whether it names a page. Blocks of pages look theirs up two blocks ahead, since the
+  // DMAs need them; rebuilt ones are tested before the loop, and in it only where a page is missing.
   const int32_t *const table = p.page_table + (int64_t)it.seq * p.page_table_stride;
-  auto entry = [&](int i) {
-    const int t = bl.at<kChunkKeys>(min(i, b1 - 1)) + 32 * (lane >> 5);
+  auto entry_of = [&](int i, int half) {
+    const int t = bl.at<kChunkKeys>(min(i, b1 - 1)) + 32 * half;
     return table[min(t >> p.page_shift, p.table_pages - 1)];
   };
+  auto entry = [&](int i) { return entry_of(i, lane >> 5); };
   auto in_pool = [&](int e) -> uint64_t { return __builtin_amdgcn_ballot_w64((uint32_t)e < (uint32_t)p.pages); };
   auto issue = [&](int i, int e) {  // e: the block's entries (pages)
     const int t0 = bl.at<kChunkKeys>(i);
@@ -79,8 +80,16 @@ __global__ __launch_bounds__((64 * Wide<D, SRC, BF>::W), (Wide<D, SRC, BF>::PER_
     }
   };
   int e0 = 0, e1 = 0;  // the entries of block i, i + 1
+  bool none_missing = true;
   if (b0 < b1) {
-    e0 = entry(b0), e1 = entry(b0 + 1);
+    if constexpr (SRC == kPages) {
+      e0 = entry(b0), e1 = entry(b0 + 1);
+    } else {
+      bool ok = true;
+#pragma unroll 4
+      for (int i = b0; i < b1; i += 32) ok &= (uint32_t)entry_of(i + (lane & 31), lane >> 5) < (uint32_t)p.pages;
+      none_missing = __builtin_amdgcn_ballot_w64(!ok) == 0;
+    }
   }
   Wave<D, SPLIT, BF> w;
   if constexpr (SRC == kCoded) w.load_turned(p, it, cs, 32 * wave);
@@ -97,13 +106,19 @@ __global__ __launch_bounds__((64 * Wide<D, SRC, BF>::W), (Wide<D, SRC, BF>::PER_
   auto arrive = [&](int i) -> uint64_t {
     wait_vm<0>();   // this wave's part of block i has landed
     lds_barrier();  // everyone's has, and everyone is done with the other buffer
-    const uint64_t there = in_pool(e0);
-    e0 = e1;
-    if (i + 1 < b1) {
-      e1 = entry(i + 2);
-      __builtin_amdgcn_sched_barrier(0);  // (ahead of the DMAs: its wait leaves them in flight)
-      issue(i + 1, e0);
+    if constexpr (SRC == kPages) {
+      const uint64_t there = in_pool(e0);
+      e0 = e1;
+      if (i + 1 < b1) {
+        e1 = entry(i + 2);
+        __builtin_amdgcn_sched_barrier(0);  // (ahead of the DMAs: its wait leaves them in flight)
+        issue(i + 1, e0);
+      }
+      return there;
     }
+    uint64_t there = ~0ull;
+    if (!none_missing) there = in_pool(entry(i));
+    if (i + 1 < b1) issue(i + 1, 0);
     return there;
   };
   auto attend = [&](auto masked_tag, int i, uint64_t there) {
@@ -122,9 +137,11 @@ __global__ __launch_bounds__((64 * Wide<D, SRC, BF>::W), (Wide<D, SRC, BF>::PER_
       seen = w.seen_bits(bl.at<kChunkKeys>(i), there);
       // A token that a query does not see has probability 0, but 0 times an infinity or a NaN of its V row is not 0.
       float z = 0.0f;
+      int mine = lane;
+      asm volatile("" : "+v"(mine));  // (not held across the loop)
 #pragma unroll
       for (int k = 0; k < PR; ++k) {
-        const u32x4 v = *reinterpret_cast<const u32x4 *>(smem + buf + TILE + (64 * k + lane) * 16);
+        const u32x4 v = *reinterpret_cast<const u32x4 *>(smem + buf + TILE + (64 * k + mine) * 16);
 #pragma unroll
         for (int e = 0; e < 4; ++e) z = odd2(v[e], z);
       }
@@ -147,7 +164,7 @@ __global__ __launch_bounds__((64 * Wide<D, SRC, BF>::W), (Wide<D, SRC, BF>::PER_
     }
     if (i < b1 && any && w.sight(bl.at<kChunkKeys>(i), kChunkKeys, lo, hi) != 0) attend(std::true_type{}, i, there);
   }
-  w.template store<false>(p, it, cs, 32 * wave, cs.count);
+  w.store(p, it, cs, 32 * wave, cs.count);
 }
 
 // The partials of split units: a workgroup per slot, the unit's work shared by

@@ -218,7 +218,7 @@ __device__ __forceinline__ void encode_tile_body(const EncodeTileJob &job, const
       if (rotation.k_norm) {
         double sum = 0.0;
 #pragma unroll
-        for (int i = 0; i < KS; ++i) sum += rot::square(x[i]);
+        for (int i = 0; i < KS; ++i) sum = rot::add_square(x[i], sum);
         const float f = rot::factor(rot::col_sum(sum), D, rotation.eps);
         const float *w = rotation.k_norm + KS * gq;
 #pragma unroll

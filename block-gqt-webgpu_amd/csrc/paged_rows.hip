@@ -92,8 +92,8 @@ __global__ __launch_bounds__(kThreads) void paged_write_kernel(PagedWriteParams 
 #pragma unroll
       for (int jl = 0; jl < JL; ++jl) x[jl] = load_one(p.k, p.k_dtype, at + 64 * jl);
       if (rotation.k_norm) {
-        double sum = rot::square(x[0]);
-        if (JL > 1) sum += rot::square(x[JL - 1]);
+        double sum = rot::add_square(x[0], 0.0);
+        if (JL > 1) sum = rot::add_square(x[JL - 1], sum);
         const float f = rot::factor(rot::col_sum(rot::lanes_sum<16>(sum)), D, rotation.eps);
 #pragma unroll
         for (int jl = 0; jl < JL; ++jl) x[jl] = (x[jl] * f) * rotation.k_norm[lane + 64 * jl];

@@ -103,7 +103,7 @@ __device__ __forceinline__ void load8_rotated(const void *src, int dtype, bool v
   if (r.k_norm) {
     double sum = 0.0;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) sum += rot::square(x[k]);
+    for (int k = 0; k < 8; ++k) sum = rot::add_square(x[k], sum);
     const float f = rot::factor(rot::lanes_sum<L>(sum), D, r.eps);
 #pragma unroll
     for (int k = 0; k < 8; ++k) {

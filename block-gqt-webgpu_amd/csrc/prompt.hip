@@ -263,11 +263,16 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 4 : 2) void prompt_kernel(Promp
   // rows 32 on: + 64 D); V, its part of rows 4 h + (lane % 16) / 4 (tile t: ^ 64 t)
   // and 8 rows on. The swizzle of a row depends on its lane's part alone.
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void *)smem;
-  const uint32_t k_at = (uint32_t)(qc * (2 * D) + ((h ^ swizzle<D>(qc)) * 16));
   const int vr = 4 * h + ((lane & 15) >> 2);
   const int v_piece = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-  const uint32_t v_at = (uint32_t)(vr * (2 * D) + ((v_piece ^ swizzle<D>(vr)) * 16) + (lane & 1) * 8);
-  const uint32_t v_at8 = (uint32_t)((vr + 8) * (2 * D) + ((v_piece ^ swizzle<D>(vr + 8)) * 16) + (lane & 1) * 8);
+  const uint32_t lane_at = (uint32_t)(qc * (2 * D) + ((h ^ swizzle<D>(qc)) * 16)) |
+                           (uint32_t)(vr * (2 * D) + ((v_piece ^ swizzle<D>(vr)) * 16) + (lane & 1) * 8) << 16;
+  // (d=64 behind a window: parted in each block; each held across the loop, they were spilled. d=128 is 12% slower so.)
+  auto parted = [&]() {
+    uint32_t x = lane_at;
+    if constexpr (WIN && D == 64) asm volatile("" : "+v"(x));
+    return x;
+  };
 
   // Every wave meets every block's barrier and loads its part of every block.
   auto arrive = [&](int j) {
@@ -288,21 +293,23 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 4 : 2) void prompt_kernel(Promp
     }
   };
   // The keys of the workgroup's block i0 for this wave's queries; DIAGONAL: some queries see only a part of them.
-  // (WIN, DIAGONAL: unless `whole`.)
-  auto attend = [&](auto diagonal_tag, int i0, bool whole = false) {
+  auto attend = [&](auto diagonal_tag, int i0) {
     constexpr bool DIAGONAL = decltype(diagonal_tag)::value;
     const int j = block(i0);
     const uint32_t buf = (uint32_t)(i0 & 1) * 2 * BLOCK;
     // Whether this lane's query sees key 4 h + k of the block; behind a window
     // from a bit for each (one comparison more per key spilled 65 registers).
-    const int d = qi - j * kKeys - 4 * h;
+    int mine = lane;
+    if constexpr (WIN) asm volatile("" : "+v"(mine));  // (not held across the loop)
+    const int d = row0 + (mine & 31) - j * kKeys - 4 * (mine >> 5);
     uint64_t seen_bits = 0;
     if constexpr (WIN && DIAGONAL) {
       auto below = [](int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : ~(~0ull << n); };  // bits 0 .. n - 1
-      seen_bits = below(d + 1) & (~below(d + 1 - p.window) | below(p.sinks - j * kKeys - 4 * h));
+      seen_bits = below(d + 1) & (~below(d + 1 - p.window) | below(p.sinks - j * kKeys - 4 * (mine >> 5)));
     }
     const uint32_t seen_lo = (uint32_t)seen_bits, seen_hi = (uint32_t)(seen_bits >> 32);
     auto sees = [&](int k) -> bool { return WIN ? (k < 32 ? seen_lo >> k : seen_hi >> (k - 32)) & 1u : k <= d; };
+    const uint32_t k_at = parted() & 0xffffu;
     f32x16 S[2];
 #pragma unroll
     for (int b = 0; b < 2; ++b)
@@ -315,7 +322,7 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 4 : 2) void prompt_kernel(Promp
         const u32x4 a = *reinterpret_cast<const u32x4 *>(smem + ((buf + k_at) ^ (32u * s)) + 64 * D * b);
         S[b] = product<BF>(a, qf[s], S[b]);
       }
-    if (DIAGONAL && !whole) {
+    if constexpr (DIAGONAL) {
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -356,72 +363,32 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 4 : 2) void prompt_kernel(Promp
     softmax_first(0);
     // O^T += V^T P^T, 16 keys a step, the next step's V on its way meanwhile.
     uint32_t va[MT], va8[MT];
+    const uint32_t v_at = lds0 + buf + BLOCK + (parted() >> 16);
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
-      va[t] = (lds0 + buf + BLOCK + v_at) ^ (64u * t);
-      va8[t] = (lds0 + buf + BLOCK + v_at8) ^ (64u * t);
+      va[t] = v_at ^ (64u * t);
+      va8[t] = ((v_at ^ 32u) + 16 * D) ^ (64u * t);  // (swizzle(vr + 8) = swizzle(vr) ^ 2)
     }
     // A key that a query does not see has probability 0, but 0 times an
-    // infinity or a NaN of its V row is not 0: such a block's products take
-    // the finite values, and what is seen of the others is added by itself.
-    bool plain = true;
-    if (DIAGONAL && !whole) {
+    // infinity or a NaN of its V row is not 0: what is seen of those is added by
+    // itself, and such a block's products take the finite values.
+    bool odd = false;
+    if constexpr (DIAGONAL) {
       typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
       u16x2 most{0, 0};
 #pragma unroll
       for (int i = 0; i < PR; ++i) {
-        const u32x4 w = *reinterpret_cast<const u32x4 *>(smem + buf + BLOCK + (64 * i + lane) * 16);
+        const u32x4 w = *reinterpret_cast<const u32x4 *>(smem + buf + BLOCK + (64 * i + mine) * 16);
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, w[e] & 0x7fff7fffu));
       }
-      plain = __builtin_amdgcn_ballot_w64(most[0] >= Odd<BF>::kInf || most[1] >= Odd<BF>::kInf) == 0;
+      odd = __builtin_amdgcn_ballot_w64(most[0] >= Odd<BF>::kInf || most[1] >= Odd<BF>::kInf) != 0;
     }
-    if (!DIAGONAL || plain) {
-      constexpr int STEP = 16 * 2 * D;  // bytes of a step's rows
-      u32x2 v[2][MT][2];
-      ds_read_tr16<MT, 0>(va, va8, v[0]);
-#pragma unroll
-      for (int s = 0; s < kKeys / 16; ++s) {
-        const u32x4 pf{P[4 * s], P[4 * s + 1], P[4 * s + 2], P[4 * s + 3]};
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {
-          const u32x2 a = v[s & 1][t][0], b = v[s & 1][t][1];
-          O[t] = product<BF>(u32x4{a[0], a[1], b[0], b[1]}, pf, O[t]);
-        }
-        if (s == 0) ds_read_tr16<MT, STEP>(va, va8, v[1]);
-        if (s == 1) ds_read_tr16<MT, 2 * STEP>(va, va8, v[0]);
-        if (s == 2) ds_read_tr16<MT, 3 * STEP>(va, va8, v[1]);
-      }
-    } else {
-      // (through an opaque copy: or the rare branch's addresses are held across the loop)
+    if (DIAGONAL && odd) {
       int rare = lane;
-      asm volatile("" : "+v"(rare));
+      asm volatile("" : "+v"(rare));  // (this branch's addresses are not held across the loop)
       const int h = rare >> 5, qc = rare & 31;
-      // V of dimension 32 t + qc, keys 16 s + 8 (e / 2) + 4 h + 2 (e % 2) + 0, 1 in word e.
-      auto column = [&](int s, int t) {
-        u32x4 a;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          a[e] = 0;
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const int r = 16 * s + 8 * (e >> 1) + 4 * h + 2 * (e & 1) + x;
-            const uint8_t *at = smem + buf + BLOCK + r * (2 * D) + (((4 * t + (qc >> 3)) ^ swizzle<D>(r)) * 16) + 2 * (qc & 7);
-            a[e] |= (uint32_t)*reinterpret_cast<const uint16_t *>(at) << (16 * x);
-          }
-        }
-        return a;
-      };
-#pragma unroll
-      for (int s = 0; s < kKeys / 16; ++s)
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {
-          u32x4 a = column(s, t);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) a[e] = Odd<BF>::finite(a[e]);
-          O[t] = product<BF>(a, u32x4{P[4 * s], P[4 * s + 1], P[4 * s + 2], P[4 * s + 3]}, O[t]);
-        }
 #pragma clang loop unroll(disable)
       for (int kind = 0; kind < 3; ++kind) {
         const float value = kind == 0 ? __builtin_nanf("") : kind == 1 ? INFINITY : -INFINITY;
@@ -432,9 +399,17 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 4 : 2) void prompt_kernel(Promp
           for (int i = 0; i < 16; ++i) n[i] = 0.0f;
 #pragma clang loop unroll(disable)
           for (int s = 0; s < kKeys / 16; ++s) {
-            u32x4 a = column(s, t), seen;
+            u32x4 a, seen;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
+              // V of dimension 32 t + qc, keys 16 s + 8 (e / 2) + 4 h + 2 (e % 2) + 0, 1.
+              a[e] = 0;
+#pragma unroll
+              for (int x = 0; x < 2; ++x) {
+                const int r = 16 * s + 8 * (e >> 1) + 4 * h + 2 * (e & 1) + x;
+                const uint8_t *at = smem + buf + BLOCK + r * (2 * D) + (((4 * t + (qc >> 3)) ^ swizzle<D>(r)) * 16) + 2 * (qc & 7);
+                a[e] |= (uint32_t)*reinterpret_cast<const uint16_t *>(at) << (16 * x);
+              }
               const int k = 16 * s + 8 * (e >> 1) + 2 * (e & 1);
               a[e] = Odd<BF>::of_kind(a[e], kind);
               seen[e] = (sees(k) ? Odd<BF>::kOne : 0u) | (sees(k + 1) ? Odd<BF>::kOne << 16 : 0u);
@@ -449,6 +424,25 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 4 : 2) void prompt_kernel(Promp
         }
       }
     }
+    constexpr int STEP = 16 * 2 * D;  // bytes of a step's rows
+    u32x2 v[2][MT][2];
+    ds_read_tr16<MT, 0>(va, va8, v[0]);
+#pragma unroll
+    for (int s = 0; s < kKeys / 16; ++s) {
+      const u32x4 pf{P[4 * s], P[4 * s + 1], P[4 * s + 2], P[4 * s + 3]};
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        u32x4 a{v[s & 1][t][0][0], v[s & 1][t][0][1], v[s & 1][t][1][0], v[s & 1][t][1][1]};
+        if (DIAGONAL && odd) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) a[e] = Odd<BF>::finite(a[e]);
+        }
+        O[t] = product<BF>(a, pf, O[t]);
+      }
+      if (s == 0) ds_read_tr16<MT, STEP>(va, va8, v[1]);
+      if (s == 1) ds_read_tr16<MT, 2 * STEP>(va, va8, v[0]);
+      if (s == 2) ds_read_tr16<MT, 3 * STEP>(va, va8, v[1]);
+    }
   };
   // One block holds the wave's diagonal (32 rows lie within one); those after
   // it hold no key that its queries see. Loops of their own, so that the full
@@ -458,13 +452,17 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 4 : 2) void prompt_kernel(Promp
   const int jd = row0 / kKeys;
   int j = 0;
   if constexpr (WIN) {
-    // (one body for both: with one for the full blocks and one for the others it spilled 97 registers)
     const int low = row0 - p.window;  // the last key that the first query does not see
     for (; j < n_blocks; ++j) {
-      const int k0 = block(j) * kKeys;
-      arrive(j);
-      const bool whole = k0 > low + 31 && k0 < jd * kKeys;
-      if (k0 <= jd * kKeys && (k0 < p.sinks || k0 + kKeys - 1 > low)) attend(std::true_type{}, j, whole);
+      int k0;
+      for (;;) {
+        k0 = block(j) * kKeys;
+        arrive(j);
+        if (k0 <= low + 31 || k0 >= jd * kKeys) break;
+        attend(std::false_type{}, j);
+        if (++j == n_blocks) break;
+      }
+      if (j < n_blocks && k0 <= jd * kKeys && (k0 < p.sinks || k0 + kKeys - 1 > low)) attend(std::true_type{}, j);
     }
   } else {
     for (; j < min(jd, n_blocks); ++j) {

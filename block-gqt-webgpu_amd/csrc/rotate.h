@@ -2,7 +2,7 @@
 // wherever a row is rotated (rotate.hip, and K on its way into pages):
 //   norm (weights given)  x' = fl(fl(x r) w), r = fl32(1 / sqrt(mean(x^2) + eps))
 //     with the sum, the root and the quotient in 64 bits: any order of the sum
-//     gives the same r but for one row in 2^28 or so, so every kernel may sum as
+//     gives the same r but for one row in 2^27 or so, so every kernel may sum as
 //     its lanes lie;
 //   pairs (i, i + D / 2) with a table row's cosine c and sine s of i:
 //     y1 = fma(x1, c, -fl(x2 s)), y2 = fma(x2, c, fl(x1 s)).
@@ -75,9 +75,14 @@ __device__ __forceinline__ double col_sum(double v) {
   v = swap_add(v, [](uint32_t x) { return __builtin_amdgcn_permlane16_swap(x, x, false, false); });
   return swap_add(v, [](uint32_t x) { return __builtin_amdgcn_permlane32_swap(x, x, false, false); });
 }
-__device__ __forceinline__ double square(float x) { return (double)x * (double)x; }
+// (a square of 24 bits is exact in 64: one rounding either way)
+__device__ __forceinline__ double add_square(float x, double sum) { return __builtin_fma((double)x, (double)x, sum); }
+// The hardware's reciprocal root, good to 2^-24 or so, and Halley's step behind it: good to 2^-52.
 __device__ __forceinline__ float factor(double sum, int dim, double eps) {
-  return (float)(1.0 / __builtin_sqrt(sum / (double)dim + eps));
+  const double v = sum / (double)dim + eps, r = __builtin_amdgcn_rsq(v);
+  const double e = __builtin_fma(-(v * r), r, 1.0);
+  const double better = __builtin_fma(r * e, __builtin_fma(e, 0.375, 0.5), r);
+  return (float)(v > 0.0 && v < (double)INFINITY ? better : r);  // (of 0 and infinity the step makes a NaN)
 }
 // One value of a pair: `other` with the sine's sign, + for the pair's second
 // value. Its FP32 rounding is its own: left open, the compiler joins the

@@ -87,6 +87,9 @@ __device__ __forceinline__ void rotate_items(const HeadRows &h, const Rotation &
   };
   const bool vin = aligned(h.src, h.src_row, h.src_head), vout = aligned(h.dst, h.dst_row, h.dst_head);
   const uint32_t n = (uint32_t)rows * (uint32_t)h.heads;
+  float wa[N], wb[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) wa[k] = h.weight ? h.weight[N * sub + k] : 1.0f, wb[k] = h.weight ? h.weight[D / 2 + N * sub + k] : 1.0f;
   for (uint32_t i = first; i < n; i += step) {
     const uint32_t local = i / (uint32_t)h.heads;
     const int head = (int)(i - local * (uint32_t)h.heads);
@@ -106,12 +109,12 @@ __device__ __forceinline__ void rotate_items(const HeadRows &h, const Rotation &
     if (h.weight) {
       double sum = 0.0;
 #pragma unroll
-      for (int k = 0; k < N; ++k) sum += square(a[k]) + square(b[k]);
+      for (int k = 0; k < N; ++k) sum = add_square(b[k], add_square(a[k], sum));
       const float f = factor(lanes_sum<L>(sum), D, r.eps);
 #pragma unroll
       for (int k = 0; k < N; ++k) {
-        a[k] = (a[k] * f) * h.weight[N * sub + k];
-        b[k] = (b[k] * f) * h.weight[D / 2 + N * sub + k];
+        a[k] = (a[k] * f) * wa[k];
+        b[k] = (b[k] * f) * wb[k];
       }
     }
     float y[N], z[N];

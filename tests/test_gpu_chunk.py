@@ -168,6 +168,56 @@ def test_long_histories(device, oracle, dtype, layout, v, dim, heads):
     pool.destroy()
 
 
+@pytest.mark.parametrize("layout,v,dim,heads,dtype", [("S", "q8", 64, 3, "float16"), ("B", "q8", 64, 2, "bfloat16"), ("f16", "q8", 128, 2, "bfloat16")])
+@pytest.mark.parametrize("max_length", [1 << 18, 1 << 20])
+def test_groups_of_sequences(device, oracle, layout, v, dim, heads, dtype, max_length):
+    """Sequences that may be long take the rebuilt rows' workspace in turns."""
+    import torch
+    rng = np.random.RandomState(4)
+    new, lengths = [c for c, _ in MIXED] * 2, [n for _, n in MIXED] * 2
+    pool, table = _written(device, layout, v, dim, heads, 64, lengths, rng, 6, spare=max_length // 64)
+    q = _rows(sum(new), heads * 3, dim, dtype, 4, 3).cuda()
+    for window, sinks in ((0, 0), (50, 3)):
+        print(layout, max_length, window, flush=True)
+        out = _call(pool, q, new, lengths, table, window, sinks, max_length=max_length)
+        torch.cuda.synchronize()
+        _check(pool, oracle, q, out, new, lengths, table, window, sinks)
+    pool.destroy()
+
+
+def test_two_rounds_of_items(device, oracle):
+    """100 equal units on 256 workgroups: two splits each leave 56 idle, five are two rounds."""
+    import torch
+    rng = np.random.RandomState(7)
+    pool, table = _written(device, "B", "q8", 128, 1, 64, [6500], rng, 5)
+    q = _rows(1600, 16, 128, "float16", 2, 3).cuda()
+    out = _call(pool, q, [1600], [6500], table)
+    torch.cuda.synchronize()
+    _check(pool, oracle, q, out, [1600], [6500], table)
+    pool.destroy()
+
+
+@pytest.mark.parametrize("new", [1, 30, 400])
+def test_a_query_of_nans(device, oracle, new):
+    """Its head's output is NaN, whether its tokens are split or not. The others' keep their limits (not their bits:
+    32 columns raise their maxima together, and FP16 probabilities are rounded relative to those)."""
+    import torch
+    rng = np.random.RandomState(8)
+    for layout, dim, dtype in (("f16", 64, "bfloat16"), ("B", 128, "bfloat16"), ("S", 64, "float16")):
+        heads = 3 if layout == "S" else 1
+        for n in (400, 5000):
+            pool, table = _written(device, layout, "q8", dim, heads, 64, [n], rng, 5)
+            q = _rows(new, 2 * heads, dim, dtype, 2, 3).cuda()
+            bad = q.clone()
+            bad[new // 2, 1, 3] = float("nan")
+            out = _call(pool, bad, [new], [n], table)
+            torch.cuda.synchronize()
+            assert bool(out[new // 2, 1].isnan().all())
+            out[new // 2, 1] = _call(pool, q, [new], [n], table)[new // 2, 1]
+            _check(pool, oracle, q, out, [new], [n], table)
+            pool.destroy()
+
+
 @pytest.mark.parametrize("sequences", [1, 64, 65, 200])
 def test_many_sequences(device, oracle, sequences):
     import torch
