@@ -1890,6 +1890,8 @@ bgtq_status bgtq_rotate(bgtq_context *ctx, const bgtq_rotation *r, int32_t dim, 
     if (bgtq_status s = check_head_rows(q, rows, dim)) return s;
   if (k)
     if (bgtq_status s = check_head_rows(k, rows, dim)) return s;
+  if (rows && q && k && (q->dst == k->dst || q->dst == k->src || q->src == k->dst))
+    return fail(BGTQ_ERR_RANGE, "rotated q and k overlap");
   if (!ctx) return fail(BGTQ_ERR_RANGE, "null context");
   if (!rows) return BGTQ_OK;
   DeviceScope scope;
@@ -2131,6 +2133,7 @@ bgtq_status bgtq_paged_prefill(bgtq_context *ctx, const bgtq_pages *g, const bgt
     if (a.row < 0 || a.head < 0 || a.row % 8 || a.head % 8 || reinterpret_cast<uintptr_t>(a.p) % 16)
       return fail(BGTQ_ERR_RANGE, "q/out: 16-byte aligned bases, strides multiples of 8 elements and not negative");
   if (!apart(d->tokens, d->out_row_stride, d->q_heads, d->out_head_stride, g->dim)) return fail(BGTQ_ERR_RANGE, "out: overlapping rows");
+  if (!none && d->out == d->q) return fail(BGTQ_ERR_RANGE, "out overlaps q");
   const size_t need = chunk_workspace(plan);
   if (!d->workspace || d->workspace_bytes < need) return fail(BGTQ_ERR_RANGE, "workspace of %zu bytes required", need);
   if (reinterpret_cast<uintptr_t>(d->workspace) % 16) return fail(BGTQ_ERR_RANGE, "workspace must be 16-byte aligned");

@@ -109,21 +109,30 @@ struct Item {
 // of the wide ones' K and V); the wide ones.
 enum { kAllUnits, kNarrowUnits, kWideUnits };
 
+// The largest value of the lanes up to and with this one, none negative.
+__device__ __forceinline__ int wave_prefix_max(int v) {
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false));
+  return v;
+}
 // A sequence's units and what each costs; a lane per sequence.
 struct SequencePlan {
-  int64_t begin;
-  int rows, n, units;
+  int begin, rows, n, units;
   bool wide;
   float cost;
 };
-__device__ __forceinline__ SequencePlan plan_of(const ChunkParams &p, int s, int which, int tile) {
-  auto offset = [&](int i) {
-    const int64_t o = p.offsets[i];
-    return o < 0 ? 0 : o > p.tokens ? p.tokens : o;
-  };
+// The offsets count as no less than those before them (`before`: the sequences' ahead of these 64), so that
+// whatever they hold, the chunks are `tokens` rows at most, which the host's counts go by.
+__device__ __forceinline__ SequencePlan plan_of(const ChunkParams &p, int s, int which, int tile, int &before) {
+  auto offset = [&](int i) { return min(max(p.offsets[i], 0), (int)p.tokens); };
   const bool real = s < p.sequences;
-  const int64_t begin = offset(min(s, p.sequences)), end = offset(min(s + 1, p.sequences));
-  const int rows = real && end > begin ? (int)(end - begin) : 0;
+  const int begin = max(before, wave_prefix_max(offset(min(s, p.sequences)))), end = max(begin, offset(min(s + 1, p.sequences)));
+  before = __builtin_amdgcn_readlane(end, 63);
+  const int rows = real ? end - begin : 0;
   const int n = (int)min(p.lengths[min(s, p.sequences - 1)], (uint32_t)p.max_length);
   const int64_t columns = (int64_t)rows * p.group;
   const bool wide = columns > 32, mine = which == kAllUnits || wide == (which == kWideUnits);
@@ -170,8 +179,9 @@ __device__ __forceinline__ Item find_item(const ChunkParams &p, int item, int wh
   const int lane = threadIdx.x & 63;
   float all = 0.0f;
   SequencePlan q{};
+  int before = 0;
   for (int s0 = 0; s0 < p.sequences; s0 += 64) {
-    q = plan_of(p, s0 + lane, which, tile);
+    q = plan_of(p, s0 + lane, which, tile, before);
     all += wave_sum_f((float)q.units * q.cost);
   }
   const float least = which == kWideUnits ? kChunkLeast : kChunkLeastNarrow;
@@ -195,8 +205,9 @@ __device__ __forceinline__ Item find_item(const ChunkParams &p, int item, int wh
   }
   int first = 0, slots = 0;
   int64_t base = 0;
+  before = 0;
   for (int s0 = 0; s0 < p.sequences; s0 += 64) {
-    if (p.sequences > 64) q = plan_of(p, s0 + lane, which, tile);
+    if (p.sequences > 64) q = plan_of(p, s0 + lane, which, tile, before);
     const int splits = splits_of(q, share), items = BY_SLOT && splits < 2 ? 0 : splits * q.units, rebuilt = rebuilt_rows(q);
     const int end = first + wave_prefix(items), slot_end = slots + wave_prefix(splits > 1 ? items : 0);
     const int base_end = wave_prefix(rebuilt);  // (64 sequences of at most 2^24 tokens)
@@ -205,7 +216,7 @@ __device__ __forceinline__ Item find_item(const ChunkParams &p, int item, int wh
       const int at = __builtin_ctzll(here);
       auto of = [&](int v) { return __builtin_amdgcn_readlane(v, at); };
       Item r;
-      r.begin = (int64_t)(uint32_t)of((int)(uint32_t)q.begin);
+      r.begin = of(q.begin);
       r.seq = s0 + at;
       r.rows = of(q.rows);
       r.n = of(q.n);
@@ -663,7 +674,7 @@ __device__ __forceinline__ void merge_pieces(const ChunkParams &p, const Item &i
     const int piece = e / cs.count, c = e - piece * cs.count;
     float M = -INFINITY, sum = 0.0f;
     f32x4 o{0.0f, 0.0f, 0.0f, 0.0f};
-    constexpr int N = 8, kPolicy = COHERENT ? kPolicySc1 : kCached;  // splits whose loads are in flight together
+    constexpr int N = COHERENT ? 8 : 4, kPolicy = COHERENT ? kPolicySc1 : kCached;  // splits whose loads are in flight together
     for (int s0 = 0; s0 < it.splits; s0 += N) {
       u32x2 ml[N];
       f32x4 x[N];

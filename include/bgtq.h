@@ -544,7 +544,7 @@ bgtq_status bgtq_paged_decode_window(bgtq_context *ctx, const bgtq_pages *pages,
  * window > 0: as bgtq_window). The pages already hold the new tokens (bgtq_paged_append
  * or _write first). A batch may mix sequences of one new token, many and none.
  * dtype: BGTQ_DTYPE_F16 or _BF16, of q and out; layouts of both as bgtq_prompt_desc's;
- * offsets are clamped to 0 .. tokens, lengths to max_length; rows of no sequence stay
+ * offsets are clamped to 0 .. tokens and to no less than those before them, lengths to max_length; rows of no sequence stay
  * as they were, rows that see nothing (negative positions, tokens without a page)
  * become zero. Tokens whose table entry is not a page of the pool are left out.
  * q_heads / kv_heads at most 16; tokens * q_heads / kv_heads below 2^31. Logits, softmax
@@ -554,9 +554,12 @@ bgtq_status bgtq_paged_decode_window(bgtq_context *ctx, const bgtq_pages *pages,
  * rows by both as pairs of FP16 values (22 bits). scale: of the logits, at most 2e38; 0 =
  * 1 / sqrt(dim). workspace: 16-byte aligned, bgtq_paged_prefill_workspace_size()
  * bytes (its first BGTQ_PAGED_PREFILL_COUNTER_BYTES zero before the first call on it,
- * left zero by every call whatever its geometry; the rest needs no contents);
- * calls sharing one must be ordered on one stream. One launch, HIP-graph capturable;
- * out overlaps neither q nor the pool. */
+ * left zero by every call whatever its geometry; the rest, partial sums and in calls
+ * of more than 512 (row, head of a group) pairs the FP16 rows that packed and 8-bit pages
+ * stand for, 1 GiB of those at most, needs no contents); calls sharing one must be
+ * ordered on one stream. One launch for up to 512 such pairs, else three; where the rows
+ * of all sequences might take more than that GiB, sequences take turns, three launches each time.
+ * HIP-graph capturable; out overlaps neither q nor the pool. */
 #define BGTQ_PAGED_PREFILL_COUNTER_BYTES (64u * 1024u)
 typedef struct {
   int32_t q_heads, dtype, sequences;

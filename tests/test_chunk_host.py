@@ -33,7 +33,7 @@ BAD = [dict(q_heads=0), dict(q_heads=5), dict(q_heads=34), dict(dtype=_lib.DTYPE
        dict(scale=float("nan")), dict(scale=3e38), dict(window=-1), dict(sinks=1), dict(window=4, sinks=-1), dict(window=4, sinks=(1 << 30) + 1),
        dict(page_table_stride=3), dict(page_table_stride=-4), dict(offsets=None), dict(lengths=None), dict(page_table=None), dict(q=None),
        dict(out=None), dict(offsets=A + 2), dict(lengths=A + 1), dict(page_table=A + 2), dict(q=A + 8), dict(out=A + 2), dict(q_row_stride=-8),
-       dict(q_head_stride=4), dict(out_row_stride=380), dict(out_row_stride=320), dict(out_head_stride=56), dict(workspace=None),
+       dict(q_head_stride=4), dict(out_row_stride=380), dict(out_row_stride=320), dict(out_head_stride=56), dict(out=A), dict(workspace=None),
        dict(workspace=A + 8), dict(workspace_bytes=1000)]
 
 

@@ -358,6 +358,64 @@ def test_captured_and_on_another_stream(device, oracle):
     pool.destroy()
 
 
+@pytest.mark.parametrize("rows", [100, 2000])
+def test_offsets_out_of_order(device, oracle, rows):
+    """Offsets count as no less than those before them, whatever they hold."""
+    import torch
+    from bgtq import batched
+    rng = np.random.RandomState(9)
+    S = 70
+    lengths = [int(n) for n in rng.randint(1, 400, S)]
+    pool, table = _written(device, "B", "q8", 64, 2, 64, lengths, rng, 5)
+    q = _rows(rows, 4, 64, "bfloat16", 4, 3).cuda()
+    for kind in range(3):
+        given = rng.randint(-rows, 2 * rows, S + 1) if kind == 0 else np.where(np.arange(S + 1) % 2, rows, 0) if kind == 1 else -np.arange(S + 1)
+        meant = np.maximum.accumulate(np.clip(given, 0, rows))
+        args = dict(pages=pool.handle, q=q, offsets=torch.tensor(given, dtype=torch.int32, device="cuda"),
+                    lengths=torch.tensor(lengths, dtype=torch.int32, device="cuda"), page_table=table)
+        out = torch.full_like(q, 7.0)
+        size = batched.paged_prefill_workspace_bytes(batched.paged_prefill_desc(out=out, **args))
+        batched.paged_prefill(device, batched.paged_prefill_desc(out=out, workspace=torch.zeros(size, dtype=torch.uint8, device="cuda"), **args))
+        torch.cuda.synchronize()
+        _check(pool, oracle, q, out, list(np.diff(meant)), lengths, table, first=int(meant[0]))
+        assert bool((out[:meant[0]] == 7).all()) and bool((out[meant[-1]:] == 7).all())
+    pool.destroy()
+
+
+def test_two_calls_at_once(device, oracle):
+    """Two contexts on streams of their own over one pool, a workspace each."""
+    import bgtq
+    import torch
+    from bgtq import batched
+    rng = np.random.RandomState(10)
+    lengths = [3000, 700, 64]
+    pool, table = _written(device, "S", "q8", 64, 3, 64, lengths, rng, 5)
+    calls = []
+    for new in ([600, 1, 0], [1, 1, 20]):
+        q = _rows(sum(new), 9, 64, "float16", sum(new), 3).cuda()
+        calls.append((new, q, _call(pool, q, new, lengths, table)))
+    torch.cuda.synchronize()
+    others, descs = [], []
+    for new, q, _ in calls:
+        stream, ctx = torch.cuda.Stream(), bgtq.Device(0)
+        ctx.set_stream(stream.cuda_stream)
+        args = dict(pages=pool.handle, q=q, out=torch.zeros_like(q), offsets=torch.tensor(np.concatenate([[0], np.cumsum(new)]), dtype=torch.int32, device="cuda"),
+                    lengths=torch.tensor(lengths, dtype=torch.int32, device="cuda"), page_table=table)
+        size = batched.paged_prefill_workspace_bytes(batched.paged_prefill_desc(**args))
+        descs.append((args["out"], batched.paged_prefill_desc(workspace=torch.zeros(size, dtype=torch.uint8, device="cuda"), **args)))
+        others.append((ctx, stream))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for (ctx, _s), (_o, desc) in zip(others, descs):
+            batched.paged_prefill(ctx, desc)
+    torch.cuda.synchronize()
+    for (_n, _q, want), (got, _d) in zip(calls, descs):
+        assert torch.equal(want, got)
+    for ctx, _s in others:
+        ctx.destroy()
+    pool.destroy()
+
+
 def test_a_step_from_rows_to_outputs(device, oracle):
     """A layer's step as a serving loop runs it: rows rotated into the pages, then all chunks attended, then single
     tokens decoded behind a window, against 64 bits from the rows themselves with K as the pages hold it."""

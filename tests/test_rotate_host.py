@@ -72,6 +72,16 @@ def test_other_refusals():
     assert b"context" in L.bgtq_last_error()
 
 
+def test_q_and_k_that_overlap():
+    """One's rows are written where the other's are read or written."""
+    for q, k in ((_heads(), _heads()), (_heads(), _heads(src=8 * A)), (_heads(dst=8 * A), _heads(src=8 * A, dst=16 * A)),
+                 (_heads(src=16 * A, dst=8 * A), _heads(src=4 * A, dst=16 * A))):
+        assert _rotate(_rotation(), q=q, k=k) == _lib.ERR_RANGE
+        assert b"overlap" in _lib.lib().bgtq_last_error()
+    _rotate(_rotation(), q=_heads(), k=_heads(src=4 * A, dst=4 * A))
+    assert b"context" in _lib.lib().bgtq_last_error()
+
+
 @pytest.mark.parametrize("bad", [None, dict(window=0), dict(window=-1), dict(sinks=-1), dict(sinks=(1 << 30) + 1)], ids=str)
 def test_bad_windows(bad):
     L, n = _lib.lib(), ctypes.c_size_t()
