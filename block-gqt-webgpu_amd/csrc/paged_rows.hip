@@ -46,7 +46,7 @@ __host__ __device__ inline WriteLds write_lds(int enc_bytes) {
 }
 
 // Rot on: K rows are normed and rotated first, and one more slice of grid y
-// takes the queries. (Rotated FP16 rows at five waves per SIMD: 5003 rows of d=128 20.2 us, 20.8 at four.)
+// takes the queries. (Rotated FP16 rows at five waves per SIMD: 5003 rows of d=128, written and read back, 20.3 us, 21.4 at four.)
 template <int D, bool WITH_K, typename Rot>
 __global__ __launch_bounds__(kThreads, Rot::kOn && !WITH_K ? 5 : 1) void paged_write_kernel(PagedWriteParams p, Rot rotation) {
   constexpr int JL = row_enc::Lane<D>::JL, L8 = D / 8;
