@@ -119,9 +119,10 @@ struct PagedDst {
 };
 
 // Waves per SIMD that the register budget leaves room for (rotated rows: the
-// table row's 2 x D / 4 values are held too).
+// table row's 2 x D / 4 values are held too; four spilled 33 registers, 16384
+// rows 41.8 us, 33.6 at three).
 constexpr int tile_waves_per_simd(int D, bool src_f32, bool rotated = false) {
-  return D != 64 || rotated ? 2 : src_f32 ? 3 : 4;
+  return D != 64 ? 2 : rotated || src_f32 ? 3 : 4;
 }
 
 // One job: its packed and norms already point at its first destination row.
@@ -671,19 +672,26 @@ __global__ __launch_bounds__(64 * tile_waves(D), tile_waves_per_simd(D, SRC_F32)
 // K rows into pages, a KV head per grid y; the workgroups share the head's V
 // rows too (16384 rows x 2 heads written and read back 20.6 us, with V in a launch
 // of its own 21.6).
-// Rot on: K rows are normed and rotated first; the workgroups share the queries too.
+// Rot on: K rows are normed and rotated first, and one more slice of grid y
+// takes the queries, beside the encoding workgroups where the chip holds both, two items
+// ahead (16384 rows of 14 + 2 heads, written and read back: shared by those 33.6
+// us; a slice one, two and four items at a time 31.3, 29.8 and 31.2).
 template <int D, int SRC, typename Rot>
 __global__ __launch_bounds__(64 * tile_waves(D), tile_waves_per_simd(D, SRC == BGTQ_DTYPE_F32, Rot::kOn)) void encode_tile_paged_kernel(
     PagedWriteParams p, Rot rotation, int max_codebooks, int max_groups, int max_row_bytes) {
   const int h = blockIdx.y;
+  if constexpr (Rot::kOn) {
+    if (h == p.kv_heads) {
+      rot::rotate_queries<D, 64 * tile_waves(D), 2>(rotation, p.slots.rows, blockIdx.x, gridDim.x);
+      return;
+    }
+  }
   const EncodeTileJob job{p.tables[h], static_cast<const uint8_t *>(p.k) + h * p.k_head_stride * (SRC == BGTQ_DTYPE_F32 ? 4 : 2),
                           p.packed + h * p.packed_head_stride, p.norms + h * p.norms_head_stride, (int32_t)p.k_row_stride, 0};
   const PagedDst<Rot> place{p.slots, p.packed_page_stride, p.norms_page_stride, rotation};
   constexpr int kThreads = 64 * tile_waves(D), kLanes = D / 8;
   write_rows<D, false>(p, h, (int64_t)blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes,
                        (int64_t)gridDim.x * (kThreads / kLanes), rotation);
-  if constexpr (Rot::kOn)
-    rot::rotate_queries<D, kThreads>(rotation, p.slots.rows, (int64_t)h * gridDim.x + blockIdx.x, (int64_t)gridDim.x * gridDim.y);
   encode_tile_body<D, SRC, true, PagedDst<Rot>>(job, p.slots.rows, max_codebooks, max_groups, max_row_bytes, place, rotation);
 }
 
@@ -751,7 +759,8 @@ hipError_t launch_encode_tile_paged(const PagedWriteParams &p, const Rotation *r
                                     const EncodeTileSizes &z, hipStream_t stream) {
   const int64_t wg_rows = encode_tile_wg_rows(dim), most = (p.slots.rows + wg_rows - 1) / wg_rows;
   const int64_t resident = resident_of(dim, tile_waves_per_simd(dim, p.k_dtype == BGTQ_DTYPE_F32, rotation != nullptr), cus, z);
-  const dim3 grid((unsigned)std::max<int64_t>(1, std::min<int64_t>(most, resident / p.kv_heads)), (unsigned)p.kv_heads);
+  const dim3 grid((unsigned)std::max<int64_t>(1, std::min<int64_t>(most, resident / p.kv_heads)),
+                  (unsigned)p.kv_heads + (rotation && rotation->q ? 1u : 0u));
   if (rotation)
     return dim == 64 ? launch_paged_src<64>(p, *rotation, grid, z, stream) : launch_paged_src<128>(p, *rotation, grid, z, stream);
   return dim == 64 ? launch_paged_src<64>(p, NoRotation{}, grid, z, stream)

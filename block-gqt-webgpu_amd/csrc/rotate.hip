@@ -9,8 +9,9 @@ namespace {
 
 constexpr int kThreads = 256;
 
+// (Eight waves per SIMD: 16384 rows of 14 + 2 heads 13.6 us; the compiler's own four 14.6.)
 template <int D>
-__global__ __launch_bounds__(kThreads) void rotate_kernel(Rotation q, Rotation k, int64_t rows) {
+__global__ __launch_bounds__(kThreads, 8) void rotate_kernel(Rotation q, Rotation k, int64_t rows) {
   if (blockIdx.y == 0) rot::rotate_queries<D, kThreads>(q, rows, blockIdx.x, gridDim.x);
   else rot::rotate_queries<D, kThreads>(k, rows, blockIdx.x, gridDim.x);
 }

@@ -14,6 +14,7 @@ namespace rot {
 typedef _Float16 half2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
+using gfx::u32x4;
 
 struct HeadRows {
   const void *src;
@@ -26,26 +27,32 @@ struct HeadRows {
 template <int DTYPE>
 constexpr int kPer = DTYPE == BGTQ_DTYPE_F32 ? 4 : 8;  // values of 16 bytes
 
-// N values from element `at` on, as FP32; vec: in one 16-byte access.
-template <int DTYPE, int N>
-__device__ __forceinline__ void load_values(const void *src, int64_t at, bool vec, float (&x)[N]) {
-  uint32_t w[4];
+// 16 bytes of values from element `at` on; vec: in one access.
+template <int DTYPE>
+__device__ __forceinline__ u32x4 load_words(const void *src, int64_t at, bool vec) {
+  u32x4 w;
   if constexpr (DTYPE == BGTQ_DTYPE_F32) {
     const uint32_t *p = static_cast<const uint32_t *>(src) + at;
-    if (vec) __builtin_memcpy(w, __builtin_assume_aligned(p, 16), 16);
+    if (vec) w = *reinterpret_cast<const u32x4 *>(p);
     else
 #pragma unroll
       for (int k = 0; k < 4; ++k) w[k] = p[k];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) x[k] = __uint_as_float(w[k]);
   } else {
     const uint16_t *p = static_cast<const uint16_t *>(src) + at;
-    if (vec) __builtin_memcpy(w, __builtin_assume_aligned(p, 16), 16);
+    if (vec) w = *reinterpret_cast<const u32x4 *>(p);
     else
 #pragma unroll
       for (int k = 0; k < 4; ++k) w[k] = (uint32_t)p[2 * k] | (uint32_t)p[2 * k + 1] << 16;
+  }
+  return w;
+}
+template <int DTYPE, int N>
+__device__ __forceinline__ void values_of(u32x4 w, float (&x)[N]) {
 #pragma unroll
-    for (int k = 0; k < N; ++k) {
+  for (int k = 0; k < N; ++k) {
+    if constexpr (DTYPE == BGTQ_DTYPE_F32) {
+      x[k] = __uint_as_float(w[k]);
+    } else {
       const uint32_t u = k & 1 ? w[k >> 1] >> 16 : w[k >> 1] & 0xffffu;
       x[k] = DTYPE == BGTQ_DTYPE_F16 ? row_enc::f16_bits_to_f32((uint16_t)u) : __uint_as_float(u << 16);
     }
@@ -77,8 +84,9 @@ __device__ __forceinline__ void store_values(void *dst, int64_t at, bool vec, co
 }
 
 // Items first, first + step, ... of rows [row0, row0 + rows) x heads, a
-// group of lanes each; `sub` is this lane's place in its group.
-template <int D, int DTYPE>
+// group of lanes each; `sub` is this lane's place in its group. U: items whose loads are in
+// flight together, where few waves share a SIMD.
+template <int D, int DTYPE, int U>
 __device__ __forceinline__ void rotate_items(const HeadRows &h, const Rotation &r, int64_t row0, int rows, uint32_t first,
                                              uint32_t step, int sub) {
   constexpr int N = kPer<DTYPE>, L = D / (2 * N), E = DTYPE == BGTQ_DTYPE_F32 ? 4 : 2;
@@ -87,50 +95,61 @@ __device__ __forceinline__ void rotate_items(const HeadRows &h, const Rotation &
   };
   const bool vin = aligned(h.src, h.src_row, h.src_head), vout = aligned(h.dst, h.dst_row, h.dst_head);
   const uint32_t n = (uint32_t)rows * (uint32_t)h.heads;
-  for (uint32_t i = first; i < n; i += step) {
-    const uint32_t local = i / (uint32_t)h.heads;
-    const int head = (int)(i - local * (uint32_t)h.heads);
-    const int64_t row = row0 + local;
-    const int64_t from = row * h.src_row + head * h.src_head + N * sub;
-    float a[N], b[N];
-    load_values<DTYPE>(h.src, from, vin, a);
-    load_values<DTYPE>(h.src, from + D / 2, vin, b);
-    const float *cs;
-    const bool ok = r.find(row, cs, D);
-    float c[N], s[N];
+  for (uint32_t i0 = first; i0 < n; i0 += U * step) {
+    int64_t row[U];
+    int head[U];
+    u32x4 raw[U][2];
+    const float *cs[U];
+    bool ok[U];
 #pragma unroll
-    for (int k = 0; k < N; ++k) {
-      c[k] = cs[N * sub + k];
-      s[k] = cs[D / 2 + N * sub + k];
+    for (int u = 0; u < U; ++u) {
+      const uint32_t i = U == 1 ? i0 : min(i0 + u * step, n - 1), local = i / (uint32_t)h.heads;
+      head[u] = (int)(i - local * (uint32_t)h.heads);
+      row[u] = row0 + local;
+      const int64_t from = row[u] * h.src_row + head[u] * h.src_head + N * sub;
+      raw[u][0] = load_words<DTYPE>(h.src, from, vin);
+      raw[u][1] = load_words<DTYPE>(h.src, from + D / 2, vin);
+      ok[u] = r.find(row[u], cs[u], D) && (U == 1 || i0 + u * step < n);
     }
-    if (h.weight) {
-      double sum = 0.0;
 #pragma unroll
-      for (int k = 0; k < N; ++k) sum = add_square(b[k], add_square(a[k], sum));
-      const float f = factor(lanes_sum<L>(sum), D, r.eps);
-      // (weights loaded ahead of the loop cost 13%: 16384 rows 14.0 / 15.8 us)
+    for (int u = 0; u < U; ++u) {
+      float a[N], b[N], c[N], s[N];
+      values_of<DTYPE>(raw[u][0], a);
+      values_of<DTYPE>(raw[u][1], b);
 #pragma unroll
       for (int k = 0; k < N; ++k) {
-        a[k] = (a[k] * f) * h.weight[N * sub + k];
-        b[k] = (b[k] * f) * h.weight[D / 2 + N * sub + k];
+        c[k] = cs[u][N * sub + k];
+        s[k] = cs[u][D / 2 + N * sub + k];
       }
-    }
-    float y[N], z[N];
+      if (h.weight) {
+        double sum = 0.0;
 #pragma unroll
-    for (int k = 0; k < N; ++k) {
-      y[k] = turn(a[k], b[k], c[k], s[k], false);
-      z[k] = turn(b[k], a[k], c[k], s[k], true);
+        for (int k = 0; k < N; ++k) sum = add_square(b[k], add_square(a[k], sum));
+        const float f = factor(lanes_sum<L>(sum), D, r.eps);
+        // (weights loaded ahead of the loop cost 13%: 16384 rows 14.0 / 15.8 us)
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+          a[k] = (a[k] * f) * h.weight[N * sub + k];
+          b[k] = (b[k] * f) * h.weight[D / 2 + N * sub + k];
+        }
+      }
+      float y[N], z[N];
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        y[k] = turn(a[k], b[k], c[k], s[k], false);
+        z[k] = turn(b[k], a[k], c[k], s[k], true);
+      }
+      if (!ok[u]) continue;
+      const int64_t to = row[u] * h.dst_row + head[u] * h.dst_head + N * sub;
+      store_values<DTYPE>(h.dst, to, vout, y);
+      store_values<DTYPE>(h.dst, to + D / 2, vout, z);
     }
-    if (!ok) continue;
-    const int64_t to = row * h.dst_row + head * h.dst_head + N * sub;
-    store_values<DTYPE>(h.dst, to, vout, y);
-    store_values<DTYPE>(h.dst, to + D / 2, vout, z);
   }
 }
 
 // The same for a dtype known at run time, shared by the TH threads of the
 // workgroups `wg` of `wgs`: each takes a run of whole rows.
-template <int D, int TH>
+template <int D, int TH, int U = 1>
 __device__ __forceinline__ void rotate_queries(const Rotation &r, int64_t rows, int64_t wg, int64_t wgs) {
   if (!r.q) return;
   const HeadRows h{r.q, r.q_out, r.q_heads, r.q_row_stride, r.q_head_stride, r.q_out_row_stride, r.q_out_head_stride, r.q_norm};
@@ -139,7 +158,7 @@ __device__ __forceinline__ void rotate_queries(const Rotation &r, int64_t rows, 
     // (a run of rows holds at most 2^16 items of a 32-bit count, and one row any number of heads)
     const int64_t run = max((int64_t)1, min((rows + wgs - 1) / wgs, (int64_t)(65536 / r.q_heads)));
     for (int64_t row0 = wg * run; row0 < rows; row0 += wgs * run)
-      rotate_items<D, DT>(h, r, row0, (int)min(run, rows - row0), threadIdx.x / L, TH / L, threadIdx.x % L);
+      rotate_items<D, DT, U>(h, r, row0, (int)min(run, rows - row0), threadIdx.x / L, TH / L, threadIdx.x % L);
   };
   if (r.q_dtype == BGTQ_DTYPE_F32) go(std::integral_constant<int, BGTQ_DTYPE_F32>{});
   else if (r.q_dtype == BGTQ_DTYPE_F16) go(std::integral_constant<int, BGTQ_DTYPE_F16>{});
