@@ -1,6 +1,6 @@
 // Attention of chunks over the paged cache (bgtq_paged_prefill): which item of
 // work a workgroup has, and a wave's part in one: 32 query columns against
-// blocks of K and V rows in LDS. chunk_kernel.h and chunk_wide.h have the kernels.
+// blocks of K and V rows in LDS. chunk_rows.h and chunk_wide.hip have the kernels.
 //
 // The products, the softmax and its lazy rescale are prompt.hip's: S^T = K Q^T
 // in 32x32x16 products leaves a lane one query's logits, and probabilities in
