@@ -94,7 +94,11 @@ __global__ __launch_bounds__((64 * Wide<D, SRC, BF>::W), (Wide<D, SRC, BF>::PER_
     } else {
       bool ok = true;
 #pragma unroll 4
-      for (int i = b0; i < b1; i += 32) ok &= (uint32_t)entry_of(i + (lane & 31), lane >> 5) < (uint32_t)p.pages;
+      for (int i = b0; i < b1; i += 32) {
+        const int at = i + (lane & 31);
+        // (a half behind the sequence's tokens is seen by nobody, and its entry may be anything)
+        ok &= (uint32_t)entry_of(at, lane >> 5) < (uint32_t)p.pages || bl.at<kChunkKeys>(min(at, b1 - 1)) + 32 * (lane >> 5) >= it.n;
+      }
       none_missing = __builtin_amdgcn_ballot_w64(!ok) == 0;
     }
   }

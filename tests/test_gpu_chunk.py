@@ -382,6 +382,40 @@ def test_offsets_out_of_order(device, oracle, rows):
     pool.destroy()
 
 
+@pytest.mark.parametrize("layout,v,dim", [("f16", "f16", 128), ("B", "q8", 64)])
+def test_pages_beyond_32_bits(device, layout, v, dim):
+    """Pages several hundred million entries apart: the same bits as from a compact pool."""
+    import torch
+    from bgtq import batched
+    rows, got = 700, []
+    k, val = _rows(rows, 1, dim, "bfloat16", 1, 1).cuda(), _rows(rows, 1, dim, "bfloat16", 1, 2).cuda()
+    q = _rows(rows, 4, dim, "bfloat16", 1, 3).cuda()
+    rope = batched.rope(table=batched.rope_table(1000, dim, 1e4))
+    positions = torch.arange(rows, device="cuda")
+    table = torch.tensor(np.random.RandomState(1).permutation(12)[None], dtype=torch.int32, device="cuda")
+    slots = table[0].long()[positions // 64] * 64 + positions % 64
+    for gap in (32, 400_000_000):
+        pool = Pool(device, layout, v, dim, 1, 12, 64, gap=gap)
+        qr = torch.empty_like(q)
+        batched.paged_append(device, pool.handle, slots, rope, positions, k, val, q=q, q_out=qr)
+        outs = [qr]
+        for new in (5, 300):
+            for window, sinks in ((0, 0), (100, 5)):
+                outs.append(_call(pool, qr[rows - new:].contiguous(), [new], [rows], table, window, sinks))
+        q1, o1 = qr[-1:].float().contiguous(), torch.empty((1, 4, dim), device="cuda")
+        args = dict(pages=pool.handle, q=q1, out=o1, lengths=torch.tensor([rows], dtype=torch.int32, device="cuda"), page_table=table, window=200, sinks=4)
+        ws = torch.zeros(batched.paged_decode_workspace_bytes(batched.paged_decode_desc(**args)), dtype=torch.uint8, device="cuda")
+        batched.paged_decode(device, batched.paged_decode_desc(workspace=ws, **args))
+        kr, vr = torch.empty_like(k), torch.empty_like(val)
+        batched.paged_read(device, pool.handle, slots, kr, vr)
+        torch.cuda.synchronize()
+        got.append([t.clone() for t in (*outs, o1, kr, vr)])
+        pool.destroy()
+        del pool
+    for a, b in zip(*got):
+        assert torch.equal(a, b) and bool(a.isfinite().all())
+
+
 def test_two_calls_at_once(device, oracle):
     """Two contexts on streams of their own over one pool, a workspace each."""
     import bgtq
