@@ -309,26 +309,28 @@ def rope(*, table, q_norm=None, k_norm=None, eps=1e-6) -> Rope:
 
 def _head_rows(index, name, t, out, rows, dim):
     """bgtq_head_rows of t [rows, heads, dim] and where it goes (None: in place)."""
-    out = t if out is None else out
-    code = _codes().get(t.dtype)
-    if code is None or t.dim() != 3 or t.shape[0] != rows or t.shape[2] != dim or t.get_device() != index:
+    shape, code = t.shape, _codes().get(t.dtype)
+    if code is None or len(shape) != 3 or shape[0] != rows or shape[2] != dim or t.get_device() != index:
         raise RangeError(f"{name} must be a [rows, heads, dim] tensor of float32, float16 or bfloat16 on the context's device")
-    if out.dtype != t.dtype or out.shape != t.shape or out.get_device() != index:
-        raise RangeError(f"{name} and its output must agree in shape, dtype and device")
-    s, o = t.stride(), out.stride()
+    s, src = t.stride(), t.data_ptr()
+    o, dst = s, src
+    if out is not None:
+        if out.dtype != t.dtype or out.shape != shape or out.get_device() != index:
+            raise RangeError(f"{name} and its output must agree in shape, dtype and device")
+        o, dst = out.stride(), out.data_ptr()
     if s[2] != 1 or o[2] != 1:
         raise RangeError(f"{name}'s last dimension must be dense")
-    several, heads = rows > 1, t.shape[1]
-    return _lib.HeadRows(t.data_ptr(), out.data_ptr(), heads, code, s[0] if several else 0, s[1] if heads > 1 else 0,
-                         o[0] if several else 0, o[1] if heads > 1 else 0)
+    heads = shape[1]
+    rs, ro = (s[0], o[0]) if rows > 1 else (0, 0)
+    hs, ho = (s[1], o[1]) if heads > 1 else (0, 0)
+    return _lib.HeadRows(src, dst, heads, code, rs, hs, ro, ho)
 
 
-def _positions(device, rope, positions):
+def _positions(index, rope, positions):
     """The number of rows, checked."""
-    index = device.index
-    _need(rope.device_index == index, "the rotation must lie on the context's device")
+    if rope.device_index != index:
+        raise RangeError("the rotation must lie on the context's device")
     _dense(index, "positions", positions, "int64", 1)
-    _need(positions.is_contiguous(), "positions must be contiguous")
     return positions.shape[0]
 
 
@@ -336,26 +338,27 @@ def rotate(device, rope, positions, q=None, k=None, q_out=None, k_out=None) -> N
     """bgtq_rotate: rows q [n, Hq, dim] and k [n, Hkv, dim] (FP32, FP16 or BF16, any strides of the first two
     dimensions) at positions [n] int64 normed and rotated into q_out and k_out (None: in place); rows whose position
     is none of the table's are left out."""
-    n = _positions(device, rope, positions)
+    index, dim = device.index, rope.dim
+    n = _positions(index, rope, positions)
     _need(q is not None or k is not None, "rotate needs q or k")
-    rows = [None if t is None else ctypes.byref(_head_rows(device.index, name, t, out, n, rope.dim))
-            for name, t, out in (("q", q, q_out), ("k", k, k_out))]
+    qr = None if q is None else ctypes.byref(_head_rows(index, "q", q, q_out, n, dim))
+    kr = None if k is None else ctypes.byref(_head_rows(index, "k", k, k_out, n, dim))
     if n:
-        check(lib().bgtq_rotate(device.handle, rope.ref, rope.dim, n, _addr(positions), *rows))
+        check(lib().bgtq_rotate(device.handle, rope.ref, dim, n, positions.data_ptr(), qr, kr))
 
 
 def paged_append(device, pool, slots, rope, positions, k, v, q=None, q_out=None) -> None:
     """bgtq_paged_append: rows k, v [n, Hkv, dim] of a step into the slots [n] int64, k normed and rotated to positions
     [n] int64 on the way, and the step's queries q [n, Hq, dim] (None: none) into q_out (None: in place). Rows of
     slots outside the pool, or of positions outside the table, are not written."""
-    n = _positions(device, rope, positions)
+    n = _positions(device.index, rope, positions)
     _need(pool.dim == rope.dim, "the pool's heads and the rotation must agree in dim")
     _need(k is not None and v is not None, "paged_append needs k and v")
     r = _paged_rows(device, pool, slots, k, v)
     _need(r.rows == n, "slots and positions must have an entry per row")
     queries = None if q is None else ctypes.byref(_head_rows(device.index, "q", q, q_out, n, rope.dim))
     if n:
-        check(lib().bgtq_paged_append(device.handle, pool.ref, ctypes.byref(r), rope.ref, _addr(positions), queries))
+        check(lib().bgtq_paged_append(device.handle, pool.ref, ctypes.byref(r), rope.ref, positions.data_ptr(), queries))
 
 
 def _window(window, sinks):
