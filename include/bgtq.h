@@ -493,7 +493,8 @@ bgtq_status bgtq_rotate(bgtq_context *ctx, const bgtq_rotation *r, int32_t dim, 
  * rotated as bgtq_rotate does in FP32, rounded to FP16 and encoded, V written as it
  * is; rows whose position is none of the table's are skipped as those of slots
  * outside the pool are. The same pool bit for bit as bgtq_rotate of K into FP32
- * rows and bgtq_paged_write of them. q (may be NULL): queries of the same rows,
+ * rows and bgtq_paged_write of them (with norms, but for one row in 2^27 or so, whose
+ * factor lies so near the middle of two FP32 values that the order of its sum decides). q (may be NULL): queries of the same rows,
  * rotated as bgtq_rotate does, also those whose slot lies outside the pool. One
  * launch, HIP-graph capturable. */
 bgtq_status bgtq_paged_append(bgtq_context *ctx, const bgtq_pages *pages, const bgtq_paged_rows *rows, const bgtq_rotation *r,

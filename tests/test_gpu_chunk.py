@@ -416,6 +416,27 @@ def test_pages_beyond_32_bits(device, layout, v, dim):
         assert torch.equal(a, b) and bool(a.isfinite().all())
 
 
+@pytest.mark.parametrize("layout,v,dim,heads", [("S", "q8", 64, 3), ("f16", "f16", 128, 2)])
+def test_shared_and_large_pages(device, oracle, layout, v, dim, heads):
+    """Sequences that share their first pages; pages of 4096 tokens; no sequences; sequences without rows."""
+    import torch
+    from bgtq import batched
+    rng = np.random.RandomState(11)
+    pool, table = _written(device, layout, v, dim, heads, 4096, [6000, 4096], rng, 5)
+    table = table[[0, 0, 1, 0]].contiguous()
+    new, lengths = [50, 1, 200, 7], [6000, 4500, 4096, 3000]
+    q = _rows(sum(new), 2 * heads, dim, "bfloat16", 4, 3).cuda()
+    for window, sinks in ((0, 0), (4100, 10)):
+        out = _call(pool, q, new, lengths, table, window, sinks)
+        torch.cuda.synchronize()
+        _check(pool, oracle, q, out, new, lengths, table, window, sinks)
+    out = _call(pool, q, [0, 0, 0, 0], lengths, table)
+    none = _call(pool, q, [], [], table[:0])
+    torch.cuda.synchronize()
+    assert bool(out.isnan().all()) and bool(none.isnan().all())
+    pool.destroy()
+
+
 def test_two_calls_at_once(device, oracle):
     """Two contexts on streams of their own over one pool, a workspace each."""
     import bgtq

@@ -91,6 +91,42 @@ def test_unaligned_strided_and_left_out(device):
             assert flat_rows.shape == dst.shape
 
 
+def test_many_heads(device):
+    """More items in a few rows than a workgroup's run of 65536 holds."""
+    import torch
+    from bgtq import batched
+    batched.bind_torch_stream(device)
+    rope, w = _rope(64, True)
+    for rows, heads in ((3, 5000), (2, 40000), (70, 1500)):
+        x = _rows(rows, heads, 64, "bfloat16", 5).cuda()
+        positions, out = torch.arange(rows, device="cuda") * 70, torch.empty_like(x)
+        batched.rotate(device, rope, positions, q=x, q_out=out)
+        torch.cuda.synchronize()
+        _check(out, x, w[0], rope, positions, f"{rows} rows of {heads} heads")
+
+
+def test_append_of_mixed_types(device):
+    """K, V and queries each of a type of its own."""
+    import torch
+    from bgtq import batched
+    batched.bind_torch_stream(device)
+    rope, w = _rope(64, True)
+    for layout, rows in (("B", 5), ("B", 9000), ("f16", 300)):
+        one, two = (Pool(device, layout, "q8", 64, 2, rows // 4096 + 2, 4096) for _ in range(2))
+        k, v, q = _rows(rows, 2, 64, "float32", 1).cuda(), _rows(rows, 2, 64, "float16", 2).cuda(), _rows(rows, 6, 64, "bfloat16", 3).cuda()
+        slots, positions = torch.arange(rows, device="cuda") + 7, torch.arange(rows, device="cuda") % 5000
+        q_out, k32 = torch.empty_like(q), torch.empty_like(k)
+        batched.paged_append(device, one.handle, slots, rope, positions, k, v, q, q_out)
+        batched.rotate(device, rope, positions, k=k, k_out=k32)
+        batched.paged_write(device, two.handle, slots, k32, v)
+        torch.cuda.synchronize()
+        _check(q_out, q, w[0], rope, positions, "q")
+        for a, b in zip(one.snapshot(), two.snapshot()):
+            assert a is None or _same_bits(a, b)
+        one.destroy()
+        two.destroy()
+
+
 def test_infinities_and_zero_rows(device):
     """A row of zeros stays zero under a norm; an infinity reaches its pair, NaN only where arithmetic makes one."""
     import torch
