@@ -2091,6 +2091,8 @@ static bgtq_status chunk_params(const bgtq_pages *g, const bgtq_paged_prefill_de
   p.group = d->q_heads / g->kv_heads;
   p.tokens = d->tokens;
   p.max_length = (int32_t)d->max_length;
+  p.window = std::min(d->window, 1 << 25);  // (past every position; positions less it stay within 32 bits)
+  p.sinks = std::min(d->sinks, 1 << 25);
   if (d->tokens * p.group > INT32_MAX) return fail(BGTQ_ERR_UNSUPPORTED, "paged prefill: too many (row, head) pairs for one call");
   *plan = plan_chunks(p, g->dim, g->key_format == BGTQ_KEYS_PACKED, g->v_format == BGTQ_DTYPE_Q8, d->dtype == BGTQ_DTYPE_BF16, device_cus());
   // (a launch counts its work-items in 32 bits)
@@ -2153,8 +2155,6 @@ bgtq_status bgtq_paged_prefill(bgtq_context *ctx, const bgtq_pages *g, const bgt
   p.q_row = d->q_row_stride, p.q_head = d->q_head_stride;
   p.out_row = d->out_row_stride, p.out_head = d->out_head_stride;
   p.c = (d->scale > 0.0f ? d->scale : (float)(1.0 / std::sqrt((double)g->dim))) * 1.4426950408889634f;
-  p.window = std::min(d->window, 1 << 25);  // (past every position; positions less it stay within 32 bits)
-  p.sinks = std::min(d->sinks, 1 << 25);
   const bgtq_paged_rows no_rows{};
   const PagedWriteParams w = rows_params(g, &no_rows);
   if (g->key_format == BGTQ_KEYS_PACKED) {

@@ -23,7 +23,11 @@ ChunkPlan plan_chunks(const ChunkParams &p, int dim, bool packed, bool q8, bool 
   const bool narrow_splits = kChunkSetup + kChunkNarrow * blocks > kChunkLeastNarrow, wide_splits = kChunkSetup + kChunkWide * blocks > kChunkLeast;
   c.narrow_aim = cus;
   const bool all_narrow = columns <= kChunkSmall;
-  c.narrow_items = (S + (all_narrow ? columns / 32 : 0)) * H + (narrow_splits ? c.narrow_aim : 0);
+  // (as many workgroups as units and splits can be: those without an item are ahead of the rebuilding ones)
+  const int64_t narrow_units = (S + (all_narrow ? columns / 32 : 0)) * H;
+  const int64_t narrow_blocks = p.window ? std::min(blocks, ((int64_t)p.window + 34 + p.sinks) / kChunkKeys + 3) : blocks;
+  const int64_t most_splits = std::max<int64_t>(1, (kChunkSetup + kChunkNarrow * narrow_blocks + kChunkLeastNarrow - 1) / kChunkLeastNarrow);
+  c.narrow_items = std::min(narrow_units + (narrow_splits ? c.narrow_aim : 0), narrow_units * most_splits);
   const int64_t narrow_bytes = narrow_splits ? 2 * (int64_t)c.narrow_aim * 32 * (dim + 2) * 4 : 0;
   c.part_bytes = narrow_bytes;
   c.wide_sequences = all_narrow ? 0 : std::min<int64_t>(S, columns / 33);
@@ -74,7 +78,7 @@ hipError_t launch_chunks(const ChunkParams &params, const ChunkPlan &plan, int d
     p.two_rounds = plan.two_rounds;
     p.slot_columns = (int32_t)std::min<int64_t>(plan.wide_columns, (p.tokens * p.group + 31) / 32 * 32);
     if (hipError_t e = launch_chunk_wide(p, dim, bf16, (int)plan.wide_items, stream)) return e;
-    return plan.slots ? launch_chunk_merge(p, dim, bf16, plan.wide_columns, (int)plan.slots, stream) : hipSuccess;
+    return plan.slots ? launch_chunk_merge(p, dim, bf16, plan.wide_columns, (int)std::min(plan.slots, plan.wide_items), stream) : hipSuccess;
   };
   if (!plan.wide_sequences) return rows(plan.narrow_items, false, false);
   const bool rebuild = plan.rebuilt_rows > 0;
