@@ -41,6 +41,7 @@ struct ChunkParams {
   const int32_t *page_table;
   int64_t page_table_stride;
   int32_t sequences, kv_heads, group;  // KV heads; query heads per KV head
+  int32_t ahead;                       // sequences of the call before these (their offsets lie before)
   int64_t tokens;
   int32_t max_length, page_shift, table_pages, pages;
   const uint16_t *q;

@@ -91,6 +91,7 @@ hipError_t launch_chunks(const ChunkParams &params, const ChunkPlan &plan, int d
     p.offsets = params.offsets + s;
     p.lengths = params.lengths + s;
     p.page_table = params.page_table + s * p.page_table_stride;
+    p.ahead = (int32_t)s;
     p.sequences = (int32_t)std::min<int64_t>(plan.group, params.sequences - s);
     if (hipError_t e = rows(0, false, true)) return e;
     if (hipError_t e = wide()) return e;

@@ -451,7 +451,7 @@ __device__ __forceinline__ void rebuild_rows(const ChunkParams &p, uint8_t *smem
   int64_t base = 0, at = (int64_t)(wg / p.kv_heads) * kChunkWaves + wave;  // blocks before these sequences; this wave's next
   R::books(p, kv, smem);
   lds_barrier();
-  int before = 0;
+  int before = offset_ahead(p);
   for (int s0 = 0; s0 < p.sequences; s0 += 64) {
     const SequencePlan q = plan_of(p, s0 + lane, kWideUnits, 32, before);
     const int count = rebuilt_rows(q) / 32, end = wave_prefix(count), all = __builtin_amdgcn_readlane(end, 63);

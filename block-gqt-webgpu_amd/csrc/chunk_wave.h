@@ -125,6 +125,12 @@ struct SequencePlan {
   bool wide;
   float cost;
 };
+// What the offsets of the sequences ahead of a group's come to.
+__device__ __forceinline__ int offset_ahead(const ChunkParams &p) {
+  int most = 0;
+  for (int i = (int)(threadIdx.x & 63) - p.ahead; i < 0; i += 64) most = max(most, min(p.offsets[i], (int)p.tokens));
+  return __builtin_amdgcn_readlane(wave_prefix_max(most), 63);
+}
 // The offsets count as no less than those before them (`before`: the sequences' ahead of these 64), so that
 // whatever they hold, the chunks are `tokens` rows at most, which the host's counts go by.
 __device__ __forceinline__ SequencePlan plan_of(const ChunkParams &p, int s, int which, int tile, int &before) {
@@ -179,7 +185,8 @@ __device__ __forceinline__ Item find_item(const ChunkParams &p, int item, int wh
   const int lane = threadIdx.x & 63;
   float all = 0.0f;
   SequencePlan q{};
-  int before = 0;
+  const int ahead = offset_ahead(p);
+  int before = ahead;
   for (int s0 = 0; s0 < p.sequences; s0 += 64) {
     q = plan_of(p, s0 + lane, which, tile, before);
     all += wave_sum_f((float)q.units * q.cost);
@@ -205,7 +212,7 @@ __device__ __forceinline__ Item find_item(const ChunkParams &p, int item, int wh
   }
   int first = 0, slots = 0;
   int64_t base = 0;
-  before = 0;
+  before = ahead;
   for (int s0 = 0; s0 < p.sequences; s0 += 64) {
     if (p.sequences > 64) q = plan_of(p, s0 + lane, which, tile, before);
     const int splits = splits_of(q, share), items = BY_SLOT && splits < 2 ? 0 : splits * q.units, rebuilt = rebuilt_rows(q);

@@ -7,7 +7,7 @@
 // rebuilt (contiguous, in the code domain).
 //
 // Measured: 2048 rows behind 30720 tokens, 14 / 2 heads of d=64 in BF16: 300 to 340 us
-// of a call's 318 to 326 (the clocks differ), 690 to 780 TFLOP/s; prompt.hip reaches 715
+// of a call's 312 to 330 (the clocks differ), 690 to 780 TFLOP/s; prompt.hip reaches 715
 // on d=64. A wave's block is 290 instructions, 1100 cycles of the vector unit's, beside 512
 // of products: 204 us of this call at four waves per SIMD without a stall. The
 // rest is set-up, partials (69 MB, read back by the merge in 22 us) and the last

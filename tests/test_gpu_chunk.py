@@ -358,21 +358,21 @@ def test_captured_and_on_another_stream(device, oracle):
     pool.destroy()
 
 
-@pytest.mark.parametrize("rows", [100, 2000])
-def test_offsets_out_of_order(device, oracle, rows):
-    """Offsets count as no less than those before them, whatever they hold."""
+@pytest.mark.parametrize("rows,max_length", [(100, 1024), (2000, 1024), (2000, 1 << 17)])
+def test_offsets_out_of_order(device, oracle, rows, max_length):
+    """Offsets count as no less than those before them, whatever they hold; also where the sequences take turns."""
     import torch
     from bgtq import batched
     rng = np.random.RandomState(9)
     S = 70
     lengths = [int(n) for n in rng.randint(1, 400, S)]
-    pool, table = _written(device, "B", "q8", 64, 2, 64, lengths, rng, 5)
+    pool, table = _written(device, "B", "q8", 64, 2, 64, lengths, rng, 5, spare=max_length // 64)
     q = _rows(rows, 4, 64, "bfloat16", 4, 3).cuda()
     for kind in range(3):
         given = rng.randint(-rows, 2 * rows, S + 1) if kind == 0 else np.where(np.arange(S + 1) % 2, rows, 0) if kind == 1 else -np.arange(S + 1)
         meant = np.maximum.accumulate(np.clip(given, 0, rows))
         args = dict(pages=pool.handle, q=q, offsets=torch.tensor(given, dtype=torch.int32, device="cuda"),
-                    lengths=torch.tensor(lengths, dtype=torch.int32, device="cuda"), page_table=table)
+                    lengths=torch.tensor(lengths, dtype=torch.int32, device="cuda"), page_table=table, max_length=max_length)
         out = torch.full_like(q, 7.0)
         size = batched.paged_prefill_workspace_bytes(batched.paged_prefill_desc(out=out, **args))
         batched.paged_prefill(device, batched.paged_prefill_desc(out=out, workspace=torch.zeros(size, dtype=torch.uint8, device="cuda"), **args))
