@@ -39,6 +39,14 @@ __device__ __forceinline__ uint32_t pack_out(float a, float b) {
   if constexpr (BF) return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
   else return pack2(a, b);
 }
+// A K value's pair: high part rounded to nearest, low part times 2^11, so that it keeps 11 bits however small the value is
+// (as it is, it would end at 2^-24: of rows of a scale of 2^-12 a pair had 13 bits in all). |x| at most 65504.
+constexpr float kLowUp = 2048.0f;
+__device__ __forceinline__ void split2_up(float x0, float x1, uint32_t &hi, uint32_t &lo) {
+  hi = pack2(x0, x1);
+  const half2 h = __builtin_bit_cast(half2, hi);
+  lo = pack2(__builtin_fmaf(-(float)h[0], kLowUp, x0 * kLowUp), __builtin_fmaf(-(float)h[1], kLowUp, x1 * kLowUp));
+}
 __device__ __forceinline__ float add2(uint32_t pair, float c) {
   return __builtin_amdgcn_fdot2(__builtin_bit_cast(half2, pair), half2{(_Float16)1.0f, (_Float16)1.0f}, c, false);
 }
@@ -504,6 +512,14 @@ struct Wave {
         if constexpr (SPLIT)
           if (low) S[b] = product(a, ql[s], S[b]);
       }
+  }
+  // S of K's low parts, which are held times 2^11, to be added to.
+  template <int NB>
+  __device__ __forceinline__ static void low_parts(f32x16 (&S)[NB]) {
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) S[b][i] *= 1.0f / kLowUp;
   }
   // What the queries of positions lo .. hi see of the block of B tokens from t0 on: 0 nothing, 1 a part, 2 all.
   __device__ __forceinline__ int sight(int t0, int B, int lo, int hi) const {

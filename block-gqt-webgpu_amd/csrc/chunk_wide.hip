@@ -140,8 +140,11 @@ __global__ __launch_bounds__((64 * Wide<D, SRC, BF>::W), (Wide<D, SRC, BF>::PER_
     for (int b = 0; b < 2; ++b)
 #pragma unroll
       for (int e = 0; e < 16; ++e) S[b][e] = 0.0f;
+    if constexpr (SPLIT) {
+      w.qk(smem, buf + 2 * TILE, S, false);
+      w.low_parts(S);
+    }
     w.qk(smem, buf, S, true);
-    if constexpr (SPLIT) w.qk(smem, buf + 2 * TILE, S, false);
     uint64_t seen = ~0ull;
     bool odd = false;
     if constexpr (MASKED) {
