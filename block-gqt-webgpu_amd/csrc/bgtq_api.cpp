@@ -1621,6 +1621,52 @@ bool apart(int64_t n0, int64_t s0, int64_t n1, int64_t s1, int64_t len) {
   return nested(n0, s0, n1, s1) || nested(n1, s1, n0, s0);
 }
 
+// Rows of heads as they lie: rows x heads pieces of `piece` bytes at byte strides.
+struct RowsAt {
+  __int128 at, rows, row, heads, head, piece;
+  RowsAt(const void *p, int64_t n0, int64_t s0, int64_t n1, int64_t s1, int64_t dim, int32_t dtype)
+      : at(reinterpret_cast<uintptr_t>(p)), rows(n0), heads(n1) {
+    const int64_t size = dtype == BGTQ_DTYPE_F32 ? 4 : 2;
+    row = (__int128)s0 * size, head = (__int128)s1 * size, piece = (__int128)dim * size;
+    // Pieces without a gap between them are one, whichever index is the inner one.
+    for (int k = 0; k < 2; ++k) {
+      if (heads <= 1 || head <= piece) piece += (heads - 1) * head, heads = 1, head = 0;
+      if (rows <= 1 || row <= piece) piece += (rows - 1) * row, rows = 1, row = 0;
+    }
+  }
+  __int128 end() const { return at + (rows - 1) * row + (heads - 1) * head + piece; }
+};
+
+// Whether a byte is in both. Exact, and next to nothing where the spans do not
+// meet, or where both are slices of the same rows: pairs of heads are looked at, and only
+// where the row strides differ pairs of a row and a head too. Layouts of more than kMostPairs such pairs
+// are left to the caller: false.
+bool meet(const RowsAt &a, const RowsAt &b) {
+  constexpr __int128 kMostPairs = 1 << 16;
+  if (a.end() <= b.at || b.end() <= a.at) return false;
+  if (std::max(a.end(), b.end()) >> 62) return false;  // (no memory lies there; below, 64 bits hold all products)
+  if (a.rows > 1 && b.rows > 1 && a.row != b.row) {
+    if (a.rows > b.rows) return meet(b, a);
+    if (a.rows * a.heads * b.heads > kMostPairs) return false;
+    RowsAt one = a;
+    one.rows = 1, one.row = 0;
+    for (; one.at < a.at + a.rows * a.row; one.at += a.row)
+      if (meet(one, b)) return true;
+    return false;
+  }
+  if (a.heads * b.heads > kMostPairs) return false;
+  auto floor_div = [](int64_t x, int64_t y) { return x / y - (x % y < 0); };
+  const int64_t r = (int64_t)std::max(a.row, b.row), k0 = (int64_t)(1 - a.rows), k1 = (int64_t)(b.rows - 1);  // rows of b less rows of a
+  const int64_t pa = (int64_t)a.piece, pb = (int64_t)b.piece;
+  for (int64_t g = 0; g < (int64_t)a.heads; ++g)
+    for (int64_t h = 0; h < (int64_t)b.heads; ++h) {
+      // -pb < d + k r < pa for a k of k0 .. k1
+      const int64_t d = (int64_t)(b.at + h * b.head - a.at - g * a.head);
+      if (r == 0 ? -pb < d && d < pa : std::max(k0, floor_div(-pb - d, r) + 1) <= std::min(k1, floor_div(pa - d - 1, r))) return true;
+    }
+  return false;
+}
+
 // One array of a pool: its base and strides in bytes, and the bytes of a page's rows of one head.
 bgtq_status check_pool_array(const char *what, const void *base, int64_t page_stride, int64_t head_stride, int64_t rows,
                              int64_t align, int64_t pages, int32_t heads) {
@@ -1841,6 +1887,13 @@ static bgtq_status check_rotation(const bgtq_rotation *r, int64_t rows, const in
   return BGTQ_OK;
 }
 
+static RowsAt rows_read(const bgtq_head_rows *h, int64_t rows, int32_t dim) {
+  return {h->src, rows, h->src_row_stride, h->heads, h->src_head_stride, dim, h->dtype};
+}
+static RowsAt rows_written(const bgtq_head_rows *h, int64_t rows, int32_t dim) {
+  return {h->dst, rows, h->dst_row_stride, h->heads, h->dst_head_stride, dim, h->dtype};
+}
+
 static bgtq_status check_head_rows(const bgtq_head_rows *h, int64_t rows, int32_t dim) {
   if (h->heads < 1 || h->heads > 65535) return fail(BGTQ_ERR_RANGE, "rotation: heads must be in 1..65535");
   if (h->dtype != BGTQ_DTYPE_F32 && h->dtype != BGTQ_DTYPE_F16 && h->dtype != BGTQ_DTYPE_BF16)
@@ -1855,6 +1908,8 @@ static bgtq_status check_head_rows(const bgtq_head_rows *h, int64_t rows, int32_
   if (h->src == h->dst && ((rows > 1 && h->src_row_stride != h->dst_row_stride) ||
                            (h->heads > 1 && h->src_head_stride != h->dst_head_stride)))
     return fail(BGTQ_ERR_RANGE, "rows rotated in place must keep their strides");
+  if (rows && h->src != h->dst && meet(rows_written(h, rows, dim), rows_read(h, rows, dim)))
+    return fail(BGTQ_ERR_RANGE, "rotated rows overlap the rows they come from");
   return BGTQ_OK;
 }
 
@@ -1890,8 +1945,11 @@ bgtq_status bgtq_rotate(bgtq_context *ctx, const bgtq_rotation *r, int32_t dim, 
     if (bgtq_status s = check_head_rows(q, rows, dim)) return s;
   if (k)
     if (bgtq_status s = check_head_rows(k, rows, dim)) return s;
-  if (rows && q && k && (q->dst == k->dst || q->dst == k->src || q->src == k->dst))
-    return fail(BGTQ_ERR_RANGE, "rotated q and k overlap");
+  if (rows && q && k) {
+    const RowsAt q_to = rows_written(q, rows, dim), k_to = rows_written(k, rows, dim);
+    if (meet(q_to, k_to) || meet(q_to, rows_read(k, rows, dim)) || meet(k_to, rows_read(q, rows, dim)))
+      return fail(BGTQ_ERR_RANGE, "rotated q and k overlap");
+  }
   if (!ctx) return fail(BGTQ_ERR_RANGE, "null context");
   if (!rows) return BGTQ_OK;
   DeviceScope scope;
@@ -1907,8 +1965,14 @@ bgtq_status bgtq_paged_append(bgtq_context *ctx, const bgtq_pages *g, const bgtq
   if (bgtq_status s = check_pages(g)) return s;
   if (bgtq_status s = check_rows(rows, g, true)) return s;
   if (bgtq_status s = check_rotation(r, rows->rows, positions)) return s;
-  if (q)
+  if (q) {
     if (bgtq_status s = check_head_rows(q, rows->rows, g->dim)) return s;
+    const RowsAt to = rows_written(q, rows->rows, g->dim);
+    if (rows->rows &&
+        (meet(to, {rows->k, rows->rows, rows->k_row_stride, g->kv_heads, rows->k_head_stride, g->dim, rows->k_dtype}) ||
+         meet(to, {rows->v, rows->rows, rows->v_row_stride, g->kv_heads, rows->v_head_stride, g->dim, rows->v_dtype})))
+      return fail(BGTQ_ERR_RANGE, "rotated queries overlap the K or V rows");
+  }
   if (!ctx) return fail(BGTQ_ERR_RANGE, "null context");
   if (!rows->rows) return BGTQ_OK;
   const Rotation rotation = rotation_of(r, positions, q, r->q_norm);
@@ -2135,7 +2199,9 @@ bgtq_status bgtq_paged_prefill(bgtq_context *ctx, const bgtq_pages *g, const bgt
     if (a.row < 0 || a.head < 0 || a.row % 8 || a.head % 8 || reinterpret_cast<uintptr_t>(a.p) % 16)
       return fail(BGTQ_ERR_RANGE, "q/out: 16-byte aligned bases, strides multiples of 8 elements and not negative");
   if (!apart(d->tokens, d->out_row_stride, d->q_heads, d->out_head_stride, g->dim)) return fail(BGTQ_ERR_RANGE, "out: overlapping rows");
-  if (!none && d->out == d->q) return fail(BGTQ_ERR_RANGE, "out overlaps q");
+  if (!none && meet({d->out, d->tokens, d->out_row_stride, d->q_heads, d->out_head_stride, g->dim, d->dtype},
+                    {d->q, d->tokens, d->q_row_stride, d->q_heads, d->q_head_stride, g->dim, d->dtype}))
+    return fail(BGTQ_ERR_RANGE, "out overlaps q");
   const size_t need = chunk_workspace(plan);
   if (!d->workspace || d->workspace_bytes < need) return fail(BGTQ_ERR_RANGE, "workspace of %zu bytes required", need);
   if (reinterpret_cast<uintptr_t>(d->workspace) % 16) return fail(BGTQ_ERR_RANGE, "workspace must be 16-byte aligned");

@@ -478,7 +478,9 @@ typedef struct {
 /* Row i of head h at src + i*row_stride + h*head_stride (dim elements of dtype
  * BGTQ_DTYPE_F32, _F16 or _BF16, aligned to their type; 16-byte aligned rows are
  * faster), its result likewise at dst. dst is src (the same strides: in place) or
- * overlaps no row that the call reads; its rows lie apart. heads: 1 .. 65535. */
+ * overlaps no row that the call reads (q, k and v of one projection may be slices of
+ * the same rows); its rows lie apart. Overlaps are refused, unless finding them takes more
+ * than 2^16 comparisons of a head's or a row's place. heads: 1 .. 65535. */
 typedef struct {
   const void *src;
   void *dst;
@@ -560,7 +562,7 @@ bgtq_status bgtq_paged_decode_window(bgtq_context *ctx, const bgtq_pages *pages,
  * stand for, 1 GiB of those at most, needs no contents); calls sharing one must be
  * ordered on one stream. One launch for up to 512 such pairs, else three; where the rows
  * of all sequences might take more than that GiB, sequences take turns, three launches each time.
- * HIP-graph capturable; out overlaps neither q nor the pool. */
+ * HIP-graph capturable; out overlaps neither q (refused as bgtq_rotate's overlaps) nor the pool. */
 #define BGTQ_PAGED_PREFILL_COUNTER_BYTES (64u * 1024u)
 typedef struct {
   int32_t q_heads, dtype, sequences;
