@@ -32,7 +32,7 @@ constexpr int kChunkRound = 64, kChunkLong = 384;
 constexpr int kChunkMostSplits = 64;
 // Calls of at most this many columns attend all units as narrow ones, in tiles of 32, in their one launch.
 constexpr int kChunkSmall = 512;
-// Bytes of rebuilt rows at most: sequences that take more are attended in groups.
+// Bytes of rebuilt rows: sequences that take more are attended in groups, one that does alone.
 constexpr int64_t kChunkRebuiltBytes = (int64_t)1 << 30;
 
 struct ChunkParams {

@@ -557,11 +557,14 @@ bgtq_status bgtq_paged_decode_window(bgtq_context *ctx, const bgtq_pages *pages,
  * rows by both as pairs of FP16 values (22 bits, of K values down to 2^-14; 2^-36 absolute below). scale: of the logits, at most 2e38; 0 =
  * 1 / sqrt(dim). workspace: 16-byte aligned, bgtq_paged_prefill_workspace_size()
  * bytes (its first BGTQ_PAGED_PREFILL_COUNTER_BYTES zero before the first call on it,
- * left zero by every call whatever its geometry; the rest, partial sums and in calls
- * of more than 512 (row, head of a group) pairs the FP16 rows that packed and 8-bit pages
- * stand for, 1 GiB of those at most, needs no contents); calls sharing one must be
- * ordered on one stream. One launch for up to 512 such pairs, else three; where the rows
- * of all sequences might take more than that GiB, sequences take turns, three launches each time.
+ * left zero by every call whatever its geometry; the rest needs no contents: partial
+ * sums, and in calls of more than 512 (row, head of a group) pairs the rotated queries and the FP16
+ * rows that packed and 8-bit pages stand for). Those rows are 4 * dim * kv_heads bytes
+ * a token, 6 where FP16 queries meet packed K, of whole sequences at max_length: as
+ * many as fit 1 GiB, and one where not even that fits (8 heads of dim 128: 4 GiB at 2^20 tokens, 6 with FP16 queries on
+ * packed K), so pass no more than the step's longest length. Calls sharing a workspace must be
+ * ordered on one stream. One launch for up to 512 such pairs, else three; where not all
+ * sequences fit, they take turns in their order: one launch, then three for each turn.
  * HIP-graph capturable; out overlaps neither q (refused as bgtq_rotate's overlaps) nor the pool. */
 #define BGTQ_PAGED_PREFILL_COUNTER_BYTES (64u * 1024u)
 typedef struct {

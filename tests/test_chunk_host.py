@@ -62,3 +62,25 @@ def test_limits_and_workspace():
     # no rows need no pointers; what is left is the context
     assert _status(tokens=0, offsets=None, lengths=None, page_table=None, q=None, out=None) == _status() == _lib.ERR_RANGE
     assert b"context" in L.bgtq_last_error()
+
+
+def test_workspace_of_rebuilt_rows():
+    """4 dim heads bytes a token, of as many sequences at max_length as fit 1 GiB, and of one at least."""
+    L, n, heads, dim = _lib.lib(), ctypes.c_size_t(), 8, 128
+    pages = _pages(kv_heads=heads, dim=dim, k_page_stride=heads * 64 * dim, k_head_stride=64 * dim, v_page_stride=heads * 64 * dim,
+                   v_head_stride=64 * dim, v_scales_page_stride=heads * 64, v_scales_head_stride=64)
+
+    def size(max_length, sequences, tokens):
+        d = _desc(q_heads=16, q_row_stride=16 * dim, q_head_stride=dim, out_row_stride=16 * dim, out_head_stride=dim, max_length=max_length,
+                  page_table_stride=1 << 18, sequences=sequences, tokens=tokens)
+        assert L.bgtq_paged_prefill_workspace_size(ctypes.byref(pages), ctypes.byref(d), ctypes.byref(n)) == _lib.OK
+        return n.value
+    few = size(64, 1, 10)  # no rebuilt rows, no partials
+    assert few == _lib.PAGED_PREFILL_COUNTER_BYTES
+    for max_length, sequences in ((1000, 1), (1 << 17, 1), (1 << 17, 2), (1 << 17, 3), (1 << 18, 50), (1 << 19, 1), (1 << 19, 50), (1 << 20, 1),
+                                  (1 << 24, 7)):
+        rows = (max_length + 63) // 64 * 64
+        one = rows * heads * dim * 4
+        held = max(1, min(sequences, (1 << 30) // one))
+        partials = size(max_length, sequences, 3)  # (a small call's: fewer than a large one's)
+        assert held * one + few <= size(max_length, sequences, 5000) <= held * one + partials + (200 << 20)
