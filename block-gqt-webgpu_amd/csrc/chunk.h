@@ -26,11 +26,26 @@ constexpr int chunk_wide_residents(int dim, bool split) {
 }
 // Costs of a unit, in eighths of a wide block: its set-up, a block of a wide
 // unit, one of a narrow unit; the least cost of a wide and of a narrow item where a unit is split.
+// us of calls that differ by more than two runs of one do (A: 13 sequences of 3 KV heads, 301 new rows among
+// single ones; B, C: 16 of five new rows behind up to 4099 tokens, 14 / 2 heads of layout B, d=64, BF16 and FP16
+// rows; D: the same on 16 / 4 heads of d=128; E: on the calibration's 9 / 3 heads; F: 8 of 36 rows, as B):
+//   set-up 4 / 16 / 32:              B 32.2 / 32.1 / 34.3, C 36.5 / 36.5 / 38.6
+//   a narrow block 2 / 3 / 6:        A 72.5 / 70.2 / 72.8, D 35.1 / 32.5 / 32.4, E 25.0 / 22.7 / 21.3, B 32.2 / 32.1 / 34.5
+//   least of a wide item 24 / 48 / 96: B 33.5 / 32.1 / 37.5, C 36.8 / 36.5 / 43.6, F 33.1 / 37.2 / 44.6
+//   of a narrow one 16 / 24 / 32 / 48: A 73.3 / 73.4 / 70.2 / 73.4, E 21.2 / 21.4 / 22.7 / 25.4, D 32.8 / 32.4 / 32.5 / 35.6
 constexpr int kChunkSetup = 16, kChunkWide = 8, kChunkNarrow = 3, kChunkLeast = 48, kChunkLeastNarrow = 32;
-// A second round of wide items costs this much more; none is made of calls whose items may cost kChunkLong at most.
+// A second round of wide items costs this much more (0 / 64 / no second round: A 71.3 / 70.2 / 70.9 us, 2048 rows behind
+// 30720 tokens on 14 / 2 heads of d=64 in FP16 pages 309.8 / 309.6 / 319.7); none is made of calls whose items may cost kChunkLong at
+// most, which leaves their workgroups the search for it (A 71.4 us with 0).
 constexpr int kChunkRound = 64, kChunkLong = 384;
+// (A bound on a merge's chain, which the shares hardly meet: 16, 32 and 128 within 1% but for 4 x 36 rows behind 8156
+// tokens, as F, 37.2 us with 16, 35.0 with 64.)
 constexpr int kChunkMostSplits = 64;
-// Calls of at most this many columns attend all units as narrow ones, in tiles of 32, in their one launch.
+// Calls of at most this many columns attend all units as narrow ones, in tiles of 32, in their one launch. us, 64 / 256 /
+// 512 / 1024 / 2048: 32 single tokens (224 columns, up to 32768 tokens) 62.8 / 53.9 / 53.8 / 53.8 / 54.5, D (320) 43.3 / 43.0 /
+// 32.5 / 32.9 / 32.8, 2 x 36 rows of B's heads (504) 32.6 / 32.6 / 23.5 / 24.0 / 23.2, 2 x 1000 rows of 8 heads of d=128 behind a window (2000) 65.3 / 66.2 / 65.9
+// / 66.1 / 94.9. From 512 to 1024 the narrow way is the faster one too in B (560: 32.1 / 21.0), C (36.5 / 23.4), 4 x 36 rows (1008: 35.0 /
+// 26.5) and 74 single tokens (518, all of which find no wide unit in two launches: 67.3 / 55.6).
 constexpr int kChunkSmall = 512;
 // Bytes of rebuilt rows: sequences that take more are attended in groups, one that does alone.
 constexpr int64_t kChunkRebuiltBytes = (int64_t)1 << 30;

@@ -43,7 +43,7 @@
 // Behind a window (WIN) a wave's blocks are the sinks', those at its 32 queries'
 // window edge and diagonal, seen in part and masked from a bit per key, and
 // between them full ones, in a loop of their own without that code: 11 prompts behind
-// 511 keys and 4 sinks, 14 / 2 heads of d=64, 61 to 62 us (470 TFLOP/s of what is seen; with one body
+// 511 keys and 4 sinks, 14 / 2 heads of d=64, 61 to 64 us (450 to 470 TFLOP/s of what is seen; with one body
 // for all blocks 80). Three or four of a wave's ten blocks are masked, and two of a
 // workgroup's twelve are not its own. At d=64 the 128 registers of four waves per SIMD leave 24 or 28 bytes
 // of scratch to the masked blocks there, none to the full ones.

@@ -1,9 +1,10 @@
 // Head norms and position rotation of query and key rows in one pass
 // (bgtq_rotate): rotate_rows.h has the arithmetic, a workgroup a run of whole
 // rows, so that the heads of a row share its table row in the L1 cache; grid y
-// is the queries, then the keys. HBM bounds many rows: 16384 of 14 + 2 heads of
-// d=64 in BF16, normed, 12.9 us (71 MB, 5.5 TB/s; a copy reaches 5.1 to 5.5); one row is a
-// launch of 2.3 us.
+// is the queries, then the keys. Memory and the norm's chain bound many rows: 16384 of 14 + 2 heads
+// of d=64 in BF16, normed (71 MB), take 12.9 to 14.3 us where they lie in the Infinity Cache (256 MB)
+// from the call before, as a layer's rows do (a copy of as much 9.6), and 19.7 over eight sets of
+// buffers in turn, from HBM (a copy 15.4); one row is a launch of 2.3 us.
 #include "rotate_rows.h"
 
 namespace bgtq {
@@ -11,7 +12,7 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// (Six waves per SIMD: 16384 rows of 14 + 2 heads 12.9 us; eight, with a register spilled, 13.6, the compiler's own four 14.6.)
+// (Six waves per SIMD: those 16384 rows, cached, 12.9 us; eight, with a register spilled, 13.6, the compiler's own four 14.6.)
 template <int D>
 __global__ __launch_bounds__(kThreads, 6) void rotate_kernel(Rotation q, Rotation k, int64_t rows) {
   if (blockIdx.y == 0) rot::rotate_queries<D, kThreads>(q, rows, blockIdx.x, gridDim.x);

@@ -553,7 +553,7 @@ bgtq_status bgtq_paged_decode_window(bgtq_context *ctx, const bgtq_pages *pages,
  * q_heads / kv_heads at most 16; tokens * q_heads / kv_heads below 2^31. Logits, softmax
  * statistics and sums are FP32; probabilities are rounded to FP16 (11 bits down to
  * 2^-25 of the largest) for the product with V. Packed K is multiplied in the code
- * domain: BF16 rows by the rotated query and K row rounded to FP16 each, FP16
+ * domain: BF16 rows by the rotated query and K row rounded to FP16 each (K values below 2^-14 to 2^-25 absolute), FP16
  * rows by both as pairs of FP16 values (22 bits, of K values down to 2^-14; 2^-36 absolute below). scale: of the logits, at most 2e38; 0 =
  * 1 / sqrt(dim). workspace: 16-byte aligned, bgtq_paged_prefill_workspace_size()
  * bytes (its first BGTQ_PAGED_PREFILL_COUNTER_BYTES zero before the first call on it,
